@@ -234,6 +234,30 @@ int moba_hip_paged_append(const void* k, const void* v, int dtype, int N, int Hk
                           int table_width, const int* token_seq, const int* token_pos,
                           void* stream);
 
+/* Rotary append (no counterpart in the reference, whose callers rotate Q and K
+ * before its append): N new tokens k/v go into the page pool
+ * k_cache/v_cache [num_pages, page_size, Hkv, D] at (token_seq[n],
+ * token_pos[n]) through table [B, table_width], the keys rotated; their
+ * queries (Hq > 0; Hq = 0: q and q_out null) are rotated into q_out [N,Hq,D].
+ * q, k, v have a token and a head stride each (elements; dims contiguous).
+ * The first rotary_dim dims of a head turn in pairs (i, i + rotary_dim/2), or
+ * (2i, 2i+1) when interleaved, by row token_pos[n] + offsets[token_seq[n]]
+ * (offsets [B] nullable) of cos_sin [max_pos][rotary_dim/2][2] fp32 (16-byte
+ * aligned): a' = a cos - b sin, b' = a sin + b cos, rounded once.  The other
+ * dims and the values are copied.  q_out must not overlap the inputs.
+ * token_seq -1 marks padding: nothing of the token is written.  A token whose
+ * slot, page or angle does not exist has no key and value written (nor, without
+ * slot or angle, its query) and sets bit 1, 2 or 4 of *status (nullable; the
+ * caller clears it first).  Two tokens of one cell leave either's data. */
+int moba_hip_append_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                           const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                           int dtype, int N, int Hq, int Hkv, int D, const float* cos_sin,
+                           int max_pos, int rotary_dim, int interleaved, void* k_cache,
+                           void* v_cache, int num_pages, int page_size, const int* table, int B,
+                           int table_width, const int* token_seq, const int* token_pos,
+                           const int* offsets, void* q_out, int* status, void* stream);
+
 /* Key means of closed chunks into means [B, max_chunks, Hkv, D] (cache dtype):
  * canonical fp32 sum (64 strided partial sums, then a fixed pairwise tree),
  * / chunk, for chunk in [1, 1024].  mode 0: item i = (item_seq[i], chunk
@@ -365,6 +389,31 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
                                    const int* ids, const int* positions, const void* means,
                                    int max_chunks, int chunk, int width, int R, int dense,
                                    int* selected, void* out, float* lse, void* stream);
+
+/* Attention of Nq query rows over a prefix that several of them share and
+ * their own tokens, both in the page pool (no counterpart in the reference,
+ * whose decode reads a row's tokens row by row: paged_decode.py:67-112).
+ * q [Nq,Hq,D]; row r attends its prefix segment and own_lengths[r] (device;
+ * cut to [0, max_length]) tokens of its own slot.  The host's plan holds the
+ * work: items [n_items][8] int32 (first entry of the segment in rows; first
+ * (row, q head of the kv head) pair; pairs, at most 128, 0 pads; page-table row;
+ * kv head; range; ranges; tokens of the segment or -1: the rows' own
+ * lengths), rows (the segments' query rows), row_parts [3][Nq] (first
+ * partial, prefix ranges, all ranges of each row).  Every range of every
+ * (row, head) belongs to exactly one item; a row's partials are those of its
+ * prefix, then its own.  Prefix tokens must fit the table
+ * (table_width * page_size).  Workspaces part_o [parts*Hq, D] and part_ml
+ * [parts*Hq, 2] fp32, parts = sum of all ranges.  out [Nq,Hq,D] (dtype),
+ * lse [Nq,Hq] fp32 natural log; nothing attended: zeros and -inf.  A token in
+ * an unmapped page is not attended.  q, k_cache, v_cache, out: 16-byte
+ * aligned.  Two launches; results do not depend on timing. */
+int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
+                              float scale, const void* k_cache, const void* v_cache,
+                              int num_pages, int page_size, const int* table, int table_width,
+                              const int* own_lengths, int max_length, const int* items,
+                              int n_items, const int* rows, const int* row_parts,
+                              float* part_o, float* part_ml, void* out, float* lse,
+                              void* stream);
 
 /* ------------------------------------------------ host page pool (CPU only)
  *

@@ -1,0 +1,178 @@
+"""Attention for a batch whose sequences share long prefixes.
+
+A prefix (a system prompt, a document, a prompt that is sampled several times)
+is stored once, in a slot of its own, and read once for all the query rows
+behind it; each row then attends the tokens of its own slot.  The plan of a
+batch is made once and serves every layer and step: which rows share what is
+fixed, their own lengths are read on the device.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import torch
+
+from .cache_layout import positive_int
+from .ops import _lib
+from .rotary import _DTYPES, _index, _pool
+
+# (row, q head of a kv head) pairs of a work item: 4 waves x 32 columns
+_BLOCK = 128
+_XCDS = 8   # workgroup L runs on XCD L % 8
+
+
+def _slots(values, name, n=None):
+    out = np.asarray(values.cpu() if isinstance(values, torch.Tensor) else values)
+    if out.ndim != 1 or out.dtype.kind not in "iu" or (n is not None and len(out) != n):
+        raise ValueError(f"{name} must be one integer per query row")
+    if len(out) and (out.min() < -1 or out.max() >= 2 ** 31):
+        raise ValueError(f"{name} entries must be -1 or more")
+    return out.astype(np.int64)
+
+
+class SharedPrefixPlan:
+    """Which query rows share which prefix, cut into work items.
+
+    ``prefix_ids``, ``prefix_lengths``, ``suffix_ids``: one entry per query
+    row.  The row attends tokens [0, prefix_length) of page-table row
+    ``prefix_id`` (-1: no prefix, with length 0) and then its own length of
+    tokens of page-table row ``suffix_id`` (-1: none).  Rows of one
+    (prefix_id, prefix_length) are served together, and so are rows of one
+    suffix_id (several query tokens of a sequence, each with its own length).
+    ``max_suffix`` bounds the own lengths (longer ones are cut to it).
+    """
+
+    def __init__(self, prefix_ids, prefix_lengths, suffix_ids, num_q_heads, num_kv_heads, head_dim,
+                 *, max_suffix, device="cuda"):
+        hq, hkv = positive_int(num_q_heads, "num_q_heads"), positive_int(num_kv_heads, "num_kv_heads")
+        d = positive_int(head_dim, "head_dim")
+        if hq % hkv:
+            raise ValueError("Hq must be a multiple of Hkv")
+        if d % 8 or d > 256:
+            raise ValueError("head_dim must be a multiple of 8 in [8,256]")
+        if isinstance(max_suffix, bool) or not isinstance(max_suffix, int) or \
+                not 0 <= max_suffix < 2 ** 31:
+            raise ValueError("max_suffix must be a length")
+        prefix = _slots(prefix_ids, "prefix_ids")
+        n = len(prefix)
+        if n < 1:
+            raise ValueError("one query row at least")
+        length = _slots(prefix_lengths, "prefix_lengths", n)
+        suffix = _slots(suffix_ids, "suffix_ids", n)
+        if length.min() < 0 or (length[prefix < 0] != 0).any():
+            raise ValueError("prefix_lengths must be 0 or more, and 0 without a prefix")
+        if n * hq >= 2 ** 31:
+            raise ValueError("query grid exceeds int32 capacity")
+        self.rows, self.num_q_heads, self.num_kv_heads, self.head_dim = n, hq, hkv, d
+        self.max_suffix = max_suffix
+        self.max_prefix = int(length.max())
+        self.max_slot = int(max(prefix[length > 0].max(initial=-1), suffix.max()))
+        flat = self._build(prefix, length, suffix)
+        self.meta = torch.from_numpy(flat).to(device)
+        self.device = self.meta.device
+
+    def _build(self, prefix, length, suffix):
+        n, hkv, group = self.rows, self.num_kv_heads, self.num_q_heads // self.num_kv_heads
+        segments = []   # (slot, tokens or -1, bound of the tokens, rows)
+        shared, alone = {}, {}
+        for row in range(n):
+            if length[row] > 0:
+                shared.setdefault((int(prefix[row]), int(length[row])), []).append(row)
+            if suffix[row] >= 0 and self.max_suffix:
+                alone.setdefault(int(suffix[row]), []).append(row)
+        segments += [(slot, tokens, tokens, rows) for (slot, tokens), rows in shared.items()]
+        segments += [(slot, -1, self.max_suffix, rows) for slot, rows in alone.items()]
+        blocks = [-(-len(rows) * group // _BLOCK) for *_, rows in segments]
+        keys = sum(b * hkv * bound for b, (_, _, bound, _) in zip(blocks, segments))
+        # about two work items per CU, ranges of 256 keys at least
+        target = max(256, -(-keys // 512))
+        n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
+        row_list, sharing = [], []
+        for (slot, tokens, bound, rows), nb in zip(segments, blocks):
+            splits = max(1, -(-bound // target))
+            (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
+            for kh in range(hkv):
+                for s in range(splits):
+                    sharing.append([
+                        (len(row_list), b * _BLOCK, min(_BLOCK, len(rows) * group - b * _BLOCK),
+                         slot, kh, s, splits, tokens) for b in range(nb)])
+            row_list += rows
+        items = self._order(sharing)
+        part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
+        self.parts = int(part_at[-1])
+        self.n_items = len(items)
+        arrays = [np.asarray(items, np.int64).ravel(), np.asarray(row_list, np.int64),
+                  part_at[:-1], n_prefix, n_prefix + n_suffix]
+        self._rows_at = 4 * arrays[0].size
+        self._parts_at = self._rows_at + 4 * arrays[1].size
+        return np.concatenate(arrays).astype(np.int32)
+
+    @staticmethod
+    def _order(sharing):
+        """Items that read the same keys go to one XCD, one after another;
+        XCDs are filled evenly, and an item of no pairs pads a short one."""
+        per = [[] for _ in range(_XCDS)]
+        for items in sharing:
+            min(per, key=len).extend(items)
+        depth = max(map(len, per))
+        pad = (0, 0, 0, 0, 0, 0, 1, 0)
+        return [per[x][i] if i < len(per[x]) else pad
+                for i in range(depth) for x in range(_XCDS)]
+
+
+@torch.no_grad()
+def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan, *, scale=None,
+                            out=None, lse=None):
+    """Softmax attention of q [Nq,Hq,D] over each row's shared prefix and its
+    own tokens in a page pool; returns (out [Nq,Hq,D], lse [Nq,Hq] fp32, natural
+    log).
+
+    k_cache, v_cache [pages,page_size,Hkv,D] and page_table [slots,width] int32
+    as in :func:`moba_hip.append_rotary`; ``suffix_lengths`` [Nq] int32: how many
+    tokens of its own slot each row attends (read on the device, cut to
+    [0, plan.max_suffix]).  ``scale`` defaults to D ** -0.5.  A row with nothing
+    to attend gives zeros and an lse of -inf; a token in an unmapped page is
+    not attended.  Nothing is read back, so a call can be captured into a graph
+    (``out`` and ``lse``, contiguous, then keep their addresses)."""
+    pages, page, hkv, d = _pool(k_cache, v_cache, page_table)
+    dev = k_cache.device
+    if not isinstance(plan, SharedPrefixPlan):
+        raise ValueError("plan must be a SharedPrefixPlan")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype != k_cache.dtype or \
+            q.device != dev or plan.device != dev:
+        raise ValueError("q must be [Nq,Hq,D] of the pool's device and dtype, and the plan on it")
+    if q.requires_grad:
+        raise ValueError("KV cache/decode is inference-only; detach Q/K/V")
+    n, hq = plan.rows, plan.num_q_heads
+    if tuple(q.shape) != (n, hq, plan.head_dim) or (hkv, d) != (plan.num_kv_heads, plan.head_dim):
+        raise ValueError("q and the pool must have the plan's rows, heads and head_dim")
+    slots, width = page_table.shape
+    if plan.max_slot >= slots or plan.max_prefix > width * page:
+        raise ValueError("the plan's slots and prefix lengths must fit page_table")
+    _index(suffix_lengths, "suffix_lengths", 1, dev, n)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
+    q = q.contiguous()
+    for t, name, shape, dtype in ((out, "out", (n, hq, d), q.dtype),
+                                  (lse, "lse", (n, hq), torch.float32)):
+        if t is not None and (not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or
+                              t.dtype != dtype or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {list(shape)} {dtype} on the pool's device")
+    if (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+        raise ValueError("q and the pool must be 16-byte aligned")
+    with torch.cuda.device(dev):
+        out = torch.empty_like(q) if out is None else out
+        lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if lse is None else lse
+        parts = plan.parts * hq
+        # partial sums [parts, D], then (max, sum) pairs
+        work = torch.empty(parts * (d + 2), dtype=torch.float32, device=dev)
+        meta = plan.meta.data_ptr()
+        _lib.call("moba_hip_shared_attention", q.data_ptr(), _DTYPES[q.dtype], n, hq, hkv, d, scale,
+                  k_cache.data_ptr(), v_cache.data_ptr(), pages, page, page_table.data_ptr(), width,
+                  suffix_lengths.data_ptr(), min(plan.max_suffix, width * page), meta,
+                  plan.n_items, meta + plan._rows_at, meta + plan._parts_at, work.data_ptr(),
+                  work.data_ptr() + 4 * parts * d, out.data_ptr(), lse.data_ptr(),
+                  _lib.stream_of(dev))
+    return out, lse
