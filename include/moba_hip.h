@@ -399,7 +399,7 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
  * (row, q head of the kv head) pair; pairs, at most 128, 0 pads; page-table row;
  * kv head; range; ranges; tokens of the segment or -1: the rows' own
  * lengths), rows (the segments' query rows), row_parts [3][Nq] (first
- * partial, prefix ranges, all ranges of each row).  Every range of every
+ * partial, prefix ranges, all ranges of each row; max_parts bounds the last).  Every range of every
  * (row, head) belongs to exactly one item; a row's partials are those of its
  * prefix, then its own.  Prefix tokens must fit the table
  * (table_width * page_size).  Workspaces part_o [parts*Hq, D] and part_ml
@@ -411,7 +411,7 @@ int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv,
                               float scale, const void* k_cache, const void* v_cache,
                               int num_pages, int page_size, const int* table, int table_width,
                               const int* own_lengths, int max_length, const int* items,
-                              int n_items, const int* rows, const int* row_parts,
+                              int n_items, const int* rows, const int* row_parts, int max_parts,
                               float* part_o, float* part_ml, void* out, float* lse,
                               void* stream);
 

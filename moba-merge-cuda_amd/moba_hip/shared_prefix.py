@@ -17,8 +17,9 @@ from .cache_layout import positive_int
 from .ops import _lib
 from .rotary import _DTYPES, _index, _pool
 
-# (row, q head of a kv head) pairs of a work item: 4 waves x 32 columns
-_BLOCK = 128
+# (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
+# or the same 32 and a quarter of the keys each
+_WIDE, _NARROW = 128, 32
 _XCDS = 8   # workgroup L runs on XCD L % 8
 
 
@@ -83,24 +84,25 @@ class SharedPrefixPlan:
                 alone.setdefault(int(suffix[row]), []).append(row)
         segments += [(slot, tokens, tokens, rows) for (slot, tokens), rows in shared.items()]
         segments += [(slot, -1, self.max_suffix, rows) for slot, rows in alone.items()]
-        blocks = [-(-len(rows) * group // _BLOCK) for *_, rows in segments]
+        sizes = [_WIDE if len(rows) * group > 2 * _NARROW else _NARROW for *_, rows in segments]
+        blocks = [-(-len(rows) * group // size) for (*_, rows), size in zip(segments, sizes)]
         keys = sum(b * hkv * bound for b, (_, _, bound, _) in zip(blocks, segments))
-        # about two work items per CU, ranges of 256 keys at least
-        target = max(256, -(-keys // 512))
+        target = max(128, -(-keys // (768 if self.head_dim <= 128 else 512)))
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
         row_list, sharing = [], []
-        for (slot, tokens, bound, rows), nb in zip(segments, blocks):
+        for (slot, tokens, bound, rows), size, nb in zip(segments, sizes, blocks):
             splits = max(1, -(-bound // target))
             (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
             for kh in range(hkv):
                 for s in range(splits):
                     sharing.append([
-                        (len(row_list), b * _BLOCK, min(_BLOCK, len(rows) * group - b * _BLOCK),
+                        (len(row_list), b * size, min(size, len(rows) * group - b * size),
                          slot, kh, s, splits, tokens) for b in range(nb)])
             row_list += rows
         items = self._order(sharing)
         part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
         self.parts = int(part_at[-1])
+        self.max_parts = int((n_prefix + n_suffix).max())
         self.n_items = len(items)
         arrays = [np.asarray(items, np.int64).ravel(), np.asarray(row_list, np.int64),
                   part_at[:-1], n_prefix, n_prefix + n_suffix]
@@ -172,7 +174,7 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
         _lib.call("moba_hip_shared_attention", q.data_ptr(), _DTYPES[q.dtype], n, hq, hkv, d, scale,
                   k_cache.data_ptr(), v_cache.data_ptr(), pages, page, page_table.data_ptr(), width,
                   suffix_lengths.data_ptr(), min(plan.max_suffix, width * page), meta,
-                  plan.n_items, meta + plan._rows_at, meta + plan._parts_at, work.data_ptr(),
-                  work.data_ptr() + 4 * parts * d, out.data_ptr(), lse.data_ptr(),
+                  plan.n_items, meta + plan._rows_at, meta + plan._parts_at, plan.max_parts,
+                  work.data_ptr(), work.data_ptr() + 4 * parts * d, out.data_ptr(), lse.data_ptr(),
                   _lib.stream_of(dev))
     return out, lse
