@@ -397,9 +397,10 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
  * cut to [0, max_length]) tokens of its own slot.  The host's plan holds the
  * work: items [n_items][8] int32 (first entry of the segment in rows; first
  * (row, q head of the kv head) pair; pairs, at most 128, 0 pads; page-table row;
- * kv head; range; ranges; tokens of the segment or -1: the rows' own
- * lengths), rows (the segments' query rows), row_parts [3][Nq] (first
- * partial, prefix ranges, all ranges of each row; max_parts bounds the last).  Every range of every
+ * kv head; range | ranges << 16; tokens of the segment or -1: the rows' own
+ * lengths; the row of all the pairs or -1: several), rows (the segments' query
+ * rows), row_parts [3][Nq] (each row's first partial of its prefix and of its
+ * own tokens, its ranges in all; max_parts bounds the last).  Every range of every
  * (row, head) belongs to exactly one item; a row's partials are those of its
  * prefix, then its own.  Prefix tokens must fit the table
  * (table_width * page_size).  Workspaces part_o [parts*Hq, D] and part_ml

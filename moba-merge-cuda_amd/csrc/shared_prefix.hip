@@ -10,6 +10,8 @@
 // (row, head) pairs against the range's K/V, read once for the block.  An item
 // leaves (O, m, z) of its range in fp32; merge_kernel joins a row's ranges in
 // their order.  Results do not depend on timing.
+#include <type_traits>
+
 #include "common.h"
 #include "../../include/moba_hip.h"
 
@@ -24,8 +26,9 @@ struct Item {
   int n_m;      // pairs of the block
   int slot;     // page-table row of the keys
   int kh;
-  int split, splits;
+  int split;    // split | splits << 16
   int length;   // tokens of the segment; -1: each row's own length
+  int row;      // the row of the block's pairs; -1: several
 };
 
 struct SharedArgs {
@@ -33,20 +36,16 @@ struct SharedArgs {
   int Hq, Hkv, D, G;
   float scale_log2;
   int num_pages, P, W;
+  uint32_t pool_bytes;      // of k_cache; 0: 4 GiB or more
   const int* table;
   const int* lengths;       // own tokens of each row
   int max_length;
   const Item* items;
   const int* rows;
-  const int *part_at, *n_prefix, *n_part;  // per row: first partial, prefix ranges, ranges
+  const int *prefix_at, *own_at, *n_part;  // per row: first partials, ranges in all
   float* part_o;
   float2* part_ml;
 };
-
-constexpr uint32_t kNoToken = 0xffffffffu;
-
-// What a key of no token loads: zeros, so that a weight of 0 meets no NaN.
-__device__ __attribute__((aligned(16))) const uint16_t g_zero[8] = {0};
 
 // 16 bytes per lane from any address straight into LDS (lane l's at
 // lds + 16 l); ordered by the caller as dma_lds16.
@@ -54,55 +53,127 @@ MOBA_DEV void dma_global16(const void* p, const void* lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds_addr(lds)), "v"(p) : "memory", "m0");
 }
+// s_waitcnt vmcnt(N) for any N, and nothing moves across it.
+template <int N> MOBA_DEV void landed() {
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | (N >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+// This wave's LDS reads are complete.
+MOBA_DEV void lds_read_done() {
+  __builtin_amdgcn_s_waitcnt(0xC07F);
+  asm volatile("" ::: "memory");
+}
 
 // Sizes of a head dim's kernel.
 template <int ND> struct Dims {
   static constexpr int DP = ND <= 64 ? 64 : ND <= 128 ? 128 : 256;  // row of the LDS layouts
   static constexpr int NKS = ND / 16, NDB = ND / 32, NB = DP / 8;
-  static constexpr int KEYS = DP <= 64 ? 64 : 32;  // keys of a tile that four waves share
+  static constexpr int KEYS = DP <= 64 ? 64 : 32;   // keys of a tile that four waves share
   static constexpr int TILE = KEYS * DP;
-  // bytes of LDS: two stages of K and V tiles, looked-up tokens and flags; or a
-  // V tile per wave and the query rows
-  static constexpr int TOK = 4 * TILE * 2, FLAGS = TOK + 2 * 256 * 4, WIDE = FLAGS + 8 * 4;
-  static constexpr int ROWS = 4 * 32 * DP * 2, NARROW = ROWS + 32 * DP * 2;
-  static constexpr int LDS = WIDE > NARROW ? WIDE : NARROW;
-  static constexpr int WAVES = ND <= 128 ? 3 : 2;  // per SIMD
+  static constexpr int OWN = DP <= 64 ? 32 : 16;    // keys of a tile that a wave has alone
+  // LDS: two stages of shared K and V tiles, or a K and a V tile per wave; the
+  // pool's token of up to CAP keys; flags
+  static constexpr int CAP = 2048;
+  static constexpr int TILES = 4 * TILE * 2;
+  static_assert(4 * 2 * OWN * DP * 2 <= TILES && 2 * NDB * 4 * 64 * 16 <= TILES, "LDS");
+  static constexpr int TOK = TILES, FLAGS = TOK + CAP * 4, LDS = FLAGS + 16;
+  static constexpr int WAVES = ND <= 128 ? 3 : 2;   // per SIMD
+};
+
+// Where a key's row of the pool is: its byte offset below 4 GiB (NEAR), else
+// its token.  A key of no token, or of an unmapped page, loads zeros, so that a
+// weight of 0 meets no NaN: its offset lies outside the buffer resource.
+constexpr uint32_t kNowhere = 0xffff0000u;
+__device__ __attribute__((aligned(16))) const uint16_t g_zero[8] = {0};
+
+// The K and V rows of a kv head in the pool.
+template <bool NEAR> struct Rows {
+  __amdgpu_buffer_rsrc_t k, v;
+  const char *kp, *vp;
+  uint32_t row_bytes;
+  MOBA_DEV Rows(const SharedArgs& a, int kh) {
+    const uint32_t head = (uint32_t)(kh * a.D * 2);
+    kp = (const char*)a.kc + head;
+    vp = (const char*)a.vc + head;
+    row_bytes = (uint32_t)(a.Hkv * a.D * 2);
+    if constexpr (NEAR) {
+      k = make_rsrc(kp, a.pool_bytes - head);
+      v = make_rsrc(vp, a.pool_bytes - head);
+    }
+  }
+  MOBA_DEV uint32_t place(uint32_t token) const { return NEAR ? token * row_bytes : token; }
+  // 64 lanes' 16-byte blocks, `byte` into the row at `at`, to lds
+  template <bool V> MOBA_DEV void bring(uint32_t at, uint32_t byte, bool on, const void* lds) const {
+    if constexpr (NEAR) {
+      dma_lds16(V ? v : k, lds, on ? at + byte : kNowhere, 0);
+    } else {
+      const char* p = (V ? vp : kp) + (uint64_t)at * row_bytes + byte;
+      dma_global16(on & (at != kNowhere) ? p : (const char*)g_zero, lds);
+    }
+  }
 };
 
 // What a lane knows of its (row, q head) pair.
 struct Pair {
-  int row, h, limit;
+  int row, h, limit;   // limit: tokens of the segment that the row attends
+  int64_t part;        // its partial
   bool valid;
 };
 MOBA_DEV Pair pair_of(const SharedArgs& a, const Item& x, int m) {
   Pair p;
   p.valid = m < x.n_m;
-  const int i = x.m0 + min(m, x.n_m - 1);
-  p.row = a.rows[x.row_at + i / a.G];
-  p.h = x.kh * a.G + i % a.G;
-  p.limit = x.length < 0 ? max(0, min(a.lengths[p.row], a.max_length)) : x.length;
+  const int i = x.m0 + min(m, x.n_m - 1), r = i / a.G;
+  p.h = x.kh * a.G + i - r * a.G;
+  if (x.row >= 0) {  // uniform: the loads are scalar ones
+    p.row = x.row;
+    p.limit = x.length < 0 ? max(0, min(a.lengths[x.row], a.max_length)) : x.length;
+    p.part = (x.length < 0 ? a.own_at : a.prefix_at)[x.row];
+  } else {
+    p.row = a.rows[x.row_at + r];
+    p.limit = x.length < 0 ? max(0, min(a.lengths[p.row], a.max_length)) : x.length;
+    p.part = (x.length < 0 ? a.own_at : a.prefix_at)[p.row];
+  }
+  p.part = (p.part + (x.split & 0xffff)) * a.Hq + p.h;
   return p;
 }
-MOBA_DEV int64_t partial_of(const SharedArgs& a, const Item& x, const Pair& p) {
-  return ((int64_t)a.part_at[p.row] + (x.length < 0 ? a.n_prefix[p.row] : 0) + x.split) * a.Hq + p.h;
+// Longest and shortest row of the lanes' 32 pairs, the same in every lane.
+MOBA_DEV int longest(int limit) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) limit = max(limit, __shfl_xor(limit, o, 64));
+  return __builtin_amdgcn_readfirstlane(limit);
+}
+MOBA_DEV int shortest(const Pair& p) {
+  int limit = p.valid ? p.limit : 0x7fffffff;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) limit = min(limit, __shfl_xor(limit, o, 64));
+  return __builtin_amdgcn_readfirstlane(limit);
 }
 // The keys [lo, hi) of an item's range: whole groups of 64 but for the last.
 MOBA_DEV void range_of(const Item& x, int length, int& lo, int& hi) {
-  const int per = ((length + 64 * x.splits - 1) / (64 * x.splits)) * 64;
-  lo = min(length, x.split * per);
-  hi = min(length, lo + per);
+  const int split = x.split & 0xffff, splits = (uint32_t)x.split >> 16;
+  const int per = (int)((length + 64ll * splits - 1) / (64 * splits)) * 64;
+  lo = (int)min((int64_t)length, (int64_t)split * per);
+  hi = (int)min((int64_t)length, (int64_t)lo + per);
 }
-// The pool's token of key `key` of a slot.
-MOBA_DEV uint32_t token_of(const SharedArgs& a, const int* trow, int key, int hi) {
-  const int k = min(key, hi - 1), lp = k / a.P, page = trow[lp];
-  const bool on = key < hi && page >= 0 && page < a.num_pages;
-  return on ? (uint32_t)page * a.P + (k - lp * a.P) : kNoToken;
+// Looks up the keys [k0, min(k0 + CAP, hi)) for the workgroup (and fills to a
+// multiple of 256 with kNowhere).  flag is set where a page is unmapped.
+template <bool NEAR, int CAP>
+MOBA_DEV void look_up(const SharedArgs& a, const Rows<NEAR>& rows, int slot, int k0, int hi,
+                      uint32_t* tok, int* flag) {
+  const int* trow = a.table + (int64_t)slot * a.W;
+  const int tid = threadIdx.x, n = min(CAP, hi - k0);
+  for (int i0 = 0; i0 < n; i0 += 256) {
+    const int key = min(k0 + i0 + tid, hi - 1), lp = key / a.P, page = trow[lp];
+    const bool in = k0 + i0 + tid < hi, mapped = page >= 0 && page < a.num_pages;
+    tok[i0 + tid] = in & mapped ? rows.place((uint32_t)page * a.P + (key - lp * a.P)) : kNowhere;
+    if (__any(!mapped) && (tid & 63) == 0) *flag = 1;
+  }
 }
 
 template <int NDB>
-MOBA_DEV void store_partial(const SharedArgs& a, int64_t slot, const f32x16_t (&o)[NDB], float m,
+MOBA_DEV void store_partial(const SharedArgs& a, int64_t part, const f32x16_t (&o)[NDB], float m,
                             float l, int hh) {
-  float* po = a.part_o + slot * a.D;
+  float* po = a.part_o + part * a.D;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -112,22 +183,24 @@ MOBA_DEV void store_partial(const SharedArgs& a, int64_t slot, const f32x16_t (&
         *reinterpret_cast<f32x4_t*>(po + d) =
             (f32x4_t){o[db][4 * j], o[db][4 * j + 1], o[db][4 * j + 2], o[db][4 * j + 3]};
     }
-  if (hh == 0) a.part_ml[slot] = make_float2(m, l);
+  if (hh == 0) a.part_ml[part] = make_float2(m, l);
 }
 
-// One tile's scores into the running (max, sum) of a lane's pair; returns the
-// 16-bit weights as operands of the product with V.
-template <int DT, int NKB, int NDB>
+// One tile's scores (the first NR registers of each block) into the running
+// (max, sum) of a lane's pair; returns the 16-bit weights as operands of the
+// product with V.  The reference stays while the scores are within 2^8 of it.
+constexpr float kSlack = 8.0f;
+template <int DT, int NKB, int NR, int NDB>
 MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, float& m_run, float& lsum,
-                           f32x16_t (&o)[NDB], u16x8_t (&pv)[NKB][2]) {
+                           f32x16_t (&o)[NDB], u16x8_t (&pv)[NKB][NR / 8]) {
   float mx = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+    for (int r = 0; r < NR; ++r) mx = fmaxf(mx, s[kb][r]);
   mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
-  const bool up = mx > m_run;
-  if (__any(up)) {
+  const bool up = mx > m_run + kSlack;
+  if (__any(up)) [[unlikely]] {
     const float mn = up ? mx : m_run;
     const float alpha = up ? fast_exp2(m_run - mn) : 1.0f;
     lsum *= alpha;
@@ -136,22 +209,39 @@ MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, float& m_run, flo
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     m_run = mn;
+    __builtin_amdgcn_sched_barrier(0);
   }
   // a row with nothing so far: weights of 0, not of exp2(-inf + inf)
   const float nm = m_run == -INFINITY ? 0.0f : -m_run;
   float ps = 0.0f;
 #pragma unroll
   for (int kb = 0; kb < NKB; ++kb) {
-    float p[16];
+    float p[NR];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = 0; r < NR; ++r) {
       p[r] = fast_exp2(fmaf(s[kb][r], c2, nm));
       ps += p[r];
     }
-    pv[kb][0] = pack8<DT>(p);
-    pv[kb][1] = pack8<DT>(p + 8);
+#pragma unroll
+    for (int t = 0; t < NR / 8; ++t) pv[kb][t] = pack8<DT>(p + 8 * t);
   }
   lsum += ps;
+}
+
+// Scores of keys behind `left` (counted from the tile's first) or, with holes,
+// of unmapped pages: -inf.  tok: the tile's keys.
+template <int NKB, int NR>
+MOBA_DEV void mask_scores(f32x16_t (&s)[NKB], int left, const uint32_t* tok, int hh) {
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+    for (int j = 0; j < NR / 4; ++j) {
+      const int k = kb * 32 + 8 * j + 4 * hh;
+      const u32x4_t t = *reinterpret_cast<const u32x4_t*>(tok + k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        s[kb][4 * j + i] = (k + i < left) & (t[i] != kNowhere) ? s[kb][4 * j + i] : -INFINITY;
+    }
 }
 
 // First byte of the 16-byte block that lane `lane` brings in a load of 64
@@ -164,27 +254,34 @@ template <int DP> MOBA_DEV uint32_t block_byte(uint32_t lane, uint32_t row0) {
   return ((lane % NB) ^ (f & NBM)) * 16;
 }
 
+template <int NKS> MOBA_DEV void load_query(const SharedArgs& a, const Pair& p, int hh, u16x8_t (&qf)[NKS]) {
+  const uint16_t* q = a.q + ((int64_t)p.row * a.Hq + p.h) * a.D;
+#pragma unroll
+  for (int ks = 0; ks < NKS; ++ks) {
+    const int d = ks * 16 + hh * 8;
+    const u16x8_t v = ld8(q + (d < a.D ? d : 0));
+    qf[ks] = d < a.D ? v : zero8();
+  }
+}
+
 // More than 32 pairs: every wave has 32 of them, and the four share tiles of
 // KEYS keys in two LDS stages.
-template <int DT, int ND>
+template <int DT, int ND, bool NEAR>
 MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
-  uint32_t (*tok)[256] = (uint32_t(*)[256])(smem + C::TOK);  // pool token of each key
-  int* flags = (int*)(smem + C::FLAGS);
   constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, KEYS = C::KEYS, NKB = KEYS / 32;
   constexpr int TILE = C::TILE, NB = C::NB, NDMA = KEYS * NB / 256;
-  constexpr int TPC = 256 / KEYS;   // tiles per 256 looked-up tokens
   uint16_t* Ks = (uint16_t*)smem;   // [2][TILE], then V
+  uint32_t* tok = (uint32_t*)(smem + C::TOK);
+  int* flags = (int*)(smem + C::FLAGS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 31, hh = lane >> 5, D = a.D;
 
   const Pair p = pair_of(a, x, wave * 32 + qi);
   int length = x.length;
   if (length < 0) {  // the block's longest row
-    int mx = p.limit;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor(mx, o, 64));
-    if (lane == 0) flags[wave] = mx;
+    const int mine = longest(p.limit);
+    if (lane == 0) flags[wave] = mine;
     lds_barrier();
     length = max(max(flags[0], flags[1]), max(flags[2], flags[3]));
     lds_barrier();
@@ -192,65 +289,41 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   int lo, hi;
   range_of(x, length, lo, hi);
   if (lo >= hi) {
-    if (p.valid && hh == 0) a.part_ml[partial_of(a, x, p)] = make_float2(-INFINITY, 0.0f);
+    if (p.valid && hh == 0) a.part_ml[p.part] = make_float2(-INFINITY, 0.0f);
     return;
   }
-
-  const int* trow = a.table + (int64_t)x.slot * a.W;
-  auto publish = [&](int c, uint32_t t) {  // this thread's key of chunk c of 256
-    tok[c & 1][tid] = t;
-    const bool any = __any(t == kNoToken);
-    if (lane == 0) flags[4 * (c & 1) + wave] = any;
-  };
-  const char *kp = (const char*)(a.kc + (int64_t)x.kh * D), *vp = (const char*)(a.vc + (int64_t)x.kh * D);
-  const uint32_t row_bytes = (uint32_t)(a.Hkv * D * 2);
-  // thread (wave w, lane l) brings 16-byte blocks j = (n * 4 + w) * 64 + l of a
-  // tile: row j / NB, physical block j % NB of the swizzled row
-  auto dma = [&](int it) {
-    const uint32_t* tk = &tok[(it / TPC) & 1][(it % TPC) * KEYS];
-    uint16_t* Kd = Ks + (it & 1) * TILE;
-    const uint32_t ln = opaque(lane);
-#pragma unroll
-    for (int n = 0; n < NDMA; ++n) {
-      const uint32_t row0 = (n * 4 + wave) * (64 / NB), byte = block_byte<DP>(ln, row0);
-      if (byte < ND * 2) {
-        const uint32_t t = tk[row0 + ln / NB];
-        const bool on = (t != kNoToken) & (byte < (uint32_t)D * 2);
-        const uint64_t off = (uint64_t)t * row_bytes + byte;
-        dma_global16(on ? kp + off : (const char*)g_zero, Kd + (n * 4 + wave) * 64 * 8);
-        dma_global16(on ? vp + off : (const char*)g_zero, Kd + 2 * TILE + (n * 4 + wave) * 64 * 8);
-      }
-    }
-  };
-
-  publish(0, token_of(a, trow, lo + tid, hi));
+  const Rows<NEAR> rows(a, x.kh);
   u16x8_t qf[NKS];
-  const uint16_t* qrow = a.q + ((int64_t)p.row * a.Hq + p.h) * D;
-#pragma unroll
-  for (int ks = 0; ks < NKS; ++ks) {
-    const int d = ks * 16 + hh * 8;
-    const u16x8_t v = ld8(qrow + (d < D ? d : 0));
-    qf[ks] = d < D ? v : zero8();
-  }
-  lds_barrier();
-  dma(0);
+  load_query<NKS>(a, p, hh, qf);
 
   f32x16_t oacc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
   float m_run = -INFINITY, lsum = 0.0f;
   const bool idle = wave * 32 >= x.n_m;
-  int wlim = p.valid ? p.limit : 0x7fffffff;  // the wave's shortest row
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) wlim = min(wlim, __shfl_xor(wlim, o, 64));
-  wlim = __builtin_amdgcn_readfirstlane(wlim);
-
+  const int wlim = min(shortest(p), hi);
   const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
-  auto tile = [&](int it) {
+
+  // wave w brings the 64-block loads n * 4 + w of a tile
+  auto dma = [&](int it) {
+    const uint32_t* tk = tok + it * KEYS;
+    uint16_t* Kd = Ks + (it & 1) * TILE;
+    const uint32_t ln = opaque(lane);
+#pragma unroll
+    for (int n = 0; n < NDMA; ++n) {
+      const uint32_t row0 = (n * 4 + wave) * (64 / NB), byte = block_byte<DP>(ln, row0);
+      if (byte < ND * 2) {
+        const uint32_t at = tk[row0 + ln / NB];
+        const bool on = byte < (uint32_t)D * 2;
+        rows.template bring<false>(at, byte, on, Kd + (n * 4 + wave) * 64 * 8);
+        rows.template bring<true>(at, byte, on, Kd + 2 * TILE + (n * 4 + wave) * 64 * 8);
+      }
+    }
+  };
+  auto tile = [&](int it, int kt0, bool holes) {
     const uint16_t *Kb = Ks + (it & 1) * TILE, *Vb = Kb + 2 * TILE;
     const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
-    const int kt0 = lo + it * KEYS;
     f32x16_t sacc[NKB];
     wave_prio<1>();
 #pragma unroll
@@ -261,22 +334,10 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
         sacc[kb] = mfma32<DT>(lds8(Kb, kb * 32 * DP * 2 + swz_b128<DP>(kq, ks)), qf[ks], sacc[kb]);
     }
     wave_prio<0>();
-    const int at = (it % TPC) * KEYS, c = (it / TPC) & 1;
-    if (kt0 + KEYS > wlim || __builtin_amdgcn_readfirstlane(flags[4 * c + at / 64])) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = kb * 32 + 8 * j + 4 * hh;
-          const u32x4_t t = *reinterpret_cast<const u32x4_t*>(&tok[c][at + k]);
-          const int left = (int)opaque(p.limit - kt0) - k;  // keys from k on below the limit
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sacc[kb][4 * j + i] = (i < left) & (t[i] != kNoToken) ? sacc[kb][4 * j + i] : -INFINITY;
-        }
-    }
+    if (kt0 + KEYS > wlim || holes)
+      mask_scores<NKB, 16>(sacc, (int)opaque(min(p.limit, hi) - kt0), tok + it * KEYS, hh);
     u16x8_t pv[NKB][2];
-    softmax_step<DT, NKB, NDB>(sacc, a.scale_log2, m_run, lsum, oacc, pv);
+    softmax_step<DT, NKB, 16, NDB>(sacc, a.scale_log2, m_run, lsum, oacc, pv);
     wave_prio<1>();
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -291,145 +352,120 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     wave_prio<0>();
   };
 
-  const int ntiles = (hi - lo + KEYS - 1) / KEYS;
-  for (int it = 0; it < ntiles; ++it) {
-    wait_vmcnt<0>();  // this wave's part of tile `it` has landed
-    lds_barrier();    // everyone's has, and tile it - 1 is read
-    uint32_t next = 0;
-    const bool more = it % TPC == 0 && (it / TPC + 1) * TPC < ntiles;
-    if (more) next = token_of(a, trow, lo + (it / TPC + 1) * 256 + tid, hi);
-    if (it + 1 < ntiles) dma(it + 1);
-    if (!idle) tile(it);
-    if (more) publish(it / TPC + 1, next);  // read from tile it + TPC - 1 on
+  for (int k0 = lo; k0 < hi; k0 += C::CAP) {
+    lds_barrier();  // the tokens and tiles before are read
+    if (tid == 0) flags[0] = 0;
+    lds_barrier();
+    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, tok, flags);
+    lds_barrier();
+    const bool holes = __builtin_amdgcn_readfirstlane(flags[0]) != 0;
+    const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
+    landed<0>();  // what the compiler has in flight: it must not wait for it below
+    dma(0);
+    for (int it = 0; it < ntiles; ++it) {
+      landed<0>();    // this wave's part of tile `it`
+      lds_barrier();  // everyone's, and tile it - 1 is read
+      if (it + 1 < ntiles) dma(it + 1);
+      if (!idle) tile(it, k0 + it * KEYS, holes);
+    }
   }
   const float l = lsum + __shfl_xor(lsum, 32, 64);
-  if (p.valid) store_partial<NDB>(a, partial_of(a, x, p), oacc, m_run, l, hh);
+  if (p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
 }
 
 // Up to 32 pairs: the four waves have the same pairs and take every fourth
-// group of 32 keys each, the K rows straight into registers, the V rows into
-// an LDS tile of their own, with no barrier between them; their results are
-// joined in LDS in a fixed order.
-template <int DT, int ND>
+// group of OWN keys each, through a K and a V tile of their own, with no barrier
+// between them; their results are joined in LDS in a fixed order.  The next
+// group's K is in flight from the scores on, its V from the product with V on.
+// 16-key groups fill half of a 32-row score product; what a narrow item waits
+// for is memory.
+template <int DT, int ND, bool NEAR>
 MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
-  constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, NB = C::NB;
+  constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, NB = C::NB, OWN = C::OWN;
+  constexpr int NDMA = OWN * NB / 64;  // loads of a K or V tile
+  constexpr int NR = OWN / 2;          // score registers in use
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 31, hh = lane >> 5, D = a.D;
-  uint16_t* Vs = (uint16_t*)smem + wave * 32 * DP;
-  uint16_t* Qs = (uint16_t*)(smem + C::ROWS);
+  uint16_t *Kt = (uint16_t*)smem + wave * 2 * OWN * DP, *Vt = Kt + OWN * DP;
+  uint32_t* tok = (uint32_t*)(smem + C::TOK);
+  int* flags = (int*)(smem + C::FLAGS);
 
   const Pair p = pair_of(a, x, qi);
-  int length = p.limit;  // the longest row (static: everyone's)
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) length = max(length, __shfl_xor(length, o, 64));
-  length = __builtin_amdgcn_readfirstlane(length);
+  const int length = longest(p.limit);
   int lo, hi;
   range_of(x, length, lo, hi);
   if (lo >= hi) {
-    if (tid < 32 && p.valid) a.part_ml[partial_of(a, x, p)] = make_float2(-INFINITY, 0.0f);
+    if (tid < 32 && p.valid) a.part_ml[p.part] = make_float2(-INFINITY, 0.0f);
     return;
   }
-
-  const int* trow = a.table + (int64_t)x.slot * a.W;
-  const char *kp = (const char*)(a.kc + (int64_t)x.kh * D), *vp = (const char*)(a.vc + (int64_t)x.kh * D);
-  const uint32_t row_bytes = (uint32_t)(a.Hkv * D * 2);
-  const int ntiles = (hi - lo + 31) / 32;
-  u16x8_t kf[NKS];
-  auto load_k = [&](uint32_t t) {
-    // a key of no token loads the pool's first one: its score is masked
-    const uint16_t* row = (const uint16_t*)(kp + (uint64_t)(t != kNoToken ? t : 0) * row_bytes);
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      const int d = ks * 16 + hh * 8;
-      const u16x8_t v = ld8(row + (d < D ? d : 0));
-      kf[ks] = d < D ? v : zero8();
-    }
-  };
-  auto load_v = [&](uint32_t t) {
-    const uint32_t ln = opaque(lane);
-#pragma unroll
-    for (int n = 0; n < NB / 2; ++n) {
-      const uint32_t row0 = n * (64 / NB), byte = block_byte<DP>(ln, row0);
-      const uint32_t tr = __shfl(t, row0 + ln / NB, 64);
-      if (byte < ND * 2) {
-        const bool on = (tr != kNoToken) & (byte < (uint32_t)D * 2);
-        dma_global16(on ? vp + ((uint64_t)tr * row_bytes + byte) : (const char*)g_zero, Vs + n * 64 * 8);
-      }
-    }
-  };
-  uint32_t t_now = token_of(a, trow, lo + wave * 32 + qi, hi), t_next = kNoToken;
-  if (wave < ntiles) {
-    load_k(t_now);
-    load_v(t_now);
-    t_next = token_of(a, trow, lo + (wave + 4) * 32 + qi, hi);
-  }
-  // the query rows, once for the four waves
-  const uint16_t* qrow = a.q + ((int64_t)p.row * a.Hq + p.h) * D;
-  const uint32_t kbase0 = swz_b128_base<DP>(lane);
-  for (int ks = wave; ks < NKS; ks += 4) {
-    const int d = ks * 16 + hh * 8;
-    const u16x8_t v = ld8(qrow + (d < D ? d : 0));
-    st8((uint16_t*)((char*)Qs + swz_b128<DP>(kbase0, ks)), d < D ? v : zero8());
-  }
-  int wlim = p.valid ? p.limit : 0x7fffffff;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) wlim = min(wlim, __shfl_xor(wlim, o, 64));
-  wlim = __builtin_amdgcn_readfirstlane(wlim);
-  lds_barrier();
+  const Rows<NEAR> rows(a, x.kh);
+  u16x8_t qf[NKS];
+  load_query<NKS>(a, p, hh, qf);
 
   f32x16_t oacc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
   float m_run = -INFINITY, lsum = 0.0f;
+  const int wlim = min(shortest(p), hi);
+  const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
-  for (int it = wave; it < ntiles; it += 4) {
-    f32x16_t s[1] = {zero16()};
-    const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
+  auto bring = [&](int it, auto v) {
+    const uint32_t ln = opaque(lane);
 #pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) s[0] = mfma32<DT>(kf[ks], lds8(Qs, swz_b128<DP>(kq, ks)), s[0]);
-    const uint32_t live = (uint32_t)__ballot(t_now != kNoToken);
-    wait_vmcnt<0>();  // the V rows of this group have landed
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);  // the next K rows take the registers of these
-    const bool more = it + 4 < ntiles;
-    if (more) {
-      t_now = t_next;
-      load_k(t_now);
-      t_next = token_of(a, trow, lo + (it + 8) * 32 + qi, hi);
+    for (int n = 0; n < NDMA; ++n) {
+      const uint32_t row0 = n * (64 / NB), byte = block_byte<DP>(ln, row0);
+      const uint32_t at = tok[it * OWN + row0 + ln / NB];
+      if (byte < ND * 2)
+        rows.template bring<decltype(v)::value>(at, byte, byte < (uint32_t)D * 2,
+                                                (decltype(v)::value ? Vt : Kt) + n * 64 * 8);
     }
-    const int kt0 = lo + it * 32;
-    if (kt0 + 32 > wlim || live != 0xffffffffu) {
-      const int left = (int)opaque(p.limit - kt0) - 4 * hh;
-      const uint32_t mine = live >> (4 * hh);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int k = 8 * (r >> 2) + (r & 3);
-        s[0][r] = (k < left) & ((mine >> k) & 1) ? s[0][r] : -INFINITY;
-      }
+  };
+  for (int k0 = lo; k0 < hi; k0 += C::CAP) {
+    lds_barrier();  // the tokens before are read
+    if (tid == 0) flags[0] = 0;
+    lds_barrier();
+    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, tok, flags);
+    lds_barrier();
+    const bool holes = __builtin_amdgcn_readfirstlane(flags[0]) != 0;
+    const int ntiles = (min(hi - k0, C::CAP) + OWN - 1) / OWN;
+    landed<0>();  // what the compiler has in flight: it must not wait for it below
+    if (wave < ntiles) {
+      bring(wave, std::false_type{});
+      bring(wave, std::true_type{});
     }
-    u16x8_t pv[1][2];
-    softmax_step<DT, 1, NDB>(s, a.scale_log2, m_run, lsum, oacc, pv);
-    asm volatile("" ::: "memory");
+    for (int it = wave; it < ntiles; it += 4) {
+      const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
+      const bool more = it + 4 < ntiles;
+      landed<NDMA>();  // K; V may be on its way
+      f32x16_t s[1] = {zero16()};
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+      for (int ks = 0; ks < NKS; ++ks) s[0] = mfma32<DT>(lds8(Kt, swz_b128<DP>(kq, ks)), qf[ks], s[0]);
+      lds_read_done();
+      if (more) bring(it + 4, std::false_type{});
+      const int kt0 = k0 + it * OWN;
+      if (kt0 + OWN > wlim || holes)
+        mask_scores<1, NR>(s, (int)opaque(min(p.limit, hi) - kt0), tok + it * OWN, hh);
+      u16x8_t pv[1][NR / 8];
+      softmax_step<DT, 1, NR, NDB>(s, a.scale_log2, m_run, lsum, oacc, pv);
+      if (more) landed<NDMA>(); else landed<0>();  // V; the next K may be on its way
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint32_t ro = t * 16 * DP * 2;
-        oacc[db] = mfma32<DT>(lds_tr8(Vs, ro + swz_tr<DP>(t0, db), ro + swz_tr<DP>(t1, db)),
-                              pv[0][t], oacc[db]);
-      }
-    if (more) {
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // the V tile is read
-      asm volatile("" ::: "memory");
-      load_v(t_now);
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int t = 0; t < NR / 8; ++t) {
+          const uint32_t ro = t * 16 * DP * 2;
+          oacc[db] = mfma32<DT>(lds_tr8(Vt, ro + swz_tr<DP>(t0, db), ro + swz_tr<DP>(t1, db)),
+                                pv[0][t], oacc[db]);
+        }
+      lds_read_done();
+      if (more) bring(it + 4, std::true_type{});
     }
   }
   float l = lsum + __shfl_xor(lsum, 32, 64);
 
   // join: waves 2, 3 into 0, 1, then 1 into 0; lane by lane
-  f32x4_t* ox = (f32x4_t*)smem;                        // [2][NDB * 4][64]
-  float2* mx = (float2*)(smem + C::ROWS);      // [2][64], where the queries were
+  f32x4_t* ox = (f32x4_t*)smem;                // [2][NDB * 4][64], where the tiles were
+  float2* mx = (float2*)(smem + C::TOK);       // [2][64]
 #pragma unroll
   for (int step = 2; step > 0; step >>= 1) {
     lds_barrier();
@@ -462,29 +498,31 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
         }
     }
   }
-  if (wave == 0 && p.valid) store_partial<NDB>(a, partial_of(a, x, p), oacc, m_run, l, hh);
+  if (wave == 0 && p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
 }
 
-template <int DT, int ND>
+template <int DT, int ND, bool NEAR>
 __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[Dims<ND>::LDS];
   const Item x = a.items[blockIdx.x];
   if (x.n_m == 0) return;
-  if (x.n_m <= 32) narrow_item<DT, ND>(a, x, smem);
-  else wide_item<DT, ND>(a, x, smem);
+  if (x.n_m <= 32) narrow_item<DT, ND, NEAR>(a, x, smem);
+  else wide_item<DT, ND, NEAR>(a, x, smem);
 }
 
-// Joins the ranges of each (row, head): a workgroup per pair (or several, PL
-// = 1), PL threads per four dims, each with every PL-th range.
-template <int DT, int PL>
+// Joins the ranges of each (row, head): PL threads per four dims, each with
+// every PL-th range, four of them at a time (their loads are in flight
+// together), then the PL sums in LDS in order.
+template <int DT>
 __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ part_o,
                                                     const float2* __restrict__ part_ml,
                                                     const int* __restrict__ part_at,
                                                     const int* __restrict__ n_part, int n_rows,
-                                                    int Hq, int D, uint16_t* __restrict__ out,
+                                                    int Hq, int D, int PL,
+                                                    uint16_t* __restrict__ out,
                                                     float* __restrict__ lse) {
-  __shared__ f32x4_t red[PL > 1 ? 256 : 1];
-  __shared__ float2 ml_red[PL > 1 ? 256 : 1];
+  __shared__ f32x4_t red[256];
+  __shared__ float2 ml_red[256];
   const int tpr = D / 4, tpp = tpr * PL, per = 256 / tpp;
   const int e = threadIdx.x / tpp, in = threadIdx.x - e * tpp, pl = in / tpr;
   const int d = (in - pl * tpr) * 4;
@@ -495,7 +533,6 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
   const int64_t s0 = (int64_t)part_at[row] * Hq + h;
   float M = -INFINITY, z = 0.0f;
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-  // four ranges at a time: their loads are in flight together
   for (int i0 = pl; i0 < n; i0 += 4 * PL) {
     float2 ml[4];
     f32x4_t v[4];
@@ -507,8 +544,10 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
       ml[k] = part_ml[s];
       v[k] = *reinterpret_cast<const f32x4_t*>(part_o + s * D + d);
       if (i >= n) ml[k].y = 0.0f;
-      if (ml[k].y != 0.0f) mn = fmaxf(mn, ml[k].x);
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (ml[k].y != 0.0f) mn = fmaxf(mn, ml[k].x);
     const float keep = M == -INFINITY ? 0.0f : fast_exp2(M - mn);
     M = mn;
     z *= keep;
@@ -516,28 +555,25 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
     for (int c = 0; c < 4; ++c) o[c] *= keep;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (ml[k].y == 0.0f) continue;  // an empty range wrote no O
-      const float w = fast_exp2(ml[k].x - mn);
-      z += w * ml[k].y;
+      const bool some = ml[k].y != 0.0f;  // an empty range wrote no O
+      const float w = some ? fast_exp2(ml[k].x - mn) : 0.0f;
+      z += some ? w * ml[k].y : 0.0f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] += w * v[k][c];
+      for (int c = 0; c < 4; ++c) o[c] += some ? w * v[k][c] : 0.0f;
     }
   }
-  if constexpr (PL > 1) {
+  if (PL > 1) {
     ml_red[threadIdx.x] = make_float2(M, z);
     red[threadIdx.x] = o;
     __syncthreads();
-    if (pl != 0) return;
-    float Mx = M;
-#pragma unroll
-    for (int k = 1; k < PL; ++k) Mx = fmaxf(Mx, ml_red[threadIdx.x + k * tpr].x);
-    const float ref = Mx == -INFINITY ? 0.0f : Mx;
-    const float w0 = fast_exp2(M - ref);
-    M = Mx;
+    if (pl != 0 || !on) return;
+    float top = M;
+    for (int k = 1; k < PL; ++k) top = fmaxf(top, ml_red[threadIdx.x + k * tpr].x);
+    const float ref = top == -INFINITY ? 0.0f : top, w0 = fast_exp2(M - ref);
+    M = top;
     z *= w0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[c] *= w0;
-#pragma unroll
     for (int k = 1; k < PL; ++k) {
       const float2 ml = ml_red[threadIdx.x + k * tpr];
       const f32x4_t v = red[threadIdx.x + k * tpr];
@@ -556,21 +592,26 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
   if (d == 0) lse[rh] = z != 0.0f ? (M + log2f(z)) * kLn2 : -INFINITY;
 }
 
-template <int DT> void launch_blocks(const SharedArgs& a, int n_items, hipStream_t st) {
+template <int DT, bool NEAR> void launch_blocks(const SharedArgs& a, int n_items, hipStream_t st) {
   const dim3 grid(n_items), block(256);
-  if (a.D <= 64) hipLaunchKernelGGL((block_kernel<DT, 64>), grid, block, 0, st, a);
-  else if (a.D <= 96) hipLaunchKernelGGL((block_kernel<DT, 96>), grid, block, 0, st, a);
-  else if (a.D <= 128) hipLaunchKernelGGL((block_kernel<DT, 128>), grid, block, 0, st, a);
-  else if (a.D <= 192) hipLaunchKernelGGL((block_kernel<DT, 192>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((block_kernel<DT, 256>), grid, block, 0, st, a);
+  if (a.D <= 64) hipLaunchKernelGGL((block_kernel<DT, 64, NEAR>), grid, block, 0, st, a);
+  else if (a.D <= 96) hipLaunchKernelGGL((block_kernel<DT, 96, NEAR>), grid, block, 0, st, a);
+  else if (a.D <= 128) hipLaunchKernelGGL((block_kernel<DT, 128, NEAR>), grid, block, 0, st, a);
+  else if (a.D <= 192) hipLaunchKernelGGL((block_kernel<DT, 192, NEAR>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((block_kernel<DT, 256, NEAR>), grid, block, 0, st, a);
 }
 
-template <int DT, int PL>
-void launch_merge(const SharedArgs& a, int Nq, uint16_t* out, float* lse, hipStream_t st) {
-  const int per = 256 / (a.D / 4 * PL);
+template <int DT>
+void launch_merge(const SharedArgs& a, int Nq, int max_parts, uint16_t* out, float* lse,
+                  hipStream_t st) {
+  // a thread takes the ranges four at a time: the fewest threads that need one
+  // round, as far as a workgroup holds them
+  int pl = 1;
+  while (4 * pl < max_parts && 2 * pl * (a.D / 4) <= 256) pl *= 2;
+  const int per = 256 / (a.D / 4 * pl);
   const dim3 grid((unsigned)(((int64_t)Nq * a.Hq + per - 1) / per));
-  hipLaunchKernelGGL((merge_kernel<DT, PL>), grid, dim3(256), 0, st, a.part_o, a.part_ml, a.part_at,
-                     a.n_part, Nq, a.Hq, a.D, out, lse);
+  hipLaunchKernelGGL((merge_kernel<DT>), grid, dim3(256), 0, st, a.part_o, a.part_ml, a.prefix_at,
+                     a.n_part, Nq, a.Hq, a.D, pl, out, lse);
 }
 
 }  // namespace
@@ -596,19 +637,18 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
   a.num_pages = num_pages; a.P = page_size; a.W = table_width; a.table = table;
   a.lengths = own_lengths; a.max_length = max_length;
   a.items = (const Item*)items; a.rows = rows;
-  a.part_at = row_parts; a.n_prefix = row_parts + Nq; a.n_part = row_parts + 2 * (int64_t)Nq;
+  const int64_t pool = (int64_t)num_pages * page_size * Hkv * D * 2;
+  a.pool_bytes = pool <= kNowhere ? (uint32_t)pool : 0;
+  a.prefix_at = row_parts; a.own_at = row_parts + Nq; a.n_part = row_parts + 2 * (int64_t)Nq;
   a.part_o = part_o; a.part_ml = (float2*)part_ml;
   hipStream_t st = (hipStream_t)stream;
   if (n_items > 0) {
-    if (dtype == 0) launch_blocks<0>(a, n_items, st);
-    else launch_blocks<1>(a, n_items, st);
+    if (a.pool_bytes) dtype == 0 ? launch_blocks<0, true>(a, n_items, st) : launch_blocks<1, true>(a, n_items, st);
+    else dtype == 0 ? launch_blocks<0, false>(a, n_items, st) : launch_blocks<1, false>(a, n_items, st);
     const int rc = moba_launch_status("shared_attention(blocks)");
     if (rc) return rc;
   }
-  const bool many = max_parts > 4;
-  if (dtype == 0)
-    many ? launch_merge<0, 4>(a, Nq, (uint16_t*)out, lse, st) : launch_merge<0, 1>(a, Nq, (uint16_t*)out, lse, st);
-  else
-    many ? launch_merge<1, 4>(a, Nq, (uint16_t*)out, lse, st) : launch_merge<1, 1>(a, Nq, (uint16_t*)out, lse, st);
+  if (dtype == 0) launch_merge<0>(a, Nq, max_parts, (uint16_t*)out, lse, st);
+  else launch_merge<1>(a, Nq, max_parts, (uint16_t*)out, lse, st);
   return moba_launch_status("shared_attention(merge)");
 }

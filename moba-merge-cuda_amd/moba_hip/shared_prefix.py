@@ -91,13 +91,14 @@ class SharedPrefixPlan:
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
         row_list, sharing = [], []
         for (slot, tokens, bound, rows), size, nb in zip(segments, sizes, blocks):
-            splits = max(1, -(-bound // target))
+            splits = min(max(1, -(-bound // target)), 2 ** 15 - 1)
             (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
             for kh in range(hkv):
                 for s in range(splits):
                     sharing.append([
                         (len(row_list), b * size, min(size, len(rows) * group - b * size),
-                         slot, kh, s, splits, tokens) for b in range(nb)])
+                         slot, kh, s | splits << 16, tokens, self._only_row(rows, group, b * size, size))
+                        for b in range(nb)])
             row_list += rows
         items = self._order(sharing)
         part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
@@ -105,10 +106,16 @@ class SharedPrefixPlan:
         self.max_parts = int((n_prefix + n_suffix).max())
         self.n_items = len(items)
         arrays = [np.asarray(items, np.int64).ravel(), np.asarray(row_list, np.int64),
-                  part_at[:-1], n_prefix, n_prefix + n_suffix]
+                  part_at[:-1], part_at[:-1] + n_prefix, n_prefix + n_suffix]
         self._rows_at = 4 * arrays[0].size
         self._parts_at = self._rows_at + 4 * arrays[1].size
         return np.concatenate(arrays).astype(np.int32)
+
+    @staticmethod
+    def _only_row(rows, group, m0, size):
+        """The row of a block's pairs, -1 if there are several."""
+        last = min(m0 + size, len(rows) * group) - 1
+        return rows[m0 // group] if m0 // group == last // group else -1
 
     @staticmethod
     def _order(sharing):
@@ -118,7 +125,7 @@ class SharedPrefixPlan:
         for items in sharing:
             min(per, key=len).extend(items)
         depth = max(map(len, per))
-        pad = (0, 0, 0, 0, 0, 0, 1, 0)
+        pad = (0,) * 8
         return [per[x][i] if i < len(per[x]) else pad
                 for i in range(depth) for x in range(_XCDS)]
 

@@ -60,13 +60,17 @@ def _covered(plan, prefix, length, suffix):
     n, hkv = plan.rows, plan.num_kv_heads
     g = plan.num_q_heads // hkv
     rows = flat[plan._rows_at // 4:plan._parts_at // 4]
-    part_at, n_prefix, n_part = flat[plan._parts_at // 4:].reshape(3, n)
+    part_at, own_at, n_part = flat[plan._parts_at // 4:].reshape(3, n)
+    n_prefix = own_at - part_at
     assert part_at[0] == 0 and (np.diff(part_at) == n_part[:-1]).all()
     assert part_at[-1] + n_part[-1] == plan.parts
     seen = np.zeros((plan.parts, plan.num_q_heads), np.int64)
-    for row_at, m0, n_m, slot, kh, split, splits, tokens in items:
+    for row_at, m0, n_m, slot, kh, packed, tokens, only in items:
         if n_m == 0:
             continue
+        split, splits = packed & 0xffff, packed >> 16
+        its = {rows[row_at + m // g] for m in range(m0, m0 + n_m)}
+        assert its == {only} if only >= 0 else len(its) > 1
         assert 0 < n_m and 0 <= split < splits and 0 <= kh < hkv
         for m in range(m0, m0 + n_m):
             row, h = rows[row_at + m // g], kh * g + m % g
