@@ -47,11 +47,15 @@ struct SharedArgs {
   float2* part_ml;
 };
 
-// 16 bytes per lane from any address straight into LDS (lane l's at
-// lds + 16 l); ordered by the caller as dma_lds16.
-MOBA_DEV void dma_global16(const void* p, const void* lds) {
+// 16 bytes per lane straight into LDS (lane l's at LDS address lds + 16 l), from
+// a buffer or from any address; ordered by the caller as dma_lds16.
+MOBA_DEV void dma_buffer16(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(voff), "s"(r) : "memory", "m0");
+}
+MOBA_DEV void dma_global16(const void* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(lds_addr(lds)), "v"(p) : "memory", "m0");
+               :: "s"(lds), "v"(p) : "memory", "m0");
 }
 // s_waitcnt vmcnt(N) for any N, and nothing moves across it.
 template <int N> MOBA_DEV void landed() {
@@ -102,13 +106,13 @@ template <bool NEAR> struct Rows {
     }
   }
   MOBA_DEV uint32_t place(uint32_t token) const { return NEAR ? token * row_bytes : token; }
-  // 64 lanes' 16-byte blocks, `byte` into the row at `at`, to lds
-  template <bool V> MOBA_DEV void bring(uint32_t at, uint32_t byte, bool on, const void* lds) const {
+  // 64 lanes' 16-byte blocks, `byte` into the row at `at`, to LDS address lds
+  template <bool V> MOBA_DEV void bring(uint32_t at, uint32_t byte, uint32_t lds) const {
     if constexpr (NEAR) {
-      dma_lds16(V ? v : k, lds, on ? at + byte : kNowhere, 0);
+      dma_buffer16(V ? v : k, lds, at + byte);
     } else {
       const char* p = (V ? vp : kp) + (uint64_t)at * row_bytes + byte;
-      dma_global16(on & (at != kNowhere) ? p : (const char*)g_zero, lds);
+      dma_global16(at != kNowhere ? p : (const char*)g_zero, lds);
     }
   }
 };
@@ -186,46 +190,62 @@ MOBA_DEV void store_partial(const SharedArgs& a, int64_t part, const f32x16_t (&
   if (hh == 0) a.part_ml[part] = make_float2(m, l);
 }
 
-// One tile's scores (the first NR registers of each block) into the running
-// (max, sum) of a lane's pair; returns the 16-bit weights as operands of the
-// product with V.  The reference stays while the scores are within 2^8 of it.
+// A lane's pair's running softmax: reference (log2 domain), sum of this lane's
+// keys, and what the next tile needs of the reference.  The reference stays
+// while the scores are within 2^8 of it.
+struct Running {
+  float m = -INFINITY, l = 0.0f;
+  float nm = 0.0f;            // -m; 0 while nothing was attended: weights of
+                              // 0, not of exp2(-inf + inf)
+  float limit = -INFINITY;    // scores above move the reference
+};
 constexpr float kSlack = 8.0f;
+
+// Maximum over the lanes l and l + 32.
+MOBA_DEV float max_halves(float x) {
+  uint32_t a = __float_as_uint(x), b = a;
+  swap_halves(a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+
+// One tile's scores (the first NR registers of each block) into the running
+// softmax; returns the 16-bit weights as operands of the product with V.
 template <int DT, int NKB, int NR, int NDB>
-MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, float& m_run, float& lsum,
-                           f32x16_t (&o)[NDB], u16x8_t (&pv)[NKB][NR / 8]) {
+MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, Running& run, f32x16_t (&o)[NDB],
+                           u16x8_t (&pv)[NKB][NR / 8]) {
   float mx = -INFINITY;
 #pragma unroll
   for (int kb = 0; kb < NKB; ++kb)
 #pragma unroll
     for (int r = 0; r < NR; ++r) mx = fmaxf(mx, s[kb][r]);
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c2;
-  const bool up = mx > m_run + kSlack;
+  mx = max_halves(mx) * c2;
+  const bool up = mx > run.limit;
   if (__any(up)) [[unlikely]] {
-    const float mn = up ? mx : m_run;
-    const float alpha = up ? fast_exp2(m_run - mn) : 1.0f;
-    lsum *= alpha;
+    const float mn = up ? mx : run.m;
+    const float alpha = up ? fast_exp2(run.m - mn) : 1.0f;
+    run.l *= alpha;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-    m_run = mn;
+    run.m = mn;
+    run.nm = mn == -INFINITY ? 0.0f : -mn;
+    run.limit = mn + kSlack;
     __builtin_amdgcn_sched_barrier(0);
   }
-  // a row with nothing so far: weights of 0, not of exp2(-inf + inf)
-  const float nm = m_run == -INFINITY ? 0.0f : -m_run;
   float ps = 0.0f;
 #pragma unroll
   for (int kb = 0; kb < NKB; ++kb) {
     float p[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      p[r] = fast_exp2(fmaf(s[kb][r], c2, nm));
+      p[r] = fast_exp2(fmaf(s[kb][r], c2, run.nm));
       ps += p[r];
     }
 #pragma unroll
     for (int t = 0; t < NR / 8; ++t) pv[kb][t] = pack8<DT>(p + 8 * t);
   }
-  lsum += ps;
+  run.l += ps;
 }
 
 // Scores of keys behind `left` (counted from the tile's first) or, with holes,
@@ -299,30 +319,37 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   f32x16_t oacc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
-  float m_run = -INFINITY, lsum = 0.0f;
+  Running run;
   const bool idle = wave * 32 >= x.n_m;
   const int wlim = min(shortest(p), hi);
   const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
 
-  // wave w brings the 64-block loads n * 4 + w of a tile
-  auto dma = [&](int it) {
-    const uint32_t* tk = tok + it * KEYS;
-    uint16_t* Kd = Ks + (it & 1) * TILE;
-    const uint32_t ln = opaque(lane);
+  // wave w brings the 64-block loads n * 4 + w of a tile; where a tile's rows
+  // are is read one tile before
+  const uint32_t lds0 = lds_addr(smem) + wave * 1024;
+  uint32_t byte[NDMA], at[NDMA];
+  bool mine[NDMA];
 #pragma unroll
-    for (int n = 0; n < NDMA; ++n) {
-      const uint32_t row0 = (n * 4 + wave) * (64 / NB), byte = block_byte<DP>(ln, row0);
-      if (byte < ND * 2) {
-        const uint32_t at = tk[row0 + ln / NB];
-        const bool on = byte < (uint32_t)D * 2;
-        rows.template bring<false>(at, byte, on, Kd + (n * 4 + wave) * 64 * 8);
-        rows.template bring<true>(at, byte, on, Kd + 2 * TILE + (n * 4 + wave) * 64 * 8);
-      }
-    }
+  for (int n = 0; n < NDMA; ++n) {
+    byte[n] = block_byte<DP>(lane, (n * 4 + wave) * (64 / NB));
+    mine[n] = byte[n] < (uint32_t)D * 2;
+  }
+  auto places = [&](int it) {
+#pragma unroll
+    for (int n = 0; n < NDMA; ++n) at[n] = tok[it * KEYS + (n * 4 + wave) * (64 / NB) + lane / NB];
   };
-  auto tile = [&](int it, int kt0, bool holes) {
-    const uint16_t *Kb = Ks + (it & 1) * TILE, *Vb = Kb + 2 * TILE;
+  auto dma = [&](auto stage) {
+    const uint32_t lds = lds0 + decltype(stage)::value * (TILE * 2);
+#pragma unroll
+    for (int n = 0; n < NDMA; ++n)
+      if (mine[n]) {
+        rows.template bring<false>(at[n], byte[n], lds + n * 4096);
+        rows.template bring<true>(at[n], byte[n], lds + 4 * TILE + n * 4096);
+      }
+  };
+  auto tile = [&](auto stage, int it, int kt0, bool holes) {
+    const uint16_t *Kb = Ks + decltype(stage)::value * TILE, *Vb = Kb + 2 * TILE;
     const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
     f32x16_t sacc[NKB];
     wave_prio<1>();
@@ -337,7 +364,7 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     if (kt0 + KEYS > wlim || holes)
       mask_scores<NKB, 16>(sacc, (int)opaque(min(p.limit, hi) - kt0), tok + it * KEYS, hh);
     u16x8_t pv[NKB][2];
-    softmax_step<DT, NKB, 16, NDB>(sacc, a.scale_log2, m_run, lsum, oacc, pv);
+    softmax_step<DT, NKB, 16, NDB>(sacc, a.scale_log2, run, oacc, pv);
     wave_prio<1>();
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -361,16 +388,27 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     const bool holes = __builtin_amdgcn_readfirstlane(flags[0]) != 0;
     const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
-    dma(0);
-    for (int it = 0; it < ntiles; ++it) {
+    typedef std::integral_constant<int, 0> S0;
+    typedef std::integral_constant<int, 1> S1;
+    auto step = [&](auto stage, auto other, int it) {
       landed<0>();    // this wave's part of tile `it`
       lds_barrier();  // everyone's, and tile it - 1 is read
-      if (it + 1 < ntiles) dma(it + 1);
-      if (!idle) tile(it, k0 + it * KEYS, holes);
+      if (it + 1 < ntiles) {
+        dma(other);
+        places(min(it + 2, ntiles - 1));
+      }
+      if (!idle) tile(stage, it, k0 + it * KEYS, holes);
+    };
+    places(0);
+    dma(S0{});
+    places(min(1, ntiles - 1));
+    for (int it = 0; it < ntiles; it += 2) {
+      step(S0{}, S1{}, it);
+      if (it + 1 < ntiles) step(S1{}, S0{}, it + 1);
     }
   }
-  const float l = lsum + __shfl_xor(lsum, 32, 64);
-  if (p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
+  const float l = run.l + __shfl_xor(run.l, 32, 64);
+  if (p.valid) store_partial<NDB>(a, p.part, oacc, run.m, l, hh);
 }
 
 // Up to 32 pairs: the four waves have the same pairs and take every fourth
@@ -406,19 +444,19 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   f32x16_t oacc[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
-  float m_run = -INFINITY, lsum = 0.0f;
+  Running run;
   const int wlim = min(shortest(p), hi);
   const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
+  const uint32_t lds0 = lds_addr(Kt);
   auto bring = [&](int it, auto v) {
     const uint32_t ln = opaque(lane);
 #pragma unroll
     for (int n = 0; n < NDMA; ++n) {
       const uint32_t row0 = n * (64 / NB), byte = block_byte<DP>(ln, row0);
       const uint32_t at = tok[it * OWN + row0 + ln / NB];
-      if (byte < ND * 2)
-        rows.template bring<decltype(v)::value>(at, byte, byte < (uint32_t)D * 2,
-                                                (decltype(v)::value ? Vt : Kt) + n * 64 * 8);
+      if (byte < (uint32_t)D * 2)
+        rows.template bring<decltype(v)::value>(at, byte, lds0 + decltype(v)::value * (OWN * DP * 2) + n * 1024);
     }
   };
   for (int k0 = lo; k0 < hi; k0 += C::CAP) {
@@ -447,7 +485,7 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       if (kt0 + OWN > wlim || holes)
         mask_scores<1, NR>(s, (int)opaque(min(p.limit, hi) - kt0), tok + it * OWN, hh);
       u16x8_t pv[1][NR / 8];
-      softmax_step<DT, 1, NR, NDB>(s, a.scale_log2, m_run, lsum, oacc, pv);
+      softmax_step<DT, 1, NR, NDB>(s, a.scale_log2, run, oacc, pv);
       if (more) landed<NDMA>(); else landed<0>();  // V; the next K may be on its way
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
@@ -461,7 +499,7 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       if (more) bring(it + 4, std::true_type{});
     }
   }
-  float l = lsum + __shfl_xor(lsum, 32, 64);
+  float m_run = run.m, l = run.l + __shfl_xor(run.l, 32, 64);
 
   // join: waves 2, 3 into 0, 1, then 1 into 0; lane by lane
   f32x4_t* ox = (f32x4_t*)smem;                // [2][NDB * 4][64], where the tiles were
@@ -506,6 +544,10 @@ __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs 
   __shared__ __attribute__((aligned(16))) char smem[Dims<ND>::LDS];
   const Item x = a.items[blockIdx.x];
   if (x.n_m == 0) return;
+  if (a.D < ND) {  // dims behind D are never loaded: zeros
+    for (int i = threadIdx.x * 16; i < Dims<ND>::TILES; i += 4096) st8((uint16_t*)(smem + i), zero8());
+    lds_barrier();
+  }
   if (x.n_m <= 32) narrow_item<DT, ND, NEAR>(a, x, smem);
   else wide_item<DT, ND, NEAR>(a, x, smem);
 }

@@ -20,6 +20,8 @@ from .rotary import _DTYPES, _index, _pool
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
 # or the same 32 and a quarter of the keys each
 _WIDE, _NARROW = 128, 32
+# work items of a launch: as many workgroups as the card holds, up to 128 dims and above
+_ITEMS = 768, 512
 _XCDS = 8   # workgroup L runs on XCD L % 8
 
 
@@ -87,7 +89,7 @@ class SharedPrefixPlan:
         sizes = [_WIDE if len(rows) * group > 2 * _NARROW else _NARROW for *_, rows in segments]
         blocks = [-(-len(rows) * group // size) for (*_, rows), size in zip(segments, sizes)]
         keys = sum(b * hkv * bound for b, (_, _, bound, _) in zip(blocks, segments))
-        target = max(128, -(-keys // (768 if self.head_dim <= 128 else 512)))
+        target = max(128, -(-keys // _ITEMS[self.head_dim > 128]))
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
         row_list, sharing = [], []
         for (slot, tokens, bound, rows), size, nb in zip(segments, sizes, blocks):
