@@ -70,13 +70,31 @@ class RotaryTable:
         return self.cos_sin.device
 
 
-def _token_tensor(t, name, n, heads, d, like):
+# The checks of a call run on every step of a decode, so a call first tests
+# whether everything holds (plain comparisons, about 2 us); only a call that
+# does not pass goes through the checks that name what is wrong.
+
+def _pool_holds(kc, vc, table, idx):
+    return (kc.dim() == 4 and idx >= 0 and kc.dtype in _DTYPES and vc.dtype == kc.dtype
+            and vc.get_device() == idx and vc.shape == kc.shape and kc.is_contiguous()
+            and vc.is_contiguous() and table.dtype == torch.int32 and table.dim() == 2
+            and table.get_device() == idx and table.is_contiguous()
+            and kc.shape[0] * kc.shape[1] < 2 ** 31 and table.shape[1] * kc.shape[1] < 2 ** 31
+            and kc.numel() > 0 and table.numel() > 0)
+
+
+def _index_holds(t, n, idx):
+    return (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == idx
+            and t.is_contiguous())
+
+
+def _check_token_tensor(t, name, n, heads, d, like):
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise ValueError(f"{name} must be [N,H,D]")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must match the page pool's device and dtype")
     shape = t.shape
-    if shape[0] != n or shape[2] != d or shape[1] != (heads or shape[1]):
+    if shape[0] != n or shape[2] != d or shape[1] < 1 or shape[1] != (heads or shape[1]):
         raise ValueError(f"{name} has an invalid shape")
     if t.stride(2) != 1:
         raise ValueError(f"{name} last dimension must be contiguous")
@@ -84,8 +102,7 @@ def _token_tensor(t, name, n, heads, d, like):
         raise ValueError("KV cache/decode is inference-only; detach Q/K/V")
 
 
-def _pool(k_cache, v_cache, page_table):
-    """Checks a page pool and its table; returns the pool's shape."""
+def _check_pool(k_cache, v_cache, page_table):
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or not k_cache.numel():
         raise ValueError("k_cache must be nonempty [pages, page_size, Hkv, D]")
     if k_cache.dtype not in _DTYPES:
@@ -97,16 +114,15 @@ def _pool(k_cache, v_cache, page_table):
         raise ValueError("v_cache must be like k_cache")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache and v_cache must be contiguous")
-    _index(page_table, "page_table", 2, k_cache.device)
+    _check_index(page_table, "page_table", 2, k_cache.device)
     if not page_table.numel():
         raise ValueError("page_table must be nonempty")
     pages, page = k_cache.shape[:2]
     if pages * page >= 2 ** 31 or page_table.shape[1] * page >= 2 ** 31:
         raise ValueError("page pool exceeds int32 token capacity")
-    return k_cache.shape
 
 
-def _index(t, name, dim, device, size=None):
+def _check_index(t, name, dim, device, size=None):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != dim or \
             t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 {dim}D tensor on the cache's device")
@@ -114,17 +130,65 @@ def _index(t, name, dim, device, size=None):
         raise ValueError(f"{name} must have {size} entries")
 
 
-def _overlap(a, b):
-    """Whether two tensors' memory spans meet."""
-    def span(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        lo = t.data_ptr()
-        return lo, lo + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+def _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets):
+    """Raises what is wrong with the arguments of an append."""
+    _check_pool(k_cache, v_cache, page_table)
+    _, _, hkv, d = k_cache.shape
+    n = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
+    _check_token_tensor(k, "k", n, hkv, d, k_cache)
+    _check_token_tensor(v, "v", n, hkv, d, k_cache)
+    if n < 1:
+        raise ValueError("k has an invalid shape")
+    dev = k_cache.device
+    _check_index(token_seq, "token_seq", 1, dev, n)
+    _check_index(token_pos, "token_pos", 1, dev, n)
+    if offsets is not None:
+        _check_index(offsets, "offsets", 1, dev, page_table.shape[0])
+    if not isinstance(rotary, RotaryTable):
+        raise ValueError("rotary must be a RotaryTable")
+    if rotary.rotary_dim > d:
+        raise ValueError("rotary_dim exceeds head_dim")
+    if rotary.device != dev:
+        raise ValueError("rotary table must be on the cache's device")
+    if q is not None:
+        _check_token_tensor(q, "q", n, None, d, k_cache)
+    if n * ((0 if q is None else q.shape[1]) + 2 * hkv) * d >= 2 ** 31:
+        raise ValueError("append exceeds 2^31 elements")
 
 
-@torch.no_grad()
+def _append_holds(k, v, kc, vc, table, seq, pos, rotary, q, offsets):
+    try:
+        idx = kc.get_device()
+        n, hkv, d = k.shape
+        dt = kc.dtype
+        return (_pool_holds(kc, vc, table, idx) and n > 0 and kc.shape[2] == hkv
+                and kc.shape[3] == d and v.shape == k.shape and k.dtype == dt and v.dtype == dt
+                and k.get_device() == idx and v.get_device() == idx and k.stride(2) == 1
+                and v.stride(2) == 1 and not k.requires_grad and not v.requires_grad
+                and _index_holds(seq, n, idx) and _index_holds(pos, n, idx)
+                and (offsets is None or _index_holds(offsets, table.shape[0], idx))
+                and type(rotary) is RotaryTable and rotary.rotary_dim <= d
+                and rotary.cos_sin.get_device() == idx
+                and (q is None or (q.dim() == 3 and q.shape[0] == n and q.shape[2] == d
+                                   and q.shape[1] > 0 and q.dtype == dt and q.get_device() == idx
+                                   and q.stride(2) == 1 and not q.requires_grad))
+                and n * ((0 if q is None else q.shape[1]) + 2 * hkv) * d < 2 ** 31)
+    except (AttributeError, ValueError, TypeError, IndexError):
+        return False
+
+
+def _span(t):
+    """[start, end) addresses of a nonempty tensor's elements."""
+    p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.numel() * t.element_size()
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _meet(a, b):
+    return a[0] < b[1] and b[0] < a[1]
+
+
 def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, *, q=None,
                   q_out=None, offsets=None, check=False):
     """Writes N new tokens into a page pool, their keys rotated, and returns
@@ -144,64 +208,55 @@ def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
     value written either; with ``check`` such tokens, and two tokens of one
     cell, raise RuntimeError after the launch (one device-to-host copy).
     Without it, two tokens of one cell leave either's data."""
-    pages, page, hkv, d = _pool(k_cache, v_cache, page_table)
-    n = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
-    _token_tensor(k, "k", n, hkv, d, k_cache)
-    _token_tensor(v, "v", n, hkv, d, k_cache)
-    if n < 1:
-        raise ValueError("k has an invalid shape")
-    dev = k_cache.device
-    _index(token_seq, "token_seq", 1, dev, n)
-    _index(token_pos, "token_pos", 1, dev, n)
-    slots, width = page_table.shape
-    if offsets is not None:
-        _index(offsets, "offsets", 1, dev, slots)
-    if not isinstance(rotary, RotaryTable):
-        raise ValueError("rotary must be a RotaryTable")
-    if rotary.rotary_dim > d:
-        raise ValueError("rotary_dim exceeds head_dim")
-    if rotary.device != dev:
-        raise ValueError("rotary table must be on the cache's device")
+    if not _append_holds(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets):
+        _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets)
+        raise ValueError("invalid append arguments")
+    pages, page, hkv, d = k_cache.shape
+    n = k.shape[0]
+    pools = _span(k_cache), _span(v_cache)
+    if _meet(*pools):
+        raise ValueError("k_cache and v_cache must not overlap")
+    for t in (k, v, q):
+        if t is not None:
+            at = _span(t)
+            if _meet(at, pools[0]) or _meet(at, pools[1]):
+                raise ValueError("append inputs must not alias KV cache storage; clone first")
     hq = 0
     if q is not None:
-        _token_tensor(q, "q", n, None, d, k_cache)
         hq = q.shape[1]
-        if hq < 1:
-            raise ValueError("q has an invalid shape")
-    if n * (hq + 2 * hkv) * d >= 2 ** 31:
-        raise ValueError("append exceeds 2^31 elements")
-    inputs = (k, v) if q is None else (q, k, v)
-    if q is None:
-        if q_out is not None:
-            raise ValueError("q_out without q")
-    elif q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
-    else:
-        _token_tensor(q_out, "q_out", n, hq, d, k_cache)
-        if not q_out.is_contiguous():
-            raise ValueError("q_out must be contiguous")
-        if any(_overlap(q_out, t) for t in (*inputs, k_cache, v_cache)):
-            raise ValueError("q_out must not overlap the inputs or the pool")
-    pools = (k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr())
-    if pools[0] == pools[1] and _overlap(k_cache, v_cache):
-        raise ValueError("k_cache and v_cache must not overlap")
-    for t in inputs:
-        if t.untyped_storage().data_ptr() in pools and \
-                (_overlap(t, k_cache) or _overlap(t, v_cache)):
-            raise ValueError("append inputs must not alias KV cache storage; clone first")
-    with torch.cuda.device(dev):
-        status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-        qa = (None, 0, 0) if q is None else (q.data_ptr(), q.stride(0), q.stride(1))
-        _lib.call("moba_hip_append_rotary", *qa, k.data_ptr(), k.stride(0), k.stride(1),
-                  v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype], n, hq, hkv, d,
-                  rotary.cos_sin.data_ptr(), rotary.max_positions, rotary.rotary_dim,
-                  rotary.interleaved, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
-                  page_table.data_ptr(), slots, width, token_seq.data_ptr(),
-                  token_pos.data_ptr(), _lib.ptr(offsets), _lib.ptr(q_out), _lib.ptr(status),
-                  _lib.stream_of(dev))
-        if check:
-            _raise_bad(status, token_seq, token_pos, width * page)
+        if q_out is None:
+            q_out = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        else:
+            _check_token_tensor(q_out, "q_out", n, hq, d, k_cache)
+            if not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous")
+            at = _span(q_out)
+            if any(_meet(at, _span(t)) for t in (q, k, v, k_cache, v_cache)):
+                raise ValueError("q_out must not overlap the inputs or the pool")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    status = torch.zeros(1, dtype=torch.int32, device=k.device) if check else None
+    qa = (None, 0, 0) if q is None else (q.data_ptr(), q.stride(0), q.stride(1))
+    _on_device(k_cache.get_device(), "moba_hip_append_rotary", *qa, k.data_ptr(), k.stride(0),
+               k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _DTYPES[k.dtype], n, hq, hkv, d,
+               rotary.cos_sin.data_ptr(), rotary.max_positions, rotary.rotary_dim,
+               rotary.interleaved, k_cache.data_ptr(), v_cache.data_ptr(), pages, page,
+               page_table.data_ptr(), page_table.shape[0], page_table.shape[1],
+               token_seq.data_ptr(), token_pos.data_ptr(), _lib.ptr(offsets), _lib.ptr(q_out),
+               _lib.ptr(status))
+    if check:
+        _raise_bad(status, token_seq, token_pos, page_table.shape[1] * page)
     return q_out
+
+
+def _on_device(idx, name, *args):
+    """Calls an entry on the current stream of device ``idx``."""
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if torch._C._cuda_getDevice() == idx:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(idx):
+            _lib.call(name, *args, stream)
 
 
 def _raise_bad(status, token_seq, token_pos, span):

@@ -15,7 +15,7 @@ import torch
 
 from .cache_layout import positive_int
 from .ops import _lib
-from .rotary import _DTYPES, _index, _pool
+from .rotary import (_DTYPES, _check_index, _check_pool, _index_holds, _on_device, _pool_holds)
 
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
 # or the same 32 and a quarter of the keys each
@@ -68,6 +68,7 @@ class SharedPrefixPlan:
         if n * hq >= 2 ** 31:
             raise ValueError("query grid exceeds int32 capacity")
         self.rows, self.num_q_heads, self.num_kv_heads, self.head_dim = n, hq, hkv, d
+        self._q_shape = (n, hq, d)
         self.max_suffix = max_suffix
         self.max_prefix = int(length.max())
         self.max_slot = int(max(prefix[length > 0].max(initial=-1), suffix.max()))
@@ -132,7 +133,46 @@ class SharedPrefixPlan:
                 for i in range(depth) for x in range(_XCDS)]
 
 
-@torch.no_grad()
+def _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan):
+    """Raises what is wrong with the arguments of a call."""
+    _check_pool(k_cache, v_cache, page_table)
+    _, page, hkv, d = k_cache.shape
+    dev = k_cache.device
+    if not isinstance(plan, SharedPrefixPlan):
+        raise ValueError("plan must be a SharedPrefixPlan")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype != k_cache.dtype or \
+            q.device != dev or plan.device != dev:
+        raise ValueError("q must be [Nq,Hq,D] of the pool's device and dtype, and the plan on it")
+    if q.requires_grad:
+        raise ValueError("KV cache/decode is inference-only; detach Q/K/V")
+    if tuple(q.shape) != plan._q_shape or (hkv, d) != (plan.num_kv_heads, plan.head_dim):
+        raise ValueError("q and the pool must have the plan's rows, heads and head_dim")
+    slots, width = page_table.shape
+    if plan.max_slot >= slots or plan.max_prefix > width * page:
+        raise ValueError("the plan's slots and prefix lengths must fit page_table")
+    _check_index(suffix_lengths, "suffix_lengths", 1, dev, plan.rows)
+
+
+def _attention_holds(q, kc, vc, table, lengths, plan):
+    try:
+        idx = kc.get_device()
+        return (type(plan) is SharedPrefixPlan and _pool_holds(kc, vc, table, idx)
+                and q.shape == plan._q_shape and q.dtype == kc.dtype and q.get_device() == idx
+                and plan.meta.get_device() == idx and not q.requires_grad
+                and kc.shape[2] == plan.num_kv_heads and kc.shape[3] == plan.head_dim
+                and plan.max_slot < table.shape[0]
+                and plan.max_prefix <= table.shape[1] * kc.shape[1]
+                and _index_holds(lengths, plan.rows, idx))
+    except (AttributeError, ValueError, TypeError, IndexError):
+        return False
+
+
+def _check_output(t, name, shape, like, dtype):
+    if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != dtype or \
+            t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {list(shape)} {dtype} on the pool's device")
+
+
 def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan, *, scale=None,
                             out=None, lse=None):
     """Softmax attention of q [Nq,Hq,D] over each row's shared prefix and its
@@ -146,44 +186,36 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     to attend gives zeros and an lse of -inf; a token in an unmapped page is
     not attended.  Nothing is read back, so a call can be captured into a graph
     (``out`` and ``lse``, contiguous, then keep their addresses)."""
-    pages, page, hkv, d = _pool(k_cache, v_cache, page_table)
-    dev = k_cache.device
-    if not isinstance(plan, SharedPrefixPlan):
-        raise ValueError("plan must be a SharedPrefixPlan")
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype != k_cache.dtype or \
-            q.device != dev or plan.device != dev:
-        raise ValueError("q must be [Nq,Hq,D] of the pool's device and dtype, and the plan on it")
-    if q.requires_grad:
-        raise ValueError("KV cache/decode is inference-only; detach Q/K/V")
+    if not _attention_holds(q, k_cache, v_cache, page_table, suffix_lengths, plan):
+        _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan)
+        raise ValueError("invalid attention arguments")
+    pages, page, hkv, d = k_cache.shape
+    width = page_table.shape[1]
     n, hq = plan.rows, plan.num_q_heads
-    if tuple(q.shape) != (n, hq, plan.head_dim) or (hkv, d) != (plan.num_kv_heads, plan.head_dim):
-        raise ValueError("q and the pool must have the plan's rows, heads and head_dim")
-    slots, width = page_table.shape
-    if plan.max_slot >= slots or plan.max_prefix > width * page:
-        raise ValueError("the plan's slots and prefix lengths must fit page_table")
-    _index(suffix_lengths, "suffix_lengths", 1, dev, n)
     scale = d ** -0.5 if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError("scale must be positive and finite")
     q = q.contiguous()
-    for t, name, shape, dtype in ((out, "out", (n, hq, d), q.dtype),
-                                  (lse, "lse", (n, hq), torch.float32)):
-        if t is not None and (not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or
-                              t.dtype != dtype or t.device != dev or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {list(shape)} {dtype} on the pool's device")
-    if (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) & 15:
+    qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (qp | kp | vp) & 15:
         raise ValueError("q and the pool must be 16-byte aligned")
-    with torch.cuda.device(dev):
-        out = torch.empty_like(q) if out is None else out
-        lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if lse is None else lse
-        parts = plan.parts * hq
-        # partial sums [parts, D], then (max, sum) pairs
-        work = torch.empty(parts * (d + 2), dtype=torch.float32, device=dev)
-        meta = plan.meta.data_ptr()
-        _lib.call("moba_hip_shared_attention", q.data_ptr(), _DTYPES[q.dtype], n, hq, hkv, d, scale,
-                  k_cache.data_ptr(), v_cache.data_ptr(), pages, page, page_table.data_ptr(), width,
-                  suffix_lengths.data_ptr(), min(plan.max_suffix, width * page), meta,
-                  plan.n_items, meta + plan._rows_at, meta + plan._parts_at, plan.max_parts,
-                  work.data_ptr(), work.data_ptr() + 4 * parts * d, out.data_ptr(), lse.data_ptr(),
-                  _lib.stream_of(dev))
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_output(out, "out", plan._q_shape, q, q.dtype)
+        if out.data_ptr() & 15:
+            raise ValueError("out must be 16-byte aligned")
+    if lse is None:
+        lse = torch.empty((n, hq), dtype=torch.float32, device=q.device)
+    else:
+        _check_output(lse, "lse", (n, hq), q, torch.float32)
+    parts = plan.parts * hq
+    # partial sums [parts, D], then (max, sum) pairs
+    work = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)
+    wp, meta = work.data_ptr(), plan.meta.data_ptr()
+    _on_device(k_cache.get_device(), "moba_hip_shared_attention", qp, _DTYPES[q.dtype], n, hq, hkv,
+               d, scale, kp, vp, pages, page, page_table.data_ptr(), width,
+               suffix_lengths.data_ptr(), min(plan.max_suffix, width * page), meta, plan.n_items,
+               meta + plan._rows_at, meta + plan._parts_at, plan.max_parts, wp, wp + 4 * parts * d,
+               out.data_ptr(), lse.data_ptr())
     return out, lse
