@@ -117,28 +117,30 @@ template <bool NEAR> struct Rows {
   }
 };
 
+// A row's own length.
+MOBA_DEV int own_length(const SharedArgs& a, int row) {
+  return max(0, min(a.lengths[row], a.max_length));
+}
 // What a lane knows of its (row, q head) pair.
 struct Pair {
   int row, h, limit;   // limit: tokens of the segment that the row attends
   int64_t part;        // its partial
   bool valid;
 };
-MOBA_DEV Pair pair_of(const SharedArgs& a, const Item& x, int m) {
+// alike: the tokens that all the rows attend, -1 if they differ.
+MOBA_DEV Pair pair_of(const SharedArgs& a, const Item& x, int m, int alike) {
   Pair p;
   p.valid = m < x.n_m;
   const int i = x.m0 + min(m, x.n_m - 1), r = i / a.G;
   p.h = x.kh * a.G + i - r * a.G;
-  if (x.row >= 0) {  // uniform: the loads are scalar ones
-    p.row = x.row;
-    p.limit = x.length < 0 ? max(0, min(a.lengths[x.row], a.max_length)) : x.length;
-    p.part = (x.length < 0 ? a.own_at : a.prefix_at)[x.row];
-  } else {
-    p.row = a.rows[x.row_at + r];
-    p.limit = x.length < 0 ? max(0, min(a.lengths[p.row], a.max_length)) : x.length;
-    p.part = (x.length < 0 ? a.own_at : a.prefix_at)[p.row];
-  }
-  p.part = (p.part + (x.split & 0xffff)) * a.Hq + p.h;
+  p.row = x.row >= 0 ? x.row : a.rows[x.row_at + r];
+  p.limit = alike >= 0 ? alike : own_length(a, p.row);
+  p.part = ((int64_t)(x.length < 0 ? a.own_at : a.prefix_at)[p.row] + (x.split & 0xffff)) * a.Hq + p.h;
   return p;
+}
+// Of a segment or of one row: a scalar load at most.
+MOBA_DEV int alike_of(const SharedArgs& a, const Item& x) {
+  return x.length >= 0 ? x.length : x.row >= 0 ? own_length(a, x.row) : -1;
 }
 // Longest and shortest row of the lanes' 32 pairs, the same in every lane.
 MOBA_DEV int longest(int limit) {
@@ -146,7 +148,8 @@ MOBA_DEV int longest(int limit) {
   for (int o = 16; o > 0; o >>= 1) limit = max(limit, __shfl_xor(limit, o, 64));
   return __builtin_amdgcn_readfirstlane(limit);
 }
-MOBA_DEV int shortest(const Pair& p) {
+MOBA_DEV int shortest(const Pair& p, int alike) {
+  if (alike >= 0) return alike;
   int limit = p.valid ? p.limit : 0x7fffffff;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) limit = min(limit, __shfl_xor(limit, o, 64));
@@ -154,24 +157,38 @@ MOBA_DEV int shortest(const Pair& p) {
 }
 // The keys [lo, hi) of an item's range: whole groups of 64 but for the last.
 MOBA_DEV void range_of(const Item& x, int length, int& lo, int& hi) {
+  length = max(length, 0);
   const int split = x.split & 0xffff, splits = (uint32_t)x.split >> 16;
   const int per = (int)((length + 64ll * splits - 1) / (64 * splits)) * 64;
   lo = (int)min((int64_t)length, (int64_t)split * per);
   hi = (int)min((int64_t)length, (int64_t)lo + per);
 }
+// The page-table entry of key k0 + threadIdx.x (of the last key behind hi).
+MOBA_DEV int entry_of(const SharedArgs& a, int slot, int k0, int hi) {
+  return a.table[(int64_t)slot * a.W + min(k0 + (int)threadIdx.x, hi - 1) / a.P];
+}
 // Looks up the keys [k0, min(k0 + CAP, hi)) for the workgroup (and fills to a
-// multiple of 256 with kNowhere).  flag is set where a page is unmapped.
+// multiple of 256 with kNowhere), the first 256 from the entries `first`.
+// flags[wave]: a page of the wave's keys is unmapped.
 template <bool NEAR, int CAP>
 MOBA_DEV void look_up(const SharedArgs& a, const Rows<NEAR>& rows, int slot, int k0, int hi,
-                      uint32_t* tok, int* flag) {
-  const int* trow = a.table + (int64_t)slot * a.W;
+                      int first, uint32_t* tok, int* flags) {
   const int tid = threadIdx.x, n = min(CAP, hi - k0);
+  bool holes = false;
   for (int i0 = 0; i0 < n; i0 += 256) {
-    const int key = min(k0 + i0 + tid, hi - 1), lp = key / a.P, page = trow[lp];
+    const int page = i0 ? entry_of(a, slot, k0 + i0, hi) : first;
+    const int key = min(k0 + i0 + tid, hi - 1), in_page = key - key / a.P * a.P;
     const bool in = k0 + i0 + tid < hi, mapped = page >= 0 && page < a.num_pages;
-    tok[i0 + tid] = in & mapped ? rows.place((uint32_t)page * a.P + (key - lp * a.P)) : kNowhere;
-    if (__any(!mapped) && (tid & 63) == 0) *flag = 1;
+    tok[i0 + tid] = in & mapped ? rows.place((uint32_t)page * a.P + in_page) : kNowhere;
+    holes |= !mapped;
   }
+  const bool any = __any(holes);
+  if ((tid & 63) == 0) flags[tid >> 6] = any;
+}
+// After a barrier: whether any wave saw one.
+MOBA_DEV bool any_hole(const int* flags) {
+  const int4 f = *reinterpret_cast<const int4*>(flags);
+  return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0;
 }
 
 template <int NDB>
@@ -297,8 +314,9 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 31, hh = lane >> 5, D = a.D;
 
-  const Pair p = pair_of(a, x, wave * 32 + qi);
-  int length = x.length;
+  const int alike = alike_of(a, x);
+  const Pair p = pair_of(a, x, wave * 32 + qi, alike);
+  int length = alike;
   if (length < 0) {  // the block's longest row
     const int mine = longest(p.limit);
     if (lane == 0) flags[wave] = mine;
@@ -313,6 +331,7 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     return;
   }
   const Rows<NEAR> rows(a, x.kh);
+  int first = entry_of(a, x.slot, lo, hi);
   u16x8_t qf[NKS];
   load_query<NKS>(a, p, hh, qf);
 
@@ -321,7 +340,7 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
   Running run;
   const bool idle = wave * 32 >= x.n_m;
-  const int wlim = min(shortest(p), hi);
+  const int wlim = min(shortest(p, alike), hi);
   const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
 
@@ -380,12 +399,13 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   };
 
   for (int k0 = lo; k0 < hi; k0 += C::CAP) {
-    lds_barrier();  // the tokens and tiles before are read
-    if (tid == 0) flags[0] = 0;
+    if (k0 > lo) {
+      lds_barrier();  // the tokens and tiles before are read
+      first = entry_of(a, x.slot, k0, hi);
+    }
+    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, first, tok, flags);
     lds_barrier();
-    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, tok, flags);
-    lds_barrier();
-    const bool holes = __builtin_amdgcn_readfirstlane(flags[0]) != 0;
+    const bool holes = any_hole(flags);
     const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
     typedef std::integral_constant<int, 0> S0;
@@ -429,10 +449,16 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   uint32_t* tok = (uint32_t*)(smem + C::TOK);
   int* flags = (int*)(smem + C::FLAGS);
 
-  const Pair p = pair_of(a, x, qi);
-  const int length = longest(p.limit);
-  int lo, hi;
-  range_of(x, length, lo, hi);
+  const int alike = alike_of(a, x);
+  int lo, hi, first = -1;
+  range_of(x, alike, lo, hi);
+  // what the keys wait for goes out first
+  if (lo < hi) first = entry_of(a, x.slot, lo, hi);
+  const Pair p = pair_of(a, x, qi, alike);
+  if (alike < 0) {
+    range_of(x, longest(p.limit), lo, hi);
+    if (lo < hi) first = entry_of(a, x.slot, lo, hi);
+  }
   if (lo >= hi) {
     if (tid < 32 && p.valid) a.part_ml[p.part] = make_float2(-INFINITY, 0.0f);
     return;
@@ -445,7 +471,7 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
 #pragma unroll
   for (int db = 0; db < NDB; ++db) oacc[db] = zero16();
   Running run;
-  const int wlim = min(shortest(p), hi);
+  const int wlim = min(shortest(p, alike), hi);
   const uint32_t kbase0 = swz_b128_base<DP>(lane);
   const uint32_t trb0 = swz_tr_base<DP>(lane, 0), trb1 = swz_tr_base<DP>(lane, 1);
   const uint32_t lds0 = lds_addr(Kt);
@@ -460,12 +486,13 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
     }
   };
   for (int k0 = lo; k0 < hi; k0 += C::CAP) {
-    lds_barrier();  // the tokens before are read
-    if (tid == 0) flags[0] = 0;
+    if (k0 > lo) {
+      lds_barrier();  // the tokens before are read
+      first = entry_of(a, x.slot, k0, hi);
+    }
+    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, first, tok, flags);
     lds_barrier();
-    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, tok, flags);
-    lds_barrier();
-    const bool holes = __builtin_amdgcn_readfirstlane(flags[0]) != 0;
+    const bool holes = any_hole(flags);
     const int ntiles = (min(hi - k0, C::CAP) + OWN - 1) / OWN;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
     if (wave < ntiles) {
@@ -526,14 +553,14 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       l = l * wa + o.y * wb;
       m_run = M;
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+      for (int db = 0; db < NDB; ++db) {
+        f32x4_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f32x4_t v = ox[(at * NDB * 4 + db * 4 + j) * 64 + lane];
+        for (int j = 0; j < 4; ++j) v[j] = ox[(at * NDB * 4 + db * 4 + j) * 64 + lane];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) oacc[db][4 * j + i] = oacc[db][4 * j + i] * wa + v[i] * wb;
-          __builtin_amdgcn_sched_barrier(0);  // 16 values at a time, not all in registers
-        }
+        for (int r = 0; r < 16; ++r) oacc[db][r] = oacc[db][r] * wa + v[r >> 2][r & 3] * wb;
+        __builtin_amdgcn_sched_barrier(0);  // a block at a time, not all in registers
+      }
     }
   }
   if (wave == 0 && p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
