@@ -75,10 +75,11 @@ template <int ND> struct Dims {
   static constexpr int KEYS = DP <= 64 ? 64 : 32;   // keys of a tile that four waves share
   static constexpr int TILE = KEYS * DP;
   static constexpr int OWN = DP <= 64 ? 32 : 16;    // keys of a tile that a wave has alone
-  // LDS: two stages of shared K and V tiles, or a K and a V tile per wave; the
-  // pool's token of up to CAP keys; flags
-  static constexpr int CAP = 2048;
-  static constexpr int TILES = 4 * TILE * 2;
+  // LDS: stages of shared K and V tiles, or a K and a V tile per wave; the
+  // pool's token of up to CAP keys; flags.  Three workgroups share a CU up to 128
+  // dims, two above.
+  static constexpr int STAGES = DP <= 128 ? 3 : 2, CAP = 1024;
+  static constexpr int TILES = STAGES * TILE * 2 * 2;
   static_assert(4 * 2 * OWN * DP * 2 <= TILES && 2 * NDB * 4 * 64 * 16 <= TILES, "LDS");
   static constexpr int TOK = TILES, FLAGS = TOK + CAP * 4, LDS = FLAGS + 16;
   static constexpr int WAVES = ND <= 128 ? 3 : 2;   // per SIMD
@@ -302,13 +303,15 @@ template <int NKS> MOBA_DEV void load_query(const SharedArgs& a, const Pair& p, 
 }
 
 // More than 32 pairs: every wave has 32 of them, and the four share tiles of
-// KEYS keys in two LDS stages.
+// KEYS keys in STAGES LDS stages: while one is in use, the loads of the others are
+// in flight.
 template <int DT, int ND, bool NEAR>
 MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
   constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, KEYS = C::KEYS, NKB = KEYS / 32;
   constexpr int TILE = C::TILE, NB = C::NB, NDMA = KEYS * NB / 256;
-  uint16_t* Ks = (uint16_t*)smem;   // [2][TILE], then V
+  constexpr int STAGES = C::STAGES;
+  uint16_t* Ks = (uint16_t*)smem;   // [STAGES][TILE], then V
   uint32_t* tok = (uint32_t*)(smem + C::TOK);
   int* flags = (int*)(smem + C::FLAGS);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -364,11 +367,11 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     for (int n = 0; n < NDMA; ++n)
       if (mine[n]) {
         rows.template bring<false>(at[n], byte[n], lds + n * 4096);
-        rows.template bring<true>(at[n], byte[n], lds + 4 * TILE + n * 4096);
+        rows.template bring<true>(at[n], byte[n], lds + STAGES * TILE * 2 + n * 4096);
       }
   };
   auto tile = [&](auto stage, int it, int kt0, bool holes) {
-    const uint16_t *Kb = Ks + decltype(stage)::value * TILE, *Vb = Kb + 2 * TILE;
+    const uint16_t *Kb = Ks + decltype(stage)::value * TILE, *Vb = Kb + STAGES * TILE;
     const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
     f32x16_t sacc[NKB];
     wave_prio<1>();
@@ -408,23 +411,30 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     const bool holes = any_hole(flags);
     const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
-    typedef std::integral_constant<int, 0> S0;
-    typedef std::integral_constant<int, 1> S1;
-    auto step = [&](auto stage, auto other, int it) {
-      landed<0>();    // this wave's part of tile `it`
+    // the loads of a tile: 2 NDMA, issued STAGES - 1 tiles ahead
+    auto step = [&](auto stage, int it) {
+      constexpr int S = decltype(stage)::value;
+      if (it + 1 < ntiles) landed<(STAGES - 2) * 2 * NDMA>();  // this wave's part of tile `it`
+      else landed<0>();
       lds_barrier();  // everyone's, and tile it - 1 is read
-      if (it + 1 < ntiles) {
-        dma(other);
-        places(min(it + 2, ntiles - 1));
+      if (it + STAGES - 1 < ntiles) {
+        dma(std::integral_constant<int, (S + STAGES - 1) % STAGES>{});
+        places(min(it + STAGES, ntiles - 1));
       }
       if (!idle) tile(stage, it, k0 + it * KEYS, holes);
     };
     places(0);
-    dma(S0{});
-    places(min(1, ntiles - 1));
-    for (int it = 0; it < ntiles; it += 2) {
-      step(S0{}, S1{}, it);
-      if (it + 1 < ntiles) step(S1{}, S0{}, it + 1);
+    dma(std::integral_constant<int, 0>{});
+    if constexpr (STAGES > 2) {
+      places(min(1, ntiles - 1));
+      if (ntiles > 1) dma(std::integral_constant<int, 1>{});
+    }
+    places(min(STAGES - 1, ntiles - 1));
+    for (int it = 0; it < ntiles; it += STAGES) {
+      step(std::integral_constant<int, 0>{}, it);
+      if (it + 1 < ntiles) step(std::integral_constant<int, 1>{}, it + 1);
+      if constexpr (STAGES > 2)
+        if (it + 2 < ntiles) step(std::integral_constant<int, 2>{}, it + 2);
     }
   }
   const float l = run.l + __shfl_xor(run.l, 32, 64);
