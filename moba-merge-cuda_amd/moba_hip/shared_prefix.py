@@ -20,8 +20,15 @@ from .rotary import (_DTYPES, _check_index, _check_pool, _index_holds, _on_devic
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
 # or the same 32 and a quarter of the keys each
 _WIDE, _NARROW = 128, 32
-# work items of a launch: as many workgroups as the card holds, up to 128 dims and above
-_ITEMS = 768, 512
+# What the length of the ranges is chosen by: workgroups that the card holds at
+# once (up to 128 dims, above); an item's time before and after its keys, us; a
+# key's time per dim with the card full, us (39 ns at 128 dims, measured with 64
+# rows behind 32K tokens), and what is left of it with few workgroups; the rate
+# at which partials are written and read, and K/V, bytes per us; the merge's
+# time per range of a row, us.
+_SLOTS = 768, 512
+_ITEM, _KEY, _ALONE = 7.0, 3.0e-4, 0.54
+_PARTIALS, _CACHE, _RANGE = 4.0e6, 4.3e6, 7.5e-3
 _XCDS = 8   # workgroup L runs on XCD L % 8
 
 
@@ -89,12 +96,13 @@ class SharedPrefixPlan:
         segments += [(slot, -1, self.max_suffix, rows) for slot, rows in alone.items()]
         sizes = [_WIDE if len(rows) * group > 2 * _NARROW else _NARROW for *_, rows in segments]
         blocks = [-(-len(rows) * group // size) for (*_, rows), size in zip(segments, sizes)]
-        keys = sum(b * hkv * bound for b, (_, _, bound, _) in zip(blocks, segments))
-        target = max(128, -(-keys // _ITEMS[self.head_dim > 128]))
+        ranges = self._ranges(np.array([b * hkv for b in blocks]),
+                              np.array([bound for _, _, bound, _ in segments]),
+                              np.array([0.5 if tokens < 0 else 1.0 for _, tokens, *_ in segments]),
+                              np.array([len(rows) for *_, rows in segments]))
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
         row_list, sharing = [], []
-        for (slot, tokens, bound, rows), size, nb in zip(segments, sizes, blocks):
-            splits = min(max(1, -(-bound // target)), 2 ** 15 - 1)
+        for (slot, tokens, _, rows), size, nb, splits in zip(segments, sizes, blocks, ranges):
             (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
             for kh in range(hkv):
                 for s in range(splits):
@@ -103,6 +111,12 @@ class SharedPrefixPlan:
                          slot, kh, s | splits << 16, tokens, self._only_row(rows, group, b * size, size))
                         for b in range(nb)])
             row_list += rows
+        # Longest first; but a few items of own tokens behind a card full of
+        # prefix ranges would start when those end, all alone
+        own = sum(len(x) for x in sharing if x[0][6] < 0)
+        slots = _SLOTS[self.head_dim > 128]
+        if own <= slots // 2 and sum(map(len, sharing)) > slots:
+            sharing.sort(key=lambda x: x[0][6] >= 0)
         items = self._order(sharing)
         part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
         self.parts = int(part_at[-1])
@@ -113,6 +127,31 @@ class SharedPrefixPlan:
         self._rows_at = 4 * arrays[0].size
         self._parts_at = self._rows_at + 4 * arrays[1].size
         return np.concatenate(arrays).astype(np.int32)
+
+    def _ranges(self, blocks, bounds, share, rows):
+        """Ranges of each segment, of ``blocks`` items per range, up to
+        ``bounds`` keys (``share`` of them on average: own lengths lie anywhere
+        below their bound) and ``rows`` query rows: of about one length, the
+        one that gives the shortest time by the figures above."""
+        if not len(blocks):
+            return []
+        d, hq, hkv = self.head_dim, self.num_q_heads, self.num_kv_heads
+        slots = _SLOTS[d > 128]
+        best, longest = None, int(bounds.max())
+        count = max(1, math.ceil(4 * math.log2(max(1.0, longest / 128)))) + 1
+        for length in np.ceil(np.geomspace(128, max(128, longest), count)):
+            splits = np.minimum(np.ceil(bounds / length), 2 ** 15 - 1)
+            items = blocks * splits
+            full = min(1.0, max(_ALONE, items.sum() / slots))
+            keys = _KEY * d * full * np.ceil(bounds / splits)
+            last = _ITEM + keys.max()
+            rounds = math.ceil(items[_ITEM + keys > 0.7 * last].sum() / slots)
+            time = max((items * (_ITEM + keys * share)).sum() / slots, rounds * last,
+                       (bounds * share).sum() * hkv * d * 4 / _CACHE)
+            time += (splits * rows).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
+            if best is None or time < best[0]:
+                best = time, splits
+        return best[1].astype(np.int64).tolist()
 
     @staticmethod
     def _only_row(rows, group, m0, size):
