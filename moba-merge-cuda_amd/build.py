@@ -1,8 +1,9 @@
-"""Build libmoba_hip.so (gfx950) in-tree with hipcc.
+"""Build libmoba_hip.so (gfx950) and the host path _calls.so in-tree.
 
 Every ``csrc/*.hip`` (device code) and ``csrc/*.cpp`` (host-only runtime:
 page pool, prepared-decode driver) file is compiled to an object under ``_build/`` and
-linked into ``moba_hip/libmoba_hip.so``.  Objects are rebuilt when their
+linked into ``moba_hip/libmoba_hip.so``.  ``csrc/python/calls.cpp`` (host-only,
+against torch's headers) becomes the extension ``moba_hip/_calls.so``.  Objects are rebuilt when their
 source or any header changed.  ``python build.py`` builds; ``--force``
 rebuilds everything.
 """
@@ -18,6 +19,7 @@ ROOT = Path(__file__).resolve().parent
 CSRC = ROOT / "csrc"
 OUT_DIR = ROOT / "_build"
 LIB = ROOT / "moba_hip" / "libmoba_hip.so"
+CALLS = ROOT / "moba_hip" / "_calls.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
@@ -58,10 +60,42 @@ def _compile(src: Path, force: bool) -> Path:
     return obj
 
 
+def _compile_calls(force: bool) -> Path:
+    src, obj = CSRC / "python" / "calls.cpp", OUT_DIR / "calls.cpp.o"
+    if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, _headers()):
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths
+        dirs = [*include_paths(), sysconfig.get_paths()["include"]]
+        abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-w",
+               f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{d}" for d in dirs], "-c", str(src), "-o",
+               str(obj)]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("g++ failed on calls.cpp")
+    return obj
+
+
+def _link_calls(obj: Path, force: bool) -> None:
+    if not force and CALLS.exists() and CALLS.stat().st_mtime >= obj.stat().st_mtime:
+        return
+    import torch
+    libs = Path(torch.__file__).parent / "lib"
+    tmp = CALLS.with_suffix(f".so.{os.getpid()}")
+    subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", str(obj), "-o", str(tmp),
+                           f"-L{LIB.parent}", "-l:libmoba_hip.so", "-Wl,-rpath,$ORIGIN",
+                           f"-L{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10"])
+    os.replace(tmp, CALLS)
+
+
 def build(force: bool = False, jobs: int = 8) -> Path:
     OUT_DIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.cpp"))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        calls = ex.submit(_compile_calls, force)
         objs = list(ex.map(lambda s: _compile(s, force), sources))
     newest = max(o.stat().st_mtime for o in objs)
     if force or not LIB.exists() or LIB.stat().st_mtime < newest:
@@ -69,6 +103,7 @@ def build(force: bool = False, jobs: int = 8) -> Path:
         cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
         subprocess.check_call(cmd)
         os.replace(tmp, LIB)
+    _link_calls(calls.result(), force)
     return LIB
 
 

@@ -130,6 +130,34 @@ def load():
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """The native host path of the paged-cache operators (once).  Raises if
+    it has not been built."""
+    global _calls
+    if _calls is None:
+        import importlib.util
+
+        import torch
+
+        from ..rotary import RotaryTable
+        from ..shared_prefix import SharedPrefixPlan
+        load()
+        path = LIB_PATH.with_name("_calls.so")
+        if not path.exists():
+            raise MobaHipError(f"{path} is missing: build it with "
+                               "`python moba-merge-cuda_amd/build.py`")
+        spec = importlib.util.spec_from_file_location("moba_hip._calls", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, MobaHipError,
+                    RotaryTable, SharedPrefixPlan)
+        _calls = module
+    return _calls
+
+
 def call(name: str, *args) -> None:
     """Invoke an entry point and raise MobaHipError on a non-zero status."""
     lib = load()

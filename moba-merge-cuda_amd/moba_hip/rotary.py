@@ -70,23 +70,9 @@ class RotaryTable:
         return self.cos_sin.device
 
 
-# The checks of a call run on every step of a decode, so a call first tests
-# whether everything holds (plain comparisons, about 2 us); only a call that
-# does not pass goes through the checks that name what is wrong.
-
-def _pool_holds(kc, vc, table, idx):
-    return (kc.dim() == 4 and idx >= 0 and kc.dtype in _DTYPES and vc.dtype == kc.dtype
-            and vc.get_device() == idx and vc.shape == kc.shape and kc.is_contiguous()
-            and vc.is_contiguous() and table.dtype == torch.int32 and table.dim() == 2
-            and table.get_device() == idx and table.is_contiguous()
-            and kc.shape[0] * kc.shape[1] < 2 ** 31 and table.shape[1] * kc.shape[1] < 2 ** 31
-            and kc.numel() > 0 and table.numel() > 0)
-
-
-def _index_holds(t, n, idx):
-    return (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.get_device() == idx
-            and t.is_contiguous())
-
+# The checks below name what is wrong with a call.  They are not on the path of
+# one that holds: the native host path (csrc/python/calls.cpp) tests the same
+# conditions, allocates and launches.
 
 def _check_token_tensor(t, name, n, heads, d, like):
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
@@ -156,32 +142,9 @@ def _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
         raise ValueError("append exceeds 2^31 elements")
 
 
-def _append_holds(k, v, kc, vc, table, seq, pos, rotary, q, offsets):
-    try:
-        idx = kc.get_device()
-        n, hkv, d = k.shape
-        dt = kc.dtype
-        return (_pool_holds(kc, vc, table, idx) and n > 0 and kc.shape[2] == hkv
-                and kc.shape[3] == d and v.shape == k.shape and k.dtype == dt and v.dtype == dt
-                and k.get_device() == idx and v.get_device() == idx and k.stride(2) == 1
-                and v.stride(2) == 1 and not k.requires_grad and not v.requires_grad
-                and _index_holds(seq, n, idx) and _index_holds(pos, n, idx)
-                and (offsets is None or _index_holds(offsets, table.shape[0], idx))
-                and type(rotary) is RotaryTable and rotary.rotary_dim <= d
-                and rotary.cos_sin.get_device() == idx
-                and (q is None or (q.dim() == 3 and q.shape[0] == n and q.shape[2] == d
-                                   and q.shape[1] > 0 and q.dtype == dt and q.get_device() == idx
-                                   and q.stride(2) == 1 and not q.requires_grad))
-                and n * ((0 if q is None else q.shape[1]) + 2 * hkv) * d < 2 ** 31)
-    except (AttributeError, ValueError, TypeError, IndexError):
-        return False
-
-
 def _span(t):
     """[start, end) addresses of a nonempty tensor's elements."""
     p = t.data_ptr()
-    if t.is_contiguous():
-        return p, p + t.numel() * t.element_size()
     return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
@@ -208,9 +171,12 @@ def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
     value written either; with ``check`` such tokens, and two tokens of one
     cell, raise RuntimeError after the launch (one device-to-host copy).
     Without it, two tokens of one cell leave either's data."""
-    if not _append_holds(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets):
-        _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets)
-        raise ValueError("invalid append arguments")
+    if not check:
+        done = _lib.calls().append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos,
+                                          rotary, q, q_out, offsets)
+        if done is not NotImplemented:
+            return done
+    _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rotary, q, offsets)
     pages, page, hkv, d = k_cache.shape
     n = k.shape[0]
     pools = _span(k_cache), _span(v_cache)

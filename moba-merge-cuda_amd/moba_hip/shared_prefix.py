@@ -9,13 +9,14 @@ fixed, their own lengths are read on the device.
 from __future__ import annotations
 
 import math
+import struct
 
 import numpy as np
 import torch
 
 from .cache_layout import positive_int
 from .ops import _lib
-from .rotary import (_DTYPES, _check_index, _check_pool, _index_holds, _on_device, _pool_holds)
+from .rotary import _DTYPES, _check_index, _check_pool, _on_device
 
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
 # or the same 32 and a quarter of the keys each
@@ -82,6 +83,10 @@ class SharedPrefixPlan:
         flat = self._build(prefix, length, suffix)
         self.meta = torch.from_numpy(flat).to(device)
         self.device = self.meta.device
+        # what a call needs of the plan, for the native host path
+        self._packed = struct.pack("12q", n, hq, hkv, d, self.max_slot, self.max_prefix, max_suffix,
+                                   self.n_items, self._rows_at, self._parts_at, self.parts,
+                                   self.max_parts)
 
     def _build(self, prefix, length, suffix):
         n, hkv, group = self.rows, self.num_kv_heads, self.num_q_heads // self.num_kv_heads
@@ -192,20 +197,6 @@ def _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan):
     _check_index(suffix_lengths, "suffix_lengths", 1, dev, plan.rows)
 
 
-def _attention_holds(q, kc, vc, table, lengths, plan):
-    try:
-        idx = kc.get_device()
-        return (type(plan) is SharedPrefixPlan and _pool_holds(kc, vc, table, idx)
-                and q.shape == plan._q_shape and q.dtype == kc.dtype and q.get_device() == idx
-                and plan.meta.get_device() == idx and not q.requires_grad
-                and kc.shape[2] == plan.num_kv_heads and kc.shape[3] == plan.head_dim
-                and plan.max_slot < table.shape[0]
-                and plan.max_prefix <= table.shape[1] * kc.shape[1]
-                and _index_holds(lengths, plan.rows, idx))
-    except (AttributeError, ValueError, TypeError, IndexError):
-        return False
-
-
 def _check_output(t, name, shape, like, dtype):
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != dtype or \
             t.device != like.device or not t.is_contiguous():
@@ -225,9 +216,11 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     to attend gives zeros and an lse of -inf; a token in an unmapped page is
     not attended.  Nothing is read back, so a call can be captured into a graph
     (``out`` and ``lse``, contiguous, then keep their addresses)."""
-    if not _attention_holds(q, k_cache, v_cache, page_table, suffix_lengths, plan):
-        _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan)
-        raise ValueError("invalid attention arguments")
+    done = _lib.calls().shared_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan, scale,
+                                         out, lse)
+    if done is not NotImplemented:
+        return done
+    _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan)
     pages, page, hkv, d = k_cache.shape
     width = page_table.shape[1]
     n, hq = plan.rows, plan.num_q_heads
