@@ -106,9 +106,10 @@ template <int DT> MOBA_DEV void rotate(float x, float y, float2 t, float& xo, fl
   yo = fmaf(x, t.y, y * t.x);
 }
 
-// Pairs in whole 16-byte pieces: unit u < R/16 turns 8 pairs (the two pieces
-// i = 8u and i + R/2, or the 16 dims from 16u when interleaved), the units
-// behind copy 16 dims each.
+// Whole 16-byte pieces, two per unit, so that neighbouring lanes have
+// neighbouring pieces in each of the two accesses: unit u < R/16 turns the
+// pieces at 8u and 8u + R/2 (8 pairs of the two, or 4 pairs within each when
+// interleaved), unit R/16 + c copies the pieces c and c + n of the 2n behind R.
 template <int DT, bool INTER>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -118,19 +119,21 @@ __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   uint16_t* dst;
   const float2* turn;
   if (!locate(a, idx, u, src, dst, turn)) return;
-  if (turn == nullptr || u >= a.R / 16) {
-    const int d = 16 * u;
-    st8(dst + d, ld8(src + d));
-    if (d + 8 < a.D) st8(dst + d + 8, ld8(src + d + 8));
+  const int turning = turn != nullptr ? a.R / 16 : 0, from = turning * 16;
+  if (u >= turning) {
+    const int n = (a.D - from + 15) / 16, d0 = from + 8 * (u - turning), d1 = d0 + 8 * n;
+    const u16x8_t x = ld8(src + d0), y = ld8(src + (d1 < a.D ? d1 : d0));
+    st8(dst + d0, x);
+    if (d1 < a.D) st8(dst + d1, y);
     return;
   }
-  const int d0 = INTER ? 16 * u : 8 * u, d1 = INTER ? d0 + 8 : d0 + a.R / 2;
+  const int d0 = 8 * u, d1 = d0 + a.R / 2;
   const u16x8_t x0 = ld8(src + d0), x1 = ld8(src + d1);
   float2 t[8];
-  const float4* tp = reinterpret_cast<const float4*>(turn + 8 * u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float4 w = tp[i];
+    const int first = !INTER ? d0 : i < 2 ? d0 / 2 : d1 / 2 - 4;  // pair of t[0]
+    const float4 w = reinterpret_cast<const float4*>(turn + first)[i];
     t[2 * i] = make_float2(w.x, w.y);
     t[2 * i + 1] = make_float2(w.z, w.w);
   }
