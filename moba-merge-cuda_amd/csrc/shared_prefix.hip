@@ -23,7 +23,8 @@ namespace {
 struct Item {
   int row_at;   // its segment's first entry of `rows`
   int m0;       // first (row, q head of the kv head) pair of the block: row m / G
-  int n_m;      // pairs of the block
+  int n_m;      // pairs of the block; 0: none; -1: each wave has the item of its
+                // own at row_at + wave
   int slot;     // page-table row of the keys
   int kh;
   int split;    // split | splits << 16
@@ -164,27 +165,26 @@ MOBA_DEV void range_of(const Item& x, int length, int& lo, int& hi) {
   lo = (int)min((int64_t)length, (int64_t)split * per);
   hi = (int)min((int64_t)length, (int64_t)lo + per);
 }
-// The page-table entry of key k0 + threadIdx.x (of the last key behind hi).
-MOBA_DEV int entry_of(const SharedArgs& a, int slot, int k0, int hi) {
-  return a.table[(int64_t)slot * a.W + min(k0 + (int)threadIdx.x, hi - 1) / a.P];
+// The page-table entry of a key (of the last key behind hi).
+MOBA_DEV int entry_of(const SharedArgs& a, int slot, int key, int hi) {
+  return a.table[(int64_t)slot * a.W + min(key, hi - 1) / a.P];
 }
-// Looks up the keys [k0, min(k0 + CAP, hi)) for the workgroup (and fills to a
-// multiple of 256 with kNowhere), the first 256 from the entries `first`.
-// flags[wave]: a page of the wave's keys is unmapped.
-template <bool NEAR, int CAP>
-MOBA_DEV void look_up(const SharedArgs& a, const Rows<NEAR>& rows, int slot, int k0, int hi,
-                      int first, uint32_t* tok, int* flags) {
-  const int tid = threadIdx.x, n = min(CAP, hi - k0);
+// Looks up the keys [k0, min(k0 + CAP, hi)) with WIDTH threads (and fills to a
+// multiple of WIDTH with kNowhere), the first WIDTH from the entries `first`.
+// Returns whether a page of the wave's keys is unmapped.
+template <bool NEAR, int CAP, int WIDTH>
+MOBA_DEV bool look_up(const SharedArgs& a, const Rows<NEAR>& rows, int slot, int k0, int hi,
+                      int first, int thread, uint32_t* tok) {
+  const int n = min(CAP, hi - k0);
   bool holes = false;
-  for (int i0 = 0; i0 < n; i0 += 256) {
-    const int page = i0 ? entry_of(a, slot, k0 + i0, hi) : first;
-    const int key = min(k0 + i0 + tid, hi - 1), in_page = key - key / a.P * a.P;
-    const bool in = k0 + i0 + tid < hi, mapped = page >= 0 && page < a.num_pages;
-    tok[i0 + tid] = in & mapped ? rows.place((uint32_t)page * a.P + in_page) : kNowhere;
+  for (int i0 = 0; i0 < n; i0 += WIDTH) {
+    const int at = k0 + i0 + thread, page = i0 ? entry_of(a, slot, at, hi) : first;
+    const int key = min(at, hi - 1), in_page = key - key / a.P * a.P;
+    const bool mapped = page >= 0 && page < a.num_pages;
+    tok[i0 + thread] = (at < hi) & mapped ? rows.place((uint32_t)page * a.P + in_page) : kNowhere;
     holes |= !mapped;
   }
-  const bool any = __any(holes);
-  if ((tid & 63) == 0) flags[tid >> 6] = any;
+  return __any(holes);
 }
 // After a barrier: whether any wave saw one.
 MOBA_DEV bool any_hole(const int* flags) {
@@ -334,7 +334,7 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     return;
   }
   const Rows<NEAR> rows(a, x.kh);
-  int first = entry_of(a, x.slot, lo, hi);
+  int first = entry_of(a, x.slot, lo + tid, hi);
   u16x8_t qf[NKS];
   load_query<NKS>(a, p, hh, qf);
 
@@ -404,9 +404,10 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   for (int k0 = lo; k0 < hi; k0 += C::CAP) {
     if (k0 > lo) {
       lds_barrier();  // the tokens and tiles before are read
-      first = entry_of(a, x.slot, k0, hi);
+      first = entry_of(a, x.slot, k0 + tid, hi);
     }
-    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, first, tok, flags);
+    const bool mine = look_up<NEAR, C::CAP, 256>(a, rows, x.slot, k0, hi, first, tid, tok);
+    if (lane == 0) flags[wave] = mine;
     lds_barrier();
     const bool holes = any_hole(flags);
     const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
@@ -446,8 +447,8 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
 // between them; their results are joined in LDS in a fixed order.  The next
 // group's K is in flight from the scores on, its V from the product with V on.
 // 16-key groups fill half of a 32-row score product; what a narrow item waits
-// for is memory.
-template <int DT, int ND, bool NEAR>
+// for is memory.  SOLO: x is this wave's alone, and it takes every group.
+template <int DT, int ND, bool NEAR, bool SOLO>
 MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
   constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, NB = C::NB, OWN = C::OWN;
@@ -456,21 +457,23 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qi = lane & 31, hh = lane >> 5, D = a.D;
   uint16_t *Kt = (uint16_t*)smem + wave * 2 * OWN * DP, *Vt = Kt + OWN * DP;
-  uint32_t* tok = (uint32_t*)(smem + C::TOK);
+  constexpr int CAP = SOLO ? C::CAP / 4 : C::CAP, STEP = SOLO ? 1 : 4;
+  uint32_t* tok = (uint32_t*)(smem + C::TOK) + (SOLO ? wave * CAP : 0);
   int* flags = (int*)(smem + C::FLAGS);
+  const int thread = SOLO ? lane : tid, begin = SOLO ? 0 : wave;
 
   const int alike = alike_of(a, x);
   int lo, hi, first = -1;
   range_of(x, alike, lo, hi);
   // what the keys wait for goes out first
-  if (lo < hi) first = entry_of(a, x.slot, lo, hi);
+  if (lo < hi) first = entry_of(a, x.slot, lo + thread, hi);
   const Pair p = pair_of(a, x, qi, alike);
   if (alike < 0) {
     range_of(x, longest(p.limit), lo, hi);
-    if (lo < hi) first = entry_of(a, x.slot, lo, hi);
+    if (lo < hi) first = entry_of(a, x.slot, lo + thread, hi);
   }
   if (lo >= hi) {
-    if (tid < 32 && p.valid) a.part_ml[p.part] = make_float2(-INFINITY, 0.0f);
+    if (thread < 32 && p.valid) a.part_ml[p.part] = make_float2(-INFINITY, 0.0f);
     return;
   }
   const Rows<NEAR> rows(a, x.kh);
@@ -495,29 +498,34 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
         rows.template bring<decltype(v)::value>(at, byte, lds0 + decltype(v)::value * (OWN * DP * 2) + n * 1024);
     }
   };
-  for (int k0 = lo; k0 < hi; k0 += C::CAP) {
+  for (int k0 = lo; k0 < hi; k0 += CAP) {
     if (k0 > lo) {
-      lds_barrier();  // the tokens before are read
-      first = entry_of(a, x.slot, k0, hi);
+      if constexpr (!SOLO) lds_barrier();  // the tokens before are read
+      first = entry_of(a, x.slot, k0 + thread, hi);
     }
-    look_up<NEAR, C::CAP>(a, rows, x.slot, k0, hi, first, tok, flags);
-    lds_barrier();
-    const bool holes = any_hole(flags);
-    const int ntiles = (min(hi - k0, C::CAP) + OWN - 1) / OWN;
+    bool holes = look_up<NEAR, CAP, SOLO ? 64 : 256>(a, rows, x.slot, k0, hi, first, thread, tok);
+    if constexpr (SOLO) {
+      wave_lds_sync();
+    } else {
+      if (lane == 0) flags[wave] = holes;
+      lds_barrier();
+      holes = any_hole(flags);
+    }
+    const int ntiles = (min(hi - k0, CAP) + OWN - 1) / OWN;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
-    if (wave < ntiles) {
-      bring(wave, std::false_type{});
-      bring(wave, std::true_type{});
+    if (begin < ntiles) {
+      bring(begin, std::false_type{});
+      bring(begin, std::true_type{});
     }
-    for (int it = wave; it < ntiles; it += 4) {
+    for (int it = begin; it < ntiles; it += STEP) {
       const uint32_t kq = opaque(kbase0), t0 = opaque(trb0), t1 = opaque(trb1);
-      const bool more = it + 4 < ntiles;
+      const bool more = it + STEP < ntiles;
       landed<NDMA>();  // K; V may be on its way
       f32x16_t s[1] = {zero16()};
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) s[0] = mfma32<DT>(lds8(Kt, swz_b128<DP>(kq, ks)), qf[ks], s[0]);
       lds_read_done();
-      if (more) bring(it + 4, std::false_type{});
+      if (more) bring(it + STEP, std::false_type{});
       const int kt0 = k0 + it * OWN;
       if (kt0 + OWN > wlim || holes)
         mask_scores<1, NR>(s, (int)opaque(min(p.limit, hi) - kt0), tok + it * OWN, hh);
@@ -533,10 +541,14 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
                                 pv[0][t], oacc[db]);
         }
       lds_read_done();
-      if (more) bring(it + 4, std::true_type{});
+      if (more) bring(it + STEP, std::true_type{});
     }
   }
   float m_run = run.m, l = run.l + __shfl_xor(run.l, 32, 64);
+  if constexpr (SOLO) {
+    if (p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
+    return;
+  }
 
   // join: waves 2, 3 into 0, 1, then 1 into 0; lane by lane
   f32x4_t* ox = (f32x4_t*)smem;                // [2][NDB * 4][64], where the tiles were
@@ -585,7 +597,10 @@ __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs 
     for (int i = threadIdx.x * 16; i < Dims<ND>::TILES; i += 4096) st8((uint16_t*)(smem + i), zero8());
     lds_barrier();
   }
-  if (x.n_m <= 32) narrow_item<DT, ND, NEAR>(a, x, smem);
+  if (x.n_m < 0) {
+    const Item own = a.items[x.row_at + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+    if (own.n_m > 0) narrow_item<DT, ND, NEAR, true>(a, own, smem);
+  } else if (x.n_m <= 32) narrow_item<DT, ND, NEAR, false>(a, x, smem);
   else wide_item<DT, ND, NEAR>(a, x, smem);
 }
 

@@ -19,7 +19,8 @@ from .ops import _lib
 from .rotary import _DTYPES, _check_index, _check_pool, _on_device
 
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
-# or the same 32 and a quarter of the keys each
+# or the same 32 and a quarter of the keys each (solo: a wave has an item's 32
+# pairs and all of its keys alone)
 _WIDE, _NARROW = 128, 32
 # What the length of the ranges is chosen by: workgroups that the card holds at
 # once (up to 128 dims, above); an item's time before and after its keys, us; a
@@ -99,23 +100,34 @@ class SharedPrefixPlan:
                 alone.setdefault(int(suffix[row]), []).append(row)
         segments += [(slot, tokens, tokens, rows) for (slot, tokens), rows in shared.items()]
         segments += [(slot, -1, self.max_suffix, rows) for slot, rows in alone.items()]
-        sizes = [_WIDE if len(rows) * group > 2 * _NARROW else _NARROW for *_, rows in segments]
+        # 33 to 128 pairs: one wide block of which a part is idle reads its keys
+        # once (16 rows of 4 heads behind 32K tokens: 41 us; two narrow ones 43)
+        sizes = [_WIDE if len(rows) * group > _NARROW else _NARROW for *_, rows in segments]
         blocks = [-(-len(rows) * group // size) for (*_, rows), size in zip(segments, sizes)]
-        ranges = self._ranges(np.array([b * hkv for b in blocks]),
-                              np.array([bound for _, _, bound, _ in segments]),
-                              np.array([0.5 if tokens < 0 else 1.0 for _, tokens, *_ in segments]),
-                              np.array([len(rows) for *_, rows in segments]))
+        ranges, solo = self._ranges(
+            np.array([b * hkv for b in blocks]), np.array([bound for _, _, bound, _ in segments]),
+            np.array([tokens < 0 for _, tokens, *_ in segments]), np.array(sizes) == _NARROW,
+            np.array([len(rows) for *_, rows in segments]))
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
-        row_list, sharing = [], []
+        row_list, sharing, singles = [], [], []
         for (slot, tokens, _, rows), size, nb, splits in zip(segments, sizes, blocks, ranges):
             (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
-            for kh in range(hkv):
-                for s in range(splits):
-                    sharing.append([
+            for s in range(splits):
+                for kh in range(hkv):
+                    same_keys = [
                         (len(row_list), b * size, min(size, len(rows) * group - b * size),
                          slot, kh, s | splits << 16, tokens, self._only_row(rows, group, b * size, size))
-                        for b in range(nb)])
+                        for b in range(nb)]
+                    if solo and tokens < 0 and size == _NARROW:
+                        singles += same_keys
+                    else:
+                        sharing.append(same_keys)
             row_list += rows
+        # four waves' items of one workgroup: the kv heads of a row next to each
+        # other, whose keys lie together and are as many
+        pad = (0,) * 8
+        singles += [pad] * (-len(singles) % 4)
+        sharing += [[(i, 0, -1, 0, 0, 0, -1, 0)] for i in range(0, len(singles), 4)]
         # Longest first; but a few items of own tokens behind a card full of
         # prefix ranges would start when those end, all alone
         own = sum(len(x) for x in sharing if x[0][6] < 0)
@@ -123,40 +135,45 @@ class SharedPrefixPlan:
         if own <= slots // 2 and sum(map(len, sharing)) > slots:
             sharing.sort(key=lambda x: x[0][6] >= 0)
         items = self._order(sharing)
+        self.n_items = len(items)
+        items = [(x[0] + len(items), *x[1:]) if x[2] < 0 else x for x in items] + singles
         part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
         self.parts = int(part_at[-1])
         self.max_parts = int((n_prefix + n_suffix).max())
-        self.n_items = len(items)
         arrays = [np.asarray(items, np.int64).ravel(), np.asarray(row_list, np.int64),
                   part_at[:-1], part_at[:-1] + n_prefix, n_prefix + n_suffix]
         self._rows_at = 4 * arrays[0].size
         self._parts_at = self._rows_at + 4 * arrays[1].size
         return np.concatenate(arrays).astype(np.int32)
 
-    def _ranges(self, blocks, bounds, share, rows):
-        """Ranges of each segment, of ``blocks`` items per range, up to
-        ``bounds`` keys (``share`` of them on average: own lengths lie anywhere
-        below their bound) and ``rows`` query rows: of about one length, the
-        one that gives the shortest time by the figures above."""
+    def _ranges(self, blocks, bounds, own, narrow, rows):
+        """How the segments are cut: (ranges of each, whether narrow items of
+        own tokens go to single waves).  A segment has ``blocks`` items per
+        range, up to ``bounds`` keys (own lengths lie anywhere below their bound:
+        half of it on average) and ``rows`` query rows.  Taken are ranges of about
+        one length, the one that gives the shortest time by the figures above."""
         if not len(blocks):
-            return []
+            return [], False
         d, hq, hkv = self.head_dim, self.num_q_heads, self.num_kv_heads
-        slots = _SLOTS[d > 128]
+        slots, share = _SLOTS[d > 128], np.where(own, 0.5, 1.0)
+        single = own & narrow
         best, longest = None, int(bounds.max())
         count = max(1, math.ceil(4 * math.log2(max(1.0, longest / 128)))) + 1
+        cache = (bounds * share).sum() * hkv * d * 4 / _CACHE
         for length in np.ceil(np.geomspace(128, max(128, longest), count)):
             splits = np.minimum(np.ceil(bounds / length), 2 ** 15 - 1)
-            items = blocks * splits
-            full = min(1.0, max(_ALONE, items.sum() / slots))
-            keys = _KEY * d * full * np.ceil(bounds / splits)
-            last = _ITEM + keys.max()
-            rounds = math.ceil(items[_ITEM + keys > 0.7 * last].sum() / slots)
-            time = max((items * (_ITEM + keys * share)).sum() / slots, rounds * last,
-                       (bounds * share).sum() * hkv * d * 4 / _CACHE)
-            time += (splits * rows).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
-            if best is None or time < best[0]:
-                best = time, splits
-        return best[1].astype(np.int64).tolist()
+            joins = (splits * rows).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
+            for solo in (False, True) if single.any() else (False,):
+                waves = np.where(single & solo, 4, 1)   # items of a workgroup
+                items = blocks * splits / waves
+                full = min(1.0, max(_ALONE, items.sum() / slots))
+                keys = _KEY * d * full * waves * np.ceil(bounds / splits)
+                last = _ITEM + keys.max()
+                rounds = math.ceil(items[_ITEM + keys > 0.7 * last].sum() / slots)
+                time = joins + max((items * (_ITEM + keys * share)).sum() / slots, rounds * last, cache)
+                if best is None or time < best[0]:
+                    best = time, splits, solo
+        return best[1].astype(np.int64).tolist(), best[2]
 
     @staticmethod
     def _only_row(rows, group, m0, size):

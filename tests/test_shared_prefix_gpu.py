@@ -121,6 +121,29 @@ def test_row_counts(cuda_device, rows, d):
          torch.bfloat16, seed=rows)
 
 
+@pytest.mark.parametrize("solo", [False, True])
+@pytest.mark.parametrize("splits", [1, 3])
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 8, 64, torch.bfloat16), (32, 4, 128, torch.float16),
+                                            (40, 1, 96, torch.bfloat16), (6, 3, 40, torch.float16),
+                                            (4, 2, 256, torch.bfloat16), (3, 1, 192, torch.bfloat16)])
+def test_ways_to_cut_the_work(cuda_device, monkeypatch, hq, hkv, d, dtype, splits, solo):
+    """Own tokens by whole workgroups and by single waves, in one and several
+    ranges, with own lengths from none to more than a lookup's 256 and 1024."""
+    from moba_hip.shared_prefix import SharedPrefixPlan
+    monkeypatch.setattr(SharedPrefixPlan, "_ranges",
+                        lambda self, blocks, *a: ([splits] * len(blocks), solo))
+    own = [0, 1, 15, 16, 17, 255, 257, 1, 1100, 64, 300]
+    n = len(own)
+    _run([500] + own, [0] * n, [500] * n, list(range(1, n + 1)), own, hq, hkv, d, 16, dtype,
+         seed=d + splits)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 64), (32, 4, 128), (48, 1, 80)])
+def test_many_short_sequences(cuda_device, hq, hkv, d):
+    own = [(7 * i) % 23 for i in range(300)]
+    _run([70] + own, [0] * 300, [70] * 300, list(range(1, 301)), own, hq, hkv, d, 16, torch.bfloat16)
+
+
 def test_groups_of_unlike_prefixes_and_rows_of_nothing(cuda_device):
     """Rows in mixed order: two prefixes, one of them at two lengths, rows
     without a prefix, without own tokens, and without either."""
