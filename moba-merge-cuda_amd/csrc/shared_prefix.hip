@@ -698,10 +698,13 @@ template <int DT, bool NEAR> void launch_blocks(const SharedArgs& a, int n_items
 template <int DT>
 void launch_merge(const SharedArgs& a, int Nq, int max_parts, uint16_t* out, float* lse,
                   hipStream_t st) {
-  // a thread takes the ranges four at a time: the fewest threads that need one
-  // round, as far as a workgroup holds them
+  // A thread takes the ranges four at a time.  One round of them is fastest
+  // while the launch is small (us with 1, 4, 16 threads per dims: 154 ranges of 28
+  // (row, head) pairs 23.6, 8.5, 5.0; 17 of 1512 5.1, 4.4, 5.9); one that fills
+  // the card by itself has its loads in flight anyway (11 of 8192: 10.8, 14.2).
   int pl = 1;
-  while (4 * pl < max_parts && 2 * pl * (a.D / 4) <= 256) pl *= 2;
+  const int64_t threads = (int64_t)Nq * a.Hq * (a.D / 4);
+  while (4 * pl < max_parts && pl * threads < 65536 && 2 * pl * (a.D / 4) <= 256) pl *= 2;
   const int per = 256 / (a.D / 4 * pl);
   const dim3 grid((unsigned)(((int64_t)Nq * a.Hq + per - 1) / per));
   hipLaunchKernelGGL((merge_kernel<DT>), grid, dim3(256), 0, st, a.part_o, a.part_ml, a.prefix_at,
