@@ -393,8 +393,8 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
 /* Attention of Nq query rows over a prefix that several of them share and
  * their own tokens, both in the page pool (no counterpart in the reference,
  * whose decode reads a row's tokens row by row: paged_decode.py:67-112).
- * q [Nq,Hq,D]; row r attends its prefix segment and own_lengths[r] (device;
- * cut to [0, max_length]) tokens of its own slot.  The host's plan holds the
+ * q [Nq,Hq,D]; row r attends its prefix segment and own_lengths[r] + length_add
+ * (device; cut to [0, max_length]) tokens of its own slot.  The host's plan holds the
  * work: items [n_items][8] int32 (first entry of the segment in rows; first
  * (row, q head of the kv head) pair; pairs, at most 128, 0 pads; page-table row;
  * kv head; range | ranges << 16; tokens of the segment or -1: the rows' own
@@ -411,7 +411,7 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
 int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
                               float scale, const void* k_cache, const void* v_cache,
                               int num_pages, int page_size, const int* table, int table_width,
-                              const int* own_lengths, int max_length, const int* items,
+                              const int* own_lengths, int length_add, int max_length, const int* items,
                               int n_items, const int* rows, const int* row_parts, int max_parts,
                               float* part_o, float* part_ml, void* out, float* lse,
                               void* stream);

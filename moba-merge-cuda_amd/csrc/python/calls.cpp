@@ -227,7 +227,7 @@ PyObject* shared_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const int rc = moba_hip_shared_attention(
       q->data_ptr(), p.code, (int)x.rows, (int)x.hq, (int)x.hkv, (int)x.d, (float)scale, p.k, p.v,
       (int)p.pages, (int)p.page, (const int*)table->data_ptr(), (int)p.width,
-      (const int*)own->data_ptr(), (int)std::min(x.max_suffix, p.width * p.page), (const int*)m,
+      (const int*)own->data_ptr(), 0, (int)std::min(x.max_suffix, p.width * p.page), (const int*)m,
       (int)x.n_items, (const int*)(m + x.rows_at), (const int*)(m + x.parts_at), (int)x.max_parts, w,
       w + parts * x.d, out.data_ptr(), (float*)lse.data_ptr(), stream);
   if (rc) return failed("moba_hip_shared_attention", rc);

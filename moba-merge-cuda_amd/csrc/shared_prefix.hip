@@ -40,7 +40,7 @@ struct SharedArgs {
   uint32_t pool_bytes;      // of k_cache; 0: 4 GiB or more
   const int* table;
   const int* lengths;       // own tokens of each row
-  int max_length;
+  int length_add, max_length;  // own length of a row: lengths[row] + length_add, cut
   const Item* items;
   const int* rows;
   const int *prefix_at, *own_at, *n_part;  // per row: first partials, ranges in all
@@ -121,7 +121,7 @@ template <bool NEAR> struct Rows {
 
 // A row's own length.
 MOBA_DEV int own_length(const SharedArgs& a, int row) {
-  return max(0, min(a.lengths[row], a.max_length));
+  return (int)max(0ll, min((long long)a.lengths[row] + a.length_add, (long long)a.max_length));
 }
 // What a lane knows of its (row, q head) pair.
 struct Pair {
@@ -716,7 +716,7 @@ void launch_merge(const SharedArgs& a, int Nq, int max_parts, uint16_t* out, flo
 extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
                                          float scale, const void* k_cache, const void* v_cache,
                                          int num_pages, int page_size, const int* table,
-                                         int table_width, const int* own_lengths, int max_length,
+                                         int table_width, const int* own_lengths, int length_add, int max_length,
                                          const int* items, int n_items, const int* rows,
                                          const int* row_parts, int max_parts, float* part_o, float* part_ml,
                                          void* out, float* lse, void* stream) {
@@ -732,7 +732,7 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
   a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.G = Hq / Hkv;
   a.scale_log2 = scale * kLog2e;
   a.num_pages = num_pages; a.P = page_size; a.W = table_width; a.table = table;
-  a.lengths = own_lengths; a.max_length = max_length;
+  a.lengths = own_lengths; a.length_add = length_add; a.max_length = max_length;
   a.items = (const Item*)items; a.rows = rows;
   const int64_t pool = (int64_t)num_pages * page_size * Hkv * D * 2;
   a.pool_bytes = pool <= kNowhere ? (uint32_t)pool : 0;

@@ -11,5 +11,6 @@ from .grouped_attention import opt_hip, opt_hip_mha  # noqa: F401
 from .merge import merge_forward  # noqa: F401
 from .kv_cache import ContiguousKVCache, DecodeResult, PagedKVCache  # noqa: F401
 from .prepared_decode import PreparedDecode  # noqa: F401
+from .prepared_shared import PreparedSharedDecode  # noqa: F401
 from .rotary import RotaryTable, append_rotary  # noqa: F401
 from .shared_prefix import SharedPrefixPlan, shared_prefix_attention  # noqa: F401

@@ -79,7 +79,7 @@ def finite(t, name):
     _require([(lambda: bool(torch.isfinite(t).all()), f"{name} contains NaN/Inf")])
 
 
-def tensors(specs, *, device, dtype, head_dim):
+def tensors(specs, *, device, dtype, head_dim, check_finite=True):
     """`tensor` for each (t, name, kwargs) in order, raising what those calls
     in sequence would raise first; the NaN/Inf test of all inputs reads one
     flag (one host synchronisation instead of one per tensor).  A callable
@@ -91,9 +91,12 @@ def tensors(specs, *, device, dtype, head_dim):
         try:
             tensor(t, name, device=device, dtype=dtype, head_dim=head_dim, finite=False, **kw)
         except ValueError:
-            for t0, n0, _ in specs[:i]:  # an earlier input's NaN/Inf comes first
-                finite(t0, n0)
+            if check_finite:
+                for t0, n0, _ in specs[:i]:  # an earlier input's NaN/Inf comes first
+                    finite(t0, n0)
             raise
+    if not check_finite:
+        return
     if len(specs) == 1 or not bool(torch.stack([torch.isfinite(t).all() for t, _, _ in specs]).all()):
         for t, name, _ in specs:
             finite(t, name)

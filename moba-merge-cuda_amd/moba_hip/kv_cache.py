@@ -20,10 +20,16 @@ Operations hold one lock and run on the stream that was current at
 construction; calls from another stream or inside an external graph capture
 are refused.  While a :class:`~moba_hip.prepared_decode.PreparedDecode`
 holds the cache, ordinary operations are refused too.
+
+Beyond the reference's cache: ``append_rotary`` takes keys before their
+rotation and turns them (and the queries of the same tokens) on the way into
+the pool; ``attend_shared`` and ``prepare_shared_decode`` let several sequences
+go on behind one prefix that is stored once, in a slot of its own.
 """
 from __future__ import annotations
 
 import threading
+from collections import OrderedDict
 from dataclasses import dataclass
 
 import numpy as np
@@ -33,6 +39,8 @@ from . import decode_contract as contract
 from .baseline_adapter import _require
 from .cache_layout import PageAllocator
 from .ops import decode as kernels
+from .rotary import RotaryTable, append_rotary
+from .shared_prefix import SharedPrefixPlan, shared_prefix_attention
 
 # names of the reference module, kept for callers that import them
 _ints = contract.int_vector
@@ -43,6 +51,13 @@ _mode = contract.decode_mode
 class AppendResult:
     sequence_ids: tuple
     positions: tuple
+
+
+@dataclass(frozen=True)
+class RotaryAppendResult:
+    sequence_ids: tuple
+    positions: tuple
+    q: object   # the rotated queries [N,Hq,D]; None if none were given
 
 
 @dataclass(frozen=True)
@@ -68,6 +83,7 @@ class PagedKVCache:
         self._lock = threading.RLock()
         self._lessee = None      # the PreparedDecode holding the cache, if any
         self._broken = False     # a device failure happened under a lease
+        self._plans = OrderedDict()   # work plans of attend_shared, the last few
         with torch.cuda.device(requested):
             self.device = torch.device("cuda", torch.cuda.current_device())
             self._stream = torch.cuda.current_stream(self.device).cuda_stream
@@ -156,18 +172,22 @@ class PagedKVCache:
             counts = contract.append_counts(k.shape[0], ids, cu_seqlens)
             return self._store(k, v, ids, counts)[0]
 
-    def _store(self, k, v, ids, counts):
+    def _store(self, k, v, ids, counts, put=None, extra=()):
         """Plans, writes and commits an append whose inputs are checked.
-        Returns (AppendResult, device token slots, device token positions)."""
+        Returns (AppendResult, device token slots, device token positions).
+        ``put`` writes the tokens in place of the plain append: it gets their
+        device slots and positions, then the device copies of ``extra``."""
         plan = self._layout.plan_append(ids, counts)
         before = self._layout._pool.clone()
         self._layout.commit(plan)
         try:
-            seq, pos, cseq, cchunk = self._publish_layout(plan.seq_arr, plan.pos_arr,
-                                                          plan.closed_arr[:, 0],
-                                                          plan.closed_arr[:, 1])
-            kernels.append_tokens(k.contiguous(), v.contiguous(), self.k_cache, self.v_cache,
-                                  self._table, seq, pos)
+            seq, pos, cseq, cchunk, *more = self._publish_layout(
+                plan.seq_arr, plan.pos_arr, plan.closed_arr[:, 0], plan.closed_arr[:, 1], *extra)
+            if put is None:
+                kernels.append_tokens(k.contiguous(), v.contiguous(), self.k_cache, self.v_cache,
+                                      self._table, seq, pos)
+            else:
+                put(seq, pos, *more)
             kernels.block_means(self.k_cache, self._table, self._means, cseq, cchunk,
                                 self.chunk_size)
         except Exception:  # a failed launch leaves the pool as it was
@@ -175,6 +195,49 @@ class PagedKVCache:
             self._publish_layout()
             raise
         return AppendResult(plan.token_sequences, plan.token_positions), seq, pos
+
+    def _check_rotary(self, rotary, last):
+        """``last``: the largest position that will be turned."""
+        _require([
+            (lambda: isinstance(rotary, RotaryTable), "rotary must be a RotaryTable"),
+            (lambda: rotary.device == self.device, "rotary table must be on the cache's device"),
+            (lambda: rotary.rotary_dim <= self.head_dim, "rotary_dim exceeds head_dim"),
+            (lambda: last < rotary.max_positions, "positions exceed the rotary table"),
+        ])
+
+    @torch.no_grad()
+    def append_rotary(self, k, v, rotary, *, sequence_ids, cu_seqlens=None, q=None, offsets=None,
+                      check_finite=True):
+        """``append`` of keys before their rotation: each turns by its position
+        (plus its sequence's entry of ``offsets``, the length of the shared
+        prefix it goes on behind) on the way into the pool, and so do the
+        queries ``q`` [N,Hq,D] of the same tokens.  Inputs may be views with a
+        contiguous last dimension."""
+        with self._lock, torch.cuda.device(self.device):
+            self._guard()
+            specs = [(k, "k", {"heads": self.num_kv_heads}),
+                     (v, "v", {"heads": self.num_kv_heads, "tokens": lambda: k.shape[0]})]
+            if q is not None:
+                specs.append((q, "q", {"tokens": lambda: k.shape[0]}))
+            contract.tensors(specs, device=self.device, dtype=self.dtype, head_dim=self.head_dim,
+                             check_finite=check_finite)
+            self._no_pool_alias(*(t for t, _, _ in specs))
+            ids = self._layout.validate_ids(_ints(sequence_ids, "sequence_ids"), unique=True)
+            counts = contract.append_counts(k.shape[0], ids, cu_seqlens)
+            shift = (0,) * len(ids) if offsets is None else _ints(offsets, "offsets")
+            _require([(lambda: len(shift) == len(ids) and min(shift) >= 0,
+                       "one offset of 0 or more per sequence required")])
+            lengths = self.lengths
+            self._check_rotary(rotary, max(lengths[s] + n + o for s, n, o in zip(ids, counts, shift)) - 1)
+            by_slot = np.zeros(self._layout.batch_size, np.int32)
+            by_slot[list(ids)] = shift
+            turned = []
+
+            def put(seq, pos, offs):
+                turned.append(append_rotary(k, v, self.k_cache, self.v_cache, self._table, seq, pos,
+                                            rotary, q=q, offsets=offs))
+            done = self._store(k, v, ids, counts, put, (by_slot,))[0]
+            return RotaryAppendResult(done.sequence_ids, done.positions, turned[0])
 
     # ----------------------------------------------------------------- attend
     def _positions(self, q, sequence_ids, positions):
@@ -233,6 +296,53 @@ class PagedKVCache:
         kernels.attention(q, self.k_cache, self.v_cache, self._table, self._lengths, dev_ids,
                           dev_pos, work, out, lse, self.chunk_size, dense, history + 1)
         return DecodeResult(out, lse, None if dense else work.selected, ids, pos)
+
+    def _prefixes(self, ids, prefix_ids):
+        """Checked prefix slots of the sequences ``ids`` (-1: none) and their
+        lengths."""
+        prefix = _ints(prefix_ids, "prefix_ids")
+        _require([(lambda: len(prefix) == len(ids), "one prefix ID per sequence required")])
+        used = [p for p in prefix if p != -1]
+        if used:
+            self._layout.validate_ids(used)
+        _require([(lambda: not set(used) & set(ids),
+                   "a sequence of the call cannot be a prefix as well")])
+        lengths = self.lengths
+        return prefix, tuple(lengths[p] if p >= 0 else 0 for p in prefix)
+
+    @torch.no_grad()
+    def attend_shared(self, q, *, sequence_ids, prefix_ids, positions=None, scale=None):
+        """Dense attention of q [Nq,Hq,D] over the whole of each row's prefix
+        slot and then its own slot up to its position.  ``prefix_ids``: one
+        slot per query row, -1 for none; the rows that share one read it once
+        for all.  Several rows of one sequence attend causally by their
+        positions.  Returns a DecodeResult."""
+        with self._lock, torch.cuda.device(self.device):
+            self._guard()
+            ids, pos = self._positions(q, sequence_ids, positions)
+            prefix, plen = self._prefixes(ids, prefix_ids)
+            # the plan serves own lengths up to the next power of two
+            bound = min(1 << max(pos).bit_length(), self._layout.max_seq_len)
+            key = (ids, prefix, plen, q.shape[1], bound)
+            plan = self._plans.get(key)
+            if plan is None:
+                plan = SharedPrefixPlan(prefix, plen, ids, q.shape[1], self.num_kv_heads,
+                                        self.head_dim, max_suffix=bound, device=self.device)
+                self._plans[key] = plan
+                while len(self._plans) > 4:
+                    self._plans.popitem(last=False)
+            own = torch.tensor([p + 1 for p in pos], dtype=torch.int32, device=self.device)
+            out, lse = shared_prefix_attention(q, self.k_cache, self.v_cache, self._table, own, plan,
+                                               scale=scale)
+            return DecodeResult(out, lse, None, ids, pos)
+
+    def prepare_shared_decode(self, sequence_ids, prefix_ids, num_q_heads, *, rotary=None,
+                              max_length=None, check_finite=True):
+        """Leases the cache for the decode of ``sequence_ids`` behind their
+        prefixes: :class:`~moba_hip.prepared_shared.PreparedSharedDecode`."""
+        from .prepared_shared import PreparedSharedDecode
+        return PreparedSharedDecode(self, sequence_ids, prefix_ids, num_q_heads, rotary=rotary,
+                                    max_length=max_length, check_finite=check_finite)
 
     @torch.no_grad()
     def append_and_attend(self, q, k, v, *, sequence_ids, cu_seqlens=None, topk=4, mode="moba"):

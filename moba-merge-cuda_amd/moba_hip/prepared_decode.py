@@ -327,8 +327,8 @@ class PreparedDecode:
                 self._lease.publish(c._layout)
             c._lessee = None
             self.closed = True
-            lib = _lib.load()
-            lib.moba_prep_destroy(self._handle)
+            if self._handle:
+                _lib.load().moba_prep_destroy(self._handle)
             self._handle = None
 
     def __del__(self):

@@ -264,7 +264,7 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     wp, meta = work.data_ptr(), plan.meta.data_ptr()
     _on_device(k_cache.get_device(), "moba_hip_shared_attention", qp, _DTYPES[q.dtype], n, hq, hkv,
                d, scale, kp, vp, pages, page, page_table.data_ptr(), width,
-               suffix_lengths.data_ptr(), min(plan.max_suffix, width * page), meta, plan.n_items,
+               suffix_lengths.data_ptr(), 0, min(plan.max_suffix, width * page), meta, plan.n_items,
                meta + plan._rows_at, meta + plan._parts_at, plan.max_parts, wp, wp + 4 * parts * d,
                out.data_ptr(), lse.data_ptr())
     return out, lse
