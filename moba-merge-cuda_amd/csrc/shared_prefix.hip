@@ -81,7 +81,7 @@ template <int ND> struct Dims {
   // dims, two above.
   static constexpr int STAGES = DP <= 128 ? 3 : 2, CAP = 1024;
   static constexpr int TILES = STAGES * TILE * 2 * 2;
-  static_assert(4 * 2 * OWN * DP * 2 <= TILES && 2 * NDB * 4 * 64 * 16 <= TILES, "LDS");
+  static_assert(4 * 2 * OWN * DP * 2 <= TILES && 4 * 3 * 4 * 64 * 16 <= TILES && CAP * 4 >= 4 * 64 * 8, "LDS");
   static constexpr int TOK = TILES, FLAGS = TOK + CAP * 4, LDS = FLAGS + 16;
   static constexpr int WAVES = ND <= 128 ? 3 : 2;   // per SIMD
 };
@@ -550,42 +550,62 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
     return;
   }
 
-  // join: waves 2, 3 into 0, 1, then 1 into 0; lane by lane
-  f32x4_t* ox = (f32x4_t*)smem;                // [2][NDB * 4][64], where the tiles were
-  float2* mx = (float2*)(smem + C::TOK);       // [2][64]
+  // Join, lane by lane, waves in order: wave w takes the 32-dim blocks db % 4 ==
+  // w from the others and writes them, four blocks a round.
+  f32x4_t* ox = (f32x4_t*)smem;                // [4 waves][3][4][64], where the tiles were
+  float2* mx = (float2*)(smem + C::TOK);       // [4][64]
+  lds_barrier();                               // tiles and tokens are read
+  mx[wave * 64 + lane] = make_float2(m_run, l);
+  float weight[4];
+  float* po = a.part_o + p.part * D;
 #pragma unroll
-  for (int step = 2; step > 0; step >>= 1) {
-    lds_barrier();
-    const bool give = wave >= step && wave < 2 * step;
-    const int at = give ? wave - step : wave;
-    if (give) {
+  for (int b0 = 0; b0 < NDB; b0 += 4) {
+    if (b0) lds_barrier();                     // the round before is read
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+    for (int i = 0; i < 4 && b0 + i < NDB; ++i)
+      if (i != wave) {
+        const int at = (wave * 3 + (i > wave ? i - 1 : i)) * 4;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          ox[(at * NDB * 4 + db * 4 + j) * 64 + lane] =
-              (f32x4_t){oacc[db][4 * j], oacc[db][4 * j + 1], oacc[db][4 * j + 2], oacc[db][4 * j + 3]};
-      mx[at * 64 + lane] = make_float2(m_run, l);
-    }
-    lds_barrier();
-    if (wave < step) {
-      const float2 o = mx[at * 64 + lane];
-      const float M = fmaxf(m_run, o.x), ref = M == -INFINITY ? 0.0f : M;
-      const float wa = fast_exp2(m_run - ref), wb = fast_exp2(o.x - ref);
-      l = l * wa + o.y * wb;
-      m_run = M;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        f32x4_t v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = ox[(at * NDB * 4 + db * 4 + j) * 64 + lane];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) oacc[db][r] = oacc[db][r] * wa + v[r >> 2][r & 3] * wb;
-        __builtin_amdgcn_sched_barrier(0);  // a block at a time, not all in registers
+          ox[(at + j) * 64 + lane] = (f32x4_t){oacc[b0 + i][4 * j], oacc[b0 + i][4 * j + 1],
+                                               oacc[b0 + i][4 * j + 2], oacc[b0 + i][4 * j + 3]};
       }
+    lds_barrier();
+    if (b0 == 0) {
+      float2 ml[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) ml[w] = mx[w * 64 + lane];
+      m_run = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+      const float ref = m_run == -INFINITY ? 0.0f : m_run;
+      l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        weight[w] = fast_exp2(ml[w].x - ref);
+        l += ml[w].y * weight[w];
+      }
+      if (wave == 0 && p.valid && hh == 0) a.part_ml[p.part] = make_float2(m_run, l);
     }
+#pragma unroll
+    for (int i = 0; i < 4 && b0 + i < NDB; ++i)
+      if (i == wave) {
+        f32x4_t sum[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4_t v = {oacc[b0 + i][4 * j], oacc[b0 + i][4 * j + 1], oacc[b0 + i][4 * j + 2],
+                         oacc[b0 + i][4 * j + 3]};
+            if (w != i) v = ox[((w * 3 + (i > w ? i - 1 : i)) * 4 + j) * 64 + lane];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[j][k] = w ? fmaf(v[k], weight[w], sum[j][k]) : v[k] * weight[0];
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int d = (b0 + i) * 32 + 8 * j + 4 * hh;
+          if (p.valid && d < D) *reinterpret_cast<f32x4_t*>(po + d) = sum[j];
+        }
+      }
   }
-  if (wave == 0 && p.valid) store_partial<NDB>(a, p.part, oacc, m_run, l, hh);
 }
 
 template <int DT, int ND, bool NEAR>
