@@ -90,60 +90,72 @@ class SharedPrefixPlan:
                                    self.max_parts)
 
     def _build(self, prefix, length, suffix):
+        """The device arrays: work items, segments' rows, rows' partials."""
         n, hkv, group = self.rows, self.num_kv_heads, self.num_q_heads // self.num_kv_heads
-        segments = []   # (slot, tokens or -1, bound of the tokens, rows)
-        shared, alone = {}, {}
-        for row in range(n):
-            if length[row] > 0:
-                shared.setdefault((int(prefix[row]), int(length[row])), []).append(row)
-            if suffix[row] >= 0 and self.max_suffix:
-                alone.setdefault(int(suffix[row]), []).append(row)
-        segments += [(slot, tokens, tokens, rows) for (slot, tokens), rows in shared.items()]
-        segments += [(slot, -1, self.max_suffix, rows) for slot, rows in alone.items()]
+        # segments: the rows of one (prefix, length), then those of one own slot
+        shared = np.nonzero(length > 0)[0]
+        alone = np.nonzero((suffix >= 0) & (self.max_suffix > 0))[0]
+        pairs, of_shared, n_shared = np.unique(prefix[shared] << 32 | length[shared],
+                                               return_inverse=True, return_counts=True)
+        slots, of_alone, n_alone = np.unique(suffix[alone], return_inverse=True, return_counts=True)
+        row_list = np.concatenate((shared[np.argsort(of_shared, kind="stable")],
+                                   alone[np.argsort(of_alone, kind="stable")]))
+        slot = np.concatenate((pairs >> 32, slots))
+        own = np.arange(len(slot)) >= len(pairs)
+        tokens = np.where(own, -1, np.concatenate((pairs & (2 ** 32 - 1), slots)))
+        bound = np.where(own, self.max_suffix, tokens)
+        n_rows = np.concatenate((n_shared, n_alone))
+        row_at = np.cumsum(n_rows) - n_rows
         # 33 to 128 pairs: one wide block of which a part is idle reads its keys
         # once (16 rows of 4 heads behind 32K tokens: 41 us; two narrow ones 43)
-        sizes = [_WIDE if len(rows) * group > _NARROW else _NARROW for *_, rows in segments]
-        blocks = [-(-len(rows) * group // size) for (*_, rows), size in zip(segments, sizes)]
-        ranges, solo = self._ranges(
-            np.array([b * hkv for b in blocks]), np.array([bound for _, _, bound, _ in segments]),
-            np.array([tokens < 0 for _, tokens, *_ in segments]), np.array(sizes) == _NARROW,
-            np.array([len(rows) for *_, rows in segments]))
+        size = np.where(n_rows * group > _NARROW, _WIDE, _NARROW)
+        blocks = -(-n_rows * group // size)
+        splits, solo = self._ranges(blocks * hkv, bound, own, size == _NARROW, n_rows)
         n_prefix, n_suffix = np.zeros(n, np.int64), np.zeros(n, np.int64)
-        row_list, sharing, singles = [], [], []
-        for (slot, tokens, _, rows), size, nb, splits in zip(segments, sizes, blocks, ranges):
-            (n_prefix if tokens >= 0 else n_suffix)[rows] = splits
-            for s in range(splits):
-                for kh in range(hkv):
-                    same_keys = [
-                        (len(row_list), b * size, min(size, len(rows) * group - b * size),
-                         slot, kh, s | splits << 16, tokens, self._only_row(rows, group, b * size, size))
-                        for b in range(nb)]
-                    if solo and tokens < 0 and size == _NARROW:
-                        singles += same_keys
-                    else:
-                        sharing.append(same_keys)
-            row_list += rows
+        of_row = np.repeat(splits, n_rows)
+        n_prefix[row_list[:len(shared)]] = of_row[:len(shared)]
+        n_suffix[row_list[len(shared):]] = of_row[len(shared):]
+
+        # one item per (segment, range, kv head, block); those of one (segment,
+        # range, kv head) read the same keys
+        count = splits * hkv * blocks
+        seg = np.repeat(np.arange(len(slot)), count)
+        local = np.arange(len(seg)) - np.repeat(np.cumsum(count) - count, count)
+        block, part = local % blocks[seg], local // blocks[seg]
+        m0 = block * size[seg]
+        n_m = np.minimum(size[seg], n_rows[seg] * group - m0)
+        first, last = m0 // group, (m0 + n_m - 1) // group
+        only = np.where(first == last, row_list[row_at[seg] + first], -1)
+        items = np.stack((row_at[seg], m0, n_m, slot[seg], part % hkv,
+                          part // hkv | splits[seg] << 16, tokens[seg], only), axis=1)
+        keys = np.cumsum(block == 0)
         # four waves' items of one workgroup: the kv heads of a row next to each
         # other, whose keys lie together and are as many
-        pad = (0,) * 8
-        singles += [pad] * (-len(singles) % 4)
-        sharing += [[(i, 0, -1, 0, 0, 0, -1, 0)] for i in range(0, len(singles), 4)]
+        single = (own & (size == _NARROW) & solo)[seg]
+        singles, items, keys = items[single], items[~single], keys[~single]
+        singles = np.concatenate((singles, np.zeros((-len(singles) % 4, 8), np.int64)))
+        carriers = np.zeros((len(singles) // 4, 8), np.int64)
+        carriers[:, 0], carriers[:, 2], carriers[:, 6] = 4 * np.arange(len(carriers)), -1, -1
+        items = np.concatenate((items, carriers))
+        keys = np.concatenate((keys, len(seg) + 1 + np.arange(len(carriers))))
         # Longest first; but a few items of own tokens behind a card full of
         # prefix ranges would start when those end, all alone
-        own = sum(len(x) for x in sharing if x[0][6] < 0)
-        slots = _SLOTS[self.head_dim > 128]
-        if own <= slots // 2 and sum(map(len, sharing)) > slots:
-            sharing.sort(key=lambda x: x[0][6] >= 0)
-        items = self._order(sharing)
+        n_own = int((items[:, 6] < 0).sum())
+        card = _SLOTS[self.head_dim > 128]
+        if n_own <= card // 2 and len(items) > card:
+            order = np.argsort(items[:, 6] >= 0, kind="stable")
+            items, keys = items[order], keys[order]
+        items = self._dealt(items, keys)
         self.n_items = len(items)
-        items = [(x[0] + len(items), *x[1:]) if x[2] < 0 else x for x in items] + singles
-        part_at = np.concatenate(([0], np.cumsum(n_prefix + n_suffix)))
-        self.parts = int(part_at[-1])
+        items[items[:, 2] < 0, 0] += len(items)
+
+        part_at = np.cumsum(n_prefix + n_suffix) - (n_prefix + n_suffix)
+        self.parts = int((n_prefix + n_suffix).sum())
         self.max_parts = int((n_prefix + n_suffix).max())
-        arrays = [np.asarray(items, np.int64).ravel(), np.asarray(row_list, np.int64),
-                  part_at[:-1], part_at[:-1] + n_prefix, n_prefix + n_suffix]
-        self._rows_at = 4 * arrays[0].size
-        self._parts_at = self._rows_at + 4 * arrays[1].size
+        arrays = [items.ravel(), singles.ravel(), row_list, part_at, part_at + n_prefix,
+                  n_prefix + n_suffix]
+        self._rows_at = 4 * (arrays[0].size + arrays[1].size)
+        self._parts_at = self._rows_at + 4 * len(row_list)
         return np.concatenate(arrays).astype(np.int32)
 
     def _ranges(self, blocks, bounds, own, narrow, rows):
@@ -153,19 +165,22 @@ class SharedPrefixPlan:
         half of it on average) and ``rows`` query rows.  Taken are ranges of about
         one length, the one that gives the shortest time by the figures above."""
         if not len(blocks):
-            return [], False
+            return np.zeros(0, np.int64), False
+        alike, index, times = np.unique(np.stack((blocks, bounds, own, narrow, rows), axis=1), axis=0,
+                                        return_inverse=True, return_counts=True)
+        blocks, bounds, own, narrow, rows = alike.T
         d, hq, hkv = self.head_dim, self.num_q_heads, self.num_kv_heads
         slots, share = _SLOTS[d > 128], np.where(own, 0.5, 1.0)
-        single = own & narrow
+        single = (own & narrow).astype(bool)
         best, longest = None, int(bounds.max())
         count = max(1, math.ceil(4 * math.log2(max(1.0, longest / 128)))) + 1
-        cache = (bounds * share).sum() * hkv * d * 4 / _CACHE
+        cache = (bounds * share * times).sum() * hkv * d * 4 / _CACHE
         for length in np.ceil(np.geomspace(128, max(128, longest), count)):
             splits = np.minimum(np.ceil(bounds / length), 2 ** 15 - 1)
-            joins = (splits * rows).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
+            joins = (splits * rows * times).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
             for solo in (False, True) if single.any() else (False,):
                 waves = np.where(single & solo, 4, 1)   # items of a workgroup
-                items = blocks * splits / waves
+                items = blocks * splits * times / waves
                 full = min(1.0, max(_ALONE, items.sum() / slots))
                 keys = _KEY * d * full * waves * np.ceil(bounds / splits)
                 last = _ITEM + keys.max()
@@ -173,25 +188,22 @@ class SharedPrefixPlan:
                 time = joins + max((items * (_ITEM + keys * share)).sum() / slots, rounds * last, cache)
                 if best is None or time < best[0]:
                     best = time, splits, solo
-        return best[1].astype(np.int64).tolist(), best[2]
+        return best[1].astype(np.int64)[index.ravel()], best[2]
 
     @staticmethod
-    def _only_row(rows, group, m0, size):
-        """The row of a block's pairs, -1 if there are several."""
-        last = min(m0 + size, len(rows) * group) - 1
-        return rows[m0 // group] if m0 // group == last // group else -1
-
-    @staticmethod
-    def _order(sharing):
-        """Items that read the same keys go to one XCD, one after another;
-        XCDs are filled evenly, and an item of no pairs pads a short one."""
-        per = [[] for _ in range(_XCDS)]
-        for items in sharing:
-            min(per, key=len).extend(items)
-        depth = max(map(len, per))
-        pad = (0,) * 8
-        return [per[x][i] if i < len(per[x]) else pad
-                for i in range(depth) for x in range(_XCDS)]
+    def _dealt(items, keys):
+        """The items as workgroups take them: those of the same ``keys`` go to
+        one XCD, one after another, the XCDs in turn; an item of no pairs pads
+        a short one."""
+        if not len(items):
+            return items
+        turn = (np.cumsum(np.concatenate(([True], keys[1:] != keys[:-1]))) - 1) % _XCDS
+        order = np.argsort(turn, kind="stable")
+        held = np.bincount(turn, minlength=_XCDS)
+        rank = np.arange(len(items)) - np.repeat(np.cumsum(held) - held, held)
+        dealt = np.zeros((int(held.max()) * _XCDS, items.shape[1]), np.int64)
+        dealt[rank * _XCDS + turn[order]] = items[order]
+        return dealt
 
 
 def _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan):

@@ -11,6 +11,7 @@ Allowed error of an output element, with A = sum_j p_j |v_j| / z:
   of 2^-24 each that add up as their root in practice and 2^-12 at worst: the
   test's sums are below 2^4 terms per step of that bound);
 * the result is rounded once: eps/2 * |out|."""
+import numpy as np
 import pytest
 import torch
 
@@ -131,7 +132,7 @@ def test_ways_to_cut_the_work(cuda_device, monkeypatch, hq, hkv, d, dtype, split
     ranges, with own lengths from none to more than a lookup's 256 and 1024."""
     from moba_hip.shared_prefix import SharedPrefixPlan
     monkeypatch.setattr(SharedPrefixPlan, "_ranges",
-                        lambda self, blocks, *a: ([splits] * len(blocks), solo))
+                        lambda self, blocks, *a: (np.full(len(blocks), splits), solo))
     own = [0, 1, 15, 16, 17, 255, 257, 1, 1100, 64, 300]
     n = len(own)
     _run([500] + own, [0] * n, [500] * n, list(range(1, n + 1)), own, hq, hkv, d, 16, dtype,
