@@ -12,6 +12,8 @@
 //
 // Bound by memory: every input is read once and every output written once; the
 // table's row is shared by all the heads of a token and stays in L1 / L2.
+#include <algorithm>
+
 #include "common.h"
 #include "../../include/moba_hip.h"
 
@@ -101,16 +103,31 @@ MOBA_DEV bool locate(const AppendArgs& a, uint32_t idx, int& unit, const uint16_
   return cell && angle;  // a token without its angle has neither key nor value written
 }
 
-template <int DT> MOBA_DEV void rotate(float x, float y, float2 t, float& xo, float& yo) {
-  xo = fmaf(x, t.x, -(y * t.y));
-  yo = fmaf(x, t.y, y * t.x);
+MOBA_DEV void rotate(float x, float y, float2 t, float& xo, float& yo) {
+  const float a = fmaf(x, t.x, -(y * t.y)), b = fmaf(x, t.y, y * t.x);
+  xo = a;
+  yo = b;
 }
 
-// Whole 16-byte pieces, two per unit, so that neighbouring lanes have
-// neighbouring pieces in each of the two accesses: unit u < R/16 turns the
-// pieces at 8u and 8u + R/2 (8 pairs of the two, or 4 pairs within each when
-// interleaved), unit R/16 + c copies the pieces c and c + n of the 2n behind R.
-template <int DT, bool INTER>
+// VEC 16-bit values of a row as one access (16, 8 or 4 bytes).
+template <int VEC> struct Piece {
+  typedef uint32_t words __attribute__((ext_vector_type(VEC / 2)));
+  words w;
+  MOBA_DEV void load(const uint16_t* p) { w = *reinterpret_cast<const words*>(p); }
+  MOBA_DEV void store(uint16_t* p) const { *reinterpret_cast<words*>(p) = w; }
+};
+template <> struct Piece<2> {
+  uint32_t w[1];
+  MOBA_DEV void load(const uint16_t* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
+  MOBA_DEV void store(uint16_t* p) const { *reinterpret_cast<uint32_t*>(p) = w[0]; }
+};
+
+// Whole pieces of VEC dims, two per unit, so that neighbouring lanes have
+// neighbouring pieces in each of the two accesses: unit u < R / 2 VEC turns the
+// pieces at VEC u and VEC u + R/2 (VEC pairs of the two, or VEC / 2 pairs within
+// each when interleaved), unit R / 2 VEC + c copies the pieces c and c + n of
+// the 2n behind R.
+template <int DT, bool INTER, int VEC>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   if (idx >= a.total) return;
@@ -119,38 +136,52 @@ __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   uint16_t* dst;
   const float2* turn;
   if (!locate(a, idx, u, src, dst, turn)) return;
-  const int turning = turn != nullptr ? a.R / 16 : 0, from = turning * 16;
+  const int turning = turn != nullptr ? a.R / (2 * VEC) : 0, from = turning * 2 * VEC;
+  Piece<VEC> x, y;
   if (u >= turning) {
-    const int n = (a.D - from + 15) / 16, d0 = from + 8 * (u - turning), d1 = d0 + 8 * n;
-    const u16x8_t x = ld8(src + d0), y = ld8(src + (d1 < a.D ? d1 : d0));
-    st8(dst + d0, x);
-    if (d1 < a.D) st8(dst + d1, y);
+    const int n = (a.D - from + 2 * VEC - 1) / (2 * VEC), d0 = from + VEC * (u - turning);
+    const int d1 = d0 + VEC * n;
+    x.load(src + d0);
+    y.load(src + (d1 < a.D ? d1 : d0));
+    x.store(dst + d0);
+    if (d1 < a.D) y.store(dst + d1);
     return;
   }
-  const int d0 = 8 * u, d1 = d0 + a.R / 2;
-  const u16x8_t x0 = ld8(src + d0), x1 = ld8(src + d1);
-  float2 t[8];
+  const int d0 = VEC * u, d1 = d0 + a.R / 2;
+  x.load(src + d0);
+  y.load(src + d1);
+  float2 t[VEC];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int first = !INTER ? d0 : i < 2 ? d0 / 2 : d1 / 2 - 4;  // pair of t[0]
-    const float4 w = reinterpret_cast<const float4*>(turn + first)[i];
-    t[2 * i] = make_float2(w.x, w.y);
-    t[2 * i + 1] = make_float2(w.z, w.w);
-  }
-  float y0[8], y1[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if constexpr (INTER) {
-      const u16x8_t& x = i < 4 ? x0 : x1;
-      float* y = i < 4 ? y0 : y1;
-      const int e = 2 * (i & 3);
-      rotate<DT>(to_f32<DT>(x[e]), to_f32<DT>(x[e + 1]), t[i], y[e], y[e + 1]);
+  for (int i = 0; i < VEC; i += 2) {  // two pairs an access, as the table has them
+    const int pair = !INTER ? d0 + i : i < VEC / 2 ? d0 / 2 + i : d1 / 2 + i - VEC / 2;
+    if constexpr (INTER && VEC == 2) {
+      t[0] = turn[d0 / 2];
+      t[1] = turn[d1 / 2];
     } else {
-      rotate<DT>(to_f32<DT>(x0[i]), to_f32<DT>(x1[i]), t[i], y0[i], y1[i]);
+      const float4 w = *reinterpret_cast<const float4*>(turn + pair);
+      t[i] = make_float2(w.x, w.y);
+      t[i + 1] = make_float2(w.z, w.w);
     }
   }
-  st8(dst + d0, pack8<DT>(y0));
-  st8(dst + d1, pack8<DT>(y1));
+  float v[2 * VEC];
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) {
+    unpack2<DT>(x.w[i], v[2 * i], v[2 * i + 1]);
+    unpack2<DT>(y.w[i], v[VEC + 2 * i], v[VEC + 2 * i + 1]);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    float& p = INTER ? v[2 * i] : v[i];
+    float& q = INTER ? v[2 * i + 1] : v[VEC + i];
+    rotate(p, q, t[i], p, q);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) {
+    x.w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+    y.w[i] = pack2<DT>(v[VEC + 2 * i], v[VEC + 2 * i + 1]);
+  }
+  x.store(dst + d0);
+  y.store(dst + d1);
 }
 
 // Any even R: unit u writes dims VEC u .. VEC u + VEC - 1, and reads the
@@ -184,7 +215,7 @@ __global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a, int inter
       const float2 t = turn[inter ? de >> 1 : (second ? de - half : de)];
       const float mine = to_f32<DT>(x[e]), theirs = to_f32<DT>(src[other]);
       float lo, hi;
-      rotate<DT>(second ? theirs : mine, second ? mine : theirs, t, lo, hi);
+      rotate(second ? theirs : mine, second ? mine : theirs, t, lo, hi);
       x[e] = from_f32<DT>(second ? hi : lo);
     }
   }
@@ -198,26 +229,35 @@ __global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a, int inter
   }
 }
 
+// Widest access that every row allows: 8, 4, 2 or 1 dims.
+int row_access(const void* p, int64_t ts, int64_t hs, int D) {
+  const uint64_t bits = ((uint64_t)(uintptr_t)p >> 1) | (uint64_t)ts | (uint64_t)hs | (uint64_t)D;
+  return ((uintptr_t)p & 1) ? 1 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+}
+
+template <int DT, int VEC> void launch_pairs(AppendArgs& a, int interleaved, hipStream_t st) {
+  const dim3 grid((a.total + 255) / 256), block(256);
+  if (interleaved) hipLaunchKernelGGL((append_pairs_kernel<DT, true, VEC>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((append_pairs_kernel<DT, false, VEC>), grid, block, 0, st, a);
+}
+
+// access: of the rows.  Pairs in whole pieces where R / 2 dims are whole pieces
+// too; else each dim finds its partner.
 template <int DT>
-void launch_append(AppendArgs& a, int interleaved, bool vec, hipStream_t st) {
-  const bool pairs = vec && a.R % 16 == 0;
-  a.units = pairs ? (a.D + 15) / 16 : vec ? a.D / 8 : a.D;
+void launch_append(AppendArgs& a, int interleaved, int access, hipStream_t st) {
+  int vec = access;
+  while (vec > 1 && a.R % (2 * vec)) vec /= 2;
+  const bool pairs = vec > 1;
+  a.units = pairs ? (a.D + 2 * vec - 1) / (2 * vec) : access == 8 ? a.D / 8 : a.D;
   a.by_head = fast_div(a.units);
   a.by_token = fast_div((a.Hq + 2 * a.Hkv) * a.units);
   a.total = (uint32_t)a.N * a.by_token.d;
   const dim3 grid((a.total + 255) / 256), block(256);
-  if (pairs && interleaved)
-    hipLaunchKernelGGL((append_pairs_kernel<DT, true>), grid, block, 0, st, a);
-  else if (pairs)
-    hipLaunchKernelGGL((append_pairs_kernel<DT, false>), grid, block, 0, st, a);
-  else if (vec)
-    hipLaunchKernelGGL((append_any_kernel<DT, 8>), grid, block, 0, st, a, interleaved);
-  else
-    hipLaunchKernelGGL((append_any_kernel<DT, 1>), grid, block, 0, st, a, interleaved);
-}
-
-bool whole_pieces(const void* p, int64_t ts, int64_t hs) {
-  return ((uintptr_t)p & 15) == 0 && ts % 8 == 0 && hs % 8 == 0;
+  if (vec == 8) launch_pairs<DT, 8>(a, interleaved, st);
+  else if (vec == 4) launch_pairs<DT, 4>(a, interleaved, st);
+  else if (vec == 2) launch_pairs<DT, 2>(a, interleaved, st);
+  else if (access == 8) hipLaunchKernelGGL((append_any_kernel<DT, 8>), grid, block, 0, st, a, interleaved);
+  else hipLaunchKernelGGL((append_any_kernel<DT, 1>), grid, block, 0, st, a, interleaved);
 }
 
 }  // namespace
@@ -250,10 +290,12 @@ extern "C" int moba_hip_append_rotary(const void* q, int64_t q_token_stride, int
   a.table = table; a.B = B; a.W = table_width;
   a.seq = token_seq; a.pos = token_pos; a.offsets = offsets;
   a.q_out = (uint16_t*)q_out; a.status = status;
-  const bool vec = D % 8 == 0 && (Hq == 0 || (whole_pieces(q, a.q_ts, a.q_hs) && whole_pieces(q_out, 0, 0))) &&
-                   whole_pieces(k, a.k_ts, a.k_hs) && whole_pieces(v, a.v_ts, a.v_hs) &&
-                   whole_pieces(k_cache, 0, 0) && whole_pieces(v_cache, 0, 0);
-  if (dtype == 0) launch_append<0>(a, interleaved, vec, (hipStream_t)stream);
-  else launch_append<1>(a, interleaved, vec, (hipStream_t)stream);
+  int access = row_access(k, a.k_ts, a.k_hs, D);
+  access = std::min(access, row_access(v, a.v_ts, a.v_hs, D));
+  access = std::min(access, row_access(k_cache, 0, 0, D));
+  access = std::min(access, row_access(v_cache, 0, 0, D));
+  if (Hq > 0) access = std::min({access, row_access(q, a.q_ts, a.q_hs, D), row_access(q_out, 0, 0, D)});
+  if (dtype == 0) launch_append<0>(a, interleaved, access, (hipStream_t)stream);
+  else launch_append<1>(a, interleaved, access, (hipStream_t)stream);
   return moba_launch_status("append_rotary");
 }

@@ -99,7 +99,7 @@ def _check(st, got_q, dtype, live=None):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("hq,hkv,d,rotary", [
     (12, 2, 128, 128), (16, 1, 96, 96), (14, 2, 64, 64), (4, 4, 256, 64), (3, 1, 40, 40),
-    (4, 2, 40, 10), (2, 2, 64, 2), (6, 3, 72, 36), (1, 1, 8, 8), (5, 1, 24, 16), (3, 3, 20, 6),
+    (4, 2, 40, 10), (2, 2, 64, 2), (6, 3, 72, 36), (1, 1, 8, 8), (5, 1, 24, 16), (3, 3, 20, 6), (2, 1, 96, 24), (3, 1, 80, 20),
     (2, 1, 7, 4)])
 def test_append_matches_fp64(cuda_device, hq, hkv, d, rotary, interleaved, dtype):
     st = _case([1, 37, 5, 64], hq, hkv, d, rotary, 16, dtype, interleaved=interleaved, seed=d)
@@ -123,15 +123,16 @@ def test_append_without_queries_offsets_and_own_output(cuda_device):
     _check(st, out, torch.bfloat16)
 
 
-def test_misaligned_views(cuda_device):
-    """Rows that are not whole 16-byte pieces: an odd token stride, an odd
-    start."""
-    st = _case([50], 2, 1, 64, 64, 16, torch.float16)
-    n = 50
-    wide = torch.randn(n, 4 * 64 + 3, device="cuda").half()
-    st["q"] = wide[:, 1:129].unflatten(1, (2, 64))
-    st["k"] = wide[:, 129:193].unflatten(1, (1, 64))
-    st["v"] = wide[:, 195:259].unflatten(1, (1, 64))
+@pytest.mark.parametrize("rotary,interleaved", [(64, False), (64, True), (24, False), (20, True), (6, False)])
+@pytest.mark.parametrize("start,pad", [(1, 3), (2, 2), (4, 4), (8, 4), (2, 8)])
+def test_misaligned_views(cuda_device, start, pad, rotary, interleaved):
+    """Rows that are whole pieces of 8, 4 and 2 bytes only: odd starts and
+    token strides."""
+    st = _case([50], 2, 1, 64, rotary, 16, torch.float16, interleaved=interleaved)
+    wide = torch.randn(50, 4 * 64 + start + pad, device="cuda").half()
+    st["q"] = wide[:, start:start + 128].unflatten(1, (2, 64))
+    st["k"] = wide[:, start + 128:start + 192].unflatten(1, (1, 64))
+    st["v"] = wide[:, start + 192:start + 256].unflatten(1, (1, 64))
     _check(st, _run(st), torch.float16)
 
 
