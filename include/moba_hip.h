@@ -400,9 +400,10 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
  * kv head; range | ranges << 16; tokens of the segment or -1: the rows' own
  * lengths; the row of all the pairs or -1: several), rows (the segments' query
  * rows), row_parts [3][Nq] (each row's first partial of its prefix and of its
- * own tokens, its ranges in all; max_parts bounds the last).  Every range of every
- * (row, head) belongs to exactly one item; a row's partials are those of its
- * prefix, then its own.  Prefix tokens must fit the table
+ * own tokens, its ranges in all; max_parts bounds the last).  uneven: several rows
+ * of one own slot may have unlike lengths; values behind a row's length that are
+ * not finite then do not reach it.  Every range of every (row, head) belongs to
+ * exactly one item; a row's partials are those of its prefix, then its own.  Prefix tokens must fit the table
  * (table_width * page_size).  Workspaces part_o [parts*Hq, D] and part_ml
  * [parts*Hq, 2] fp32, parts = sum of all ranges.  out [Nq,Hq,D] (dtype),
  * lse [Nq,Hq] fp32 natural log; nothing attended: zeros and -inf.  A token in
@@ -413,7 +414,7 @@ int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv,
                               int num_pages, int page_size, const int* table, int table_width,
                               const int* own_lengths, int length_add, int max_length, const int* items,
                               int n_items, const int* rows, const int* row_parts, int max_parts,
-                              float* part_o, float* part_ml, void* out, float* lse,
+                              int uneven, float* part_o, float* part_ml, void* out, float* lse,
                               void* stream);
 
 /* ------------------------------------------------ host page pool (CPU only)

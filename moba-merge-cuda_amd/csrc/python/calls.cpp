@@ -186,7 +186,7 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
 // The numbers of a plan, as SharedPrefixPlan packs them.
 struct Plan {
   int64_t rows, hq, hkv, d, max_slot, max_prefix, max_suffix, n_items, rows_at, parts_at, parts,
-      max_parts;
+      max_parts, uneven;
 };
 
 // shared_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan, scale,
@@ -228,8 +228,8 @@ PyObject* shared_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
       q->data_ptr(), p.code, (int)x.rows, (int)x.hq, (int)x.hkv, (int)x.d, (float)scale, p.k, p.v,
       (int)p.pages, (int)p.page, (const int*)table->data_ptr(), (int)p.width,
       (const int*)own->data_ptr(), 0, (int)std::min(x.max_suffix, p.width * p.page), (const int*)m,
-      (int)x.n_items, (const int*)(m + x.rows_at), (const int*)(m + x.parts_at), (int)x.max_parts, w,
-      w + parts * x.d, out.data_ptr(), (float*)lse.data_ptr(), stream);
+      (int)x.n_items, (const int*)(m + x.rows_at), (const int*)(m + x.parts_at), (int)x.max_parts,
+      (int)x.uneven, w, w + parts * x.d, out.data_ptr(), (float*)lse.data_ptr(), stream);
   if (rc) return failed("moba_hip_shared_attention", rc);
   THPObjectPtr po(THPVariable_Wrap(std::move(out))), pl(THPVariable_Wrap(std::move(lse)));
   return po && pl ? PyTuple_Pack(2, po.get(), pl.get()) : nullptr;

@@ -292,6 +292,92 @@ template <int DP> MOBA_DEV uint32_t block_byte(uint32_t lane, uint32_t row0) {
   return ((lane % NB) ^ (f & NBM)) * 16;
 }
 
+// A weight of 0 times an infinite or NaN value is NaN, which a row must not get
+// from a key behind its own length that another row of the block attends.  In
+// tiles with such keys, values that are not finite are replaced by zeros; where
+// that happened, the tiles are read again after the others, and every row gets
+// what it attends of them: +inf or -inf if there is only the one, else NaN.
+// Only kernels of plans where several rows have one own slot (UNEVEN) do this: it
+// takes registers and branches from all their items (64 rows behind 32K tokens:
+// 114 us without, 123 with).
+//
+// 0xffff for each of a word's two values that is not finite; for each that has
+// no mantissa bits (no carries: a half's bits plus 0x7fff stay below 2^16).
+MOBA_DEV uint32_t zero_halves(uint32_t w) {
+  const uint32_t z = ~(w + 0x7fff7fffu) & 0x80008000u;
+  return z | (z - (z >> 15));
+}
+template <int DT> MOBA_DEV uint32_t not_finite(uint32_t w) {
+  return zero_halves(~w & (DT == 0 ? 0x7f807f80u : 0x7c007c00u));
+}
+template <int DT> MOBA_DEV uint32_t no_mantissa(uint32_t w) {
+  return zero_halves(w & (DT == 0 ? 0x007f007fu : 0x03ff03ffu));
+}
+// Zeros in the place of what is not finite in the wave's share (from thread
+// `thread` of WIDTH) of a tile of N values; whether there was any.
+template <int DT, int N, int WIDTH> MOBA_DEV bool odd_in(uint16_t* V, int thread) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < N / (8 * WIDTH); ++i) {
+    u32x4_t* at = reinterpret_cast<u32x4_t*>(V) + i * WIDTH + thread;
+    u32x4_t v = *at;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t b = not_finite<DT>(v[k]);
+      bad |= b;
+      v[k] &= ~b;
+    }
+    *at = v;
+  }
+  return __any(bad != 0);
+}
+// o += what is not finite among the values of a tile of NG groups of 16 keys,
+// for the lane's row, which attends the keys before `left`.
+template <int DT, int DP, int NDB, int NG>
+MOBA_DEV void add_odd(const uint16_t* V, int lane, int left, const uint32_t* tok, f32x16_t (&o)[NDB]) {
+  constexpr uint32_t one = DT == 0 ? 0x3f803f80u : 0x3c003c00u;
+  const int hh = lane >> 5;
+  u32x4_t on[NG];  // 1 for the keys that the row attends, laid out as weights
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = g * 16 + 8 * j + 4 * hh;
+      const u32x4_t t = *reinterpret_cast<const u32x4_t*>(tok + k);
+      uint32_t m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = (k + i < left) & (t[i] != kNowhere) ? one : 0;
+      on[g][2 * j] = (m[0] & 0xffffu) | (m[1] << 16);
+      on[g][2 * j + 1] = (m[2] & 0xffffu) | (m[3] << 16);
+    }
+  const uint32_t t0 = swz_tr_base<DP>(lane, 0), t1 = swz_tr_base<DP>(lane, 1);
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) {
+    f32x16_t odd = zero16(), sign = zero16();
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t ro = g * 16 * DP * 2;
+      const u32x4_t v = __builtin_bit_cast(
+          u32x4_t, lds_tr8(V, ro + swz_tr<DP>(opaque(t0), db), ro + swz_tr<DP>(opaque(t1), db)));
+      u32x4_t c, s;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t bad = not_finite<DT>(v[k]);
+        c[k] = bad & one;
+        s[k] = bad & no_mantissa<DT>(v[k]) & ((v[k] & 0x80008000u) | one);
+      }
+      odd = mfma32<DT>(__builtin_bit_cast(u16x8_t, c), __builtin_bit_cast(u16x8_t, on[g]), odd);
+      sign = mfma32<DT>(__builtin_bit_cast(u16x8_t, s), __builtin_bit_cast(u16x8_t, on[g]), sign);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float bad = fabsf(sign[r]) == odd[r] ? copysignf(INFINITY, sign[r]) : NAN;
+      o[db][r] += odd[r] != 0.0f ? bad : 0.0f;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // a block at a time
+  }
+}
+
 template <int NKS> MOBA_DEV void load_query(const SharedArgs& a, const Pair& p, int hh, u16x8_t (&qf)[NKS]) {
   const uint16_t* q = a.q + ((int64_t)p.row * a.Hq + p.h) * a.D;
 #pragma unroll
@@ -305,7 +391,7 @@ template <int NKS> MOBA_DEV void load_query(const SharedArgs& a, const Pair& p, 
 // More than 32 pairs: every wave has 32 of them, and the four share tiles of
 // KEYS keys in STAGES LDS stages: while one is in use, the loads of the others are
 // in flight.
-template <int DT, int ND, bool NEAR>
+template <int DT, int ND, bool NEAR, bool UNEVEN>
 MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
   constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, KEYS = C::KEYS, NKB = KEYS / 32;
@@ -319,13 +405,20 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
 
   const int alike = alike_of(a, x);
   const Pair p = pair_of(a, x, wave * 32 + qi, alike);
-  int length = alike;
-  if (length < 0) {  // the block's longest row
+  int length = alike, block_least = 0x7fffffff;
+  if (length < 0) {  // the block's longest and shortest row
     const int mine = longest(p.limit);
     if (lane == 0) flags[wave] = mine;
     lds_barrier();
     length = max(max(flags[0], flags[1]), max(flags[2], flags[3]));
     lds_barrier();
+    if constexpr (UNEVEN) {
+      const int least = shortest(p, alike);
+      if (lane == 0) flags[wave] = least;
+      lds_barrier();
+      block_least = min(min(flags[0], flags[1]), min(flags[2], flags[3]));
+      lds_barrier();
+    }
   }
   int lo, hi;
   range_of(x, length, lo, hi);
@@ -401,17 +494,22 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     wave_prio<0>();
   };
 
+  // Looks up the keys from k0 on; returns whether a page of theirs is unmapped.
+  auto chunk = [&](int k0) {
+    const bool mine = look_up<NEAR, C::CAP, 256>(a, rows, x.slot, k0, hi, first, tid, tok);
+    if (lane == 0) flags[wave] = mine;
+    lds_barrier();
+    landed<0>();  // what the compiler has in flight: it must not wait for it below
+    return any_hole(flags);
+  };
+  bool odd = false;
   for (int k0 = lo; k0 < hi; k0 += C::CAP) {
     if (k0 > lo) {
       lds_barrier();  // the tokens and tiles before are read
       first = entry_of(a, x.slot, k0 + tid, hi);
     }
-    const bool mine = look_up<NEAR, C::CAP, 256>(a, rows, x.slot, k0, hi, first, tid, tok);
-    if (lane == 0) flags[wave] = mine;
-    lds_barrier();
-    const bool holes = any_hole(flags);
+    const bool holes = chunk(k0);
     const int ntiles = (min(hi - k0, C::CAP) + KEYS - 1) / KEYS;
-    landed<0>();  // what the compiler has in flight: it must not wait for it below
     // the loads of a tile: 2 NDMA, issued STAGES - 1 tiles ahead
     auto step = [&](auto stage, int it) {
       constexpr int S = decltype(stage)::value;
@@ -422,7 +520,13 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
         dma(std::integral_constant<int, (S + STAGES - 1) % STAGES>{});
         places(min(it + STAGES, ntiles - 1));
       }
-      if (!idle) tile(stage, it, k0 + it * KEYS, holes);
+      const int kt0 = k0 + it * KEYS;
+      if constexpr (UNEVEN)
+        if (kt0 + KEYS > block_least) {  // rows of unlike lengths end in this tile
+          odd |= odd_in<DT, TILE, 256>(Ks + (STAGES + S) * TILE, tid);
+          lds_barrier();
+        }
+      if (!idle) tile(stage, it, kt0, holes);
     };
     places(0);
     dma(std::integral_constant<int, 0>{});
@@ -438,6 +542,30 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
         if (it + 2 < ntiles) step(std::integral_constant<int, 2>{}, it + 2);
     }
   }
+  if (UNEVEN && alike < 0) {
+    lds_barrier();
+    if (lane == 0) flags[wave] = odd;
+    lds_barrier();
+    if (any_hole(flags)) [[unlikely]] {
+      for (int k0 = lo; k0 < hi; k0 += C::CAP) {
+        if (k0 + C::CAP <= block_least) continue;
+        lds_barrier();
+        first = entry_of(a, x.slot, k0 + tid, hi);
+        chunk(k0);
+        for (int it = 0; it * KEYS < min(hi - k0, C::CAP); ++it) {
+          if (k0 + (it + 1) * KEYS <= block_least) continue;
+          places(it);
+          dma(std::integral_constant<int, 0>{});
+          landed<0>();
+          lds_barrier();
+          if (!idle)
+            add_odd<DT, DP, NDB, KEYS / 16>(Ks + STAGES * TILE, lane, min(p.limit, hi) - k0 - it * KEYS,
+                                            tok + it * KEYS, oacc);
+          lds_barrier();
+        }
+      }
+    }
+  }
   const float l = run.l + __shfl_xor(run.l, 32, 64);
   if (p.valid) store_partial<NDB>(a, p.part, oacc, run.m, l, hh);
 }
@@ -448,7 +576,7 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
 // group's K is in flight from the scores on, its V from the product with V on.
 // 16-key groups fill half of a 32-row score product; what a narrow item waits
 // for is memory.  SOLO: x is this wave's alone, and it takes every group.
-template <int DT, int ND, bool NEAR, bool SOLO>
+template <int DT, int ND, bool NEAR, bool UNEVEN, bool SOLO>
 MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
   constexpr int DP = C::DP, NKS = C::NKS, NDB = C::NDB, NB = C::NB, OWN = C::OWN;
@@ -498,11 +626,7 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
         rows.template bring<decltype(v)::value>(at, byte, lds0 + decltype(v)::value * (OWN * DP * 2) + n * 1024);
     }
   };
-  for (int k0 = lo; k0 < hi; k0 += CAP) {
-    if (k0 > lo) {
-      if constexpr (!SOLO) lds_barrier();  // the tokens before are read
-      first = entry_of(a, x.slot, k0 + thread, hi);
-    }
+  auto chunk = [&](int k0) {
     bool holes = look_up<NEAR, CAP, SOLO ? 64 : 256>(a, rows, x.slot, k0, hi, first, thread, tok);
     if constexpr (SOLO) {
       wave_lds_sync();
@@ -511,8 +635,17 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       lds_barrier();
       holes = any_hole(flags);
     }
-    const int ntiles = (min(hi - k0, CAP) + OWN - 1) / OWN;
     landed<0>();  // what the compiler has in flight: it must not wait for it below
+    return holes;
+  };
+  bool odd = false;
+  for (int k0 = lo; k0 < hi; k0 += CAP) {
+    if (k0 > lo) {
+      if constexpr (!SOLO) lds_barrier();  // the tokens before are read
+      first = entry_of(a, x.slot, k0 + thread, hi);
+    }
+    const bool holes = chunk(k0);
+    const int ntiles = (min(hi - k0, CAP) + OWN - 1) / OWN;
     if (begin < ntiles) {
       bring(begin, std::false_type{});
       bring(begin, std::true_type{});
@@ -527,11 +660,16 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       lds_read_done();
       if (more) bring(it + STEP, std::false_type{});
       const int kt0 = k0 + it * OWN;
+      const bool ends = UNEVEN && alike < 0 && kt0 + OWN > wlim;  // rows of unlike lengths
       if (kt0 + OWN > wlim || holes)
         mask_scores<1, NR>(s, (int)opaque(min(p.limit, hi) - kt0), tok + it * OWN, hh);
       u16x8_t pv[1][NR / 8];
       softmax_step<DT, 1, NR, NDB>(s, a.scale_log2, run, oacc, pv);
       if (more) landed<NDMA>(); else landed<0>();  // V; the next K may be on its way
+      if (ends) {
+        odd |= odd_in<DT, OWN * DP, 64>(Vt, lane);
+        wave_lds_sync();
+      }
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -543,6 +681,28 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
       lds_read_done();
       if (more) bring(it + STEP, std::true_type{});
     }
+  }
+  if (UNEVEN && alike < 0) {
+    if constexpr (!SOLO) {
+      lds_barrier();
+      if (lane == 0) flags[wave] = odd;
+      lds_barrier();
+      odd = any_hole(flags);
+    }
+    if (odd) [[unlikely]]
+      for (int k0 = lo; k0 < hi; k0 += CAP) {
+        if (k0 + CAP <= wlim) continue;
+        if constexpr (!SOLO) lds_barrier();
+        first = entry_of(a, x.slot, k0 + thread, hi);
+        chunk(k0);
+        for (int it = begin; it * OWN < min(hi - k0, CAP); it += STEP) {
+          if (k0 + (it + 1) * OWN <= wlim) continue;
+          bring(it, std::true_type{});
+          landed<0>();
+          add_odd<DT, DP, NDB, OWN / 16>(Vt, lane, min(p.limit, hi) - k0 - it * OWN, tok + it * OWN, oacc);
+          lds_read_done();
+        }
+      }
   }
   float m_run = run.m, l = run.l + __shfl_xor(run.l, 32, 64);
   if constexpr (SOLO) {
@@ -608,20 +768,21 @@ MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   }
 }
 
-template <int DT, int ND, bool NEAR>
+template <int DT, int ND, bool NEAR, bool UNEVEN>
 __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[Dims<ND>::LDS];
   const Item x = a.items[blockIdx.x];
   if (x.n_m == 0) return;
-  if (a.D < ND) {  // dims behind D are never loaded: zeros
+  // Dims behind D are never loaded: zeros where they are multiplied, or looked at
+  if (a.D < ND || (UNEVEN && a.D < Dims<ND>::DP && x.length < 0)) {
     for (int i = threadIdx.x * 16; i < Dims<ND>::TILES; i += 4096) st8((uint16_t*)(smem + i), zero8());
     lds_barrier();
   }
   if (x.n_m < 0) {
     const Item own = a.items[x.row_at + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
-    if (own.n_m > 0) narrow_item<DT, ND, NEAR, true>(a, own, smem);
-  } else if (x.n_m <= 32) narrow_item<DT, ND, NEAR, false>(a, x, smem);
-  else wide_item<DT, ND, NEAR>(a, x, smem);
+    if (own.n_m > 0) narrow_item<DT, ND, NEAR, UNEVEN, true>(a, own, smem);
+  } else if (x.n_m <= 32) narrow_item<DT, ND, NEAR, UNEVEN, false>(a, x, smem);
+  else wide_item<DT, ND, NEAR, UNEVEN>(a, x, smem);
 }
 
 // Joins the ranges of each (row, head): PL threads per four dims, each with
@@ -706,13 +867,13 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
   if (d == 0) lse[rh] = z != 0.0f ? (M + log2f(z)) * kLn2 : -INFINITY;
 }
 
-template <int DT, bool NEAR> void launch_blocks(const SharedArgs& a, int n_items, hipStream_t st) {
+template <int DT, bool NEAR, bool UNEVEN> void launch_blocks(const SharedArgs& a, int n_items, hipStream_t st) {
   const dim3 grid(n_items), block(256);
-  if (a.D <= 64) hipLaunchKernelGGL((block_kernel<DT, 64, NEAR>), grid, block, 0, st, a);
-  else if (a.D <= 96) hipLaunchKernelGGL((block_kernel<DT, 96, NEAR>), grid, block, 0, st, a);
-  else if (a.D <= 128) hipLaunchKernelGGL((block_kernel<DT, 128, NEAR>), grid, block, 0, st, a);
-  else if (a.D <= 192) hipLaunchKernelGGL((block_kernel<DT, 192, NEAR>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((block_kernel<DT, 256, NEAR>), grid, block, 0, st, a);
+  if (a.D <= 64) hipLaunchKernelGGL((block_kernel<DT, 64, NEAR, UNEVEN>), grid, block, 0, st, a);
+  else if (a.D <= 96) hipLaunchKernelGGL((block_kernel<DT, 96, NEAR, UNEVEN>), grid, block, 0, st, a);
+  else if (a.D <= 128) hipLaunchKernelGGL((block_kernel<DT, 128, NEAR, UNEVEN>), grid, block, 0, st, a);
+  else if (a.D <= 192) hipLaunchKernelGGL((block_kernel<DT, 192, NEAR, UNEVEN>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((block_kernel<DT, 256, NEAR, UNEVEN>), grid, block, 0, st, a);
 }
 
 template <int DT>
@@ -738,7 +899,7 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
                                          int num_pages, int page_size, const int* table,
                                          int table_width, const int* own_lengths, int length_add, int max_length,
                                          const int* items, int n_items, const int* rows,
-                                         const int* row_parts, int max_parts, float* part_o, float* part_ml,
+                                         const int* row_parts, int max_parts, int uneven, float* part_o, float* part_ml,
                                          void* out, float* lse, void* stream) {
   if (dtype != 0 && dtype != 1) { moba_set_error("shared_attention: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
   if (D < 8 || D > 256 || D % 8) { moba_set_error("shared_attention: head_dim must be a multiple of 8 in [8,256]"); return MOBA_ERR_ARG; }
@@ -760,8 +921,10 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
   a.part_o = part_o; a.part_ml = (float2*)part_ml;
   hipStream_t st = (hipStream_t)stream;
   if (n_items > 0) {
-    if (a.pool_bytes) dtype == 0 ? launch_blocks<0, true>(a, n_items, st) : launch_blocks<1, true>(a, n_items, st);
-    else dtype == 0 ? launch_blocks<0, false>(a, n_items, st) : launch_blocks<1, false>(a, n_items, st);
+    // Pools above 4 GiB have the one kernel for all plans
+    if (!a.pool_bytes) dtype == 0 ? launch_blocks<0, false, true>(a, n_items, st) : launch_blocks<1, false, true>(a, n_items, st);
+    else if (uneven) dtype == 0 ? launch_blocks<0, true, true>(a, n_items, st) : launch_blocks<1, true, true>(a, n_items, st);
+    else dtype == 0 ? launch_blocks<0, true, false>(a, n_items, st) : launch_blocks<1, true, false>(a, n_items, st);
     const int rc = moba_launch_status("shared_attention(blocks)");
     if (rc) return rc;
   }

@@ -62,7 +62,7 @@ SIGNATURES = {
     "moba_hip_append_rotary": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _P, _I, _I, _I,
                                _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P],
     "moba_hip_shared_attention": [_P, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I,
-                                  _P, _P, _I, _P, _P, _P, _P, _P],
+                                  _P, _P, _I, _I, _P, _P, _P, _P, _P],
     # host page pool (CPU only)
     "moba_pool_create": [_I, _I, _I, _I, _I, _PP],
     "moba_pool_destroy": [_P],

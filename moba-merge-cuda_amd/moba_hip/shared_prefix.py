@@ -85,9 +85,9 @@ class SharedPrefixPlan:
         self.meta = torch.from_numpy(flat).to(device)
         self.device = self.meta.device
         # what a call needs of the plan, for the native host path
-        self._packed = struct.pack("12q", n, hq, hkv, d, self.max_slot, self.max_prefix, max_suffix,
+        self._packed = struct.pack("13q", n, hq, hkv, d, self.max_slot, self.max_prefix, max_suffix,
                                    self.n_items, self._rows_at, self._parts_at, self.parts,
-                                   self.max_parts)
+                                   self.max_parts, self.uneven)
 
     def _build(self, prefix, length, suffix):
         """The device arrays: work items, segments' rows, rows' partials."""
@@ -151,6 +151,7 @@ class SharedPrefixPlan:
 
         part_at = np.cumsum(n_prefix + n_suffix) - (n_prefix + n_suffix)
         self.parts = int((n_prefix + n_suffix).sum())
+        self.uneven = int(n_alone.max(initial=0) > 1)  # rows of one own slot, of any lengths
         self.max_parts = int((n_prefix + n_suffix).max())
         arrays = [items.ravel(), singles.ravel(), row_list, part_at, part_at + n_prefix,
                   n_prefix + n_suffix]
@@ -277,6 +278,6 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     _on_device(k_cache.get_device(), "moba_hip_shared_attention", qp, _DTYPES[q.dtype], n, hq, hkv,
                d, scale, kp, vp, pages, page, page_table.data_ptr(), width,
                suffix_lengths.data_ptr(), 0, min(plan.max_suffix, width * page), meta, plan.n_items,
-               meta + plan._rows_at, meta + plan._parts_at, plan.max_parts, wp, wp + 4 * parts * d,
-               out.data_ptr(), lse.data_ptr())
+               meta + plan._rows_at, meta + plan._parts_at, plan.max_parts, plan.uneven, wp,
+               wp + 4 * parts * d, out.data_ptr(), lse.data_ptr())
     return out, lse

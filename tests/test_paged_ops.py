@@ -168,6 +168,6 @@ def test_append_entry_refuses_before_any_device_work(change, text):
     (dict(max_length=-1), "max_length"), (dict(max_length=17), "max_length")])
 def test_attention_entry_refuses_before_any_device_work(change, text):
     base = dict(q=64, dtype=0, Nq=1, hq=2, hkv=2, D=64, scale=1.0, kc=64, vc=64, pages=1, page=16,
-                table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0, rows=64, parts=64, max_parts=1,
+                table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0, rows=64, parts=64, max_parts=1, uneven=0,
                 part_o=64, part_ml=64, out=64, lse=64, stream=None)
     _refused("moba_hip_shared_attention", base, change, text)

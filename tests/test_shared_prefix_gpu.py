@@ -219,6 +219,46 @@ def test_infinities_and_nan_stay_in_their_rows(cuda_device):
     assert torch.isnan(out[3]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,tokens,solo", [(4, 2, 128, 60, False), (8, 1, 96, 3, False),
+                                                  (8, 1, 96, 3, True), (2, 2, 64, 40, False),
+                                                  (4, 4, 40, 7, True), (2, 1, 256, 40, False)])
+def test_values_behind_a_row_do_not_reach_it(cuda_device, monkeypatch, hq, hkv, d, tokens, solo, dtype):
+    """Several query tokens of a sequence: an infinite or NaN value reaches the
+    rows at and behind its position, as the sum has it, and no row before."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    monkeypatch.setattr(SharedPrefixPlan, "_ranges",
+                        lambda self, blocks, *a: (np.full(len(blocks), 1), solo))
+    n = 1500
+    kc, vc, table, ks, vs = _pool([50, n], hkv, d, 16, dtype, 4)
+    rows = list(range(n - tokens, n))          # row r attends r + 1 tokens
+    q = torch.randn(tokens, hq, d, generator=torch.Generator().manual_seed(2)).to("cuda", dtype)
+    plan = SharedPrefixPlan([0] * tokens, [50] * tokens, [1] * tokens, hq, hkv, d, max_suffix=n)
+    own = torch.tensor([r + 1 for r in rows], dtype=torch.int32, device="cuda")
+    clean, clean_lse = shared_prefix_attention(q, kc, vc, table, own, plan)
+    inf, nan = float("inf"), float("nan")
+    odd = {n - 1: [(0, nan), (1, inf)], n - 2: [(1, -inf), (2, inf)]}
+    for at, values in odd.items():
+        for dim, x in values:
+            vc[int(table[1, at // 16]), at % 16, 0, dim] = x
+    out, lse = shared_prefix_attention(q, kc, vc, table, own, plan)
+    assert torch.equal(lse, clean_lse)
+    g = hq // hkv
+    want = clean.clone()
+    want[tokens - 2:, :g, 1:3] = torch.tensor([-inf, inf], device="cuda", dtype=dtype)
+    want[tokens - 1, :g, :2] = nan             # NaN alone; -inf and inf together
+    assert torch.equal(torch.nan_to_num(out, nan=123.0), torch.nan_to_num(want, nan=123.0))
+
+
+def test_plan_of_nothing_runs(cuda_device):
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    kc, vc, table, _, _ = _pool([20], 1, 64, 16, torch.bfloat16, 1)
+    plan = SharedPrefixPlan([-1, -1], [0, 0], [-1, -1], 2, 1, 64, max_suffix=5)
+    out, lse = shared_prefix_attention(torch.ones(2, 2, 64, device="cuda").bfloat16(), kc, vc, table,
+                                       torch.tensor([3, 4], dtype=torch.int32, device="cuda"), plan)
+    assert (out == 0).all() and (lse == float("-inf")).all()
+
+
 def test_far_cells(cuda_device):
     """Pages behind 2^31 elements of the pool."""
     from moba_hip import SharedPrefixPlan, shared_prefix_attention
