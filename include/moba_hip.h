@@ -403,10 +403,10 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
  * own tokens, its ranges in all; max_parts bounds the last).  uneven: several rows
  * of one own slot may have unlike lengths; values behind a row's length that are
  * not finite then do not reach it.  Every range of every (row, head) belongs to
- * exactly one item; a row's partials are those of its prefix, then its own.  Prefix tokens must fit the table
- * (table_width * page_size).  Workspaces part_o [parts*Hq, D] and part_ml
- * [parts*Hq, 2] fp32, parts = sum of all ranges.  out [Nq,Hq,D] (dtype),
- * lse [Nq,Hq] fp32 natural log; nothing attended: zeros and -inf.  A token in
+ * exactly one item; a row's partials are those of its prefix, then its own.
+ * Prefix tokens must fit the table (table_width * page_size); no length passes
+ * 2^30.  Workspaces part_o [parts*Hq, D] and part_ml [parts*Hq, 2] fp32, parts =
+ * sum of all ranges.  out [Nq,Hq,D] (dtype), lse [Nq,Hq] fp32 natural log; nothing attended: zeros and -inf.  A token in
  * an unmapped page is not attended.  q, k_cache, v_cache, out: 16-byte
  * aligned.  Two launches; results do not depend on timing. */
 int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,

@@ -907,7 +907,9 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
   if (!(scale > 0.0f) || scale > 1e30f) { moba_set_error("shared_attention: scale must be positive and finite"); return MOBA_ERR_ARG; }
   if (num_pages < 1 || page_size < 1 || table_width < 1 || (int64_t)num_pages * page_size >= 1ll << 31 ||
       (int64_t)table_width * page_size >= 1ll << 31) { moba_set_error("shared_attention: nonempty page pool and table below 2^31 tokens required"); return MOBA_ERR_ARG; }
-  if (n_items < 0 || max_length < 0 || max_length > table_width * page_size) { moba_set_error("shared_attention: max_length must fit the page table"); return MOBA_ERR_ARG; }
+  if ((int64_t)Hkv * D >= 1ll << 30) { moba_set_error("shared_attention: Hkv * D below 2^30 required"); return MOBA_ERR_ARG; }
+  // (at most 2^30: a group of keys behind the last still counts in 32 bits)
+  if (n_items < 0 || max_length < 0 || max_length > table_width * page_size || max_length > 1 << 30) { moba_set_error("shared_attention: max_length must be at most 2^30 and fit the page table"); return MOBA_ERR_ARG; }
   SharedArgs a;
   a.q = (const uint16_t*)q; a.kc = (const uint16_t*)k_cache; a.vc = (const uint16_t*)v_cache;
   a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.G = Hq / Hkv;

@@ -64,8 +64,8 @@ class SharedPrefixPlan:
         if d % 8 or d > 256:
             raise ValueError("head_dim must be a multiple of 8 in [8,256]")
         if isinstance(max_suffix, bool) or not isinstance(max_suffix, int) or \
-                not 0 <= max_suffix < 2 ** 31:
-            raise ValueError("max_suffix must be a length")
+                not 0 <= max_suffix <= 2 ** 30:
+            raise ValueError("max_suffix must be a length, at most 2^30")
         prefix = _slots(prefix_ids, "prefix_ids")
         n = len(prefix)
         if n < 1:
@@ -74,6 +74,8 @@ class SharedPrefixPlan:
         suffix = _slots(suffix_ids, "suffix_ids", n)
         if length.min() < 0 or (length[prefix < 0] != 0).any():
             raise ValueError("prefix_lengths must be 0 or more, and 0 without a prefix")
+        if length.max() > 2 ** 30:
+            raise ValueError("prefix_lengths must be at most 2^30")
         if n * hq >= 2 ** 31:
             raise ValueError("query grid exceeds int32 capacity")
         self.rows, self.num_q_heads, self.num_kv_heads, self.head_dim = n, hq, hkv, d

@@ -119,7 +119,8 @@ def test_plan_of_nothing():
     dict(prefix_ids=[]), dict(prefix_ids=[0.5]), dict(prefix_ids=[-2]), dict(prefix_lengths=[1, 2]),
     dict(prefix_lengths=[-1]), dict(prefix_ids=[-1]), dict(suffix_ids=[[0]]), dict(num_q_heads=3),
     dict(num_kv_heads=0), dict(head_dim=60), dict(head_dim=264), dict(max_suffix=-1),
-    dict(max_suffix=True), dict(max_suffix=2 ** 31), dict(suffix_ids=[2 ** 31])])
+    dict(max_suffix=True), dict(max_suffix=2 ** 31), dict(max_suffix=2 ** 30 + 1),
+    dict(prefix_lengths=[2 ** 30 + 1]), dict(suffix_ids=[2 ** 31])])
 def test_plan_refusals(kw):
     base = dict(prefix_ids=[0], prefix_lengths=[5], suffix_ids=[1], num_q_heads=4, num_kv_heads=2,
                 head_dim=64, max_suffix=8, device="cpu")
@@ -165,9 +166,12 @@ def test_append_entry_refuses_before_any_device_work(change, text):
     (dict(Nq=0), "Nq"), (dict(hq=3), "multiple of Hkv"), (dict(Nq=1 << 30, hq=8), "Nq"),
     (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(pages=1 << 28), "pool"), (dict(page=0), "pool"), (dict(width=1 << 28), "pool"),
-    (dict(max_length=-1), "max_length"), (dict(max_length=17), "max_length")])
+    (dict(max_length=-1), "max_length"), (dict(max_length=17), "max_length"),
+    (dict(max_length=(1 << 30) + 1, width=(1 << 27) - 1), "max_length"), (dict(hq=1 << 24, hkv=1 << 24), "Hkv")])
 def test_attention_entry_refuses_before_any_device_work(change, text):
     base = dict(q=64, dtype=0, Nq=1, hq=2, hkv=2, D=64, scale=1.0, kc=64, vc=64, pages=1, page=16,
-                table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0, rows=64, parts=64, max_parts=1, uneven=0,
+                table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0,
+                rows=64, parts=64, max_parts=1,
+                uneven=0,
                 part_o=64, part_ml=64, out=64, lse=64, stream=None)
     _refused("moba_hip_shared_attention", base, change, text)
