@@ -102,7 +102,8 @@ class PreparedSharedDecode(PreparedDecode):
         calls.append(("moba_hip_shared_attention", (
             ptr(self._turned), code, rows, hq, hkv, d, d ** -0.5, kc, vc, pages, page, table, width,
             pos, 1, self.max_length, meta, plan.n_items, meta + plan._rows_at, meta + plan._parts_at,
-            plan.max_parts, plan.uneven, work, work + 4 * plan.parts * hq * d, ptr(self.output), ptr(self.lse))))
+            plan.max_parts, plan.uneven, work, work + 4 * plan.parts * hq * d, ptr(self.output),
+            ptr(self.lse))))
         return calls
 
     # parts of a step, as PreparedDecode has them for whole-model steps

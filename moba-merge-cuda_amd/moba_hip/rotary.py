@@ -31,6 +31,8 @@ class RotaryTable:
                  interleaved=False, device="cuda"):
         self._shape(positive_int(rotary_dim, "rotary_dim"), interleaved)
         n = positive_int(max_positions, "max_positions")
+        if n >= 2 ** 31:
+            raise ValueError("max_positions exceeds int32 capacity")
         half = self.rotary_dim // 2
         if inv_freq is None:
             inv = float(base) ** (-torch.arange(half, dtype=torch.float64, device=device) / half)
@@ -47,7 +49,8 @@ class RotaryTable:
         rotary_dim / 2]."""
         ok = all(isinstance(t, torch.Tensor) and t.dim() == 2 and t.is_floating_point()
                  for t in (cos, sin))
-        if not ok or cos.shape != sin.shape or cos.device != sin.device or not cos.numel():
+        if not ok or cos.shape != sin.shape or cos.device != sin.device or not cos.numel() or \
+                cos.shape[0] >= 2 ** 31:
             raise ValueError("cos and sin must be alike, nonempty [positions, rotary_dim / 2]")
         self = cls.__new__(cls)
         self._shape(2 * cos.shape[1], interleaved)
@@ -62,7 +65,7 @@ class RotaryTable:
         self.rotary_dim, self.interleaved = rotary_dim, interleaved
 
     def _store(self, cos, sin):
-        self.cos_sin = torch.stack((cos, sin), dim=-1).to(torch.float32).contiguous()
+        self.cos_sin = torch.stack((cos, sin), dim=-1).detach().to(torch.float32).contiguous()
         self.max_positions = self.cos_sin.shape[0]
 
     @property
@@ -168,9 +171,11 @@ def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
 
     A token of slot -1 is padding: nothing of it is written.  A token outside
     the table, in an unmapped page or past the rotary table has no key and
-    value written either; with ``check`` such tokens, and two tokens of one
-    cell, raise RuntimeError after the launch (one device-to-host copy).
-    Without it, two tokens of one cell leave either's data."""
+    value written either, nor, past the rotary table, its query; with ``check`` such
+    tokens, and two tokens of one slot and position, raise RuntimeError after the
+    launch (one device-to-host copy).  Without it, two tokens of one cell leave
+    either's data.  A tensor of the call, the table's too, that is used on
+    another stream than its own must be kept until that work is done."""
     if not check:
         done = _lib.calls().append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos,
                                           rotary, q, q_out, offsets)

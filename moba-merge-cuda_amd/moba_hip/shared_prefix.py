@@ -16,7 +16,7 @@ import torch
 
 from .cache_layout import positive_int
 from .ops import _lib
-from .rotary import _DTYPES, _check_index, _check_pool, _on_device
+from .rotary import _DTYPES, _check_index, _check_pool, _meet, _on_device, _span
 
 # (row, q head of a kv head) pairs of a work item: its four waves have 32 each,
 # or the same 32 and a quarter of the keys each (solo: a wave has an item's 32
@@ -52,7 +52,9 @@ class SharedPrefixPlan:
     tokens of page-table row ``suffix_id`` (-1: none).  Rows of one
     (prefix_id, prefix_length) are served together, and so are rows of one
     suffix_id (several query tokens of a sequence, each with its own length).
-    ``max_suffix`` bounds the own lengths (longer ones are cut to it).
+    ``max_suffix`` bounds the own lengths (longer ones are cut to it).  A plan
+    used on a stream other than the one it was made on is kept until that
+    stream's work is done; a captured graph needs it as long as it is replayed.
     """
 
     def __init__(self, prefix_ids, prefix_lengths, suffix_ids, num_q_heads, num_kv_heads, head_dim,
@@ -269,10 +271,14 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
         _check_output(out, "out", plan._q_shape, q, q.dtype)
         if out.data_ptr() & 15:
             raise ValueError("out must be 16-byte aligned")
+        if _meet(_span(out), _span(k_cache)) or _meet(_span(out), _span(v_cache)):
+            raise ValueError("out must not overlap the pool")
     if lse is None:
         lse = torch.empty((n, hq), dtype=torch.float32, device=q.device)
     else:
         _check_output(lse, "lse", (n, hq), q, torch.float32)
+        if any(_meet(_span(lse), _span(t)) for t in (out, k_cache, v_cache)):
+            raise ValueError("lse must not overlap out or the pool")
     parts = plan.parts * hq
     # partial sums [parts, D], then (max, sum) pairs
     work = torch.empty(parts * (d + 2), dtype=torch.float32, device=q.device)

@@ -33,10 +33,12 @@ def test_table_from_tensors_and_frequencies():
     b = RotaryTable.from_cos_sin(ang.cos(), ang.sin(), interleaved=True)
     assert torch.equal(a.cos_sin, b.cos_sin) and b.rotary_dim == 6 and b.interleaved
     assert b.max_positions == 10
+    c = RotaryTable.from_cos_sin(ang.cos().requires_grad_(True), ang.sin(), interleaved=True)
+    assert torch.equal(c.cos_sin, b.cos_sin) and not c.cos_sin.requires_grad
 
 
 @pytest.mark.parametrize("kw", [dict(rotary_dim=3), dict(rotary_dim=0), dict(rotary_dim=258),
-                                dict(max_positions=0), dict(interleaved=1),
+                                dict(max_positions=0), dict(max_positions=2 ** 31), dict(interleaved=1),
                                 dict(inv_freq=[1.0, 2.0])])
 def test_table_refusals(kw):
     with pytest.raises(ValueError):
@@ -45,7 +47,8 @@ def test_table_refusals(kw):
 
 @pytest.mark.parametrize("cos,sin", [(torch.ones(3, 2), torch.ones(3, 3)), (None, torch.ones(3, 2)),
                                      (torch.ones(3), torch.ones(3)), (torch.ones(0, 2),) * 2,
-                                     (torch.ones(3, 2, dtype=torch.int32),) * 2])
+                                     (torch.ones(3, 2, dtype=torch.int32),) * 2,
+                                     (torch.ones(1, 1).expand(2 ** 31, 1),) * 2])
 def test_table_from_tensors_refusals(cos, sin):
     with pytest.raises(ValueError, match="alike"):
         RotaryTable.from_cos_sin(cos, sin)
@@ -171,7 +174,6 @@ def test_append_entry_refuses_before_any_device_work(change, text):
 def test_attention_entry_refuses_before_any_device_work(change, text):
     base = dict(q=64, dtype=0, Nq=1, hq=2, hkv=2, D=64, scale=1.0, kc=64, vc=64, pages=1, page=16,
                 table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0,
-                rows=64, parts=64, max_parts=1,
-                uneven=0,
+                rows=64, parts=64, max_parts=1, uneven=0,
                 part_o=64, part_ml=64, out=64, lse=64, stream=None)
     _refused("moba_hip_shared_attention", base, change, text)

@@ -350,6 +350,8 @@ def test_shared_refusals(cuda_device):
     bad("scale", scale=float("inf"))
     bad("out must be", out=q.float())
     bad("lse must be", lse=torch.empty(1, 4, 2, device="cuda"))
+    bad("out must not overlap", out=kc.view(-1)[:256].view(1, 4, 64))
+    bad("lse must not overlap", lse=vc.view(-1)[:8].view(torch.float32).view(1, 4))
     bad("page_table", table=table.t())
     bad("cache dtype", kc=kc.float(), vc=vc.float())
     wide = torch.empty(4 * 64 + 8, dtype=torch.bfloat16, device="cuda")
