@@ -177,23 +177,25 @@ class SharedPrefixPlan:
         d, hq, hkv = self.head_dim, self.num_q_heads, self.num_kv_heads
         slots, share = _SLOTS[d > 128], np.where(own, 0.5, 1.0)
         single = (own & narrow).astype(bool)
-        best, longest = None, int(bounds.max())
+        longest = int(bounds.max())
         count = max(1, math.ceil(4 * math.log2(max(1.0, longest / 128)))) + 1
         cache = (bounds * share * times).sum() * hkv * d * 4 / _CACHE
-        for length in np.ceil(np.geomspace(128, max(128, longest), count)):
-            splits = np.minimum(np.ceil(bounds / length), 2 ** 15 - 1)
-            joins = (splits * rows * times).sum() * hq * d * 8 / _PARTIALS + _RANGE * splits.max()
-            for solo in (False, True) if single.any() else (False,):
-                waves = np.where(single & solo, 4, 1)   # items of a workgroup
-                items = blocks * splits * times / waves
-                full = min(1.0, max(_ALONE, items.sum() / slots))
-                keys = _KEY * d * full * waves * np.ceil(bounds / splits)
-                last = _ITEM + keys.max()
-                rounds = math.ceil(items[_ITEM + keys > 0.7 * last].sum() / slots)
-                time = joins + max((items * (_ITEM + keys * share)).sum() / slots, rounds * last, cache)
-                if best is None or time < best[0]:
-                    best = time, splits, solo
-        return best[1].astype(np.int64)[index.ravel()], best[2]
+        # a row per length tried
+        lengths = np.ceil(np.geomspace(128, max(128, longest), count))[:, None]
+        splits = np.minimum(np.ceil(bounds / lengths), 2 ** 15 - 1)
+        joins = splits @ (rows * times) * hq * d * 8 / _PARTIALS + _RANGE * splits.max(axis=1)
+        each, ways = np.ceil(bounds / splits), []
+        for solo in (False, True) if single.any() else (False,):
+            waves = np.where(single & solo, 4, 1)   # items of a workgroup
+            items = blocks * splits * times / waves
+            full = np.clip(items.sum(axis=1, keepdims=True) / slots, _ALONE, 1.0)
+            keys = _KEY * d * full * waves * each
+            last = _ITEM + keys.max(axis=1)
+            rounds = np.ceil((items * (_ITEM + keys > 0.7 * last[:, None])).sum(axis=1) / slots)
+            full_card = (items * (_ITEM + keys * share)).sum(axis=1) / slots
+            ways.append(joins + np.maximum(np.maximum(full_card, rounds * last), cache))
+        best, solo = np.unravel_index(np.argmin(np.stack(ways, axis=1)), (len(lengths), len(ways)))
+        return splits[best].astype(np.int64)[index.ravel()], bool(solo)
 
     @staticmethod
     def _dealt(items, keys):
