@@ -22,15 +22,18 @@ from .rotary import _DTYPES, _check_index, _check_pool, _meet, _on_device, _span
 # or the same 32 and a quarter of the keys each (solo: a wave has an item's 32
 # pairs and all of its keys alone)
 _WIDE, _NARROW = 128, 32
-# What the length of the ranges is chosen by: workgroups that the card holds at
-# once (up to 128 dims, above); an item's time before and after its keys, us; a
-# key's time per dim with the card full, us (39 ns at 128 dims, measured with 64
-# rows behind 32K tokens), and what is left of it with few workgroups; the rate
-# at which partials are written and read, and K/V, bytes per us; the merge's
-# time per range of a row, us.
-_SLOTS = 768, 512
-_ITEM, _KEY, _ALONE = 7.0, 3.0e-4, 0.54
-_PARTIALS, _CACHE, _RANGE = 4.0e6, 4.3e6, 7.5e-3
+# What the length of the ranges is chosen by: workgroups that a CU holds (up to
+# 128 dims, above); an item's time beside its keys, us, the last one's and one of
+# many; a key's, per dim, times what the items of one CU make of each other
+# (alone, and per item; wide items, narrow ones); the rates at which partials are
+# written and read, and K/V, bytes per us; the merge's time per range of a row, us.
+# Fitted to 140 batches, each timed cut in 6 to 30 ways (prefixes to 128K tokens,
+# 1 to 400 rows, 40 to 256 dims): what is taken is 2% behind the best of them on
+# average.
+_CUS, _HELD = 256, (3, 2)
+_ITEM, _OF_MANY, _KEY = 6.4, 5.0, 2.2e-4
+_ON_A_CU = (0.8, 0.27), (0.65, 0.5)
+_PARTIALS, _CACHE, _RANGE = 3.5e6, 4.5e6, 7.5e-3
 _XCDS = 8   # workgroup L runs on XCD L % 8
 
 
@@ -145,7 +148,7 @@ class SharedPrefixPlan:
         # Longest first; but a few items of own tokens behind a card full of
         # prefix ranges would start when those end, all alone
         n_own = int((items[:, 6] < 0).sum())
-        card = _SLOTS[self.head_dim > 128]
+        card = _CUS * _HELD[self.head_dim > 128]
         if n_own <= card // 2 and len(items) > card:
             order = np.argsort(items[:, 6] >= 0, kind="stable")
             items, keys = items[order], keys[order]
@@ -168,33 +171,52 @@ class SharedPrefixPlan:
         own tokens go to single waves).  A segment has ``blocks`` items per
         range, up to ``bounds`` keys (own lengths lie anywhere below their bound:
         half of it on average) and ``rows`` query rows.  Taken are ranges of about
-        one length, the one that gives the shortest time by the figures above."""
+        one length, the one that gives the shortest time by the figures above:
+        as many heavy items as the CUs hold alike (256 rows behind 32K tokens, 8
+        kv heads: 512 items, two a CU, 192 us; 640 204; 768 220)."""
         if not len(blocks):
             return np.zeros(0, np.int64), False
         alike, index, times = np.unique(np.stack((blocks, bounds, own, narrow, rows), axis=1), axis=0,
                                         return_inverse=True, return_counts=True)
         blocks, bounds, own, narrow, rows = alike.T
-        d, hq, hkv = self.head_dim, self.num_q_heads, self.num_kv_heads
-        slots, share = _SLOTS[d > 128], np.where(own, 0.5, 1.0)
-        single = (own & narrow).astype(bool)
-        longest = int(bounds.max())
-        count = max(1, math.ceil(4 * math.log2(max(1.0, longest / 128)))) + 1
-        cache = (bounds * share * times).sum() * hkv * d * 4 / _CACHE
-        # a row per length tried
-        lengths = np.ceil(np.geomspace(128, max(128, longest), count))[:, None]
-        splits = np.minimum(np.ceil(bounds / lengths), 2 ** 15 - 1)
+        hq, hkv, d = self.num_q_heads, self.num_kv_heads, self.head_dim
+        held, share, narrow = _HELD[d > 128], np.where(own, 0.5, 1.0), narrow.astype(bool)
+        alone, each = np.where(narrow[:, None], *_ON_A_CU[::-1]).T
+        single = own.astype(bool) & narrow
+        read = (bounds * share * times).sum() * hkv * d * 4 / _CACHE
+        # ranges of the longest segment: a row of the arrays each
+        top = int(bounds.argmax())
+        most, row = max(1.0, int(bounds[top]) / 128), int(blocks[top] * hkv * times[top])
+        tried = np.unique(np.concatenate((
+            np.geomspace(1, most, 1 + math.ceil(8 * math.log2(most))).round(),
+            np.clip(np.arange(1, held + 1) * _CUS // row, 1, most))))
+        splits = np.minimum(np.ceil(bounds / np.ceil(bounds[top] / tried)[:, None]), 2 ** 15 - 1)
         joins = splits @ (rows * times) * hq * d * 8 / _PARTIALS + _RANGE * splits.max(axis=1)
-        each, ways = np.ceil(bounds / splits), []
+        count, keys = blocks * splits * times, _KEY * d * np.ceil(bounds / splits)
+        ways = []
         for solo in (False, True) if single.any() else (False,):
             waves = np.where(single & solo, 4, 1)   # items of a workgroup
-            items = blocks * splits * times / waves
-            full = np.clip(items.sum(axis=1, keepdims=True) / slots, _ALONE, 1.0)
-            keys = _KEY * d * full * waves * each
-            last = _ITEM + keys.max(axis=1)
-            rounds = np.ceil((items * (_ITEM + keys > 0.7 * last[:, None])).sum(axis=1) / slots)
-            full_card = (items * (_ITEM + keys * share)).sum(axis=1) / slots
-            ways.append(joins + np.maximum(np.maximum(full_card, rounds * last), cache))
-        best, solo = np.unravel_index(np.argmin(np.stack(ways, axis=1)), (len(lengths), len(ways)))
+            items, time = count / waves, keys * waves * share
+            # the longest ones: rounds that fill the CUs, then each CU has the rest
+            likely = _ITEM + time
+            heavy = likely > 0.83 * likely.max(axis=1, keepdims=True)
+            many = np.where(heavy, items, 0.0).sum(axis=1)
+            rounds = np.ceil(many / (held * _CUS)) - 1
+            rest = np.ceil(many / _CUS) - rounds * held
+            full, last = [np.where(heavy, _ITEM + time * np.maximum(alone, each * n), 0.0).max(axis=1)
+                          for n in (held, rest[:, None])]
+            # the others, beside the last round; what it leaves no room for starts
+            # when that ends, some of it earlier
+            work = items * (_OF_MANY + time * each * held) / (held * _CUS)
+            room = last * (rounds + 1 - many / (held * _CUS))
+            late = np.where(heavy, 0.0, _ITEM + time * alone).max(axis=1)
+            late = np.where(np.where(heavy, 0.0, work).sum(axis=1) > room, late, 0.0)
+            longest = np.maximum(rounds * full + last + 0.5 * late,
+                                 (_ITEM + keys * waves * alone).max(axis=1))
+            work = work.sum(axis=1)   # of the whole card
+            # what is far the longest hides the others
+            ways.append(joins + (longest ** 7 + work ** 7 + read ** 7) ** (1 / 7))
+        best, solo = np.unravel_index(np.argmin(np.stack(ways, axis=1)), (len(tried), len(ways)))
         return splits[best].astype(np.int64)[index.ravel()], bool(solo)
 
     @staticmethod
