@@ -11,7 +11,9 @@
 // each component fused into the sum), rounded once to the 16-bit type.
 //
 // Bound by memory: every input is read once and every output written once; the
-// table's row is shared by all the heads of a token and stays in L1 / L2.
+// table's row is shared by all the heads of a token and stays in L1 / L2.  A
+// 32K-token prompt of 32 + 8 + 8 heads of 128 dims (822 MB with the table): 143
+// us, 5.7 TB/s (a copy of 2 GiB: 4.9); 8 tokens: 3 us, what a launch takes.
 #include <algorithm>
 
 #include "common.h"
@@ -126,7 +128,9 @@ template <> struct Piece<2> {
 // neighbouring pieces in each of the two accesses: unit u < R / 2 VEC turns the
 // pieces at VEC u and VEC u + R/2 (VEC pairs of the two, or VEC / 2 pairs within
 // each when interleaved), unit R / 2 VEC + c copies the pieces c and c + n of
-// the 2n behind R.
+// the 2n behind R.  8-byte pieces where R / 2 is no multiple of 8 took 10.3 us
+// instead of 17.3 (8K tokens, 16 + 4 + 4 heads of 40 dims); a unit that turns
+// neighbouring pieces of its own 45 instead of 40 (256 dims, 64 rotated).
 template <int DT, bool INTER, int VEC>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;

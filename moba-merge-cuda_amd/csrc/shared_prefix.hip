@@ -10,6 +10,18 @@
 // (row, head) pairs against the range's K/V, read once for the block.  An item
 // leaves (O, m, z) of its range in fp32; merge_kernel joins a row's ranges in
 // their order.  Results do not depend on timing.
+//
+// Scores, softmax and sums are fp32.  Two roundings to 16 bits are the matrix
+// units' price: the weights e^{s - m} before their product with V (their sum z
+// takes them unrounded; at most half a step, 2^-8 or 2^-11 of each weight's
+// share), and the result.
+//
+// What bounds it: with many pairs to a block the products and the exponentials,
+// which share a SIMD's issue slots (D 128, 1024 rows behind 16K tokens: matrix
+// units busy 57% of the cycles, vector instructions 57%, together 89%, at 1.65
+// GHz, to which the chip's power limit takes the clock); with few the reads of
+// K and V; with few tokens the chain launch, page entries, keys, values, partials
+// and the second launch.
 #include <type_traits>
 
 #include "common.h"
@@ -403,7 +415,12 @@ template <int NKS> MOBA_DEV void load_query(const SharedArgs& a, const Pair& p, 
 
 // More than 32 pairs: every wave has 32 of them, and the four share tiles of
 // KEYS keys in STAGES LDS stages: while one is in use, the loads of the others are
-// in flight.
+// in flight.  S^T = K Q^T and O^T += V^T P^T: a lane holds one pair's column of
+// both, so that its maximum and sum take one exchange with lane + 32 and the
+// weights are the second product's operand where they are.  128 pairs: K and V
+// are read from L2 once for 128 x 4 D operations a key; 64 rows to a wave spilled
+// at 64 dims and gave 2% at 128.  Bound by products and exponentials: 1024 rows
+// of 4 heads a kv head behind 16K tokens, D 128, 296 us, 0.93 PFLOP/s.
 template <int DT, int ND, bool NEAR, bool UNEVEN>
 MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
@@ -590,7 +607,11 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
 // between them; their results are joined in LDS in a fixed order.  The next
 // group's K is in flight from the scores on, its V from the product with V on.
 // 16-key groups fill half of a 32-row score product; what a narrow item waits
-// for is memory.  SOLO: x is this wave's alone, and it takes every group.
+// for is memory: 2 rows of 7 heads a kv head behind 128K tokens, D 64, 67 MB, 15
+// us, 4.4 TB/s (a block of 128 pairs with 14 in use took 225).  SOLO: x is this
+// wave's alone, and it takes every group: a short sequence's few keys are not
+// worth a workgroup (225 sequences of up to 4 own tokens, 32 kv heads: 25 us, 58
+// with a workgroup each), many are (64 of up to 2048: 174, 108).
 template <int DT, int ND, bool NEAR, bool UNEVEN, bool SOLO>
 MOBA_DEV void narrow_item(const SharedArgs& a, const Item& x, char* smem) {
   typedef Dims<ND> C;
@@ -802,7 +823,10 @@ __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs 
 
 // Joins the ranges of each (row, head): PL threads per four dims, each with
 // every PL-th range, four of them at a time (their loads are in flight
-// together), then the PL sums in LDS in order.
+// together), then the PL sums in LDS in order.  Bound by the reads of the
+// partials: 5 ranges of 16384 (row, head)s of 256 dims, 84 MB, 16.5 us, 5.1 TB/s
+// (they come from the last-level cache); with few rows by the latency of the two
+// dependent loads, 3 to 5 us.
 template <int DT>
 __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ part_o,
                                                     const float2* __restrict__ part_ml,
