@@ -299,17 +299,40 @@ MOBA_DEV void mask_scores(f32x16_t (&s)[NKB], int left, const uint32_t* tok, int
 // blocks of the swizzled layout whose first row is row0: physical block lane %
 // NB of row row0 + lane / NB.  The swizzle's bit reversal takes row0 and lane /
 // NB apart, which share no bits.
-// In the block before: N products, each with READS LDS reads of its own that go
-// out two products before it (1024 rows behind 16K tokens: 299 us as the compiler
-// orders them, 296 so; 2 to 4 products alike, 6 and more 2% slower).
-template <int N, int READS> MOBA_DEV void ahead() {
-  constexpr int F = N < 2 ? N : 2;
-  __builtin_amdgcn_sched_group_barrier(0x100, F * READS, 0);
+// N products in order, what each reads from LDS (in READS instructions) sent out
+// before the one two or three before it.  FIXED: exactly so; the compiler, left to
+// it, sends a read out right before its product where registers are short (1024
+// rows of 256 dims behind 8K tokens: 176 us, 162 so; two ahead 163, four 172), and
+// at 128 dims does 1% better from the wish alone (1024 rows behind 16K: 299 us as it
+// orders them, 296 so).
+template <int N, int READS, bool FIXED, class Load, class Use> MOBA_DEV void in_order(Load load, Use use) {
+  constexpr int AHEAD = N < 3 ? N : FIXED ? 3 : 2;
+  u16x8_t f[N];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) f[i] = load(i);
+  if constexpr (FIXED) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    if (i + F < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    use(i, f[i]);
+    if (i + AHEAD < N) f[i + AHEAD] = load(i + AHEAD);
+    if constexpr (FIXED) __builtin_amdgcn_sched_barrier(0);
   }
+  if constexpr (!FIXED) {
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+  }
+}
+// The i-th of N fragments in an order where those a constant apart (PER of
+// them) follow each other: one address in a register serves them.
+template <int N, int PER> constexpr int by_address(int i) {
+  constexpr int G = (N + PER - 1) / PER, LONG = N - PER * (G - 1);  // LONG runs of G, then of G - 1
+  if (G == 1) return i;
+  const int j = i - G * LONG;
+  return j < 0 ? i / G + i % G * PER : LONG + j / (G - 1) + j % (G - 1) * PER;
 }
 template <int DP> MOBA_DEV uint32_t block_byte(uint32_t lane, uint32_t row0) {
   constexpr uint32_t NB = DP / 8, NBM = (uint32_t)swz_nbm<DP>();
@@ -473,13 +496,12 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   // wave w brings the 64-block loads n * 4 + w of a tile; where a tile's rows
   // are is read one tile before
   const uint32_t lds0 = lds_addr(smem) + wave * 1024;
-  uint32_t byte[NDMA], at[NDMA];
+  const uint32_t byte0 = block_byte<DP>(lane, wave * (64 / NB));
+  auto byte = [&](int n) { return opaque(byte0) ^ block_byte<DP>(0, n * 4 * (64 / NB)); };
+  uint32_t at[NDMA];
   bool mine[NDMA];
 #pragma unroll
-  for (int n = 0; n < NDMA; ++n) {
-    byte[n] = block_byte<DP>(lane, (n * 4 + wave) * (64 / NB));
-    mine[n] = byte[n] < (uint32_t)D * 2;
-  }
+  for (int n = 0; n < NDMA; ++n) mine[n] = byte(n) < (uint32_t)D * 2;
   auto places = [&](int it) {
 #pragma unroll
     for (int n = 0; n < NDMA; ++n) at[n] = tok[it * KEYS + (n * 4 + wave) * (64 / NB) + lane / NB];
@@ -489,8 +511,8 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
 #pragma unroll
     for (int n = 0; n < NDMA; ++n)
       if (mine[n]) {
-        rows.template bring<false>(at[n], byte[n], lds + n * 4096);
-        rows.template bring<true>(at[n], byte[n], lds + STAGES * TILE * 2 + n * 4096);
+        rows.template bring<false>(at[n], byte(n), lds + n * 4096);
+        rows.template bring<true>(at[n], byte(n), lds + STAGES * TILE * 2 + n * 4096);
       }
   };
   auto tile = [&](auto stage, int it, int kt0, bool holes) {
@@ -499,30 +521,30 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     f32x16_t sacc[NKB];
     wave_prio<1>();
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) {
-      sacc[kb] = zero16();
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        sacc[kb] = mfma32<DT>(lds8(Kb, kb * 32 * DP * 2 + swz_b128<DP>(kq, ks)), qf[ks], sacc[kb]);
-    }
-    ahead<NKB * NKS, 1>();
+    for (int kb = 0; kb < NKB; ++kb) sacc[kb] = zero16();
+    in_order<NKB * NKS, 1, (DP > 128)>(
+        [&](int i) {
+          return lds8(Kb, i / NKS * 32 * DP * 2 + swz_b128<DP>(kq, by_address<NKS, 8>(i % NKS)));
+        },
+        [&](int i, u16x8_t k) {
+          sacc[i / NKS] = mfma32<DT>(k, qf[by_address<NKS, 8>(i % NKS)], sacc[i / NKS]);
+        });
     wave_prio<0>();
     if (kt0 + KEYS > wlim || holes)
       mask_scores<NKB, 16>(sacc, min(p.limit, hi) - kt0, tok + it * KEYS, hh);
     u16x8_t pv[NKB][2];
     softmax_step<DT, NKB, 16, NDB>(sacc, a.scale_log2, run, oacc, pv);
     wave_prio<1>();
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint32_t ro = (kb * 32 + t * 16) * DP * 2;
-          oacc[db] = mfma32<DT>(lds_tr8(Vb, ro + swz_tr<DP>(t0, db), ro + swz_tr<DP>(t1, db)),
-                                pv[kb][t], oacc[db]);
-        }
-    ahead<NDB * NKB * 2, 2>();
+    in_order<NDB * NKB * 2, 2, (DP > 128)>(
+        [&](int i) {
+          const uint32_t ro = i % (2 * NKB) * 16 * DP * 2;
+          const int db = by_address<NDB, 4>(i / (2 * NKB));
+          return lds_tr8(Vb, ro + swz_tr<DP>(t0, db), ro + swz_tr<DP>(t1, db));
+        },
+        [&](int i, u16x8_t v) {
+          const int db = by_address<NDB, 4>(i / (2 * NKB));
+          oacc[db] = mfma32<DT>(v, pv[i % (2 * NKB) / 2][i % 2], oacc[db]);
+        });
     wave_prio<0>();
   };
 
@@ -599,7 +621,12 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
     }
   }
   const float l = run.l + __shfl_xor(run.l, 32, 64);
-  if (p.valid) store_partial<NDB>(a, p.part, oacc, run.m, l, hh);
+  if constexpr (ND > 192) {  // looked up again: its registers are the loop's
+    const Pair e = pair_of(a, x, wave * 32 + (int)opaque(qi), alike);
+    if (e.valid) store_partial<NDB>(a, e.part, oacc, run.m, l, hh);
+  } else if (p.valid) {
+    store_partial<NDB>(a, p.part, oacc, run.m, l, hh);
+  }
 }
 
 // Up to 32 pairs: the four waves have the same pairs and take every fourth
