@@ -497,7 +497,8 @@ MOBA_DEV void wide_item(const SharedArgs& a, const Item& x, char* smem) {
   // are is read one tile before
   const uint32_t lds0 = lds_addr(smem) + wave * 1024;
   const uint32_t byte0 = block_byte<DP>(lane, wave * (64 / NB));
-  auto byte = [&](int n) { return opaque(byte0) ^ block_byte<DP>(0, n * 4 * (64 / NB)); };
+  // (above 128 dims recomputed at each load: registers are short there)
+  auto byte = [&](int n) { return (DP > 128 ? opaque(byte0) : byte0) ^ block_byte<DP>(0, n * 4 * (64 / NB)); };
   uint32_t at[NDMA];
   bool mine[NDMA];
 #pragma unroll
