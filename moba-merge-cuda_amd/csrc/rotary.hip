@@ -46,6 +46,7 @@ struct AppendArgs {
   const uint16_t *q, *k, *v;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // token and head strides, elements
   int N, Hq, Hkv, D, R, units;                 // units: pieces of work per head
+  int wide;                                    // what is copied is whole 16-byte pieces
   uint32_t total;                              // N * (Hq + 2 Hkv) * units
   FastDiv by_token, by_head, by_page;
   const float2* cos_sin;
@@ -124,13 +125,25 @@ template <> struct Piece<2> {
   MOBA_DEV void store(uint16_t* p) const { *reinterpret_cast<uint32_t*>(p) = w[0]; }
 };
 
+// The pieces c and c + n of the 2n of VEC dims from `from` on.
+template <int VEC> MOBA_DEV void copy_pieces(const AppendArgs& a, const uint16_t* src, uint16_t* dst, int from, int c) {
+  const int n = (a.D - from + 2 * VEC - 1) / (2 * VEC), d0 = from + VEC * c, d1 = d0 + VEC * n;
+  if (c >= n) return;
+  Piece<VEC> x, y;
+  x.load(src + d0);
+  y.load(src + (d1 < a.D ? d1 : d0));
+  x.store(dst + d0);
+  if (d1 < a.D) y.store(dst + d1);
+}
+
 // Whole pieces of VEC dims, two per unit, so that neighbouring lanes have
 // neighbouring pieces in each of the two accesses: unit u < R / 2 VEC turns the
 // pieces at VEC u and VEC u + R/2 (VEC pairs of the two, or VEC / 2 pairs within
 // each when interleaved), unit R / 2 VEC + c copies the pieces c and c + n of
-// the 2n behind R.  8-byte pieces where R / 2 is no multiple of 8 took 10.3 us
-// instead of 17.3 (8K tokens, 16 + 4 + 4 heads of 40 dims); a unit that turns
-// neighbouring pieces of its own 45 instead of 40 (256 dims, 64 rotated).
+// the 2n behind R.  8K tokens, 16 + 4 + 4 heads: of 40 dims, all rotated, 10.3 us
+// in 8-byte pieces, 17.3 dim by dim; of 256 dims, 24 rotated, 44 with the others in
+// 16-byte pieces (wide), 54 in 8-byte ones too; 64 rotated, 40, 45 where a unit has
+// two neighbouring pieces.
 template <int DT, bool INTER, int VEC>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
@@ -143,12 +156,8 @@ __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const int turning = turn != nullptr ? a.R / (2 * VEC) : 0, from = turning * 2 * VEC;
   Piece<VEC> x, y;
   if (u >= turning) {
-    const int n = (a.D - from + 2 * VEC - 1) / (2 * VEC), d0 = from + VEC * (u - turning);
-    const int d1 = d0 + VEC * n;
-    x.load(src + d0);
-    y.load(src + (d1 < a.D ? d1 : d0));
-    x.store(dst + d0);
-    if (d1 < a.D) y.store(dst + d1);
+    if (VEC < 8 && a.wide) copy_pieces<8>(a, src, dst, from, u - turning);
+    else copy_pieces<VEC>(a, src, dst, from, u - turning);
     return;
   }
   const int d0 = VEC * u, d1 = d0 + a.R / 2;
@@ -252,7 +261,9 @@ void launch_append(AppendArgs& a, int interleaved, int access, hipStream_t st) {
   int vec = access;
   while (vec > 1 && a.R % (2 * vec)) vec /= 2;
   const bool pairs = vec > 1;
-  a.units = pairs ? (a.D + 2 * vec - 1) / (2 * vec) : access == 8 ? a.D / 8 : a.D;
+  a.wide = access == 8 && a.R % 8 == 0;
+  const int copy = a.wide ? 16 : 2 * vec;  // dims that a unit copies
+  a.units = pairs ? a.R / (2 * vec) + (a.D - a.R + copy - 1) / copy : access == 8 ? a.D / 8 : a.D;
   a.by_head = fast_div(a.units);
   a.by_token = fast_div((a.Hq + 2 * a.Hkv) * a.units);
   a.total = (uint32_t)a.N * a.by_token.d;

@@ -98,6 +98,7 @@ def _check(st, got_q, dtype, live=None):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("hq,hkv,d,rotary", [
+    (4, 2, 256, 24), (3, 1, 96, 24), (2, 2, 80, 40), (2, 1, 72, 8),  # copied in wider pieces than turned
     (12, 2, 128, 128), (16, 1, 96, 96), (14, 2, 64, 64), (4, 4, 256, 64), (3, 1, 40, 40),
     (4, 2, 40, 10), (2, 2, 64, 2), (6, 3, 72, 36), (1, 1, 8, 8), (5, 1, 24, 16), (3, 3, 20, 6), (2, 1, 96, 24), (3, 1, 80, 20),
     (2, 1, 7, 4)])
