@@ -302,7 +302,7 @@ MOBA_DEV void mask_scores(f32x16_t (&s)[NKB], int left, const uint32_t* tok, int
 // N products in order, what each reads from LDS (in READS instructions) sent out
 // before the one two or three before it.  FIXED: exactly so; the compiler, left to
 // it, sends a read out right before its product where registers are short (1024
-// rows of 256 dims behind 8K tokens: 176 us, 162 so; two ahead 163, four 172), and
+// rows of 256 dims behind 8K tokens: 176 us, 162 so; two before 163, four 172), and
 // at 128 dims does 1% better from the wish alone (1024 rows behind 16K: 299 us as it
 // orders them, 296 so).
 template <int N, int READS, bool FIXED, class Load, class Use> MOBA_DEV void in_order(Load load, Use use) {
@@ -852,7 +852,7 @@ __global__ __launch_bounds__(256, Dims<ND>::WAVES) void block_kernel(SharedArgs 
 // Joins the ranges of each (row, head): PL threads per four dims, each with
 // every PL-th range, four of them at a time (their loads are in flight
 // together), then the PL sums in LDS in order.  Bound by the reads of the
-// partials: 5 ranges of 16384 (row, head)s of 256 dims, 84 MB, 16.5 us, 5.1 TB/s
+// partials: 5 ranges of 16384 (row, head)s of 256 dims, 84 MB, 16.8 us, 5.0 TB/s
 // (they come from the last-level cache); with few rows by the latency of the two
 // dependent loads, 3 to 5 us.
 template <int DT>
