@@ -222,7 +222,8 @@ def test_infinities_and_nan_stay_in_their_rows(cuda_device):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("hq,hkv,d,tokens,solo", [(4, 2, 128, 60, False), (8, 1, 96, 3, False),
                                                   (8, 1, 96, 3, True), (2, 2, 64, 40, False),
-                                                  (4, 4, 40, 7, True), (2, 1, 256, 40, False)])
+                                                  (4, 4, 40, 7, True), (2, 1, 256, 40, False),
+                                                  (4, 1, 192, 9, False), (5, 1, 200, 3, True)])
 def test_values_behind_a_row_do_not_reach_it(cuda_device, monkeypatch, hq, hkv, d, tokens, solo, dtype):
     """Several query tokens of a sequence: an infinite or NaN value reaches the
     rows at and behind its position, as the sum has it, and no row before."""
