@@ -141,7 +141,12 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   THPObjectPtr cs_ref(cs_obj);
   const at::Tensor* cs = tensor_in(cs_obj);
   if (!int_attr(a[7], s_rotary_dim, rotary_dim) || !int_attr(a[7], s_interleaved, inter)) return nullptr;
-  if (!cs || !plain(*cs, p.idx) || rotary_dim > p.d) return not_here();
+  // the table is an attribute that a caller may replace
+  if (!cs || !plain(*cs, p.idx) || cs->scalar_type() != at::kFloat || cs->dim() != 3 ||
+      !cs->is_contiguous() || cs->size(0) < 1 || cs->size(0) >= (1ll << 31) ||
+      2 * cs->size(1) != rotary_dim || cs->size(2) != 2 || rotary_dim > p.d ||
+      ((uintptr_t)cs->data_ptr() & 15))
+    return not_here();
 
   const Span pools[2] = {{p.k, p.k + p.bytes}, {p.v, p.v + p.bytes}};
   if (meet(pools[0], pools[1])) return not_here();

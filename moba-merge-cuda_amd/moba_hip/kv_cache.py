@@ -198,12 +198,9 @@ class PagedKVCache:
 
     def _check_rotary(self, rotary, last):
         """``last``: the largest position that will be turned."""
-        _require([
-            (lambda: isinstance(rotary, RotaryTable), "rotary must be a RotaryTable"),
-            (lambda: rotary.device == self.device, "rotary table must be on the cache's device"),
-            (lambda: rotary.rotary_dim <= self.head_dim, "rotary_dim exceeds head_dim"),
-            (lambda: last < rotary.max_positions, "positions exceed the rotary table"),
-        ])
+        _require([(lambda: isinstance(rotary, RotaryTable), "rotary must be a RotaryTable")])
+        rotary._check(self.head_dim, self.device)
+        _require([(lambda: last < rotary.max_positions, "positions exceed the rotary table")])
 
     @torch.no_grad()
     def append_rotary(self, k, v, rotary, *, sequence_ids, cu_seqlens=None, q=None, offsets=None,

@@ -49,6 +49,7 @@ class PreparedSharedDecode(PreparedDecode):
             self.rotary = rotary
             if rotary is not None:
                 cache._check_rotary(rotary, max(self.prefix_lengths))
+                self._angles = rotary.cos_sin   # what the launches hold the address of
             self._plan = SharedPrefixPlan(self.prefix_ids, self.prefix_lengths, self.ids,
                                           self.num_q_heads, cache.num_kv_heads, cache.head_dim,
                                           max_suffix=self.max_length, device=cache.device)
@@ -92,7 +93,7 @@ class PreparedSharedDecode(PreparedDecode):
             r = self.rotary
             calls.append(("moba_hip_append_rotary", (
                 ptr(self.q), hq * d, d, ptr(self.k), hkv * d, d, ptr(self.v), hkv * d, d, code, rows,
-                hq, hkv, d, ptr(r.cos_sin), r.max_positions, r.rotary_dim, int(r.interleaved), kc, vc,
+                hq, hkv, d, ptr(self._angles), r.max_positions, r.rotary_dim, int(r.interleaved), kc, vc,
                 pages, page, table, c._table.shape[0], width, ids, pos, ptr(self._offsets),
                 ptr(self._turned), None)))
         calls.append(("moba_hip_block_means", (kc, code, hkv, d, page, table, width, ids, pos, rows, 1,
@@ -113,7 +114,7 @@ class PreparedSharedDecode(PreparedDecode):
         step = self._lease.plan()
         if max(step.positions) >= self.max_length:
             raise ValueError("append exceeds max_length")
-        if self.rotary is not None and self.rotary.max_positions <= max(
+        if self.rotary is not None and self._angles.shape[0] <= max(
                 p + n for p, n in zip(step.positions, self.prefix_lengths)):
             raise ValueError("positions exceed the rotary table")
         if step.updates or self._uploaded:

@@ -66,11 +66,29 @@ class RotaryTable:
 
     def _store(self, cos, sin):
         self.cos_sin = torch.stack((cos, sin), dim=-1).detach().to(torch.float32).contiguous()
-        self.max_positions = self.cos_sin.shape[0]
+
+    @property
+    def max_positions(self):
+        return self.cos_sin.shape[0]
 
     @property
     def device(self):
         return self.cos_sin.device
+
+    def _check(self, head_dim, device):
+        """Raises what keeps heads of ``head_dim`` on ``device`` from being turned.
+        ``cos_sin`` is the caller's to replace (on another device, say): what
+        the kernels read is tested at each use."""
+        cs = self.cos_sin
+        if not isinstance(cs, torch.Tensor) or cs.dtype != torch.float32 or cs.dim() != 3 or \
+                cs.layout != torch.strided or not cs.is_contiguous() or cs.data_ptr() & 15 or \
+                not 0 < cs.shape[0] < 2 ** 31 or (2 * cs.shape[1], cs.shape[2]) != (self.rotary_dim, 2):
+            raise ValueError("rotary.cos_sin must be contiguous, 16-byte aligned fp32 "
+                             "[positions, rotary_dim / 2, 2]")
+        if self.rotary_dim > head_dim:
+            raise ValueError("rotary_dim exceeds head_dim")
+        if self.device != device:
+            raise ValueError("rotary table must be on the cache's device")
 
 
 # The checks below name what is wrong with a call.  They are not on the path of
@@ -135,10 +153,7 @@ def _check_append(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
         _check_index(offsets, "offsets", 1, dev, page_table.shape[0])
     if not isinstance(rotary, RotaryTable):
         raise ValueError("rotary must be a RotaryTable")
-    if rotary.rotary_dim > d:
-        raise ValueError("rotary_dim exceeds head_dim")
-    if rotary.device != dev:
-        raise ValueError("rotary table must be on the cache's device")
+    rotary._check(d, dev)
     if q is not None:
         _check_token_tensor(q, "q", n, None, d, k_cache)
     if n * ((0 if q is None else q.shape[1]) + 2 * hkv) * d >= 2 ** 31:

@@ -1,0 +1,41 @@
+"""CPU tests of what the paged-cache operators, their prepared step and the
+Qwen2 session refuse, and of how they leave things when a part of them fails."""
+import pytest
+import torch
+
+from moba_hip import RotaryTable
+
+
+# ------------------------------------------------------------- rotary tables
+REPLACED = {
+    "16 bits": lambda t: t.half(),
+    "64 bits": lambda t: t.double(),
+    "flat": lambda t: t.flatten(1),
+    "strided": lambda t: t.transpose(0, 1).contiguous().transpose(0, 1),
+    "fewer pairs": lambda t: t[:, :2].contiguous(),
+    "cos alone": lambda t: t[..., :1].contiguous(),
+    "no rows": lambda t: t[:0],
+    "no tensor": lambda t: t.tolist(),
+    "misaligned": lambda t: torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape),
+}
+
+
+@pytest.mark.parametrize("how", REPLACED)
+def test_replaced_rotary_table_is_checked(how):
+    """A kernel reads what ``cos_sin`` holds at the call, so that is what a call tests."""
+    t = RotaryTable(8, 6, device="cpu")
+    t._check(64, torch.device("cpu"))
+    t.cos_sin = REPLACED[how](t.cos_sin)
+    with pytest.raises(ValueError, match="cos_sin must be"):
+        t._check(64, torch.device("cpu"))
+
+
+def test_rotary_table_length_is_that_of_its_rows():
+    t = RotaryTable(8, 6, device="cpu")
+    t.cos_sin = t.cos_sin[:4]
+    assert t.max_positions == 4
+    t._check(8, torch.device("cpu"))
+    with pytest.raises(ValueError, match="exceeds head_dim"):
+        t._check(6, torch.device("cpu"))
+    with pytest.raises(ValueError, match="cache's device"):
+        t._check(8, torch.device("cuda", 0))

@@ -1,0 +1,69 @@
+"""Calls of the paged-cache operators beside the ordinary ones: replaced tables
+and plans, failures inside a step, and the kernels that only far pools, unmapped
+pages or long lookups reach."""
+import pytest
+import torch
+
+from test_paged_contract import REPLACED
+from test_rotary_append_gpu import SENTINEL, _case, _run
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------- rotary tables
+@pytest.mark.parametrize("how", REPLACED)
+@pytest.mark.parametrize("check", [False, True])
+def test_append_refuses_a_replaced_table(cuda_device, how, check):
+    st = _case([4, 9], 4, 2, 64, 64, 16, torch.bfloat16)
+    st["rotary"].cos_sin = REPLACED[how](st["rotary"].cos_sin)
+    with pytest.raises(ValueError, match="cos_sin must be"):
+        _run(st, check=check)
+    torch.cuda.synchronize()
+    assert (st["k_cache"] == SENTINEL).all() and (st["v_cache"] == SENTINEL).all()
+
+
+def test_append_uses_the_rows_a_replaced_table_has(cuda_device):
+    """A shorter table: tokens past its end are dropped as past any table's."""
+    st = _case([9], 4, 2, 64, 64, 16, torch.bfloat16, context=[0])
+    whole = _run(st)
+    st["rotary"].cos_sin = st["rotary"].cos_sin[:5]
+    st["k_cache"].fill_(SENTINEL)
+    out = torch.full_like(whole, SENTINEL)
+    _run(st, q_out=out)
+    assert torch.equal(out[:5], whole[:5]) and (out[5:] == SENTINEL).all()
+    with pytest.raises(RuntimeError, match="rotary table"):
+        _run(st, check=True)
+
+
+@pytest.mark.parametrize("how", REPLACED)
+def test_cache_and_lease_refuse_a_replaced_table(cuda_device, how):
+    from moba_hip import PagedKVCache, RotaryTable
+    cache, table = PagedKVCache(2, 64, 2, 64, chunk_size=32), RotaryTable(64, 100)
+    table.cos_sin = REPLACED[how](table.cos_sin)
+    k = torch.randn(3, 2, 64, device="cuda").bfloat16()
+    with pytest.raises(ValueError, match="cos_sin must be"):
+        cache.append_rotary(k, k, table, sequence_ids=[0], cu_seqlens=[0, 3])
+    with pytest.raises(ValueError, match="cos_sin must be"):
+        cache.prepare_shared_decode([0], [-1], 4, rotary=table)
+    assert cache.lengths == (0, 0)
+
+
+def test_lease_keeps_the_table_it_was_made_with(cuda_device):
+    """The launches hold the address of the angles: replacing the attribute
+    later changes nothing of them."""
+    from moba_hip import PagedKVCache, RotaryTable
+    outs = []
+    for replace in (False, True):
+        cache, table = PagedKVCache(2, 64, 2, 64, chunk_size=32), RotaryTable(64, 100)
+        with cache.prepare_shared_decode([0, 1], [-1, -1], 4, rotary=table) as plan:
+            if replace:
+                table.cos_sin = None
+                torch.cuda.empty_cache()
+                junk = [torch.full((100, 32, 2), 9.0, device="cuda") for _ in range(8)]
+            for t in range(3):
+                g = torch.Generator().manual_seed(t)
+                q, k, v = (torch.randn(2, h, 64, generator=g).to("cuda", torch.bfloat16) for h in (4, 2, 2))
+                out = plan.step(q, k, v).output.clone()
+            torch.cuda.synchronize()
+        outs.append(out)
+    assert torch.equal(*outs) and len(junk) == 8
