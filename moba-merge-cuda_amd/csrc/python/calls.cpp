@@ -210,6 +210,9 @@ PyObject* shared_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     return not_here();
   Plan x;
   memcpy(&x, PyBytes_AS_STRING(packed.get()), sizeof(x));
+  if (meta->scalar_type() != at::kInt || meta->dim() != 1 || !meta->is_contiguous() ||
+      meta->size(0) != x.parts_at / 4 + 3 * x.rows || ((uintptr_t)meta->data_ptr() & 15))
+    return not_here();  // the records are an attribute that a caller may replace
   if (!q || !tokens_of(q, p, x.rows) || !q->is_contiguous() || q->size(1) != x.hq || p.hkv != x.hkv ||
       p.d != x.d || x.max_slot >= p.slots || x.max_prefix > p.width * p.page ||
       !index_of(own, p.idx, x.rows))

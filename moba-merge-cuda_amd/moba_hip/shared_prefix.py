@@ -90,11 +90,23 @@ class SharedPrefixPlan:
         self.max_slot = int(max(prefix[length > 0].max(initial=-1), suffix.max()))
         flat = self._build(prefix, length, suffix)
         self.meta = torch.from_numpy(flat).to(device)
-        self.device = self.meta.device
         # what a call needs of the plan, for the native host path
         self._packed = struct.pack("13q", n, hq, hkv, d, self.max_slot, self.max_prefix, max_suffix,
                                    self.n_items, self._rows_at, self._parts_at, self.parts,
                                    self.max_parts, self.uneven)
+
+    @property
+    def device(self):
+        return self.meta.device
+
+    def _check(self):
+        """Raises where ``meta``, which a caller may replace, is not what the
+        kernels index."""
+        m = self.meta
+        if not isinstance(m, torch.Tensor) or m.dtype != torch.int32 or m.layout != torch.strided or \
+                m.dim() != 1 or not m.is_contiguous() or \
+                m.numel() != self._parts_at // 4 + 3 * self.rows or m.data_ptr() & 15:
+            raise ValueError("plan.meta must be the plan's int32 records, contiguous and 16-byte aligned")
 
     def _build(self, prefix, length, suffix):
         """The device arrays: work items, segments' rows, rows' partials."""
@@ -242,6 +254,7 @@ def _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan):
     dev = k_cache.device
     if not isinstance(plan, SharedPrefixPlan):
         raise ValueError("plan must be a SharedPrefixPlan")
+    plan._check()
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype != k_cache.dtype or \
             q.device != dev or plan.device != dev:
         raise ValueError("q must be [Nq,Hq,D] of the pool's device and dtype, and the plan on it")

@@ -3,7 +3,7 @@ Qwen2 session refuse, and of how they leave things when a part of them fails."""
 import pytest
 import torch
 
-from moba_hip import RotaryTable
+from moba_hip import RotaryTable, SharedPrefixPlan
 
 
 # ------------------------------------------------------------- rotary tables
@@ -39,3 +39,24 @@ def test_rotary_table_length_is_that_of_its_rows():
         t._check(6, torch.device("cpu"))
     with pytest.raises(ValueError, match="cache's device"):
         t._check(8, torch.device("cuda", 0))
+
+
+# ------------------------------------------------------------------ the plan
+RECORDS = {
+    "64 bits": lambda t: t.long(),
+    "cut": lambda t: t[:-1],
+    "longer": lambda t: torch.cat((t, t[:1])),
+    "2D": lambda t: t[None],
+    "strided": lambda t: torch.stack((t, t), 1)[:, 0],
+    "no tensor": lambda t: t.tolist(),
+    "misaligned": lambda t: torch.cat((t.new_zeros(1), t))[1:],
+}
+
+
+@pytest.mark.parametrize("how", RECORDS)
+def test_replaced_records_of_a_plan_are_checked(how):
+    plan = SharedPrefixPlan([0, 0, -1], [70, 70, 0], [1, 2, 2], 4, 2, 64, max_suffix=9, device="cpu")
+    plan._check()
+    plan.meta = RECORDS[how](plan.meta)
+    with pytest.raises(ValueError, match="plan.meta must be"):
+        plan._check()

@@ -4,8 +4,9 @@ pages or long lookups reach."""
 import pytest
 import torch
 
-from test_paged_contract import REPLACED
+from test_paged_contract import RECORDS, REPLACED
 from test_rotary_append_gpu import SENTINEL, _case, _run
+from test_shared_prefix_gpu import _pool
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,18 @@ def test_lease_keeps_the_table_it_was_made_with(cuda_device):
             torch.cuda.synchronize()
         outs.append(out)
     assert torch.equal(*outs) and len(junk) == 8
+
+
+# ------------------------------------------------------------------ the plan
+@pytest.mark.parametrize("how", [*RECORDS, "host"])
+@pytest.mark.parametrize("given", [False, True])
+def test_attention_refuses_replaced_records(cuda_device, how, given):
+    """Without outputs of the caller's (the native entry's calls) and with them."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    kc, vc, table, _, _ = _pool([100, 5], 2, 64, 16, torch.bfloat16, 2)
+    plan = SharedPrefixPlan([0], [100], [1], 4, 2, 64, max_suffix=5)
+    plan.meta = plan.meta.cpu() if how == "host" else RECORDS[how](plan.meta)
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    own = torch.tensor([5], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="the plan on it" if how == "host" else "plan.meta must be"):
+        shared_prefix_attention(q, kc, vc, table, own, plan, out=torch.empty_like(q) if given else None)
