@@ -233,16 +233,26 @@ class Qwen2Session:
         self.close()
 
 
+# rope types whose frequencies are the same at every length
+_FIXED_ROPE = ("default", "linear", "yarn", "llama3")
+
+
 class Qwen2Branches:
     """``branches`` continuations of one prompt.  ``capacity`` bounds the
     prompt, ``new_tokens`` what each branch adds.  Keys and queries turn inside
-    the cache's append (fp32, rounded once)."""
+    the cache's append (fp32, rounded once), by one table of angles: models whose
+    frequencies change with the length of the input ("dynamic", "longrope") are
+    refused."""
 
     def __init__(self, model, capacity, branches, new_tokens, *, chunk=128, page=16,
                  backend="eager"):
         if backend not in ("eager", "model_graph"):
             raise ValueError("backend")
         cfg = _checked(model)
+        rope = model.model.rotary_emb
+        kind = getattr(rope, "rope_type", "default")
+        if kind not in _FIXED_ROPE:
+            raise ValueError(f"rope type {kind!r} unsupported: its frequencies may depend on the length")
         self.capacity = positive_int(capacity, "capacity")
         self.branches = positive_int(branches, "branches")
         self.new_tokens = positive_int(new_tokens, "new_tokens")
@@ -254,7 +264,6 @@ class Qwen2Branches:
         hk, self.hq = cfg.num_key_value_heads, cfg.num_attention_heads
         self.dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.hq
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        rope = model.model.rotary_emb
         self.rotary = RotaryTable(self.dim, self.capacity + self.new_tokens, inv_freq=rope.inv_freq,
                                   scaling=rope.attention_scaling, device=self.device)
         pages = -(-self.capacity // page) + self.branches * -(-self.new_tokens // page)

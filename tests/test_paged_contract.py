@@ -60,3 +60,44 @@ def test_replaced_records_of_a_plan_are_checked(how):
     plan.meta = RECORDS[how](plan.meta)
     with pytest.raises(ValueError, match="plan.meta must be"):
         plan._check()
+
+
+# -------------------------------------------------------------- Qwen2 session
+ROPE = {
+    "default": {},
+    "linear": dict(factor=2.0),
+    "yarn": dict(factor=4.0),
+    "llama3": dict(factor=4.0, low_freq_factor=1.0, high_freq_factor=4.0,
+                   original_max_position_embeddings=64),
+    "dynamic": dict(factor=2.0),
+    "longrope": dict(short_factor=[1.0] * 32, long_factor=[3.0] * 32,
+                     original_max_position_embeddings=64),
+}
+
+
+def qwen2_model(rope="default", device="cpu", max_positions=128):
+    from transformers import Qwen2Config, Qwen2ForCausalLM
+    torch.manual_seed(0)
+    cfg = Qwen2Config(vocab_size=256, hidden_size=256, intermediate_size=256, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2,
+                      max_position_embeddings=max_positions, attn_implementation="eager",
+                      rope_parameters={"rope_type": rope, "rope_theta": 10000.0, **ROPE[rope]})
+    m = Qwen2ForCausalLM(cfg).to(device, torch.bfloat16).eval()
+    for p in m.parameters():
+        p.requires_grad_(False)
+    return m
+
+
+@pytest.mark.parametrize("rope", ROPE)
+def test_frequencies_that_depend_on_the_length_are_refused(rope):
+    """The session's angles are one table, made when it is: of the rope types
+    only those that keep their frequencies past the original length pass."""
+    from moba_hip.qwen2 import Qwen2Branches
+    model = qwen2_model(rope)
+    emb = model.model.rotary_emb
+    before = emb.inv_freq.clone()
+    emb(torch.zeros(1, 300, 256), torch.arange(300)[None])
+    fixed = torch.equal(before, emb.inv_freq)
+    assert fixed == (rope not in ("dynamic", "longrope"))
+    with pytest.raises(ValueError, match="CUDA model required" if fixed else "rope type"):
+        Qwen2Branches(model, 64, 2, 8)

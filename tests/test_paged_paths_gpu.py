@@ -4,7 +4,7 @@ pages or long lookups reach."""
 import pytest
 import torch
 
-from test_paged_contract import RECORDS, REPLACED
+from test_paged_contract import RECORDS, REPLACED, qwen2_model
 from test_rotary_append_gpu import SENTINEL, _case, _run
 from test_shared_prefix_gpu import _pool
 
@@ -83,3 +83,25 @@ def test_attention_refuses_replaced_records(cuda_device, how, given):
     own = torch.tensor([5], dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="the plan on it" if how == "host" else "plan.meta must be"):
         shared_prefix_attention(q, kc, vc, table, own, plan, out=torch.empty_like(q) if given else None)
+
+
+# -------------------------------------------------------------- Qwen2 session
+@pytest.mark.parametrize("rope", ["linear", "yarn", "llama3"])
+def test_branches_of_models_with_fixed_frequencies(cuda_device, rope):
+    """Angles, and the attention factor of yarn, past the original length."""
+    from moba_hip.qwen2 import Qwen2Branches
+    model = qwen2_model(rope, "cuda")
+    g = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, 256, (1, 300), generator=g).to("cuda")
+    extra = torch.randint(0, 256, (6, 2), generator=g).tolist()
+    with Qwen2Branches(model, 300, 2, 8, chunk=64) as s:
+        out = [s.prefill(ids)]
+        s.prepare()
+        out += [s.step(t).clone() for t in extra]
+    for b in range(2):
+        full = torch.cat([ids, torch.tensor([[t[b] for t in extra]], device="cuda")], 1)
+        with torch.no_grad():
+            ref = model(full).logits[0].float()
+        for i, got in enumerate(out):
+            x, y = got[b if i else 0].float(), ref[299 + i]
+            assert torch.nn.functional.cosine_similarity(x, y, dim=0) > 0.999, (b, i)
