@@ -12,9 +12,12 @@
 // their order.  Results do not depend on timing.
 //
 // Scores, softmax and sums are fp32.  Two roundings to 16 bits are the matrix
-// units' price: the weights e^{s - m} before their product with V (their sum z
-// takes them unrounded; at most half a step, 2^-8 or 2^-11 of each weight's
-// share), and the result.
+// units' price: the weights e^{s - m} before their product with V, and the result.
+// A weight is off by at most half a step of its own, 2^-8 (bf16) or 2^-11 (fp16),
+// its sum z takes it unrounded.  fp16 weights reach from 2^7 or more for the
+// largest of a wave's keys to 2^15 (m lies below the maximum by that), so that
+// only what is 2^21 below the largest is subnormal, off by 2^-32 of the largest:
+// a flat tail of 2^17 keys behind one strong key is right to 2^-15.
 //
 // What bounds it: with many pairs to a block the products and the exponentials,
 // which share a SIMD's issue slots (D 128, 1024 rows behind 16K tokens: matrix
@@ -221,8 +224,10 @@ MOBA_DEV void store_partial(const SharedArgs& a, int64_t part, const f32x16_t (&
 }
 
 // A lane's pair's running softmax: reference (log2 domain), sum of this lane's
-// keys, and what the next tile needs of the reference.  The reference stays
-// while the scores are within 2^8 of it.
+// keys, and what the next tile needs of the reference.  The reference is set
+// kBelow below the largest score and stays while the scores are at most kSlack
+// above that one: weights, which are relative to it, reach 2^8 in bf16 and 2^15
+// in fp16 (whose largest value is 65504), where small weights need the room.
 struct Running {
   float m = -INFINITY, l = 0.0f;
   float nm = 0.0f;            // -m; 0 while nothing was attended: weights of
@@ -230,6 +235,7 @@ struct Running {
   float limit = -INFINITY;    // scores above move the reference
 };
 constexpr float kSlack = 8.0f;
+template <int DT> constexpr float kBelow = DT == 0 ? 0.0f : 7.0f;
 
 // Maximum over the lanes l and l + 32.
 MOBA_DEV float max_halves(float x) {
@@ -251,7 +257,7 @@ MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, Running& run, f32
   mx = max_halves(mx) * c2;
   const bool up = mx > run.limit;
   if (__any(up)) [[unlikely]] {
-    const float mn = up ? mx : run.m;
+    const float mn = up ? mx - kBelow<DT> : run.m;
     const float alpha = up ? fast_exp2(run.m - mn) : 1.0f;
     run.l *= alpha;
 #pragma unroll
@@ -260,7 +266,7 @@ MOBA_DEV void softmax_step(const f32x16_t (&s)[NKB], float c2, Running& run, f32
       for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
     run.m = mn;
     run.nm = mn == -INFINITY ? 0.0f : -mn;
-    run.limit = mn + kSlack;
+    run.limit = mn + (kBelow<DT> + kSlack);
     __builtin_amdgcn_sched_barrier(0);
   }
   float ps = 0.0f;

@@ -1,6 +1,9 @@
 """Calls of the paged-cache operators beside the ordinary ones: replaced tables
 and plans, failures inside a step, and the kernels that only far pools, unmapped
 pages or long lookups reach."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
@@ -83,6 +86,46 @@ def test_attention_refuses_replaced_records(cuda_device, how, given):
     own = torch.tensor([5], dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="the plan on it" if how == "host" else "plan.meta must be"):
         shared_prefix_attention(q, kc, vc, table, own, plan, out=torch.empty_like(q) if given else None)
+
+
+# ------------------------------------------------------ small weights in fp16
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("nats", [12.0, 17.0, 17.5, 19.0])
+@pytest.mark.parametrize("rows,d", [(1, 64), (1, 128), (1, 256), (40, 64), (40, 128), (40, 256)])
+def test_flat_tail_behind_one_strong_key_in_fp16(cuda_device, monkeypatch, rows, d, nats, first):
+    """One key of a value of 0 and 16000 keys `nats` below it of values of 1, in
+    one range: the output is the tail's share.  first: the strong key comes
+    before the others; else behind them, when the tail's sums are scaled down.
+
+    A weight lies in fp16 relative to its wave's largest, which is at least 2^7
+    there (at most 2^15), so that it is off by at most half a step, 2^-11 of
+    itself, or below 2^-14 by 2^-25: 2^-32 of the largest weight.  Numerator and z
+    are fp32 sums of positive terms: a lane adds to them at most 16001 / 16 + 16 <
+    2^10 times, each off by at most 2^-24 of the sum (equal terms round alike, so
+    that these add up), 2^-14 in all for each.  The result is rounded by 2^-11 of
+    itself or 2^-25.  Scores are sums of exact products; scaled they are below 2^5,
+    off by 2^-19 at most, 2^-18 of a weight."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    monkeypatch.setattr(SharedPrefixPlan, "_ranges",
+                        lambda self, blocks, *a: (np.full(len(blocks), 1), False))
+    n, page = 16001, 64
+    pages = -(-n // page)
+    kc = torch.zeros((pages, page, 1, d), dtype=torch.float16)
+    vc = torch.ones_like(kc)
+    at = 0 if first else n - 1
+    kc.view(-1, d)[at, 0], vc.view(-1, d)[at] = nats, 0.0
+    q = torch.zeros((rows, 1, d), dtype=torch.float16)
+    q[..., 0] = 1.0
+    table = torch.arange(pages, dtype=torch.int32)[None].cuda()
+    plan = SharedPrefixPlan([0] * rows, [n] * rows, [-1] * rows, 1, 1, d, max_suffix=0)
+    own = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    out, lse = shared_prefix_attention(q.cuda(), kc.cuda(), vc.cuda(), table, own, plan, scale=1.0)
+    tail = (n - 1) * math.exp(-nats)           # relative to the strong key
+    share = tail / (1 + tail)
+    allowed = (2.0 ** -10 + 2.0 ** -13 + 2.0 ** -17) * share + 2.0 ** -25 + (n - 1) * 2.0 ** -32 / (1 + tail)
+    assert (out.double().cpu() - share).abs().max() <= allowed
+    want = nats + math.log1p(tail)
+    assert (lse.double().cpu() - want).abs().max() <= 2.0 ** -14 + 2.0 ** -18 + 2.0 ** -22 * want
 
 
 # -------------------------------------------------------------- Qwen2 session
