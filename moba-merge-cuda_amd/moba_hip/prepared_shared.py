@@ -118,19 +118,18 @@ class PreparedSharedDecode(PreparedDecode):
                 p + n for p, n in zip(step.positions, self.prefix_lengths)):
             raise ValueError("positions exceed the rotary table")
         if step.updates or self._uploaded:
-            # from pinned memory, which torch keeps until the copy is done
-            self.delta.copy_(torch.from_numpy(step.delta).pin_memory(), non_blocking=True)
+            try:   # from pinned memory, which torch keeps until the copy is done
+                self.delta.copy_(torch.from_numpy(step.delta).pin_memory(), non_blocking=True)
+            except BaseException:
+                self.failed = True
+                raise
             self._uploaded = bool(step.updates)
         self._step = step
         return step.positions
 
     def _launch_step(self, stream):
-        try:
-            for name, args in self._calls:
-                _lib.call(name, *args, stream)
-        except _lib.MobaHipError:
-            self.failed = True
-            raise
+        for name, args in self._calls:
+            _lib.call(name, *args, stream)
 
     def _commit_step(self):
         self._lease.commit(self._step)
@@ -144,14 +143,18 @@ class PreparedSharedDecode(PreparedDecode):
             if use_graph and self._graph is None:
                 raise ValueError("capture('step') first")
             positions = self._plan_step(stream)
-            with torch.no_grad():
-                for given, buffer in copies:
-                    buffer.copy_(given)
-            if use_graph:
-                self._graph.replay()
-            else:
-                self._launch_step(stream)
-            self._commit_step()
+            try:
+                with torch.no_grad():
+                    for given, buffer in copies:
+                        buffer.copy_(given)
+                if use_graph:
+                    self._graph.replay()
+                else:
+                    self._launch_step(stream)
+                self._commit_step()
+            except BaseException:   # the device may be a token ahead of the host, or on its way
+                self.failed = True
+                raise
             return self._result(positions)
 
     def attend(self, q, *, use_graph=False):

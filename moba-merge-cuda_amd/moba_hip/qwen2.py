@@ -372,7 +372,7 @@ class Qwen2Branches:
                 self._compute_step()
             for p in self.plans:
                 p._commit_step()
-        except Exception:
+        except BaseException:
             self.failed = True
             for p in self.plans:
                 p.failed = True

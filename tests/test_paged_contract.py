@@ -1,9 +1,14 @@
 """CPU tests of what the paged-cache operators, their prepared step and the
 Qwen2 session refuse, and of how they leave things when a part of them fails."""
+import contextlib
+from types import SimpleNamespace
+
+import numpy as np
 import pytest
 import torch
 
-from moba_hip import RotaryTable, SharedPrefixPlan
+from moba_hip import PreparedSharedDecode, RotaryTable, SharedPrefixPlan, prepared_decode
+from moba_hip.ops import _lib
 
 
 # ------------------------------------------------------------- rotary tables
@@ -62,6 +67,53 @@ def test_replaced_records_of_a_plan_are_checked(how):
         plan._check()
 
 
+# ------------------------------------------------------ failures inside a step
+class _Stop(BaseException):
+    pass
+
+
+@pytest.mark.parametrize("where", ["upload", "copy", "launch", "replay", "commit"])
+@pytest.mark.parametrize("error", [RuntimeError, _lib.MobaHipError, _Stop])
+def test_a_step_that_fails_marks_its_lease(monkeypatch, where, error):
+    """Between its plan and its commit a step may leave the device ahead of the
+    host: such a lease is done with, and its cache when the lease is closed."""
+    def fail(*a, **k):
+        raise error(where)
+
+    def maybe(name):
+        return fail if where == name else (lambda *a, **k: None)
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: SimpleNamespace(cuda_stream=0))
+    monkeypatch.setattr(prepared_decode, "_raw_stream", lambda i: 0)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", maybe("upload"))
+    monkeypatch.setattr(_lib, "call", maybe("launch"))
+    plan = PreparedSharedDecode.__new__(PreparedSharedDecode)
+    step = SimpleNamespace(positions=(0,), updates=(1,) if where == "upload" else (),
+                           delta=np.zeros((2, 1), np.int32))
+    plan.cache = SimpleNamespace(_lock=contextlib.nullcontext(), device=torch.device("cpu"), _stream=0,
+                                 _lessee=plan, _broken=False)
+    plan._lease = SimpleNamespace(plan=lambda: step, commit=maybe("commit"))
+    plan._dev, plan._handle, plan.max_length, plan.rotary = 0, None, 4, None
+    plan._uploaded = plan.closed = plan.failed = plan.check_finite = False
+    plan._calls, plan.delta = [("entry", ())], torch.zeros((2, 1), dtype=torch.int32)
+    plan._graph = SimpleNamespace(replay=maybe("replay"))
+    plan.ids, plan.dense = (0,), True
+    plan.output = plan.lse = None
+    plan.q, plan.k, plan.v = (torch.zeros(1, 1, 8) for _ in range(3))
+    q = SimpleNamespace()
+    monkeypatch.setattr(plan, "_bind_all",
+                        lambda specs: [(q, SimpleNamespace(copy_=maybe("copy")))], raising=False)
+    with pytest.raises(error, match=where):
+        plan.step(q, q, q, use_graph=where == "replay")
+    assert plan.failed
+    with pytest.raises(RuntimeError, match="discard prepared decode"):
+        plan.step(q, q, q)
+    plan.close()
+    assert plan.cache._broken and plan.closed
+
+
 # -------------------------------------------------------------- Qwen2 session
 ROPE = {
     "default": {},
@@ -101,3 +153,28 @@ def test_frequencies_that_depend_on_the_length_are_refused(rope):
     assert fixed == (rope not in ("dynamic", "longrope"))
     with pytest.raises(ValueError, match="CUDA model required" if fixed else "rope type"):
         Qwen2Branches(model, 64, 2, 8)
+
+
+def _branches(monkeypatch, caches, backend="eager"):
+    """A session of two branches on stand-ins for its caches."""
+    from moba_hip.qwen2 import Qwen2Branches
+    monkeypatch.setattr(Qwen2Branches, "_check", lambda self: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: SimpleNamespace(cuda_stream=0))
+    s = Qwen2Branches.__new__(Qwen2Branches)
+    s.caches, s.branches, s.new_tokens, s.hq, s.rotary = caches, 2, 8, 4, None
+    s.device, s.backend, s.tokens = torch.device("cpu"), backend, torch.zeros((2, 1), dtype=torch.long)
+    s.plans, s.graph, s.closed, s.failed, s.logits = [], None, False, False, None
+    s.model = SimpleNamespace(config=SimpleNamespace(vocab_size=9))
+    return s
+
+
+@pytest.mark.parametrize("error", [RuntimeError, _Stop])
+def test_a_session_step_that_fails_marks_every_lease(monkeypatch, error):
+    def fail():
+        raise error("step")
+    s = _branches(monkeypatch, [])
+    s.plans = [SimpleNamespace(_plan_step=lambda stream: None, failed=False) for _ in range(3)]
+    monkeypatch.setattr(s, "_compute_step", fail, raising=False)
+    with pytest.raises(error, match="step"):
+        s.step([1, 2])
+    assert s.failed and all(p.failed for p in s.plans)

@@ -88,6 +88,46 @@ def test_attention_refuses_replaced_records(cuda_device, how, given):
         shared_prefix_attention(q, kc, vc, table, own, plan, out=torch.empty_like(q) if given else None)
 
 
+# ------------------------------------------------------ failures inside a step
+def test_a_failed_replay_ends_the_lease(cuda_device):
+    from moba_hip import PagedKVCache
+    cache = PagedKVCache(2, 64, 2, 64, chunk_size=32)
+    q, k, v = (torch.randn(2, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+    plan = cache.prepare_shared_decode([0, 1], [-1, -1], 4)
+    plan.capture()
+    plan.step(q, k, v, use_graph=True)
+
+    class Broken:
+        def replay(self):
+            raise RuntimeError("replay")
+    plan._graph = Broken()
+    with pytest.raises(RuntimeError, match="replay"):
+        plan.step(q, k, v, use_graph=True)
+    with pytest.raises(RuntimeError, match="discard prepared decode"):
+        plan.step(q, k, v)
+    plan.close()
+    with pytest.raises(RuntimeError, match="discard this cache"):
+        cache.attend_shared(q, sequence_ids=[0, 1], prefix_ids=[-1, -1])
+
+
+def test_a_failed_capture_leaves_the_lease(cuda_device, monkeypatch):
+    """Nothing runs in a capture: the lease goes on, and can be captured later."""
+    from moba_hip import PagedKVCache
+    cache = PagedKVCache(2, 64, 2, 64, chunk_size=32)
+    q, k, v = (torch.randn(2, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+    with cache.prepare_shared_decode([0, 1], [-1, -1], 4) as plan:
+        calls, plan._calls = plan._calls, [("moba_hip_no_such_entry", ())]
+        with pytest.raises(Exception):
+            plan.capture()
+        plan._calls = calls
+        a = plan.step(q, k, v).output.clone()
+        plan.capture()
+        b = plan.step(q, k, v, use_graph=True).output.clone()
+    assert cache.lengths == (2, 2)
+    # the second token's key and value are the first's: the same average
+    assert torch.equal(a, b)
+
+
 # ------------------------------------------------------ small weights in fp16
 @pytest.mark.parametrize("first", [True, False])
 @pytest.mark.parametrize("nats", [12.0, 17.0, 17.5, 19.0])
