@@ -317,24 +317,34 @@ class Qwen2Branches:
         if not self.caches[0].lengths[0]:
             raise ValueError("prefill first")
         ids = list(range(1, 1 + self.branches))
-        self.plans = [c.prepare_shared_decode(ids, [0] * self.branches, self.hq, rotary=self.rotary,
-                                              max_length=self.new_tokens, check_finite=False)
-                      for c in self.caches]
-        if self.backend == "model_graph":
-            side = torch.cuda.Stream(device=self.device)
-            side.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(side):   # lazy torch kernels, on work that changes no cache
-                m = self.model.model
-                h = m.embed_tokens(self.tokens)
-                for layer in m.layers:
-                    project_raw(layer.self_attn, layer.input_layernorm(h))
-                    layer.mlp(layer.post_attention_layernorm(h))
-                self.model.lm_head(m.norm(h))
-            torch.cuda.current_stream(self.device).wait_stream(side)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph, stream=side):
-                self._compute_step()
-            self.graph = graph
+        try:
+            for c in self.caches:
+                self.plans.append(c.prepare_shared_decode(
+                    ids, [0] * self.branches, self.hq, rotary=self.rotary,
+                    max_length=self.new_tokens, check_finite=False))
+            if self.backend == "model_graph":
+                self._capture()
+        except BaseException:   # all layers or none: the caches as before, to be prepared again
+            made, self.plans, self.logits = self.plans, [], None
+            for p in made:
+                p.close()
+            raise
+
+    def _capture(self):
+        side = torch.cuda.Stream(device=self.device)
+        side.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(side):   # lazy torch kernels, on work that changes no cache
+            m = self.model.model
+            h = m.embed_tokens(self.tokens)
+            for layer in m.layers:
+                project_raw(layer.self_attn, layer.input_layernorm(h))
+                layer.mlp(layer.post_attention_layernorm(h))
+            self.model.lm_head(m.norm(h))
+        torch.cuda.current_stream(self.device).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            self._compute_step()
+        self.graph = graph
 
     def _compute_step(self):
         """Device work of one step on the current stream (capturable)."""

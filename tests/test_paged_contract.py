@@ -178,3 +178,37 @@ def test_a_session_step_that_fails_marks_every_lease(monkeypatch, error):
     with pytest.raises(error, match="step"):
         s.step([1, 2])
     assert s.failed and all(p.failed for p in s.plans)
+
+
+@pytest.mark.parametrize("fails", [0, 2, "capture"])
+@pytest.mark.parametrize("error", [ValueError, _Stop])
+def test_a_session_that_cannot_be_prepared_keeps_no_lease(monkeypatch, fails, error):
+    """A failure at any layer, or in the capture, gives back what was leased
+    before it; the session can be prepared again."""
+    leased = set()
+
+    def lease(i):
+        def make(*a, **k):
+            if fails == i:
+                raise error("prepare")
+            assert i not in leased
+            leased.add(i)
+            return SimpleNamespace(close=lambda: leased.remove(i))
+        return make
+
+    def capture():
+        if fails == "capture":
+            raise error("prepare")
+    s = _branches(monkeypatch, [SimpleNamespace(lengths=(5, 0, 0), prepare_shared_decode=lease(i))
+                                for i in range(3)], "model_graph")
+    monkeypatch.setattr(s, "_capture", capture, raising=False)
+    with pytest.raises(error, match="prepare"):
+        s.prepare()
+    assert not leased and not s.plans and s.graph is None
+    with pytest.raises(ValueError, match="prepare first"):
+        s.step([1, 2])
+    fails = None
+    s.prepare()
+    assert leased == {0, 1, 2} and len(s.plans) == 3
+    s.close()
+    assert not leased

@@ -188,3 +188,31 @@ def test_branches_of_models_with_fixed_frequencies(cuda_device, rope):
         for i, got in enumerate(out):
             x, y = got[b if i else 0].float(), ref[299 + i]
             assert torch.nn.functional.cosine_similarity(x, y, dim=0) > 0.999, (b, i)
+
+
+def test_branches_prepared_again_after_a_failure(cuda_device, monkeypatch):
+    """A capture that fails in the second layer's launches, then one that holds:
+    the steps are those of a session that never failed."""
+    from moba_hip.qwen2 import Qwen2Branches
+    model = qwen2_model("default", "cuda")
+    ids = torch.randint(0, 256, (1, 100), generator=torch.Generator().manual_seed(2)).to("cuda")
+    outs = []
+    for failing in (False, True):
+        with Qwen2Branches(model, 100, 2, 8, chunk=64, backend="model_graph") as s:
+            s.prefill(ids)
+            if failing:
+                with monkeypatch.context() as m:
+                    def broken(self, stream):
+                        if self is s.plans[1]:
+                            raise RuntimeError("launch")
+                        launch(self, stream)
+                    from moba_hip import PreparedSharedDecode
+                    launch = PreparedSharedDecode._launch_step
+                    m.setattr(PreparedSharedDecode, "_launch_step", broken)
+                    with pytest.raises(RuntimeError):
+                        s.prepare()
+                assert not s.plans and s.graph is None
+            s.prepare()
+            outs.append([s.step([3 + i, 7 * i]).clone() for i in range(4)])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
