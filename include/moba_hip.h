@@ -408,7 +408,7 @@ int moba_hip_decode_attend_noalloc(const void* q, int dtype, int Nq, int Hq, int
  * 2^30.  Workspaces part_o [parts*Hq, D] and part_ml [parts*Hq, 2] fp32, parts =
  * sum of all ranges.  out [Nq,Hq,D] (dtype), lse [Nq,Hq] fp32 natural log;
  * nothing attended: zeros and -inf.  A token in an unmapped page is not attended.
- * q, k_cache, v_cache, out: 16-byte aligned.  Two launches; results do not depend on timing. */
+ * scale in [2^-126, 1e30].  q, k_cache, v_cache, out: 16-byte aligned.  Two launches; results do not depend on timing. */
 int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
                               float scale, const void* k_cache, const void* v_cache,
                               int num_pages, int page_size, const int* table, int table_width,

@@ -219,7 +219,7 @@ PyObject* shared_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     return not_here();
   const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)x.d)
                        : PyFloat_Check(a[6]) ? PyFloat_AS_DOUBLE(a[6]) : 0.0;
-  if (!(scale > 0.0 && scale < 1e30)) return not_here();
+  if (!(scale >= 0x1p-126 && scale < 1e30)) return not_here();
   if ((((uintptr_t)q->data_ptr()) | (uintptr_t)p.k | (uintptr_t)p.v) & 15) return not_here();
   if (a[7] != Py_None || a[8] != Py_None) return not_here();
   void* stream;

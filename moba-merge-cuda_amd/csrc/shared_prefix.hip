@@ -977,7 +977,7 @@ extern "C" int moba_hip_shared_attention(const void* q, int dtype, int Nq, int H
   if (dtype != 0 && dtype != 1) { moba_set_error("shared_attention: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
   if (D < 8 || D > 256 || D % 8) { moba_set_error("shared_attention: head_dim must be a multiple of 8 in [8,256]"); return MOBA_ERR_ARG; }
   if (Nq < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || (int64_t)Nq * Hq >= 1ll << 31) { moba_set_error("shared_attention: Nq * Hq in [1, 2^31) and Hq a multiple of Hkv required"); return MOBA_ERR_ARG; }
-  if (!(scale > 0.0f) || scale > 1e30f) { moba_set_error("shared_attention: scale must be positive and finite"); return MOBA_ERR_ARG; }
+  if (!(scale >= 0x1p-126f) || scale > 1e30f) { moba_set_error("shared_attention: scale must be positive and finite, in [2^-126, 1e30]"); return MOBA_ERR_ARG; }
   if (num_pages < 1 || page_size < 1 || table_width < 1 || (int64_t)num_pages * page_size >= 1ll << 31 ||
       (int64_t)table_width * page_size >= 1ll << 31) { moba_set_error("shared_attention: nonempty page pool and table below 2^31 tokens required"); return MOBA_ERR_ARG; }
   if ((int64_t)Hkv * D >= 1ll << 30) { moba_set_error("shared_attention: Hkv * D below 2^30 required"); return MOBA_ERR_ARG; }

@@ -268,6 +268,15 @@ def _check_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan):
     _check_index(suffix_lengths, "suffix_lengths", 1, dev, plan.rows)
 
 
+def _scale(scale):
+    """A scale that fp32 holds: one that it flushed to 0 would make NaN of masked
+    scores, -inf times 0."""
+    scale = float(scale)
+    if not 2.0 ** -126 <= scale <= 1e30:
+        raise ValueError("scale must be positive and finite, in [2^-126, 1e30]")
+    return scale
+
+
 def _check_output(t, name, shape, like, dtype):
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != dtype or \
             t.device != like.device or not t.is_contiguous():
@@ -283,9 +292,10 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     k_cache, v_cache [pages,page_size,Hkv,D] and page_table [slots,width] int32
     as in :func:`moba_hip.append_rotary`; ``suffix_lengths`` [Nq] int32: how many
     tokens of its own slot each row attends (read on the device, cut to
-    [0, plan.max_suffix]).  ``scale`` defaults to D ** -0.5.  A row with nothing
-    to attend gives zeros and an lse of -inf; a token in an unmapped page is
-    not attended.  Nothing is read back, so a call can be captured into a graph
+    [0, plan.max_suffix]).  ``scale`` (in [2^-126, 1e30]) defaults to D ** -0.5.
+    q, the pool and ``out`` must be 16-byte aligned.  A row with nothing to
+    attend gives zeros and an lse of -inf; a token in an unmapped page is not
+    attended.  Nothing is read back, so a call can be captured into a graph
     (``out`` and ``lse``, contiguous, then keep their addresses)."""
     done = _lib.calls().shared_attention(q, k_cache, v_cache, page_table, suffix_lengths, plan, scale,
                                          out, lse)
@@ -295,9 +305,7 @@ def shared_prefix_attention(q, k_cache, v_cache, page_table, suffix_lengths, pla
     pages, page, hkv, d = k_cache.shape
     width = page_table.shape[1]
     n, hq = plan.rows, plan.num_q_heads
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite")
+    scale = d ** -0.5 if scale is None else _scale(scale)
     q = q.contiguous()
     qp, kp, vp = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
     if (qp | kp | vp) & 15:

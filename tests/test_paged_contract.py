@@ -9,6 +9,7 @@ import torch
 
 from moba_hip import PreparedSharedDecode, RotaryTable, SharedPrefixPlan, prepared_decode
 from moba_hip.ops import _lib
+from moba_hip.shared_prefix import _scale
 
 
 # ------------------------------------------------------------- rotary tables
@@ -65,6 +66,26 @@ def test_replaced_records_of_a_plan_are_checked(how):
     plan.meta = RECORDS[how](plan.meta)
     with pytest.raises(ValueError, match="plan.meta must be"):
         plan._check()
+
+
+# ------------------------------------------------------------------- the scale
+SCALES = [0.0, -1.0, 1e-46, 1e-39, 1.1e30, 1e39, float("inf"), float("nan")]
+
+
+@pytest.mark.parametrize("scale", SCALES)
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    with pytest.raises(ValueError, match="scale must be"):
+        _scale(scale)
+    lib = _lib.load()
+    args = dict(q=64, dtype=0, Nq=1, hq=2, hkv=2, D=64, scale=scale, kc=64, vc=64, pages=1, page=16,
+                table=64, width=1, lengths=64, add=0, max_length=16, items=64, n_items=0, rows=64,
+                parts=64, max_parts=1, uneven=0, part_o=64, part_ml=64, out=64, lse=64, stream=None)
+    assert lib.moba_hip_shared_attention(*args.values()) == _lib.MOBA_ERR_ARG
+    assert "scale" in lib.moba_hip_last_error().decode()
+
+
+def test_scales_at_the_border():
+    assert _scale(2.0 ** -126) == 2.0 ** -126 and _scale(1) == 1.0 and _scale(1e30) == 1e30
 
 
 # ------------------------------------------------------ failures inside a step

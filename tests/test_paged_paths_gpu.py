@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_paged_contract import RECORDS, REPLACED, qwen2_model
+from test_paged_contract import RECORDS, REPLACED, SCALES, qwen2_model
 from test_rotary_append_gpu import SENTINEL, _case, _run
 from test_shared_prefix_gpu import _pool
 
@@ -86,6 +86,41 @@ def test_attention_refuses_replaced_records(cuda_device, how, given):
     own = torch.tensor([5], dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="the plan on it" if how == "host" else "plan.meta must be"):
         shared_prefix_attention(q, kc, vc, table, own, plan, out=torch.empty_like(q) if given else None)
+
+
+@pytest.mark.parametrize("scale", [*SCALES, 2e30, 2])
+def test_scales(cuda_device, scale):
+    """Refused in one way by calls with and without an output of the caller's;
+    a whole number is a scale."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    kc, vc, table, _, _ = _pool([100, 5], 2, 64, 16, torch.bfloat16, 2)
+    plan = SharedPrefixPlan([0], [100], [1], 4, 2, 64, max_suffix=5)
+    q = torch.randn(1, 4, 64, device="cuda").bfloat16()
+    own = torch.tensor([5], dtype=torch.int32, device="cuda")
+    for out in (None, torch.empty_like(q)):
+        def call(scale):
+            return shared_prefix_attention(q, kc, vc, table, own, plan, scale=scale, out=out)
+        if scale == 2:
+            assert torch.equal(call(2)[0].clone(), call(2.0)[0])
+        else:
+            with pytest.raises(ValueError, match="scale must be"):
+                call(scale)
+
+
+def test_smallest_scale_with_masked_tiles(cuda_device):
+    """All scores near 0: the mean of the attended values, whatever is masked."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    kc, vc, table, _, vs = _pool([100, 70], 1, 64, 16, torch.bfloat16, 2)
+    plan = SharedPrefixPlan([-1] * 3, [0] * 3, [1] * 3, 2, 1, 64, max_suffix=70)
+    q = torch.randn(3, 2, 64, device="cuda").bfloat16()
+    own = torch.tensor([1, 70, 0], dtype=torch.int32, device="cuda")
+    out, lse = shared_prefix_attention(q, kc, vc, table, own, plan, scale=2.0 ** -126)
+    assert torch.equal(out[0], vs[1][0].cuda().expand(2, 64)) and (out[2] == 0).all()
+    mean = vs[1].double().mean(0)
+    # weights of 1 exactly; sums of 70 terms in fp32, one rounding
+    tol = 2.0 ** -8 * mean.abs() + 70 * 2.0 ** -24 * vs[1].double().abs().mean(0) + 2.0 ** -20
+    assert ((out[1].double().cpu() - mean).abs() <= tol).all()
+    assert (lse[1] - math.log(70)).abs().max() < 1e-5 and (lse[2] == float("-inf")).all()
 
 
 # ------------------------------------------------------ failures inside a step
