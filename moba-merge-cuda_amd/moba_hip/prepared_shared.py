@@ -56,6 +56,7 @@ class PreparedSharedDecode(PreparedDecode):
             self._shared_buffers(len(self.ids))
             self._calls = self._launches(len(self.ids))
             self._uploaded = False    # the device delta holds a grant not yet committed
+            self._delta_uploads = 0
             self._graph = None
             self.closed = self.failed = False
             cache._lessee = self   # the lease starts once everything above succeeded
@@ -107,6 +108,10 @@ class PreparedSharedDecode(PreparedDecode):
             ptr(self.lse))))
         return calls
 
+    @property
+    def delta_uploads(self):
+        return self._delta_uploads
+
     # parts of a step, as PreparedDecode has them for whole-model steps
     def _plan_step(self, stream):
         """Plans one token per row and uploads its page grants; changes nothing
@@ -124,6 +129,7 @@ class PreparedSharedDecode(PreparedDecode):
                 self.failed = True
                 raise
             self._uploaded = bool(step.updates)
+            self._delta_uploads += 1
         self._step = step
         return step.positions
 

@@ -117,6 +117,7 @@ def test_a_step_that_fails_marks_its_lease(monkeypatch, where, error):
                                  _lessee=plan, _broken=False)
     plan._lease = SimpleNamespace(plan=lambda: step, commit=maybe("commit"))
     plan._dev, plan._handle, plan.max_length, plan.rotary = 0, None, 4, None
+    plan._delta_uploads = 0
     plan._uploaded = plan.closed = plan.failed = plan.check_finite = False
     plan._calls, plan.delta = [("entry", ())], torch.zeros((2, 1), dtype=torch.int32)
     plan._graph = SimpleNamespace(replay=maybe("replay"))

@@ -145,6 +145,28 @@ def test_a_failed_replay_ends_the_lease(cuda_device):
         cache.attend_shared(q, sequence_ids=[0, 1], prefix_ids=[-1, -1])
 
 
+def test_page_grants_are_uploaded_when_a_page_begins(cuda_device):
+    """delta_uploads counts as PreparedDecode's does: rows of 0 and 5 tokens on
+    pages of 16, 40 steps."""
+    from moba_hip import PagedKVCache
+    counts = []
+    for shared in (False, True):
+        cache = PagedKVCache(2, 64, 2, 64, page_size=16, chunk_size=32)
+        k = torch.randn(5, 2, 64, device="cuda").bfloat16()
+        cache.append(k, k, sequence_ids=[1], cu_seqlens=[0, 5])
+        q, k, v = (torch.randn(2, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+        with (cache.prepare_shared_decode([0, 1], [-1, -1], 4) if shared else
+              cache.prepare_decode([0, 1], 4, mode="dense")) as plan:
+            assert plan.delta_uploads == 0
+            seen = []
+            for _ in range(40):
+                plan.step(q, k, v)
+                seen.append(plan.delta_uploads)
+            counts.append(seen)
+    assert counts[0] == counts[1]
+    assert counts[1][0] == 1 and counts[1][-1] == 5   # at tokens 0, 16, 32 and 16, 32 of the rows
+
+
 def test_a_failed_capture_leaves_the_lease(cuda_device, monkeypatch):
     """Nothing runs in a capture: the lease goes on, and can be captured later."""
     from moba_hip import PagedKVCache
