@@ -256,6 +256,7 @@ class Qwen2Branches:
         self.capacity = positive_int(capacity, "capacity")
         self.branches = positive_int(branches, "branches")
         self.new_tokens = positive_int(new_tokens, "new_tokens")
+        page = positive_int(page, "page_size")
         self.model, self.backend, self.chunk = model, backend, positive_int(chunk, "chunk")
         self.device = next(model.parameters()).device
         if self.device.type != "cuda":

@@ -234,3 +234,14 @@ def test_a_session_that_cannot_be_prepared_keeps_no_lease(monkeypatch, fails, er
     assert leased == {0, 1, 2} and len(s.plans) == 3
     s.close()
     assert not leased
+
+
+@pytest.mark.parametrize("kw,match", [(dict(page=0), "page_size"), (dict(page=None), "page_size"),
+                                      (dict(page=16.0), "page_size"), (dict(branches=0), "branches"),
+                                      (dict(new_tokens=True), "new_tokens"), (dict(chunk=-1), "chunk"),
+                                      (dict(capacity="9"), "capacity"), (dict(backend="graph"), "backend")])
+def test_sizes_of_a_session_are_checked(kw, match):
+    """Before anything is divided by them or asked of a device."""
+    from moba_hip.qwen2 import Qwen2Branches
+    with pytest.raises(ValueError, match=match):
+        Qwen2Branches(qwen2_model(), **{"capacity": 64, "branches": 2, "new_tokens": 8, **kw})
