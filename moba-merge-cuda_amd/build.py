@@ -3,9 +3,11 @@
 Every ``csrc/*.hip`` (device code) and ``csrc/*.cpp`` (host-only runtime:
 page pool, prepared-decode driver) file is compiled to an object under ``_build/`` and
 linked into ``moba_hip/libmoba_hip.so``.  ``csrc/python/calls.cpp`` (host-only,
-against torch's headers) becomes the extension ``moba_hip/_calls.so``.  Objects are rebuilt when their
-source or any header changed.  ``python build.py`` builds; ``--force``
-rebuilds everything.
+against torch's headers) becomes the extension ``moba_hip/_calls.so``, for the
+torch and Python that build it; without torch the library alone is built, which is
+all that callers of the C-ABI need.  Objects are rebuilt when their source or any
+header changed, the extension's also when its torch or Python did.  ``python
+build.py`` builds; ``--force`` rebuilds everything.
 """
 from __future__ import annotations
 
@@ -60,30 +62,46 @@ def _compile(src: Path, force: bool) -> Path:
     return obj
 
 
-def _compile_calls(force: bool) -> Path:
-    src, obj = CSRC / "python" / "calls.cpp", OUT_DIR / "calls.cpp.o"
-    if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, _headers()):
-        import sysconfig
-
+def _calls_target():
+    """(what _calls.so is built for, include paths, library folder), or None
+    without torch, whose headers it needs."""
+    try:
         import torch
         from torch.utils.cpp_extension import include_paths
-        dirs = [*include_paths(), sysconfig.get_paths()["include"]]
-        abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-w",
-               f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *[f"-I{d}" for d in dirs], "-c", str(src), "-o",
-               str(obj)]
+    except ImportError:
+        return None
+    import sysconfig
+    dirs = [*include_paths(), sysconfig.get_paths()["include"]]
+    flags = [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *[f"-I{d}" for d in dirs]]
+    built_for = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
+    return built_for, flags, Path(torch.__file__).parent / "lib"
+
+
+def _compile_calls(force: bool):
+    target = _calls_target()
+    if target is None:
+        return None
+    built_for, flags, _ = target
+    src, obj, stamp = CSRC / "python" / "calls.cpp", OUT_DIR / "calls.cpp.o", OUT_DIR / "calls.cpp.for"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-w", *flags,
+           f'-DMOBA_BUILT_FOR="{built_for}"', "-c", str(src), "-o", str(obj)]
+    made = stamp.read_text() if stamp.exists() else None
+    if force or made != " ".join(cmd) or not obj.exists() or \
+            obj.stat().st_mtime < max(src.stat().st_mtime, _headers()):
+        stamp.unlink(missing_ok=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("g++ failed on calls.cpp")
+        stamp.write_text(" ".join(cmd))
     return obj
 
 
 def _link_calls(obj: Path, force: bool) -> None:
     if not force and CALLS.exists() and CALLS.stat().st_mtime >= obj.stat().st_mtime:
         return
-    import torch
-    libs = Path(torch.__file__).parent / "lib"
+    libs = _calls_target()[2]
     tmp = CALLS.with_suffix(f".so.{os.getpid()}")
     subprocess.check_call([os.environ.get("CXX", "g++"), "-shared", str(obj), "-o", str(tmp),
                            f"-L{LIB.parent}", "-l:libmoba_hip.so", "-Wl,-rpath,$ORIGIN",
@@ -103,7 +121,10 @@ def build(force: bool = False, jobs: int = 8) -> Path:
         cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
         subprocess.check_call(cmd)
         os.replace(tmp, LIB)
-    _link_calls(calls.result(), force)
+    if calls.result() is None:
+        sys.stderr.write("no torch: libmoba_hip.so alone is built, without the Python host path\n")
+    else:
+        _link_calls(calls.result(), force)
     return LIB
 
 

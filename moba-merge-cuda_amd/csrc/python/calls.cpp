@@ -271,5 +271,7 @@ PyMODINIT_FUNC PyInit__calls(void) {
   s_interleaved = PyUnicode_InternFromString("interleaved");
   s_packed = PyUnicode_InternFromString("_packed");
   s_meta = PyUnicode_InternFromString("meta");
-  return PyModule_Create(&module);
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", MOBA_BUILT_FOR)) Py_CLEAR(m);
+  return m;
 }

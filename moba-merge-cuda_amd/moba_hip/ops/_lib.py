@@ -139,6 +139,7 @@ def calls():
     global _calls
     if _calls is None:
         import importlib.util
+        import sys
 
         import torch
 
@@ -149,9 +150,17 @@ def calls():
         if not path.exists():
             raise MobaHipError(f"{path} is missing: build it with "
                                "`python moba-merge-cuda_amd/build.py`")
+        # its calls are compiled against torch's classes: another torch's may
+        # lie otherwise in memory
+        here = f"torch {torch.__version__}, Python {sys.version_info[0]}.{sys.version_info[1]}"
         spec = importlib.util.spec_from_file_location("moba_hip._calls", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise MobaHipError(f"{path} does not load with {here}: build it again ({e})") from e
+        if module.built_for != here:
+            raise MobaHipError(f"{path} is built for {module.built_for}, this is {here}: build it again")
         module.bind(torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, MobaHipError,
                     RotaryTable, SharedPrefixPlan)
         _calls = module
