@@ -9,7 +9,8 @@ import torch
 
 from test_paged_contract import RECORDS, REPLACED, SCALES, qwen2_model
 from test_rotary_append_gpu import SENTINEL, _case, _run
-from test_shared_prefix_gpu import _pool
+from test_shared_prefix_gpu import _exact, _pool
+from test_shared_prefix_gpu import _run as _attend
 
 pytestmark = pytest.mark.gpu
 
@@ -183,6 +184,124 @@ def test_a_failed_capture_leaves_the_lease(cuda_device, monkeypatch):
     assert cache.lengths == (2, 2)
     # the second token's key and value are the first's: the same average
     assert torch.equal(a, b)
+
+
+# ------------------------------------------- every kernel against 64 bits
+@pytest.fixture(scope="module")
+def far_memory(cuda_device):
+    """Room for a K and a V pool of more than 4 GiB (and 2^31 elements) each."""
+    flat = [torch.empty(2400 << 20, dtype=torch.int16, device="cuda") for _ in range(2)]
+    yield flat
+    flat.clear()
+    torch.cuda.empty_cache()
+
+
+def _laid_out(lengths, holes, hkv, d, page, dtype, far, seed):
+    """Pools and table of sequences, whose logical pages `holes` (slot, page) are
+    unmapped; (k_cache, v_cache, table, cells, ks, vs): tensors of the mapped
+    tokens alone, and their cells.  Cells of no token hold NaN."""
+    g = torch.Generator().manual_seed(seed)
+    width = max(-(-n // page) for n in lengths) + 1
+    need = sum(-(-n // page) for n in lengths) + 2
+    if far is None:
+        pages = need
+        kc, vc = (torch.empty((pages, page, hkv, d), dtype=dtype, device="cuda") for _ in range(2))
+        ids = torch.randperm(pages, generator=g).tolist()
+    else:   # over the whole of the pool, its first and last pages among them
+        pages = far[0].numel() // (page * hkv * d)
+        kc, vc = (t[:pages * page * hkv * d].view(dtype).view(pages, page, hkv, d) for t in far)
+        assert kc.numel() * 2 > 2 ** 32
+        ids = torch.linspace(0, pages - 1, need, dtype=torch.float64).long()
+        ids = ids[torch.randperm(need, generator=g)].tolist()
+    used = torch.tensor(ids, device="cuda")
+    kc[used], vc[used] = float("nan"), float("nan")
+    table = torch.full((len(lengths), width), -1, dtype=torch.int32)
+    at, cells, ks, vs = 0, [], [], []
+    for slot, n in enumerate(lengths):
+        for lp in range(-(-n // page)):
+            if (slot, lp) not in holes:
+                table[slot, lp] = ids[at]
+            elif lp % 2:
+                table[slot, lp] = pages + 5     # no page of the pool either
+            at += 1
+        i = torch.tensor([t for t in range(n) if (slot, t // page) not in holes], dtype=torch.long)
+        cell = (table[slot].long()[i // page] * page + i % page).cuda()
+        k, v = (torch.randn(len(i), hkv, d, generator=g).to("cuda", dtype) for _ in range(2))
+        kc.view(-1, hkv, d)[cell], vc.view(-1, hkv, d)[cell] = k, v
+        cells.append(cell), ks.append(k), vs.append(v)
+    return kc, vc, table.cuda(), cells, ks, vs
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [40, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("form,rows", [("wide", 20), ("narrow", 6), ("solo", 6)])
+@pytest.mark.parametrize("slots", ["each", "one"])
+@pytest.mark.parametrize("where", ["near", "far"])
+def test_every_kernel_against_64_bits(far_memory, monkeypatch, where, slots, form, rows, d, dtype):
+    """Items of four waves with 32 pairs each, of four with the same pairs and of
+    single waves, each with more keys than one lookup holds (1024, 256) and
+    unmapped pages among them; rows with an own slot each, and all with one at
+    lengths of their own; pools below and above 4 GiB.
+
+    Allowed, with A = sum_j p_j |v_j| / z: half a step of A for the weights and
+    of the result; scores and their scale 2 (D + 4) 2^-24 S of A, S the largest
+    sum of |q_d k_d| scale; 2^-15 of A for fp32 sums of at most 3800 / 16 + 16 < 2^8
+    additions in numerator and z; in fp16 2^-32 of the largest weight for weights
+    and 2^-25 for results below the normal ones.  Values that are not finite then go
+    in at two tokens of the one slot, and reach the rows that attend them."""
+    from moba_hip import SharedPrefixPlan, shared_prefix_attention
+    monkeypatch.setattr(SharedPrefixPlan, "_ranges",
+                        lambda self, blocks, *a: (np.full(len(blocks), 1), form == "solo"))
+    hq, hkv, page, plen = 4, 2, 64 if where == "far" else 16, 2500
+    own = [[1300, 700, 1, 1201, 64, 1025, 0, 1024, 701, 1100][i % 10] for i in range(rows)]
+    suffix = [1 + i if slots == "each" else 1 for i in range(rows)]
+    lengths = [plen] + (own if slots == "each" else [1300])
+    holes = {(0, 3), (0, 1100 // page), (1, 2)}
+    kc, vc, table, cells, ks, vs = _laid_out(lengths, holes, hkv, d, page, dtype,
+                                             far_memory if where == "far" else None, d + rows)
+    g = torch.Generator().manual_seed(7)
+    q = torch.randn(rows, hq, d, generator=g).to("cuda", dtype)
+    plan = SharedPrefixPlan([0] * rows, [plen] * rows, suffix, hq, hkv, d, max_suffix=1300)
+    dev_own = torch.tensor(own, dtype=torch.int32, device="cuda")
+    out, lse = shared_prefix_attention(q, kc, vc, table, dev_own, plan)
+
+    mapped = [sum((s, t // page) not in holes for t in range(n)) for s, n in zip(suffix, own)]
+    want, wl, A, S, V = [t.cuda() for t in _exact(q, ks, vs, [0] * rows, [len(ks[0])] * rows, suffix,
+                                                  mapped, d ** -0.5)]
+    eps = torch.finfo(dtype).eps
+    rel = 2 * (d + 4) * 2.0 ** -24 * S + 2.0 ** -15
+    tol = eps / 2 * (A + want.abs()) * (1 + 2.0 ** -6) + rel[..., None] * A
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -32 * V + 2.0 ** -25
+    assert ((out.double() - want).abs() <= tol).all()
+    assert ((lse.double() - wl).abs() <= rel + 2.0 ** -22 * wl.abs()).all()
+
+    if slots == "one":
+        inf, nan = float("inf"), float("nan")
+        before = sum((1, t // page) not in holes for t in range(700))
+        later = sum((1, t // page) not in holes for t in range(1200))
+        flat = vc.view(-1, hkv, d)
+        flat[cells[1][before], 0, :2] = torch.tensor([-inf, inf], dtype=dtype, device="cuda")
+        flat[cells[1][later], 0, :3] = torch.tensor([inf, inf, nan], dtype=dtype, device="cuda")
+        odd, odd_lse = shared_prefix_attention(q, kc, vc, table, dev_own, plan)
+        want = out.clone()
+        for i, n in enumerate(own):
+            if n > 700:    # the heads of kv head 0
+                want[i, :2, :2] = torch.tensor([-inf, inf], dtype=dtype, device="cuda")
+            if n > 1200:   # -inf and inf; inf twice; NaN
+                want[i, :2, :3] = torch.tensor([nan, inf, nan], dtype=dtype, device="cuda")
+        assert torch.equal(odd_lse, lse)
+        assert torch.equal(torch.nan_to_num(odd, nan=123.0), torch.nan_to_num(want, nan=123.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,d", [(513, 64), (300, 256)])
+def test_long_extension_of_one_sequence(cuda_device, tokens, d, dtype):
+    """Several hundred new tokens behind a prefix: blocks of one sequence's rows
+    whose lengths end in tiles of their own."""
+    n = tokens + 150
+    _attend([200, n], [0] * tokens, [200] * tokens, [1] * tokens, list(range(n - tokens + 1, n + 1)),
+            2, 1, d, 16, dtype)
 
 
 # ------------------------------------------------------ small weights in fp16
