@@ -248,7 +248,8 @@ int moba_hip_paged_append(const void* k, const void* v, int dtype, int N, int Hk
  * token_seq -1 marks padding: nothing of the token is written.  A token whose
  * slot, page or angle does not exist has no key and value written (nor, without
  * slot or angle, its query) and sets bit 1, 2 or 4 of *status (nullable; the
- * caller clears it first).  Two tokens of one cell leave either's data. */
+ * caller clears it first).  Two tokens of one cell leave it undefined: key and
+ * value may each hold pieces of both. */
 int moba_hip_append_rotary(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                            const void* k, int64_t k_token_stride, int64_t k_head_stride,
                            const void* v, int64_t v_token_stride, int64_t v_head_stride,

@@ -188,9 +188,10 @@ def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
     the table, in an unmapped page or past the rotary table has no key and
     value written either, nor, past the rotary table, its query; with ``check`` such
     tokens, and two tokens of one slot and position, raise RuntimeError after the
-    launch (one device-to-host copy).  Without it, two tokens of one cell leave
-    either's data.  A tensor of the call, the table's too, that is used on
-    another stream than its own must be kept until that work is done."""
+    launch (one device-to-host copy).  Two tokens of one cell leave it undefined:
+    its key and its value may each hold pieces of both.  A tensor of the call, the
+    table's too, that is used on another stream than its own must be kept until
+    that work is done."""
     if not check:
         done = _lib.calls().append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos,
                                           rotary, q, q_out, offsets)

@@ -174,7 +174,8 @@ def test_a_failed_capture_leaves_the_lease(cuda_device, monkeypatch):
     cache = PagedKVCache(2, 64, 2, 64, chunk_size=32)
     q, k, v = (torch.randn(2, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
     with cache.prepare_shared_decode([0, 1], [-1, -1], 4) as plan:
-        calls, plan._calls = plan._calls, [("moba_hip_no_such_entry", ())]
+        calls = plan._calls
+        plan._calls = [calls[0], ("moba_hip_no_such_entry", ())]
         with pytest.raises(Exception):
             plan.capture()
         plan._calls = calls
