@@ -5,8 +5,10 @@ persistent buffers overwritten by the next call, ``step`` / ``capture`` /
 ``close``).  A step takes one token per leased row before its rotation, turns
 its key and query by prefix length plus own position, appends it and attends
 the row's prefix and its own tokens: the page delta and positions, the rotary
-append, the mean of a chunk that it closes, and shared-prefix attention, six
-launches whose arguments never change, so that one hipGraph replays them.
+append, the mean of a chunk that it closes, and the two of shared-prefix attention,
+five launches whose arguments never change, so that one hipGraph replays them.  A
+lease makes the plan of its batch and holds the partials of its step; a model's
+layers have one each.
 """
 from __future__ import annotations
 

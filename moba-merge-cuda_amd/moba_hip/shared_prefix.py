@@ -3,8 +3,10 @@
 A prefix (a system prompt, a document, a prompt that is sampled several times)
 is stored once, in a slot of its own, and read once for all the query rows
 behind it; each row then attends the tokens of its own slot.  The plan of a
-batch is made once and serves every layer and step: which rows share what is
-fixed, their own lengths are read on the device.
+batch holds which rows share what; their own lengths are read on the device, so
+one plan serves every call on that batch, of whichever layer and step, that its
+maker passes it to.  (The cache's ``attend_shared`` and its prepared steps make
+plans of their own, one per cache and so one per layer.)
 """
 from __future__ import annotations
 
@@ -27,9 +29,10 @@ _WIDE, _NARROW = 128, 32
 # many; a key's, per dim, times what the items of one CU make of each other
 # (alone, and per item; wide items, narrow ones); the rates at which partials are
 # written and read, and K/V, bytes per us; the merge's time per range of a row, us.
-# Fitted to 140 batches, each timed cut in 6 to 30 ways (prefixes to 128K tokens,
-# 1 to 400 rows, 40 to 256 dims): what is taken is 2% behind the best of them on
-# average.
+# These ten, and three that stand in the formulas below (an item is long from 0.83 of
+# the longest, half of a late one counts, a norm of order 7), are fitted to 140
+# batches, each timed cut in 6 to 30 ways (prefixes to 128K tokens, 1 to 400 rows, 40
+# to 256 dims): what is taken is 2% behind the best of them on average.
 _CUS, _HELD = 256, (3, 2)
 _ITEM, _OF_MANY, _KEY = 6.4, 5.0, 2.2e-4
 _ON_A_CU = (0.8, 0.27), (0.65, 0.5)
