@@ -168,6 +168,43 @@ def test_page_grants_are_uploaded_when_a_page_begins(cuda_device):
     assert counts[1][0] == 1 and counts[1][-1] == 5   # at tokens 0, 16, 32 and 16, 32 of the rows
 
 
+@pytest.mark.parametrize("graph", [False, True])
+def test_rows_that_begin_their_pages_at_steps_of_their_own(cuda_device, graph):
+    """Rows of 0, 5, 16 and 31 tokens behind prefixes of 40, 0 and 77: the grant of
+    one row's page is replayed with the steps after it and changes no other row's.
+    Outputs against 64 bits over what the cache holds, within half a bf16 step of
+    the weights' sum and of the result, and fp32's 2^-12 of it."""
+    from moba_hip import PagedKVCache, RotaryTable
+    hq, hkv, d, starts = 4, 2, 64, (0, 5, 16, 31)
+    cache, rt = PagedKVCache(7, 160, hkv, d, page_size=16, chunk_size=32), RotaryTable(d, 300)
+    g = torch.Generator().manual_seed(3)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g).to("cuda", torch.bfloat16)
+    for slot, n in [(4, 40), (6, 77), *((i, n) for i, n in enumerate(starts) if n)]:
+        cache.append_rotary(rand(n, hkv, d), rand(n, hkv, d), rt, sequence_ids=[slot], cu_seqlens=[0, n])
+    prefix = [4, -1, 6, 6]
+    with cache.prepare_shared_decode([0, 1, 2, 3], prefix, hq, rotary=rt, max_length=100) as plan:
+        if graph:
+            plan.capture()
+        for t in range(45):
+            q, k, v = rand(4, hq, d), rand(4, hkv, d), rand(4, hkv, d)
+            res = plan.step(q, k, v, use_graph=graph)
+            assert res.positions == tuple(n + t for n in starts)
+            if t % 4:
+                continue
+            for r, own in enumerate(starts):
+                ks, vs = zip(*(cache.materialize(s) for s in ([prefix[r]] if prefix[r] >= 0 else []) + [r]))
+                kk, vv = (torch.cat(x).double().repeat_interleave(hq // hkv, 1) for x in (ks, vs))
+                assert len(kk) == own + t + 1 + (cache.lengths[prefix[r]] if prefix[r] >= 0 else 0)
+                x = plan._turned[r].double()
+                p = torch.softmax((x * kk).sum(-1) * d ** -0.5, 0)[..., None]
+                want, A = (p * vv).sum(0), (p * vv.abs()).sum(0)
+                tol = 2.0 ** -8 * (A + want.abs()) * (1 + 2.0 ** -6) + 2.0 ** -12 * A
+                assert ((res.output[r].double() - want).abs() <= tol).all(), (t, r)
+    assert cache.lengths[:4] == tuple(n + 45 for n in starts)
+
+
 def test_a_failed_capture_leaves_the_lease(cuda_device, monkeypatch):
     """Nothing runs in a capture: the lease goes on, and can be captured later."""
     from moba_hip import PagedKVCache
