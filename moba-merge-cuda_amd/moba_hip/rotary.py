@@ -191,7 +191,7 @@ def append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos, rota
     launch (one device-to-host copy).  Two tokens of one cell leave it undefined:
     its key and its value may each hold pieces of both.  A tensor of the call, the
     table's too, that is used on another stream than its own must be kept until
-    that work is done."""
+    that work is done, and those of a captured call for as long as it is replayed."""
     if not check:
         done = _lib.calls().append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos,
                                           rotary, q, q_out, offsets)
