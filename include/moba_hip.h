@@ -418,6 +418,71 @@ int moba_hip_shared_attention(const void* q, int dtype, int Nq, int Hq, int Hkv,
                               int uneven, float* part_o, float* part_ml, void* out, float* lse,
                               void* stream);
 
+/* -------------------------------------------------------- 8-bit KV pages
+ *
+ * No counterpart in the reference, whose caches hold 16 bits.  A pool holds codes
+ * k_codes/v_codes [num_pages][Hkv][page_size][Dp], one byte each (format 0: int8, 1:
+ * the 8-bit float e4m3; Dp = D rounded up to 16), and scales k_scale/v_scale
+ * [num_pages][Hkv][page_size] fp32, one per token and kv head.  A row x of D values (a
+ * multiple of 8 in [8,256]) has a = max(max |x|, 2^-100), scale a / top and codes x
+ * top / a, rounded to the nearest, ties to even (top 127 or 448); a row with an infinity
+ * or a NaN has codes 0 and scale NaN.  Codes are 16-byte aligned, at most 64 GiB.
+ * table [B][table_width]: physical page per logical page, -1 none. */
+
+/* N new tokens k/v [N,Hkv,D] go into the pool at (token_seq[n], token_pos[n]); with
+ * a table of angles cos_sin (nullable) the keys turn first and the queries q (Hq > 0)
+ * of the same tokens turn into q_out [N,Hq,D].  Arguments, padding (slot -1), what is
+ * left unwritten and the bits of *status as in moba_hip_append_rotary; the rotation's
+ * products are rounded each, and a key is quantised from fp32. */
+int moba_hip_quantized_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                              const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                              int dtype, int N, int Hq, int Hkv, int D, const float* cos_sin,
+                              int max_pos, int rotary_dim, int interleaved, int format,
+                              void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                              int num_pages, int page_size, const int* table, int B,
+                              int table_width, const int* token_seq, const int* token_pos,
+                              const int* offsets, void* q_out, int* status, void* stream);
+
+/* The values of N stored tokens, code times scale rounded to dtype: k_out/v_out
+ * [N,Hkv,D], 16-byte aligned.  A token of slot -1, and one without a cell (which sets
+ * bit 1 or 2 of *status, nullable), reads as zeros. */
+int moba_hip_quantized_read(int format, const void* k_codes, const void* v_codes,
+                            const float* k_scale, const float* v_scale, int num_pages,
+                            int page_size, int Hkv, int D, const int* table, int B,
+                            int table_width, const int* token_seq, const int* token_pos, int N,
+                            int dtype, void* k_out, void* v_out, int* status, void* stream);
+
+/* moba_hip_block_means of an 8-bit pool: the means of the stored values of closed chunks,
+ * in the same canonical order, rounded to dtype. */
+int moba_hip_quantized_means(int format, const void* k_codes, const float* k_scale, int num_pages,
+                             int page_size, int Hkv, int D, const int* table, int B,
+                             int table_width, const int* item_seq, const int* item_chunk_or_pos,
+                             int n_items, int mode, int chunk, int dtype, void* means,
+                             int max_chunks, void* stream);
+
+/* Attention of q [Nq,Hq,D] over the pool: row r attends the first lengths[r] + length_add
+ * (device; cut to [0, max_length]) tokens of slot q_seq[r], or with selected
+ * [Nq,Hq,slots] (nullable, slots in [1,16]) those of them in the chunks of `chunk` tokens
+ * that each head selected (-1 none, any order; chunks behind the length hold nothing).
+ * out [Nq,Hq,D] (dtype), lse [Nq,Hq] fp32 natural log; a row or head that attends nothing
+ * (a slot outside [0, B) too) gets zeros and -inf.  A token in an unmapped page is not
+ * attended.  scale in [2^-126, 1e30].  work: moba_hip_quantized_attention_work bytes, of
+ * this call alone until it is done.  q, out and work 16-byte aligned.  Two launches,
+ * three with selected; results do not depend on timing. */
+int moba_hip_quantized_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
+                                 float scale, int format, const void* k_codes,
+                                 const void* v_codes, const float* k_scale, const float* v_scale,
+                                 int num_pages, int page_size, const int* table, int B,
+                                 int table_width, const int* q_seq, const int* lengths,
+                                 int length_add, int max_length, const int* selected, int slots,
+                                 int chunk, void* work, void* out, float* lse, void* stream);
+
+/* Bytes of that workspace for the same arguments (-1 for bad ones), max_length before or
+ * after it is cut to the table's table_width * page_size tokens. */
+int64_t moba_hip_quantized_attention_work(int Nq, int Hq, int Hkv, int D, int slots, int chunk,
+                                          int max_length);
+
 /* ------------------------------------------------ host page pool (CPU only)
  *
  * The page allocator of the paged KV cache as a host object (no device

@@ -361,6 +361,25 @@ template <int ROWS, typename Args> MOBA_DEV ExpertTile expert_tile(const Args& a
           min(ROWS, a.counts[lo] - first)};
 }
 
+// n / d by multiplication, exact for n < 2^31 (mul 0 stands for d = 1):
+// mul = ceil(2^(31 + s) / d) with 2^(s - 1) < d <= 2^s exceeds 2^(31 + s) / d by
+// less than 1, so the product is too large by less than n / 2^(31 + s) < 1 / d.
+struct FastDiv {
+  uint32_t mul, shift, d;
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f{0, 0, d};
+  if (d <= 1) return f;
+  uint32_t s = 1;
+  while ((1ull << s) < d) ++s;
+  f.shift = s - 1;
+  f.mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+  return f;
+}
+MOBA_DEV uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return f.mul ? __umulhi(n, f.mul) >> f.shift : n;
+}
+
 // Wave issue priority (0 or 1): a wave in an MFMA-heavy phase is set ahead of
 // a wave in an element-wise phase on the same SIMD, which keeps the matrix
 // unit fed.  No scheduling fences: the compiler keeps s_setprio in order with

@@ -1,0 +1,441 @@
+// 8-bit paged KV cache on gfx950: tokens quantised as they are written, read back,
+// and the chunk means that routing takes of the stored keys.  Formats, layout and
+// rounding: quant.h.  The attention that reads the pool: quant_attn.hip.
+//
+// Append: keys turn by their positions first (as in rotary.hip: pairs (i, i + R/2) or
+// (2i, 2i + 1), y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos, fp32, here with
+// each product rounded), and are quantised from fp32, so that a stored key is
+// rounded once.  Several lanes hold a row; the maximum of |x| goes through them.
+#include <algorithm>
+
+#include "quant.h"
+#include "../../include/moba_hip.h"
+
+using namespace moba;
+
+namespace moba {
+int quant_pool_of(const char* what, int format, const void* k, const void* v, const float* ks,
+                  const float* vs, int num_pages, int page_size, int Hkv, int D, const int* table,
+                  int B, int W, QuantPool& p) {
+  if (format != 0 && format != 1) { moba_set_error("%s: format must be 0 (int8) or 1 (fp8)", what); return MOBA_ERR_ARG; }
+  if (num_pages < 1 || page_size < 1 || Hkv < 1 || B < 1 || W < 1) { moba_set_error("%s: nonempty page pool and table required", what); return MOBA_ERR_ARG; }
+  if (D < 8 || D > 256 || D % 8) { moba_set_error("%s: head_dim must be a multiple of 8 in [8,256]", what); return MOBA_ERR_ARG; }
+  if ((int64_t)num_pages * page_size >= 1ll << 31 || (int64_t)W * page_size >= 1ll << 31) { moba_set_error("%s: page pool exceeds int32 token capacity", what); return MOBA_ERR_ARG; }
+  p.Dp = code_width(D);
+  // rows and 16-byte pieces of codes are counted in 32 bits: 64 GiB of codes
+  if ((int64_t)num_pages * page_size * Hkv > 0xfffffff0ll / (p.Dp / 16)) { moba_set_error("%s: page pool exceeds 64 GiB of codes", what); return MOBA_ERR_ARG; }
+  if ((((uintptr_t)k | (uintptr_t)v) & 15) || (((uintptr_t)ks | (uintptr_t)vs) & 3)) { moba_set_error("%s: codes must be 16-byte aligned", what); return MOBA_ERR_ARG; }
+  p.k = (uint8_t*)k; p.v = (uint8_t*)v; p.ks = (float*)ks; p.vs = (float*)vs;
+  p.num_pages = num_pages; p.P = page_size; p.Hkv = Hkv; p.D = D;
+  p.by_page = fast_div(page_size);
+  p.table = table; p.B = B; p.W = W;
+  return MOBA_OK;
+}
+}  // namespace moba
+
+namespace {
+
+enum { kBadSlot = 1, kBadCell = 2, kBadAngle = 4 };
+
+MOBA_DEV void report(int* status, int what) {
+  if (status != nullptr) atomicOr(status, what);
+}
+
+// ------------------------------------------------------------------ append
+struct AppendArgs {
+  QuantPool pool;
+  const uint16_t *q, *k, *v;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // token and head strides, elements
+  int Hq, R, lanes, inter;                     // lanes of a row, a power of two
+  uint32_t rows;                               // N * (Hq + 2 Hkv)
+  FastDiv by_token;                            // Hq + 2 Hkv
+  const float2* cos_sin;
+  int max_pos;
+  const int *seq, *pos, *offsets;
+  uint16_t* q_out;
+  int* status;
+};
+
+// A row of work: its input, its row of angles (null: it does not turn), and where
+// it goes: q_out's row (cell -1), or a cell of the pool.
+struct Row {
+  const uint16_t* src;
+  const float2* turn;
+  uint16_t* q_dst;
+  int64_t cell;
+  bool is_v;
+};
+// False: nothing of the row is written.
+MOBA_DEV bool locate(const AppendArgs& a, uint32_t row, bool first_lane, Row& r) {
+  const uint32_t t = div_by(row, a.by_token);
+  const uint32_t h = row - t * a.by_token.d;
+  const int s = a.seq[t], p = a.pos[t];
+  if (s < 0 || s >= a.pool.B) {  // padding (-1), or no such slot: left as it was
+    if (s != -1 && h == 0 && first_lane) report(a.status, kBadSlot);
+    return false;
+  }
+  bool angle = true;
+  r.turn = nullptr;
+  if (a.cos_sin != nullptr) {
+    // the table's row, in 64 bits: position + offset may pass 31
+    const int64_t rp = (int64_t)p + (a.offsets != nullptr ? a.offsets[s] : 0);
+    angle = rp >= 0 && rp < a.max_pos;
+    if (!angle && h == 0 && first_lane) report(a.status, kBadAngle);
+    r.turn = a.cos_sin + (angle ? rp : 0) * (a.R / 2);
+  }
+  r.cell = -1;
+  r.is_v = false;
+  if (h < (uint32_t)a.Hq) {
+    r.src = a.q + (int64_t)t * a.q_ts + (int64_t)h * a.q_hs;
+    r.q_dst = a.q_out + ((int64_t)t * a.Hq + h) * a.pool.D;
+    return angle;
+  }
+  const uint32_t kv = h - a.Hq;
+  r.is_v = kv >= (uint32_t)a.pool.Hkv;
+  const int kh = (int)(r.is_v ? kv - a.pool.Hkv : kv);
+  r.cell = pool_row(a.pool, s, p, kh);
+  if (r.cell < 0 && kv == 0 && first_lane) report(a.status, kBadCell);
+  r.src = r.is_v ? a.v + (int64_t)t * a.v_ts + (int64_t)kh * a.v_hs
+                 : a.k + (int64_t)t * a.k_ts + (int64_t)kh * a.k_hs;
+  if (r.is_v) r.turn = nullptr;
+  return r.cell >= 0 && angle;  // a token without its angle has neither key nor value written
+}
+
+MOBA_DEV void rotate(float& x, float& y, float2 t) {
+  const float a = x * t.x - y * t.y, b = x * t.y + y * t.x;
+  x = a;
+  y = b;
+}
+
+// The largest |x| of a row, as bits, over its lanes (on: the lane has dims of it).
+template <int N> MOBA_DEV uint32_t row_max(const float (&v)[N], bool on, int lanes) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  m = on ? m : 0u;
+  for (int off = 1; off < lanes; off <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
+  return m;
+}
+
+// Eight codes of v from dim d on.
+template <int FMT> MOBA_DEV void store_codes(uint8_t* dst, const float* v, const RowScale& r) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = r.finite ? to_code<FMT>(v[i], r) : 0.0f;
+  uint2 w;
+  w.x = codes4<FMT>(y[0], y[1], y[2], y[3]);
+  w.y = codes4<FMT>(y[4], y[5], y[6], y[7]);
+  *reinterpret_cast<uint2*>(dst) = w;
+}
+
+MOBA_DEV void store_scale(const AppendArgs& a, const Row& r, float scale) {
+  (r.is_v ? a.pool.vs : a.pool.ks)[r.cell] = scale;
+}
+
+// Rows of whole 16-byte pieces, R a multiple of 16 (0: nothing turns): a lane has
+// two pieces of 8 dims, those at 8u and 8u + R/2 of what turns, or the pieces c and
+// c + n of the 2n behind R, so that a pair's two values are in one lane and
+// neighbouring lanes have neighbouring pieces.
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = idx / a.lanes;
+  if (row >= a.rows) return;
+  const int u = (int)(idx & (a.lanes - 1)), D = a.pool.D;
+  Row r;
+  if (!locate(a, row, u == 0, r)) return;
+  const int turning = r.turn != nullptr ? a.R / 16 : 0, from = turning * 16;
+  const int n = (D - from) / 16, c = u - turning;
+  const bool on = u < D / 16, turns = u < turning;
+  const int d0 = turns ? 8 * u : on ? from + 8 * c : 0, d1 = turns ? d0 + a.R / 2 : on ? d0 + 8 * n : 0;
+  const u32x4_t x = *reinterpret_cast<const u32x4_t*>(r.src + d0);
+  const u32x4_t y = *reinterpret_cast<const u32x4_t*>(r.src + d1);
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unpack2<DT>(x[i], v[2 * i], v[2 * i + 1]);
+    unpack2<DT>(y[i], v[8 + 2 * i], v[9 + 2 * i]);
+  }
+  if (turns) {
+    if (a.inter) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {  // two pairs an access, as the table has them
+        const float4 w = *reinterpret_cast<const float4*>(r.turn + (i < 4 ? d0 / 2 + i : d1 / 2 + i - 4));
+        rotate(v[2 * i], v[2 * i + 1], make_float2(w.x, w.y));
+        rotate(v[2 * i + 2], v[2 * i + 3], make_float2(w.z, w.w));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float4 w = *reinterpret_cast<const float4*>(r.turn + d0 + i);
+        rotate(v[i], v[8 + i], make_float2(w.x, w.y));
+        rotate(v[i + 1], v[9 + i], make_float2(w.z, w.w));
+      }
+    }
+  }
+  if (r.cell < 0) {
+    if (!on) return;
+    st8(r.q_dst + d0, pack8<DT>(v));
+    st8(r.q_dst + d1, pack8<DT>(v + 8));
+    return;
+  }
+  const RowScale s = row_scale<FMT>(row_max(v, on, a.lanes));
+  if (u == 0) store_scale(a, r, s.scale);
+  if (!on) return;
+  uint8_t* dst = (r.is_v ? a.pool.v : a.pool.k) + r.cell * a.pool.Dp;
+  store_codes<FMT>(dst + d0, v, s);
+  store_codes<FMT>(dst + d1, v + 8, s);
+}
+
+// Any other row: a lane has 8 neighbouring dims and reads the partner of each one
+// that turns by itself.  WIDE: rows are whole 16-byte pieces.
+template <int DT, int FMT, bool WIDE>
+__global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t row = idx / a.lanes;
+  if (row >= a.rows) return;
+  const int u = (int)(idx & (a.lanes - 1)), D = a.pool.D, half = a.R / 2;
+  Row r;
+  if (!locate(a, row, u == 0, r)) return;
+  const bool on = 8 * u < D;
+  const int d = on ? 8 * u : 0;
+  float v[8];
+  if constexpr (WIDE) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(r.src + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack2<DT>(x[i], v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to_f32<DT>(r.src[d + e]);
+  }
+  if (r.turn != nullptr && d < a.R) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int de = d + e;
+      if (de >= a.R) continue;
+      const bool second = a.inter ? de & 1 : de >= half;
+      const int other = a.inter ? de ^ 1 : (second ? de - half : de + half);
+      const float2 t = r.turn[a.inter ? de >> 1 : (second ? de - half : de)];
+      float mine = v[e], theirs = to_f32<DT>(r.src[other]);
+      if (second) rotate(theirs, mine, t);
+      else rotate(mine, theirs, t);
+      v[e] = mine;
+    }
+  }
+  if (r.cell < 0) {
+    if (!on) return;
+    if constexpr (WIDE) {
+      st8(r.q_dst + d, pack8<DT>(v));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r.q_dst[d + e] = from_f32<DT>(v[e]);
+    }
+    return;
+  }
+  const RowScale s = row_scale<FMT>(row_max(v, on, a.lanes));
+  if (u == 0) store_scale(a, r, s.scale);
+  uint8_t* dst = (r.is_v ? a.pool.v : a.pool.k) + r.cell * a.pool.Dp;
+  if (on) store_codes<FMT>(dst + d, v, s);
+  else if (8 * u < a.pool.Dp) *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(0, 0);  // behind D
+}
+
+template <int DT, int FMT> void launch_append(AppendArgs& a, bool wide, hipStream_t st) {
+  const int D = a.pool.D;
+  const bool pairs = wide && D % 16 == 0 && a.R % 16 == 0;
+  const int units = pairs ? D / 16 : a.pool.Dp / 8;
+  a.lanes = 1;
+  while (a.lanes < units) a.lanes *= 2;
+  const dim3 grid((unsigned)(((uint64_t)a.rows * a.lanes + 255) / 256)), block(256);
+  if (pairs) hipLaunchKernelGGL((append_pairs_kernel<DT, FMT>), grid, block, 0, st, a);
+  else if (wide) hipLaunchKernelGGL((append_any_kernel<DT, FMT, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((append_any_kernel<DT, FMT, false>), grid, block, 0, st, a);
+}
+
+// Whether every row begins at a 16-byte border.
+bool whole_pieces(const void* p, int64_t ts, int64_t hs) {
+  return (uintptr_t)p % 16 == 0 && ts % 8 == 0 && hs % 8 == 0;
+}
+
+// -------------------------------------------------------------------- read
+struct ReadArgs {
+  QuantPool pool;
+  uint32_t total;  // N * Hkv * 2 * (D / 8) pieces of 8 codes
+  FastDiv by_row, by_token;
+  const int *seq, *pos;
+  uint16_t *k_out, *v_out;
+  int* status;
+};
+
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= a.total) return;
+  const uint32_t row = div_by(idx, a.by_row), u = idx - row * a.by_row.d;
+  const uint32_t t = div_by(row, a.by_token), h = row - t * a.by_token.d;  // keys, then values
+  const bool is_v = h >= (uint32_t)a.pool.Hkv;
+  const int kh = (int)(is_v ? h - a.pool.Hkv : h), s = a.seq[t];
+  const int64_t cell = pool_row(a.pool, s, a.pos[t], kh);
+  uint16_t* dst = (is_v ? a.v_out : a.k_out) + ((int64_t)t * a.pool.Hkv + kh) * a.pool.D + 8 * u;
+  if (cell < 0) {  // padding, or no such cell: zeros
+    if (s != -1 && h == 0 && u == 0) report(a.status, s < 0 || s >= a.pool.B ? kBadSlot : kBadCell);
+    st8(dst, zero8());
+    return;
+  }
+  const uint2 w = *reinterpret_cast<const uint2*>((is_v ? a.pool.v : a.pool.k) + cell * a.pool.Dp + 8 * u);
+  const float scale = (is_v ? a.pool.vs : a.pool.ks)[cell];
+  float x[4], y[4], v[8];
+  numbers4<FMT>(w.x, x);
+  numbers4<FMT>(w.y, y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = x[i] * scale;
+    v[4 + i] = y[i] * scale;
+  }
+  st8(dst, pack8<DT>(v));
+}
+
+// ------------------------------------------------------------------- means
+constexpr int kMeansPer = 16;  // tokens of a lane: chunks of up to 1024
+
+// One wave per (item, kv head, 8 dims): lane j sums the stored numbers of tokens
+// j, j + 64, ... in order, then canon_tree, as the 16-bit cache's means do.  All
+// lookups, then all loads, then the sums; a token without a cell adds nothing.
+// A wave of modest size: a chunk closes once in `chunk` tokens.
+template <int DT, int FMT>
+__global__ __launch_bounds__(64) void means_kernel(QuantPool p, const int* __restrict__ seq,
+                                                   const int* __restrict__ chunk_or_pos, int mode,
+                                                   int C, uint16_t* __restrict__ means,
+                                                   int max_chunks) {
+  const int nd = p.D / 8, db = blockIdx.x % nd, kh = (blockIdx.x / nd) % p.Hkv;
+  const int i = blockIdx.x / (nd * p.Hkv), lane = threadIdx.x;
+  const int sid = seq[i];
+  int chunk = chunk_or_pos[i];
+  if (mode == 1) {
+    if ((chunk + 1) % C != 0) return;
+    chunk = chunk / C;
+  }
+  if (sid < 0 || sid >= p.B || chunk < 0 || chunk >= max_chunks) return;
+  int64_t row[kMeansPer];
+#pragma unroll
+  for (int k = 0; k < kMeansPer; ++k) {
+    const int j = lane + 64 * k;
+    row[k] = j < C ? pool_row(p, sid, chunk * C + j, kh) : -1;
+  }
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMeansPer; ++k) {
+    const int64_t at = row[k] >= 0 ? row[k] : 0;
+    const uint2 w = *reinterpret_cast<const uint2*>(p.k + at * p.Dp + 8 * db);
+    const float scale = p.ks[at];
+    float x[4], y[4];
+    numbers4<FMT>(w.x, x);
+    numbers4<FMT>(w.y, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[e] += row[k] >= 0 ? x[e] * scale : 0.0f;
+      acc[4 + e] += row[k] >= 0 ? y[e] * scale : 0.0f;
+    }
+  }
+  uint16_t res[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) res[e] = from_f32<DT>(canon_tree(acc[e]) / (float)C);
+  if (lane == 0) {
+    uint16_t* dst = means + (((int64_t)sid * max_chunks + chunk) * p.Hkv + kh) * p.D + 8 * db;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dst[e] = res[e];
+  }
+}
+
+}  // namespace
+
+extern "C" int moba_hip_quantized_append(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                                         const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                                         int dtype, int N, int Hq, int Hkv, int D,
+                                         const float* cos_sin, int max_pos, int rotary_dim,
+                                         int interleaved, int format, void* k_codes, void* v_codes,
+                                         float* k_scale, float* v_scale, int num_pages, int page_size,
+                                         const int* table, int B, int table_width,
+                                         const int* token_seq, const int* token_pos,
+                                         const int* offsets, void* q_out, int* status, void* stream) {
+  AppendArgs a;
+  const int rc = quant_pool_of("quantized_append", format, k_codes, v_codes, k_scale, v_scale, num_pages,
+                               page_size, Hkv, D, table, B, table_width, a.pool);
+  if (rc) return rc;
+  if (dtype != 0 && dtype != 1) { moba_set_error("quantized_append: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
+  if (N < 1 || Hq < 0) { moba_set_error("quantized_append: nonempty N required"); return MOBA_ERR_ARG; }
+  if (cos_sin != nullptr && (rotary_dim < 2 || rotary_dim > D || rotary_dim % 2 || max_pos < 1)) { moba_set_error("quantized_append: rotary_dim must be even, in [2, D], and the table nonempty"); return MOBA_ERR_ARG; }
+  if ((uintptr_t)cos_sin & 15) { moba_set_error("quantized_append: the cos / sin table must be 16-byte aligned"); return MOBA_ERR_ARG; }
+  if ((Hq > 0) != (q != nullptr) || (Hq > 0) != (q_out != nullptr) || (Hq > 0 && cos_sin == nullptr)) { moba_set_error("quantized_append: q, q_out and the cos / sin table go together with Hq > 0"); return MOBA_ERR_ARG; }
+  if ((int64_t)N * (Hq + 2ll * Hkv) * a.pool.Dp >= 1ll << 31) { moba_set_error("quantized_append: more than 2^31 elements in one call"); return MOBA_ERR_ARG; }
+  a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
+  a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.k_ts = k_token_stride; a.k_hs = k_head_stride;
+  a.v_ts = v_token_stride; a.v_hs = v_head_stride;
+  a.Hq = Hq; a.R = cos_sin != nullptr ? rotary_dim : 0; a.inter = interleaved;
+  a.by_token = fast_div(Hq + 2 * Hkv);
+  a.rows = (uint32_t)N * a.by_token.d;
+  a.cos_sin = (const float2*)cos_sin; a.max_pos = max_pos;
+  a.seq = token_seq; a.pos = token_pos; a.offsets = offsets;
+  a.q_out = (uint16_t*)q_out; a.status = status;
+  const bool wide = whole_pieces(k, a.k_ts, a.k_hs) && whole_pieces(v, a.v_ts, a.v_hs) &&
+                    (Hq == 0 || (whole_pieces(q, a.q_ts, a.q_hs) && whole_pieces(q_out, 0, 0)));
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0) { if (format == 0) launch_append<0, 0>(a, wide, st); else launch_append<0, 1>(a, wide, st); }
+  else { if (format == 0) launch_append<1, 0>(a, wide, st); else launch_append<1, 1>(a, wide, st); }
+  return moba_launch_status("quantized_append");
+}
+
+extern "C" int moba_hip_quantized_read(int format, const void* k_codes, const void* v_codes,
+                                       const float* k_scale, const float* v_scale, int num_pages,
+                                       int page_size, int Hkv, int D, const int* table, int B,
+                                       int table_width, const int* token_seq, const int* token_pos,
+                                       int N, int dtype, void* k_out, void* v_out, int* status,
+                                       void* stream) {
+  ReadArgs a;
+  const int rc = quant_pool_of("quantized_read", format, k_codes, v_codes, k_scale, v_scale, num_pages,
+                               page_size, Hkv, D, table, B, table_width, a.pool);
+  if (rc) return rc;
+  if (dtype != 0 && dtype != 1) { moba_set_error("quantized_read: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
+  if (N < 1) { moba_set_error("quantized_read: nonempty N required"); return MOBA_ERR_ARG; }
+  if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) { moba_set_error("quantized_read: outputs must be 16-byte aligned"); return MOBA_ERR_ARG; }
+  if ((int64_t)N * 2 * Hkv * D >= 1ll << 31) { moba_set_error("quantized_read: more than 2^31 elements in one call"); return MOBA_ERR_ARG; }
+  a.by_row = fast_div(D / 8);
+  a.by_token = fast_div(2 * Hkv);
+  a.total = (uint32_t)N * 2 * Hkv * (D / 8);
+  a.seq = token_seq; a.pos = token_pos;
+  a.k_out = (uint16_t*)k_out; a.v_out = (uint16_t*)v_out; a.status = status;
+  const dim3 grid((a.total + 255) / 256), block(256);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == 0 && format == 0) hipLaunchKernelGGL((read_kernel<0, 0>), grid, block, 0, st, a);
+  else if (dtype == 0) hipLaunchKernelGGL((read_kernel<0, 1>), grid, block, 0, st, a);
+  else if (format == 0) hipLaunchKernelGGL((read_kernel<1, 0>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((read_kernel<1, 1>), grid, block, 0, st, a);
+  return moba_launch_status("quantized_read");
+}
+
+extern "C" int moba_hip_quantized_means(int format, const void* k_codes, const float* k_scale,
+                                        int num_pages, int page_size, int Hkv, int D, const int* table,
+                                        int B, int table_width, const int* item_seq,
+                                        const int* item_chunk_or_pos, int n_items, int mode, int chunk,
+                                        int dtype, void* means, int max_chunks, void* stream) {
+  if (n_items <= 0) return MOBA_OK;
+  QuantPool p;
+  const int rc = quant_pool_of("quantized_means", format, k_codes, k_codes, k_scale, k_scale, num_pages,
+                               page_size, Hkv, D, table, B, table_width, p);
+  if (rc) return rc;
+  if (dtype != 0 && dtype != 1) { moba_set_error("quantized_means: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
+  if (chunk < 1 || chunk > 64 * kMeansPer || max_chunks < 1) { moba_set_error("quantized_means: chunk must be in [1,1024], the means nonempty"); return MOBA_ERR_ARG; }
+  if ((int64_t)n_items * Hkv * (D / 8) >= 1ll << 31 || (int64_t)max_chunks * chunk >= 1ll << 31) { moba_set_error("quantized_means: more than 2^31 pieces or positions"); return MOBA_ERR_ARG; }
+  const dim3 grid((unsigned)((int64_t)n_items * Hkv * (D / 8))), block(64);
+  hipStream_t st = (hipStream_t)stream;
+#define MOBA_MEANS(DT_, FMT_)                                                                       \
+  hipLaunchKernelGGL((means_kernel<DT_, FMT_>), grid, block, 0, st, p, item_seq, item_chunk_or_pos, \
+                     mode, chunk, (uint16_t*)means, max_chunks)
+  if (dtype == 0) { if (format == 0) MOBA_MEANS(0, 0); else MOBA_MEANS(0, 1); }
+  else { if (format == 0) MOBA_MEANS(1, 0); else MOBA_MEANS(1, 1); }
+#undef MOBA_MEANS
+  return moba_launch_status("quantized_means");
+}

@@ -12,5 +12,6 @@ from .merge import merge_forward  # noqa: F401
 from .kv_cache import ContiguousKVCache, DecodeResult, PagedKVCache  # noqa: F401
 from .prepared_decode import PreparedDecode  # noqa: F401
 from .prepared_shared import PreparedSharedDecode  # noqa: F401
+from .quantized import QuantizedPages, quantized_append, quantized_attention, quantized_read  # noqa: F401
 from .rotary import RotaryTable, append_rotary  # noqa: F401
 from .shared_prefix import SharedPrefixPlan, shared_prefix_attention  # noqa: F401

@@ -63,6 +63,15 @@ SIGNATURES = {
                                _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P],
     "moba_hip_shared_attention": [_P, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I,
                                   _P, _P, _I, _I, _P, _P, _P, _P, _P],
+    "moba_hip_quantized_append": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _P, _I, _I, _I,
+                                  _I, _P, _P, _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P],
+    "moba_hip_quantized_read": [_I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _P, _P,
+                                _P, _P],
+    "moba_hip_quantized_means": [_I, _P, _P, _I, _I, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _I, _P, _I,
+                                 _P],
+    "moba_hip_quantized_attention": [_P, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _I, _I, _P, _I, _I,
+                                     _P, _P, _I, _I, _P, _I, _I, _P, _P, _P, _P],
+    "moba_hip_quantized_attention_work": [_I, _I, _I, _I, _I, _I, _I],
     # host page pool (CPU only)
     "moba_pool_create": [_I, _I, _I, _I, _I, _PP],
     "moba_pool_destroy": [_P],
@@ -95,7 +104,8 @@ _I32P = ctypes.POINTER(ctypes.c_int32)
 _RESTYPES = {"moba_hip_merge_work": ctypes.c_int64, "moba_pool_destroy": None, "moba_prep_destroy": None,
              "moba_prep_delta_uploads": ctypes.c_int64, "moba_pool_table": _I32P, "moba_pool_lengths": _I32P,
              "moba_pool_free": _I32P, "moba_hip_last_error": ctypes.c_char_p, "moba_hip_pack_experts_work": ctypes.c_int64,
-             "moba_hip_prefill_bwd_work": ctypes.c_int64}
+             "moba_hip_prefill_bwd_work": ctypes.c_int64,
+             "moba_hip_quantized_attention_work": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()
