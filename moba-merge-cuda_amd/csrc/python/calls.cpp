@@ -25,7 +25,7 @@ PyObject* g_stream;   // torch._C._cuda_getCurrentRawStream
 PyObject* g_device;   // torch._C._cuda_getDevice
 PyObject* g_error;    // MobaHipError
 PyObject *s_cos_sin, *s_rotary_dim, *s_interleaved, *s_packed, *s_meta;
-PyTypeObject *t_rotary, *t_plan;
+PyTypeObject *t_rotary, *t_plan, *t_pages;
 
 // Borrowed tensor of a Python argument, null if it is none.
 const at::Tensor* tensor_in(PyObject* o) {
@@ -116,6 +116,25 @@ bool int_attr(PyObject* o, PyObject* name, int64_t& out) {
   return !PyErr_Occurred();
 }
 
+// The table of a RotaryTable, an attribute that a caller may replace.
+struct Angles {
+  THPObjectPtr ref;
+  const at::Tensor* cs = nullptr;
+  int64_t rotary_dim = 0, inter = 0;
+};
+// 1: it serves heads of d on device idx; 0: not here; -1: an error is set.
+int angles_of(PyObject* o, int idx, int64_t d, Angles& x) {
+  if (Py_TYPE(o) != t_rotary) return 0;
+  x.ref = THPObjectPtr(PyObject_GetAttr(o, s_cos_sin));
+  if (!x.ref) return -1;
+  if (!int_attr(o, s_rotary_dim, x.rotary_dim) || !int_attr(o, s_interleaved, x.inter)) return -1;
+  const at::Tensor* cs = x.cs = tensor_in(x.ref.get());
+  return cs && plain(*cs, idx) && cs->scalar_type() == at::kFloat && cs->dim() == 3 &&
+         cs->is_contiguous() && cs->size(0) >= 1 && cs->size(0) < (1ll << 31) &&
+         2 * cs->size(1) == x.rotary_dim && cs->size(2) == 2 && x.rotary_dim <= d &&
+         !((uintptr_t)cs->data_ptr() & 15);
+}
+
 // append_rotary(k, v, k_cache, v_cache, page_table, token_seq, token_pos,
 //               rotary, q, q_out, offsets) -> q_out or None
 PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
@@ -134,19 +153,9 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   if (a[10] != Py_None && !((offsets = tensor_in(a[10])) && index_of(offsets, p.idx, p.slots)))
     return not_here();
   const int64_t hq = q ? q->size(1) : 0;
-  if (n * (hq + 2 * p.hkv) * p.d >= (1ll << 31) || Py_TYPE(a[7]) != t_rotary) return not_here();
-  int64_t rotary_dim, inter;
-  PyObject* cs_obj = PyObject_GetAttr(a[7], s_cos_sin);
-  if (!cs_obj) return nullptr;
-  THPObjectPtr cs_ref(cs_obj);
-  const at::Tensor* cs = tensor_in(cs_obj);
-  if (!int_attr(a[7], s_rotary_dim, rotary_dim) || !int_attr(a[7], s_interleaved, inter)) return nullptr;
-  // the table is an attribute that a caller may replace
-  if (!cs || !plain(*cs, p.idx) || cs->scalar_type() != at::kFloat || cs->dim() != 3 ||
-      !cs->is_contiguous() || cs->size(0) < 1 || cs->size(0) >= (1ll << 31) ||
-      2 * cs->size(1) != rotary_dim || cs->size(2) != 2 || rotary_dim > p.d ||
-      ((uintptr_t)cs->data_ptr() & 15))
-    return not_here();
+  if (n * (hq + 2 * p.hkv) * p.d >= (1ll << 31)) return not_here();
+  Angles turn;
+  if (angles_of(a[7], p.idx, p.d, turn) != 1) return not_here();
 
   const Span pools[2] = {{p.k, p.k + p.bytes}, {p.v, p.v + p.bytes}};
   if (meet(pools[0], pools[1])) return not_here();
@@ -173,8 +182,8 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const int rc = moba_hip_append_rotary(
       q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, k->data_ptr(),
       k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), p.code, (int)n, (int)hq,
-      (int)p.hkv, (int)p.d, (const float*)cs->data_ptr(), (int)cs->size(0), (int)rotary_dim,
-      (int)inter, (void*)p.k, (void*)p.v, (int)p.pages, (int)p.page, (const int*)table->data_ptr(),
+      (int)p.hkv, (int)p.d, (const float*)turn.cs->data_ptr(), (int)turn.cs->size(0), (int)turn.rotary_dim,
+      (int)turn.inter, (void*)p.k, (void*)p.v, (int)p.pages, (int)p.page, (const int*)table->data_ptr(),
       (int)p.slots, (int)p.width, (const int*)seq->data_ptr(), (const int*)pos->data_ptr(),
       offsets ? (const int*)offsets->data_ptr() : nullptr, q ? out.data_ptr() : nullptr, nullptr,
       stream);
@@ -244,14 +253,217 @@ PyObject* shared_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(get_stream, get_device, error class, RotaryTable, SharedPrefixPlan)
+// A QuantizedPages and its table.
+struct QPool {
+  int code, idx;   // format of the codes
+  int64_t pages, hkv, page, d, width, slots, table_width;
+  const at::Tensor *k, *v, *ks, *vs, *table;
+  Span spans[4];
+  bool meets(const Span& x) const {
+    return meet(x, spans[0]) || meet(x, spans[1]) || meet(x, spans[2]) || meet(x, spans[3]);
+  }
+};
+bool qpool_of(PyObject* o, PyObject* table, QPool& p) {
+  if (Py_TYPE(o) != t_pages || PyTuple_GET_SIZE(o) != 5 || !PyLong_CheckExact(PyTuple_GET_ITEM(o, 4))) return false;
+  const at::Tensor* t[5];
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = tensor_in(PyTuple_GET_ITEM(o, i)))) return false;
+  if (!(t[4] = tensor_in(table))) return false;
+  p.k = t[0]; p.v = t[1]; p.ks = t[2]; p.vs = t[3]; p.table = t[4];
+  p.d = PyLong_AsLongLong(PyTuple_GET_ITEM(o, 4));
+  if (PyErr_Occurred() || p.d < 8 || p.d > 256 || p.d % 8 || !p.k->is_cuda() || p.k->dim() != 4) return false;
+  p.idx = p.k->get_device();
+  const auto kind = p.k->scalar_type();
+  p.code = kind == at::kChar ? 0 : kind == at::kFloat8_e4m3fn ? 1 : -1;
+  p.pages = p.k->size(0); p.hkv = p.k->size(1); p.page = p.k->size(2); p.width = p.k->size(3);
+  if (p.code < 0 || p.width != (p.d + 15) / 16 * 16 || p.k->numel() == 0) return false;
+  for (int i = 0; i < 4; ++i) {
+    if (!plain(*t[i], p.idx) || !t[i]->is_contiguous()) return false;
+    if (i == 1 && (p.v->scalar_type() != kind || p.v->sizes() != p.k->sizes())) return false;
+    if (i > 1 && (t[i]->scalar_type() != at::kFloat || t[i]->dim() != 3 || t[i]->size(0) != p.pages ||
+                  t[i]->size(1) != p.hkv || t[i]->size(2) != p.page))
+      return false;
+    p.spans[i] = span_of(*t[i]);
+    for (int j = 0; j < i; ++j)
+      if (meet(p.spans[i], p.spans[j])) return false;
+  }
+  if (((uintptr_t)p.spans[0].lo | (uintptr_t)p.spans[1].lo) & 15) return false;
+  if (!plain(*p.table, p.idx) || p.table->scalar_type() != at::kInt || p.table->dim() != 2 ||
+      !p.table->is_contiguous() || p.table->numel() == 0)
+    return false;
+  p.slots = p.table->size(0); p.table_width = p.table->size(1);
+  return p.pages * p.page < (1ll << 31) && p.table_width * p.page < (1ll << 31) &&
+         p.pages * p.page * p.hkv <= 0xfffffff0ll / (p.width / 16);
+}
+// [n, heads, d] in 16 bits on the pool's device, dims contiguous.
+bool rows_of(const at::Tensor* t, const QPool& p, int64_t n, int type) {
+  return t && plain(*t, p.idx) && t->dim() == 3 && type >= 0 && type_code(t->scalar_type()) == type &&
+         t->size(0) == n && t->size(1) > 0 && t->size(2) == p.d && t->stride(2) == 1 &&
+         t->stride(0) >= 0 && t->stride(1) >= 0 && !t->requires_grad();
+}
+
+// quantized_append(k, v, pages, page_table, token_seq, token_pos, rotary, q,
+//                  q_out, offsets) -> q_out or None
+PyObject* quantized_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 10) return PyErr_Format(PyExc_TypeError, "quantized_append takes 10 arguments");
+  const at::Tensor *k = tensor_in(a[0]), *v = tensor_in(a[1]), *seq = tensor_in(a[4]), *pos = tensor_in(a[5]);
+  QPool p;
+  if (!qpool_of(a[2], a[3], p) || !k || k->dim() != 3) return not_here();
+  const int64_t n = k->size(0);
+  const int type = type_code(k->scalar_type());
+  if (n < 1 || !rows_of(k, p, n, type) || !rows_of(v, p, n, type) || k->size(1) != p.hkv ||
+      v->size(1) != p.hkv || !index_of(seq, p.idx, n) || !index_of(pos, p.idx, n))
+    return not_here();
+  const at::Tensor *q = nullptr, *offsets = nullptr;
+  Angles turn;
+  if (a[6] == Py_None) {
+    if (a[7] != Py_None || a[8] != Py_None || a[9] != Py_None) return not_here();
+  } else {
+    if (angles_of(a[6], p.idx, p.d, turn) != 1) return not_here();
+    if (a[7] != Py_None && !((q = tensor_in(a[7])) && rows_of(q, p, n, type))) return not_here();
+    if (a[9] != Py_None && !((offsets = tensor_in(a[9])) && index_of(offsets, p.idx, p.slots))) return not_here();
+  }
+  const int64_t hq = q ? q->size(1) : 0;
+  if (n * (hq + 2 * p.hkv) * p.width >= (1ll << 31)) return not_here();
+  const at::Tensor* ins[3] = {k, v, q};
+  Span spans[3];
+  for (int i = 0; i < (q ? 3 : 2); ++i) {
+    spans[i] = span_of(*ins[i]);
+    if (p.meets(spans[i])) return not_here();
+  }
+  at::Tensor out;
+  if (a[8] != Py_None) {
+    const at::Tensor* given = tensor_in(a[8]);
+    if (!q || !rows_of(given, p, n, type) || given->size(1) != hq || !given->is_contiguous()) return not_here();
+    const Span o = span_of(*given);
+    if (p.meets(o) || meet(o, spans[0]) || meet(o, spans[1]) || meet(o, spans[2])) return not_here();
+    out = *given;
+  }
+  void* stream;
+  if (!stream_of(p.idx, stream)) return not_here();
+  if (q && !out.defined()) out = at::empty({n, hq, p.d}, q->options().requires_grad(false));
+  const int rc = moba_hip_quantized_append(
+      q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, k->data_ptr(), k->stride(0),
+      k->stride(1), v->data_ptr(), v->stride(0), v->stride(1), type, (int)n, (int)hq, (int)p.hkv, (int)p.d,
+      turn.cs ? (const float*)turn.cs->data_ptr() : nullptr, turn.cs ? (int)turn.cs->size(0) : 0,
+      (int)turn.rotary_dim, (int)turn.inter, p.code, p.k->data_ptr(), p.v->data_ptr(),
+      (float*)p.ks->data_ptr(), (float*)p.vs->data_ptr(), (int)p.pages, (int)p.page,
+      (const int*)p.table->data_ptr(), (int)p.slots, (int)p.table_width, (const int*)seq->data_ptr(),
+      (const int*)pos->data_ptr(), offsets ? (const int*)offsets->data_ptr() : nullptr,
+      q ? out.data_ptr() : nullptr, nullptr, stream);
+  if (rc) return failed("moba_hip_quantized_append", rc);
+  if (!q) Py_RETURN_NONE;
+  if (a[8] != Py_None) {
+    Py_INCREF(a[8]);
+    return a[8];
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// quantized_read(pages, page_table, token_seq, token_pos, 0 bf16 or 1 fp16) -> (k, v)
+PyObject* quantized_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) return PyErr_Format(PyExc_TypeError, "quantized_read takes 5 arguments");
+  const at::Tensor *seq = tensor_in(a[2]), *pos = tensor_in(a[3]);
+  const long type = PyLong_AsLong(a[4]);
+  QPool p;
+  if (PyErr_Occurred() || !qpool_of(a[0], a[1], p) || !seq || seq->dim() != 1) return not_here();
+  const int64_t n = seq->size(0);
+  if (n < 1 || !index_of(seq, p.idx, n) || !index_of(pos, p.idx, n) || n * 2 * p.hkv * p.d >= (1ll << 31))
+    return not_here();
+  void* stream;
+  if (!stream_of(p.idx, stream)) return not_here();
+  const auto options = seq->options().dtype(type == 0 ? at::kBFloat16 : at::kHalf);
+  at::Tensor k = at::empty({n, p.hkv, p.d}, options), v = at::empty({n, p.hkv, p.d}, options);
+  const int rc = moba_hip_quantized_read(
+      p.code, p.k->data_ptr(), p.v->data_ptr(), (const float*)p.ks->data_ptr(), (const float*)p.vs->data_ptr(),
+      (int)p.pages, (int)p.page, (int)p.hkv, (int)p.d, (const int*)p.table->data_ptr(), (int)p.slots,
+      (int)p.table_width, (const int*)seq->data_ptr(), (const int*)pos->data_ptr(), (int)n, (int)type,
+      k.data_ptr(), v.data_ptr(), nullptr, stream);
+  if (rc) return failed("moba_hip_quantized_read", rc);
+  THPObjectPtr pk(THPVariable_Wrap(std::move(k))), pv(THPVariable_Wrap(std::move(v)));
+  return pk && pv ? PyTuple_Pack(2, pk.get(), pv.get()) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// A positive int32 of a Python int; 0: none.
+int64_t positive_of(PyObject* o) {
+  if (!PyLong_CheckExact(o)) return 0;
+  int over;
+  const int64_t x = PyLong_AsLongLongAndOverflow(o, &over);
+  return over || x < 1 || x >= (1ll << 31) ? 0 : x;
+}
+
+// quantized_attention(q, pages, page_table, q_seq, lengths, selected, chunk_size,
+//                     max_length, scale) -> (out, lse)
+PyObject* quantized_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 9) return PyErr_Format(PyExc_TypeError, "quantized_attention takes 9 arguments");
+  const at::Tensor *q = tensor_in(a[0]), *seq = tensor_in(a[3]), *lengths = tensor_in(a[4]);
+  QPool p;
+  if (!qpool_of(a[1], a[2], p) || !q || q->dim() != 3) return not_here();
+  const int64_t n = q->size(0), hq = q->size(1);
+  const int type = type_code(q->scalar_type());
+  if (n < 1 || !rows_of(q, p, n, type) || hq % p.hkv || !q->is_contiguous() || ((uintptr_t)q->data_ptr() & 15) ||
+      !index_of(seq, p.idx, n) || !index_of(lengths, p.idx, n))
+    return not_here();
+  int64_t limit = p.table_width * p.page, slots = 0, chunk = 0;
+  if (a[7] != Py_None) {
+    const int64_t given = positive_of(a[7]);
+    if (!given) return not_here();
+    limit = std::min(limit, given);
+  }
+  const at::Tensor* selected = nullptr;
+  if (a[5] != Py_None) {
+    selected = tensor_in(a[5]);
+    chunk = positive_of(a[6]);
+    if (!selected || !chunk || !plain(*selected, p.idx) || selected->scalar_type() != at::kInt ||
+        selected->dim() != 3 || !selected->is_contiguous() || selected->size(0) != n || selected->size(1) != hq)
+      return not_here();
+    slots = selected->size(2);
+    if (slots < 1 || slots > 16) return not_here();
+    chunk = std::min(chunk, limit);
+  } else if (a[6] != Py_None) {
+    return not_here();
+  }
+  const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)p.d)
+                       : PyFloat_Check(a[8]) ? PyFloat_AS_DOUBLE(a[8]) : 0.0;
+  if (!(scale >= 0x1p-126 && scale < 1e30)) return not_here();
+  const int64_t blocks = (hq / p.hkv + 31) / 32;
+  if (n * hq >= (1ll << 31) || limit > 0x7fffff00 ||
+      n * p.hkv * blocks * std::max<int64_t>(32, (limit + 127) / 128) >= (1ll << 31))
+    return not_here();
+  void* stream;
+  if (!stream_of(p.idx, stream)) return not_here();
+  const auto options = q->options().requires_grad(false);
+  at::Tensor out = at::empty({n, hq, p.d}, options);
+  at::Tensor lse = at::empty({n, hq}, options.dtype(at::kFloat));
+  at::Tensor work = at::empty({moba_hip_quantized_attention_work((int)n, (int)hq, (int)p.hkv, (int)p.d, (int)slots,
+                                                                 (int)chunk, (int)limit)},
+                              options.dtype(at::kByte));
+  const int rc = moba_hip_quantized_attention(
+      q->data_ptr(), type, (int)n, (int)hq, (int)p.hkv, (int)p.d, (float)scale, p.code, p.k->data_ptr(),
+      p.v->data_ptr(), (const float*)p.ks->data_ptr(), (const float*)p.vs->data_ptr(), (int)p.pages, (int)p.page,
+      (const int*)p.table->data_ptr(), (int)p.slots, (int)p.table_width, (const int*)seq->data_ptr(),
+      (const int*)lengths->data_ptr(), 0, (int)limit, selected ? (const int*)selected->data_ptr() : nullptr,
+      (int)slots, (int)chunk, work.data_ptr(), out.data_ptr(), (float*)lse.data_ptr(), stream);
+  if (rc) return failed("moba_hip_quantized_attention", rc);
+  THPObjectPtr po(THPVariable_Wrap(std::move(out))), pl(THPVariable_Wrap(std::move(lse)));
+  return po && pl ? PyTuple_Pack(2, po.get(), pl.get()) : nullptr;
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(get_stream, get_device, error class, RotaryTable, SharedPrefixPlan, QuantizedPages)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
-  if (nargs != 5 || !PyType_Check(a[3]) || !PyType_Check(a[4]))
-    return PyErr_Format(PyExc_TypeError, "bind takes two functions and three classes");
-  for (int i = 0; i < 5; ++i) Py_INCREF(a[i]);  // for the life of the process
+  if (nargs != 6 || !PyType_Check(a[3]) || !PyType_Check(a[4]) || !PyType_Check(a[5]))
+    return PyErr_Format(PyExc_TypeError, "bind takes two functions and four classes");
+  for (int i = 0; i < 6; ++i) Py_INCREF(a[i]);  // for the life of the process
   g_stream = a[0]; g_device = a[1]; g_error = a[2];
   t_rotary = (PyTypeObject*)a[3];
   t_plan = (PyTypeObject*)a[4];
+  t_pages = (PyTypeObject*)a[5];
   Py_RETURN_NONE;
 }
 
@@ -259,6 +471,9 @@ PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr},
     {"append_rotary", (PyCFunction)(void (*)(void))append_rotary, METH_FASTCALL, nullptr},
     {"shared_attention", (PyCFunction)(void (*)(void))shared_attention, METH_FASTCALL, nullptr},
+    {"quantized_append", (PyCFunction)(void (*)(void))quantized_append, METH_FASTCALL, nullptr},
+    {"quantized_read", (PyCFunction)(void (*)(void))quantized_read, METH_FASTCALL, nullptr},
+    {"quantized_attention", (PyCFunction)(void (*)(void))quantized_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

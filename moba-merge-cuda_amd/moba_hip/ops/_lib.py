@@ -153,6 +153,7 @@ def calls():
 
         import torch
 
+        from ..quantized import QuantizedPages
         from ..rotary import RotaryTable
         from ..shared_prefix import SharedPrefixPlan
         load()
@@ -172,7 +173,7 @@ def calls():
         if module.built_for != here:
             raise MobaHipError(f"{path} is built for {module.built_for}, this is {here}: build it again")
         module.bind(torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice, MobaHipError,
-                    RotaryTable, SharedPrefixPlan)
+                    RotaryTable, SharedPrefixPlan, QuantizedPages)
         _calls = module
     return _calls
 

@@ -151,6 +151,11 @@ def quantized_append(k, v, pages, page_table, token_seq, token_pos, *, rotary=No
     last dimension.  page_table, token_seq, token_pos, offsets, q_out and check, and
     what becomes of tokens without a cell or an angle: as in
     :func:`moba_hip.append_rotary`."""
+    if not check:
+        done = _lib.calls().quantized_append(k, v, pages, page_table, token_seq, token_pos, rotary, q, q_out,
+                                             offsets)
+        if done is not NotImplemented:
+            return done
     n_pages, hkv, page, d = _check_pages(pages, page_table)
     dev = pages.k.device
     n = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
@@ -212,6 +217,10 @@ def quantized_read(pages, page_table, token_seq, token_pos, *, dtype=torch.bfloa
     :func:`quantized_append`; a cell may be named more than once.  A token of slot -1 is
     padding and reads as zeros; so does one outside the table or in an unmapped page,
     which ``check`` makes a RuntimeError after the launch."""
+    if not check and dtype in _DTYPES:
+        done = _lib.calls().quantized_read(pages, page_table, token_seq, token_pos, _DTYPES[dtype])
+        if done is not NotImplemented:
+            return done
     n_pages, hkv, page, d = _check_pages(pages, page_table)
     dev = pages.k.device
     if dtype not in _DTYPES:
@@ -254,6 +263,11 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     zeros and an lse of -inf; a token in an unmapped page is not attended.  ``scale``
     (in [2^-126, 1e30]) defaults to D ** -0.5.  q and ``out`` are contiguous and 16-byte
     aligned.  Nothing is read back, so a call can be captured into a graph."""
+    if out is None and lse is None:
+        done = _lib.calls().quantized_attention(q, pages, page_table, q_seq, lengths, selected, chunk_size,
+                                                max_length, scale)
+        if done is not NotImplemented:
+            return done
     n_pages, hkv, page, d = _check_pages(pages, page_table)
     dev = pages.k.device
     n = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
