@@ -153,21 +153,61 @@ MOBA_DEV void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_
   out[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302);
 }
 
-template <int NC> struct Words {
-  typedef uint32_t type __attribute__((ext_vector_type(NC)));
+// A read of bytes that this call reads once.
+template <typename T> MOBA_DEV T load_once(const T* p) { return __builtin_nontemporal_load(p); }
+
+// Keys of a step: 16 dims at 64 c + 16 g of token 16 t + l % 16.
+template <int NC> struct Keys {
+  u32x4_t reg[2][NC];
 };
-template <> struct Words<1> {
-  struct type {
-    uint32_t x;
-    MOBA_DEV uint32_t& operator[](int) { return x; }
-    MOBA_DEV uint32_t operator[](int) const { return x; }
-  };
+// Values of a step: the lane's 4 NC dims of tokens 4 g + j (j < 4) and 16 + 4 g + j - 4.
+template <int NC> struct Values {
+  uint32_t reg[8][NC];
+  MOBA_DEV void load(int j, const uint8_t* p) {
+    if constexpr (NC == 1) {
+      reg[j][0] = load_once(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      typedef uint32_t words __attribute__((ext_vector_type(NC)));
+      const words x = load_once(reinterpret_cast<const words*>(p));
+#pragma unroll
+      for (int d = 0; d < NC; ++d) reg[j][d] = x[d];
+    }
+  }
+  // The 8 tokens of each of the four dims of dword d, in bf16.
+  template <int FMT> MOBA_DEV void operands(int d, u32x4_t (&out)[4]) const {
+    if constexpr (FMT == 1) {  // 16 permutations, then two codes an instruction
+      uint32_t x[4], y[4];
+      transpose4(reg[0][d], reg[1][d], reg[2][d], reg[3][d], x);
+      transpose4(reg[4][d], reg[5][d], reg[6][d], reg[7][d], y);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint32_t lo, hi;
+        numbers4_16<1, 0>(x[b], lo, hi); out[b][0] = lo; out[b][1] = hi;
+        numbers4_16<1, 0>(y[b], lo, hi); out[b][2] = lo; out[b][3] = hi;
+      }
+    } else {  // int8: a conversion takes any byte of a word, and the halves are put together
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lo = (float)(int8_t)(reg[2 * j][d] >> (8 * b)), hi = (float)(int8_t)(reg[2 * j + 1][d] >> (8 * b));
+          out[b][j] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
+        }
+    }
+  }
+};
+// What a lane knows of a step: the scales of token l % 32 and the heads that attend it;
+// which of the step's tokens there are, and whether all heads attend all 32.
+struct Step {
+  float ks, vs;
+  uint32_t mask, live;
+  bool whole;
 };
 
 // Waves of a workgroup.
 constexpr int kWaves = 4;
 // Workgroups of a CU that the registers allow.
-template <int NC> constexpr int occupancy() { return NC == 4 ? 2 : NC == 2 ? 3 : 4; }
+template <int NC> constexpr int occupancy() { return NC == 1 ? 3 : 2; }
 
 // Where a step's tokens are, before the pool's rows are known.
 struct Look {
@@ -296,23 +336,19 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
       x.at = ok ? t - lp * a.pool.by_page.d : ~0u;
       return x;
     };
-    // registers of a step: codes, scales of the lane's token, who attends it
-    u32x4_t kreg[2][NC];
-    typename Words<NC>::type vreg[8];
-    float ks = 0.f, vs = 0.f;
-    uint32_t lane_mask = 0, live = 0;  // live: bit t: token t of the step is there
-    bool whole = false;
-    uint32_t voff[8];
-    // a step's places, from its page entries; loads its keys and scales
-    auto locate = [&](const Look& x) __attribute__((always_inline)) {
+    // Puts a step's places, from its page entries, where all lanes see them; loads its
+    // keys and the scales of the lane's token.  A step behind the last reads the pool's
+    // first row over and over: its loads are cheaper than a branch around them, behind
+    // which the compiler would wait for every load in flight.
+    auto fetch_keys = [&](const Look& x, Keys<NC>& k, Step& s, uint32_t (&voff)[8]) __attribute__((always_inline)) {
       const bool ok = x.at != ~0u && x.page >= 0 && x.page < a.pool.num_pages;
       const uint32_t row = ok ? ((uint32_t)x.page * a.pool.Hkv + kh) * a.pool.P + x.at : 0u;
       off_s[w][lane & 31] = row * pieces;
-      live = (uint32_t)__ballot(ok);
-      lane_mask = x.mask;
-      whole = live == ~0u && (!moba || __all(x.mask == heads_mask));
-      ks = a.pool.ks[row] * a.scale_log2;
-      vs = a.pool.vs[row];
+      s.live = (uint32_t)__ballot(ok);
+      s.mask = x.mask;
+      s.whole = s.live == ~0u && (!moba || __all(x.mask == heads_mask));
+      s.ks = a.pool.ks[row];
+      s.vs = a.pool.vs[row];
       wave_lds_sync();
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -320,7 +356,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int d = 64 * c + 16 * g;
-          kreg[t][c] = *reinterpret_cast<const u32x4_t*>(p + (d < a.pool.Dp ? d : 0));
+          k.reg[t][c] = load_once(reinterpret_cast<const u32x4_t*>(p + (d < a.pool.Dp ? d : 0)));
         }
         const u32x4_t o = *reinterpret_cast<const u32x4_t*>(&off_s[w][16 * t + 4 * g]);
 #pragma unroll
@@ -329,129 +365,155 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
       wave_lds_sync();
     };
     const int vd = 4 * NC * c16 < a.pool.Dp ? 4 * NC * c16 : 0;
-    auto load_v = [&]() __attribute__((always_inline)) {
+    auto fetch_values = [&](Values<NC>& v, const uint32_t (&voff)[8]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        vreg[j] = *reinterpret_cast<const typename Words<NC>::type*>(a.pool.v + ((uint64_t)voff[j] << 4) + vd);
+      for (int j = 0; j < 8; ++j) v.load(j, a.pool.v + ((uint64_t)voff[j] << 4) + vd);
+    };
+    // Scales of a step, from a lane per token to the scores' layout, and its scores in log2.
+    f32x4_t sc[2], vv[2];
+    u32x4_t mk[2];
+    auto scores = [&](const Keys<NC>& k, const Step& s) __attribute__((always_inline)) {
+      if (lane < 32) {
+        ks_s[w][lane] = s.ks * a.scale_log2;
+        vs_s[w][lane] = s.vs;
+        if (moba) mask_s[w][lane] = s.mask;
+      }
+      wave_lds_sync();
+      f32x4_t kk[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        kk[t] = *reinterpret_cast<const f32x4_t*>(&ks_s[w][16 * t + 4 * g]);
+        vv[t] = *reinterpret_cast<const f32x4_t*>(&vs_s[w][16 * t + 4 * g]);
+        if (moba) mk[t] = *reinterpret_cast<const u32x4_t*>(&mask_s[w][16 * t + 4 * g]);
+      }
+      wave_lds_sync();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          u32x4_t lo, hi;
+          uint32_t x, y;
+          numbers4_16<FMT, DT>(k.reg[t][c][0], x, y); lo[0] = x; lo[1] = y;
+          numbers4_16<FMT, DT>(k.reg[t][c][1], x, y); lo[2] = x; lo[3] = y;
+          numbers4_16<FMT, DT>(k.reg[t][c][2], x, y); hi[0] = x; hi[1] = y;
+          numbers4_16<FMT, DT>(k.reg[t][c][3], x, y); hi[2] = x; hi[3] = y;
+          sc[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, lo), qf[2 * c], sc[t]);
+          sc[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, hi), qf[2 * c + 1], sc[t]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] *= kk[t][i];
+      }
+    };
+    // The softmax of those scores and their product with the values.
+    auto weigh = [&](Values<NC>& v, const Step& s) __attribute__((always_inline)) {
+      bool on[8];
+      float p[8], wt[8], top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = j >> 2, i = j & 3;
+        p[j] = sc[t][i];
+        on[j] = true;
+        if (!s.whole) {
+          on[j] = (s.live >> (16 * t + 4 * g + i)) & 1;
+          if (moba) on[j] = on[j] && ((mk[t][i] >> my_head) & 1);
+          p[j] = on[j] ? p[j] : -INFINITY;
+        }
+        top = fmaxf(top, p[j]);
+      }
+      // the maximum moves when a score passes it by a margin (the first finite score
+      // does): weights of up to 2^6 lose nothing in fp32 and bf16
+      if (__any(top > m + kSlack)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float to = fmaxf(m, top), shrink = m == -INFINITY ? 0.0f : fast_exp2(m - to);
+        m = to;
+        l *= shrink;
+#pragma unroll
+        for (int t = 0; t < 4 * NC; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] *= shrink;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = fast_exp2(p[j] - ref);
+        l += p[j];
+        wt[j] = p[j] * vv[j >> 2][j & 3];
+        if (!s.whole) wt[j] = on[j] ? wt[j] : 0.0f;  // a NaN scale that is not attended
+      }
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        hi[j] = pack2<0>(wt[2 * j], wt[2 * j + 1]);
+        float x, y;
+        unpack2<0>(hi[j], x, y);
+        lo[j] = pack2<0>(wt[2 * j] - x, wt[2 * j + 1] - y);
+      }
+      if (!s.whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool there = (s.live >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1;
+#pragma unroll
+          for (int d = 0; d < NC; ++d) v.reg[j][d] = there ? v.reg[j][d] : 0;  // never written: may be a NaN's code
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < NC; ++d) {
+        u32x4_t vt[4];
+        v.template operands<FMT>(d, vt);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt[b]), __builtin_bit_cast(u16x8_t, hi), acc[4 * d + b]);
+          acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt[b]), __builtin_bit_cast(u16x8_t, lo), acc[4 * d + b]);
+        }
+      }
     };
 
     int k = stream;
     if (k < steps) {
+      uint32_t voff[8];
       Look next = look(k);
-      locate(next);
-      load_v();
-      next = look(min(k + streams, steps - 1));
-      for (; k < steps; k += streams) {
-        // ---- scales of the step, from a lane per token to the scores' layout
-        const bool now_whole = whole;
-        const uint32_t now_live = live;
-        if (lane < 32) {
-          ks_s[w][lane] = ks;
-          vs_s[w][lane] = vs;
-          if (moba) mask_s[w][lane] = lane_mask;
+      if constexpr (NC <= 2) {
+        // two steps in registers: one is on its way while the other is worked on
+        Keys<NC> ka, kb;
+        Values<NC> va, vb;
+        Step sa, sb;
+        fetch_keys(next, ka, sa, voff);
+        fetch_values(va, voff);
+        next = look(k + streams);
+        for (;;) {
+          fetch_keys(next, kb, sb, voff);
+          fetch_values(vb, voff);
+          next = look(k + 2 * streams);
+          scores(ka, sa);
+          weigh(va, sa);
+          k += streams;
+          if (k >= steps) break;
+          fetch_keys(next, ka, sa, voff);
+          fetch_values(va, voff);
+          next = look(k + 2 * streams);
+          scores(kb, sb);
+          weigh(vb, sb);
+          k += streams;
+          if (k >= steps) break;
         }
-        wave_lds_sync();
-        f32x4_t kk[2], vv[2];
-        u32x4_t mk[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          kk[t] = *reinterpret_cast<const f32x4_t*>(&ks_s[w][16 * t + 4 * g]);
-          vv[t] = *reinterpret_cast<const f32x4_t*>(&vs_s[w][16 * t + 4 * g]);
-          if (moba) mk[t] = *reinterpret_cast<const u32x4_t*>(&mask_s[w][16 * t + 4 * g]);
+      } else {
+        // registers for one: its keys make room after the scores, its values after theirs
+        Keys<NC> ka;
+        Values<NC> va;
+        Step sa, sb;
+        fetch_keys(next, ka, sa, voff);
+        fetch_values(va, voff);
+        next = look(k + streams);
+        for (; k < steps; k += streams) {
+          scores(ka, sa);
+          fetch_keys(next, ka, sb, voff);
+          next = look(k + 2 * streams);
+          weigh(va, sa);
+          fetch_values(va, voff);
+          sa = sb;
         }
-        wave_lds_sync();
-        // ---- scores
-        f32x4_t s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          s[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            u32x4_t lo, hi;
-            uint32_t x, y;
-            numbers4_16<FMT, DT>(kreg[t][c][0], x, y); lo[0] = x; lo[1] = y;
-            numbers4_16<FMT, DT>(kreg[t][c][1], x, y); lo[2] = x; lo[3] = y;
-            numbers4_16<FMT, DT>(kreg[t][c][2], x, y); hi[0] = x; hi[1] = y;
-            numbers4_16<FMT, DT>(kreg[t][c][3], x, y); hi[2] = x; hi[3] = y;
-            s[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, lo), qf[2 * c], s[t]);
-            s[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, hi), qf[2 * c + 1], s[t]);
-          }
-        }
-        // ---- the next step's keys go out, and the page entries of the one after
-        const bool more = k + streams < steps;
-        if (more) {
-          locate(next);
-          next = look(min(k + 2 * streams, steps - 1));
-        }
-        // ---- softmax
-        bool on[8];
-        float p[8], wt[8], top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int t = j >> 2, i = j & 3;
-          p[j] = s[t][i] * kk[t][i];
-          on[j] = true;
-          if (!now_whole) {
-            on[j] = (now_live >> (16 * t + 4 * g + i)) & 1;
-            if (moba) on[j] = on[j] && ((mk[t][i] >> my_head) & 1);
-            p[j] = on[j] ? p[j] : -INFINITY;
-          }
-          top = fmaxf(top, p[j]);
-        }
-        // the maximum moves when a score passes it by a margin (the first finite score
-        // does): weights of up to 2^6 lose nothing in fp32 and bf16
-        if (__any(top > m + kSlack)) {
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float to = fmaxf(m, top), shrink = m == -INFINITY ? 0.0f : fast_exp2(m - to);
-          m = to;
-          l *= shrink;
-#pragma unroll
-          for (int t = 0; t < 4 * NC; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][i] *= shrink;
-        }
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          p[j] = fast_exp2(p[j] - ref);
-          l += p[j];
-          wt[j] = p[j] * vv[j >> 2][j & 3];
-          if (!now_whole) wt[j] = on[j] ? wt[j] : 0.0f;  // a NaN scale that is not attended
-        }
-        u32x4_t hi, lo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          hi[j] = pack2<0>(wt[2 * j], wt[2 * j + 1]);
-          float x, y;
-          unpack2<0>(hi[j], x, y);
-          lo[j] = pack2<0>(wt[2 * j] - x, wt[2 * j + 1] - y);
-        }
-        // ---- values
-        if (!now_whole) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!((now_live >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1)) {
-#pragma unroll
-              for (int d = 0; d < NC; ++d) vreg[j][d] = 0;  // never written: may be a NaN's code
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < NC; ++d) {
-          uint32_t x[4], y[4];
-          transpose4(vreg[0][d], vreg[1][d], vreg[2][d], vreg[3][d], x);
-          transpose4(vreg[4][d], vreg[5][d], vreg[6][d], vreg[7][d], y);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            u32x4_t vt;
-            uint32_t p0, p1;
-            numbers4_16<FMT, 0>(x[b], p0, p1); vt[0] = p0; vt[1] = p1;
-            numbers4_16<FMT, 0>(y[b], p0, p1); vt[2] = p0; vt[3] = p1;
-            acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt), __builtin_bit_cast(u16x8_t, hi), acc[4 * d + b]);
-            acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt), __builtin_bit_cast(u16x8_t, lo), acc[4 * d + b]);
-          }
-        }
-        if (more) load_v();
       }
     }
 
@@ -506,14 +568,16 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
 }
 
 // One workgroup per (entry, head) that spans several workgroups of the first launch:
-// their partials, weighted by 2^(m_j - m), in groups of parts whose sums are then added
-// in order.  An entry without tokens gets zeros and -inf.
-template <int DT>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, int wgs, int cols, int per_entry) {
+// their partials, weighted by 2^(m_j - m); cols (a power of two) threads of 4 dims each,
+// B / cols parts at once, whose sums are added in a fixed order.  An entry without
+// tokens gets zeros and -inf.
+template <int DT, int B>
+__global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int cols, int per_entry) {
   __shared__ float weight[kMaxWgs];
-  __shared__ float red[256];
-  __shared__ __attribute__((aligned(16))) f32x4_t sums[256];
-  const int hpe = 16 * a.HB, e = blockIdx.x / per_entry, h = blockIdx.x % per_entry, tid = threadIdx.x;
+  __shared__ float red[2][B / 64];
+  __shared__ __attribute__((aligned(16))) f32x4_t sums[B / 64][64];
+  const int hpe = 16 * a.HB, e = blockIdx.x / per_entry, h = blockIdx.x % per_entry;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int r = e / a.per_row, kh = (e % a.per_row) / a.NHB, blk = e % a.NHB;
   if (h >= a.G - blk * hpe) return;
   const int D = a.pool.D;
@@ -521,7 +585,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, int wgs, int cols
   const uint32_t T = a.start[a.scan_n], s0 = a.start[si], u = (a.start[si + 1] - s0) / a.scan_mult;
   const int64_t row = (int64_t)r * a.Hq + kh * a.G + blk * hpe + h;
   if (u == 0) {
-    for (int d = tid; d < D; d += 256) a.out[row * D + d] = 0;
+    for (int d = tid; d < D; d += B) a.out[row * D + d] = 0;
     if (tid == 0) a.lse[row] = -INFINITY;
     return;
   }
@@ -529,56 +593,50 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, int wgs, int cols
   const Deal deal(T, W);
   const uint32_t w0 = deal.owner(from), w1 = deal.owner(from + u - 1), parts = w1 - w0 + 1;
   if (parts == 1) return;  // written by that workgroup
-  // workgroup w's partial of this entry: its first segment's, if its run begins within
-  // the entry, else its last one's
-  auto slot = [&](uint32_t w) { return ((int64_t)2 * w + (deal.first(w) < from ? 1 : 0)) * hpe + h; };
+  // workgroup x's partial of this entry: its first segment's, if its run begins within
+  // the entry (all but w0's do), else its last one's
+  const int64_t slot0 = ((int64_t)2 * w0 + (deal.first(w0) < from ? 1 : 0)) * hpe + h;
+  auto slot = [&](uint32_t j) { return j == 0 ? slot0 : (int64_t)2 * (w0 + j) * hpe + h; };
   float top = -INFINITY;
-  for (uint32_t j = tid; j < parts; j += 256) {
-    const float m = a.part_ml[2 * slot(w0 + j)];
-    weight[j] = m;
-    top = fmaxf(top, m);
-  }
-  red[tid] = top;
-  __syncthreads();
+  for (uint32_t j = tid; j < parts; j += B) top = fmaxf(top, a.part_ml[2 * slot(j)]);
 #pragma unroll
-  for (int off = 128; off > 0; off >>= 1) {
-    if (tid < off) red[tid] = fmaxf(red[tid], red[tid + off]);
-    __syncthreads();
-  }
-  top = red[0];
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) red[0][w] = top;
   __syncthreads();
+  for (int x = 0; x < B / 64; ++x) top = fmaxf(top, red[0][x]);
   float z = 0.0f;
-  for (uint32_t j = tid; j < parts; j += 256) {
-    const float f = weight[j] == -INFINITY ? 0.0f : fast_exp2(weight[j] - top);
+  for (uint32_t j = tid; j < parts; j += B) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(j));
+    const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
     weight[j] = f;
-    z += f * a.part_ml[2 * slot(w0 + j) + 1];
+    z += f * ml.y;
   }
-  red[tid] = z;
-  __syncthreads();
 #pragma unroll
-  for (int off = 128; off > 0; off >>= 1) {
-    if (tid < off) red[tid] += red[tid + off];
-    __syncthreads();
-  }
-  z = red[0];
-  // cols (a power of two) threads of 4 dims each, 256 / cols parts at once
-  const int c = tid & (cols - 1), d = 4 * c, group = tid / cols, groups = 256 / cols;
+  for (int off = 32; off > 0; off >>= 1) z += __shfl_xor(z, off, 64);
+  if (lane == 0) red[1][w] = z;
+  __syncthreads();
+  z = 0.0f;
+  for (int x = 0; x < B / 64; ++x) z += red[1][x];
+  const int c = tid & (cols - 1), d = 4 * c, groups = B / cols;
+  const int at = d < D ? d : 0;  // columns behind D repeat the first
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  if (d < D) {
-    for (uint32_t j = group; j < parts; j += groups) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + slot(w0 + j) * D + d);
+#pragma unroll 4
+  for (uint32_t j = tid / cols; j < parts; j += groups) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + slot(j) * D + at);
+    const float f = weight[j];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += x[i] * weight[j];
-    }
+    for (int i = 0; i < 4; ++i) o[i] += x[i] * f;
   }
-  sums[tid] = o;
+  for (int off = cols; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], off, 64);
+  if (lane < cols) sums[w][lane] = o;
   __syncthreads();
-  if (group > 0 || d >= D) return;
-  for (int y = 1; y < groups; ++y) {
-    const f32x4_t x = sums[y * cols + c];
+  if (tid >= cols || d >= D) return;
+  o = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  for (int x = 0; x < B / 64; ++x)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += x[i];
-  }
+    for (int i = 0; i < 4; ++i) o[i] += sums[x][c][i];
   const float f = z == 0.0f ? 0.0f : 1.0f / z;
   *reinterpret_cast<uint2*>(a.out + row * D + d) =
       make_uint2(pack2<DT>(o[0] * f, o[1] * f), pack2<DT>(o[2] * f, o[3] * f));
@@ -598,7 +656,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.entries = (int64_t)Nq * Hkv * s.NHB;
   s.max_items = std::min(s.G, 16 * s.HB) * slots;
   // as many workgroups as the card holds at once, but no more than there can be units
-  const int per_cu = D > 128 ? 2 : D > 64 ? 3 : 4;
+  const int per_cu = D > 64 ? 2 : 3;
   const int64_t longest = slots > 0 ? std::min<int64_t>((int64_t)s.max_items * chunk, max_length) : max_length;
   const int64_t units = s.entries * ((longest + kUnit - 1) / kUnit);
   s.wgs = (int)std::min<int64_t>(256 * per_cu, (units + 7) / 8 * 8);
@@ -619,6 +677,12 @@ template <int DT, int FMT> void launch_attend(const AttnArgs& a, int wgs, hipStr
   if (a.pool.Dp <= 64) hipLaunchKernelGGL((attend_kernel<DT, FMT, 1>), grid, block, 0, st, a);
   else if (a.pool.Dp <= 128) hipLaunchKernelGGL((attend_kernel<DT, FMT, 2>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((attend_kernel<DT, FMT, 4>), grid, block, 0, st, a);
+}
+
+// Few joins have many parts each: wide workgroups then.
+template <int DT> void launch_join(const AttnArgs& a, unsigned joins, int wgs, int cols, int per_entry, hipStream_t st) {
+  if (joins <= 256) hipLaunchKernelGGL((join_kernel<DT, 1024>), dim3(joins), dim3(1024), 0, st, a, wgs, cols, per_entry);
+  else hipLaunchKernelGGL((join_kernel<DT, 256>), dim3(joins), dim3(256), 0, st, a, wgs, cols, per_entry);
 }
 
 }  // namespace
@@ -678,8 +742,8 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   int cols = 16;
   while (cols * 4 < D) cols *= 2;
   const int per_entry = std::min(s.G, 16 * s.HB);
-  const dim3 grid((unsigned)(s.entries * per_entry)), block(256);
-  if (dtype == 0) hipLaunchKernelGGL((join_kernel<0>), grid, block, 0, st, a, s.wgs, cols, per_entry);
-  else hipLaunchKernelGGL((join_kernel<1>), grid, block, 0, st, a, s.wgs, cols, per_entry);
+  const unsigned joins = (unsigned)(s.entries * per_entry);
+  if (dtype == 0) launch_join<0>(a, joins, s.wgs, cols, per_entry, st);
+  else launch_join<1>(a, joins, s.wgs, cols, per_entry, st);
   return moba_launch_status("quantized_attention");
 }
