@@ -407,18 +407,22 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
     };
     // The softmax of those scores and their product with the values.
     auto weigh = [&](Values<NC>& v, const Step& s) __attribute__((always_inline)) {
-      bool on[8];
       float p[8], wt[8], top = -INFINITY;
+      uint32_t on = 0xff;  // bit j: the lane's head attends its token j
+      if (!s.whole) {
+        on = ((s.live >> (4 * g)) & 15) | (((s.live >> (16 + 4 * g)) & 15) << 4);
+        if (moba) {
+          uint32_t takes = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) takes |= ((mk[j >> 2][j & 3] >> my_head) & 1) << j;
+          on &= takes;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j >> 2][j & 3] = (on >> j) & 1 ? sc[j >> 2][j & 3] : -INFINITY;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int t = j >> 2, i = j & 3;
-        p[j] = sc[t][i];
-        on[j] = true;
-        if (!s.whole) {
-          on[j] = (s.live >> (16 * t + 4 * g + i)) & 1;
-          if (moba) on[j] = on[j] && ((mk[t][i] >> my_head) & 1);
-          p[j] = on[j] ? p[j] : -INFINITY;
-        }
+        p[j] = sc[j >> 2][j & 3];
         top = fmaxf(top, p[j]);
       }
       // the maximum moves when a score passes it by a margin (the first finite score
@@ -440,7 +444,10 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         p[j] = fast_exp2(p[j] - ref);
         l += p[j];
         wt[j] = p[j] * vv[j >> 2][j & 3];
-        if (!s.whole) wt[j] = on[j] ? wt[j] : 0.0f;  // a NaN scale that is not attended
+      }
+      if (!s.whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) wt[j] = (on >> j) & 1 ? wt[j] : 0.0f;  // a NaN scale that is not attended
       }
       u32x4_t hi, lo;
 #pragma unroll
@@ -472,27 +479,28 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
 
     int k = stream;
     if (k < steps) {
+      // Loads return in order: the page entries of a step are asked for before the keys
+      // and values of the one before it, so that waiting for them waits for nothing else.
       uint32_t voff[8];
-      Look next = look(k);
+      Look now = look(k), next = look(k + streams), after;
       if constexpr (NC <= 2) {
         // two steps in registers: one is on its way while the other is worked on
         Keys<NC> ka, kb;
         Values<NC> va, vb;
         Step sa, sb;
-        fetch_keys(next, ka, sa, voff);
+        fetch_keys(now, ka, sa, voff);
         fetch_values(va, voff);
-        next = look(k + streams);
         for (;;) {
+          after = look(k + 2 * streams);
           fetch_keys(next, kb, sb, voff);
           fetch_values(vb, voff);
-          next = look(k + 2 * streams);
           scores(ka, sa);
           weigh(va, sa);
           k += streams;
           if (k >= steps) break;
-          fetch_keys(next, ka, sa, voff);
-          fetch_values(va, voff);
           next = look(k + 2 * streams);
+          fetch_keys(after, ka, sa, voff);
+          fetch_values(va, voff);
           scores(kb, sb);
           weigh(vb, sb);
           k += streams;
@@ -503,13 +511,13 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         Keys<NC> ka;
         Values<NC> va;
         Step sa, sb;
-        fetch_keys(next, ka, sa, voff);
+        fetch_keys(now, ka, sa, voff);
         fetch_values(va, voff);
-        next = look(k + streams);
         for (; k < steps; k += streams) {
           scores(ka, sa);
+          after = look(k + 2 * streams);
           fetch_keys(next, ka, sb, voff);
-          next = look(k + 2 * streams);
+          next = after;
           weigh(va, sa);
           fetch_values(va, voff);
           sa = sb;
