@@ -19,13 +19,16 @@
 // partial (o, m, z), and a second launch joins them in order: nothing depends on
 // timing.
 //
-// A wave takes 32 tokens a step, straight from memory into registers:
-//   S^T = K Q^T (16x16x32): a lane supplies 16 dims of a token at a time; what it then
-//         holds are the scores of 4 + 4 tokens for one head;
+// A wave works on 32 tokens at a time.  Their codes come from memory into LDS by loads
+// that pass no register, in whole rows and with no barrier, as the tile is the wave's
+// own: it reads the tile into registers, sends for the next one, and computes.
+//   S^T = K Q^T (16x16x32): a lane supplies 8 dims of a token; what it then holds are
+//         the scores of 4 + 4 tokens for one head;
 //   O^T = V^T P^T: those 8 weights are a lane's share of P^T as they are, if V^T is
-//         supplied with the same 8 tokens, which a lane loads for 4 NC neighbouring
-//         dims each and turns into operands by byte permutations.
-// No LDS tile and no barrier in the loop; LDS holds where the step's tokens are.
+//         supplied with the same 8 tokens, which the transposed LDS read does.
+// Three waves a SIMD up to 128 dims then have 96 KB of a CU's reads on their way; with
+// tiles in registers it were two and 64 KB (64 rows of up to 32K tokens, 32/8 heads of
+// 128 dims, int8: 172 us against XX).
 #include <algorithm>
 
 #include "quant.h"
@@ -35,8 +38,13 @@ using namespace moba;
 
 namespace {
 
+typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
+
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
-constexpr int kMaxWgs = 1024;   // of a launch, at most
+constexpr int kMaxWgs = 1280;   // of a launch, at most
+constexpr int kRun = 4;         // units of a workgroup, at least
+constexpr int kBegin = 2;       // units' worth of time that beginning an entry takes
+constexpr int kManyParts = 16;  // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects
 constexpr int kMaxItems = 32 * kMaxSlots;
 constexpr float kSlack = 6.0f;  // log2 by which scores may pass the running maximum
@@ -46,32 +54,45 @@ struct AttnArgs {
   const uint16_t* q;
   int Hq, G, HB, NHB;           // query heads per kv head; blocks of 16 in an entry (1, 2); entries per kv head
   int per_row;                  // entries per row: Hkv * NHB
+  FastDiv by_row, by_nhb;       // per_row, NHB
   const int *q_seq, *lengths;
   int length_add, max_length;
   const int* selected;          // null: dense
   int slots, chunk, max_items;
-  FastDiv by_chunk, by_d4;
+  FastDiv by_chunk, by_d4, by_pieces;
   int2* items;                  // [entries][max_items]: chunk, mask of heads
   int* tokens;                  // [entries] tokens of the items, end to end
   int scan_n, scan_mult;        // dense: rows, entries per row; else entries, 1
   uint32_t* start;              // [scan_n + 1] first unit of each
+  int* run_entry;               // [workgroups] entry of each run's first unit
   float scale_log2;
   float *part_o, *part_ml;      // [2 workgroups][16 HB heads][D], [..][2]
   uint16_t* out;
   float* lse;
 };
 
+MOBA_DEV int cut_length(const AttnArgs& a, int length) {
+  const int64_t n = (int64_t)length + a.length_add;
+  return (int)(n < 0 ? 0 : n < a.max_length ? n : a.max_length);
+}
 // Tokens that row r attends at most: none for a slot that does not exist.
 MOBA_DEV int row_length(const AttnArgs& a, int r) {
   const int s = a.q_seq[r];
   if (s < 0 || s >= a.pool.B) return 0;
-  const int64_t n = (int64_t)a.lengths[r] + a.length_add;
-  return (int)(n < 0 ? 0 : n < a.max_length ? n : a.max_length);
+  return cut_length(a, a.lengths[r]);
 }
 MOBA_DEV int scan_tokens(const AttnArgs& a, int i) {
   return a.selected != nullptr ? a.tokens[i] : row_length(a, i);
 }
+// Workgroups that share T units: all of the launch's, where each then has kRun units or
+// more (a run that ends inside an entry writes its sums of 16 heads, as much as a quarter
+// of a unit's codes), else fewer of them; up to one a CU for fewer units than that.
+MOBA_DEV uint32_t sharers(uint32_t launched, uint32_t T) {
+  return min(launched, max((T + kRun - 1) / kRun, min(T, 256u)));
+}
 MOBA_DEV uint32_t units_of(int tokens) { return ((uint32_t)tokens + kUnit - 1) / kUnit; }
+// What an entry counts for in the deal: its units, and what beginning and ending it costs.
+MOBA_DEV uint32_t shares_of(int tokens) { return tokens > 0 ? units_of(tokens) + kBegin : 0; }
 
 // Workgroup w of W has units [first(w), first(w + 1)) of T >= W.
 struct Deal {
@@ -142,72 +163,10 @@ __global__ __launch_bounds__(64) void union_kernel(AttnArgs a) {
 }
 
 // ------------------------------------------------------------------ attention
-// Bytes of 4 tokens, dword by dword, to the bytes of each place: out[b] holds byte b
-// of a, b, c and d.
-MOBA_DEV void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&out)[4]) {
-  const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400), ab2 = __builtin_amdgcn_perm(b, a, 0x07030602);
-  const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400), cd2 = __builtin_amdgcn_perm(d, c, 0x07030602);
-  out[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100);
-  out[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302);
-  out[2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100);
-  out[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302);
-}
-
-// A read of bytes that this call reads once.
-template <typename T> MOBA_DEV T load_once(const T* p) { return __builtin_nontemporal_load(p); }
-
-// Keys of a step: 16 dims at 64 c + 16 g of token 16 t + l % 16.
-template <int NC> struct Keys {
-  u32x4_t reg[2][NC];
-};
-// Values of a step: the lane's 4 NC dims of tokens 4 g + j (j < 4) and 16 + 4 g + j - 4.
-template <int NC> struct Values {
-  uint32_t reg[8][NC];
-  MOBA_DEV void load(int j, const uint8_t* p) {
-    if constexpr (NC == 1) {
-      reg[j][0] = load_once(reinterpret_cast<const uint32_t*>(p));
-    } else {
-      typedef uint32_t words __attribute__((ext_vector_type(NC)));
-      const words x = load_once(reinterpret_cast<const words*>(p));
-#pragma unroll
-      for (int d = 0; d < NC; ++d) reg[j][d] = x[d];
-    }
-  }
-  // The 8 tokens of each of the four dims of dword d, in bf16.
-  template <int FMT> MOBA_DEV void operands(int d, u32x4_t (&out)[4]) const {
-    if constexpr (FMT == 1) {  // 16 permutations, then two codes an instruction
-      uint32_t x[4], y[4];
-      transpose4(reg[0][d], reg[1][d], reg[2][d], reg[3][d], x);
-      transpose4(reg[4][d], reg[5][d], reg[6][d], reg[7][d], y);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        uint32_t lo, hi;
-        numbers4_16<1, 0>(x[b], lo, hi); out[b][0] = lo; out[b][1] = hi;
-        numbers4_16<1, 0>(y[b], lo, hi); out[b][2] = lo; out[b][3] = hi;
-      }
-    } else {  // int8: a conversion takes any byte of a word, and the halves are put together
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lo = (float)(int8_t)(reg[2 * j][d] >> (8 * b)), hi = (float)(int8_t)(reg[2 * j + 1][d] >> (8 * b));
-          out[b][j] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
-        }
-    }
-  }
-};
-// What a lane knows of a step: the scales of token l % 32 and the heads that attend it;
-// which of the step's tokens there are, and whether all heads attend all 32.
-struct Step {
-  float ks, vs;
-  uint32_t mask, live;
-  bool whole;
-};
-
-// Waves of a workgroup.
-constexpr int kWaves = 4;
-// Workgroups of a CU that the registers allow.
-template <int NC> constexpr int occupancy() { return NC == 1 ? 3 : 2; }
+constexpr int kWaves = 4;  // of a workgroup
+// NT: 16-dim tiles of a head that the registers hold.  Workgroups of a CU: what registers
+// and LDS allow.
+template <int NT> constexpr int occupancy() { return NT <= 4 ? 5 : NT <= 6 ? 4 : NT <= 8 ? 3 : 2; }
 
 // Where a step's tokens are, before the pool's rows are known.
 struct Look {
@@ -216,13 +175,138 @@ struct Look {
   uint32_t mask;  // heads that attend it (chunks)
 };
 
-template <int DT, int FMT, int NC>
-__global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a) {
-  constexpr int LD = 64 * NC + 4;  // floats of a joined row: neighbouring heads 4 banks apart
-  __shared__ __attribute__((aligned(16))) float join_o[kWaves][16][LD];
+// 16 bytes a lane from memory to LDS, lane l's to lds + 16 l; read once.  Out of the
+// compiler's sight, which would wait for it before every later read of LDS; `receive`
+// waits where the bytes are read.  (One wait state between M0 and the load that uses it.)
+MOBA_DEV void load_tile(const uint8_t* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+               :: "s"(lds), "v"(from) : "memory", "m0");
+}
+// Four words at a 16-byte border.
+template <typename T> MOBA_DEV T lds4(const void* p) {
+  return *reinterpret_cast<const T*>(__builtin_assume_aligned(p, 16));
+}
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
+// ds_read_b64_tr_b8: in each 16 lanes, lane i gets byte i of 8 rows of 16 bytes when lane
+// i' addresses row i' / 2, byte 8 (i' % 2).
+MOBA_DEV i32x2_t read_tr8(const uint8_t* p) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t*)p);
+}
+
+// What a lane knows of a step: the scales of token l of its 64 and the heads that attend
+// it; which of the tokens there are, and which of those all heads attend.
+struct Step {
+  float ks, vs;
+  uint32_t mask;
+  uint64_t live, all;
+};
+
+// The query of a lane's head in the dims that the lane multiplies: as it is, for keys that
+// are turned into its type; or, for int8 keys, which go to the matrix unit as they are, as
+// three 8-bit digits of a 24-bit integer q 2^k with max |q| 2^k in [2^21, 2^22): off by
+// at most 2^-22 of the largest |q|, and exact for what lies less than 2^11 (fp16) or
+// 2^14 (bf16) below it.  Turning 128 dims of 32 int8 keys takes a wave 96
+// instructions; joining three integer sums of 8 scores takes 40.
+template <int FMT, int NT> constexpr bool digits() { return FMT == 0 && NT > 4; }
+template <int DT, int NT, bool DIGITS> struct Query;
+template <int DT, int NT> struct Query<DT, NT, false> {
+  static constexpr int kSteps = (NT + 1) / 2, kBytes = 8;  // of 32 dims: 8 of a lane's token
+  static constexpr int kRaw = kSteps;
+  static MOBA_DEV int dim(int c, int g) { return 32 * c + 8 * g; }
+  u16x8_t part[kSteps];
+  MOBA_DEV void set(const u16x8_t (&raw)[kRaw]) {
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) part[c] = raw[c];
+  }
+  struct Codes {
+    uint2 step[kSteps];
+    MOBA_DEV void read(int c, const uint8_t* p) { step[c] = *reinterpret_cast<const uint2*>(p); }
+  };
+  // q . c of a token's codes
+  template <int FMT> MOBA_DEV f32x4_t dot(const Codes& k) const {
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      uint32_t w[4];
+      numbers4_16<FMT, DT>(k.step[c].x, w[0], w[1]);
+      numbers4_16<FMT, DT>(k.step[c].y, w[2], w[3]);
+      s = mfma16<DT>(__builtin_bit_cast(u16x8_t, (u32x4_t){w[0], w[1], w[2], w[3]}), part[c], s);
+    }
+    return s;
+  }
+};
+template <int DT, int NT> struct Query<DT, NT, true> {
+  static constexpr int kSteps = (NT + 3) / 4, kBytes = 16;  // of 64 dims: 16 of a lane's token
+  i32x4_t digit[3][kSteps];  // lowest first
+  float unit;                // 2^-k
+  static constexpr int kRaw = 2 * kSteps;
+  static MOBA_DEV int dim(int c, int g) { return 64 * (c >> 1) + 16 * g + 8 * (c & 1); }
+  MOBA_DEV void set(const u16x8_t (&raw)[kRaw]) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < kRaw; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits = max(bits, __float_as_uint(to_f32<DT>(raw[c][e])) & 0x7fffffffu);
+    }
+    bits = max(bits, (uint32_t)__shfl_xor((int)bits, 16, 64));
+    bits = max(bits, (uint32_t)__shfl_xor((int)bits, 32, 64));
+    // a query that is not finite: its scores are NaN
+    const bool finite = bits < 0x7f800000u;
+    const int e = max((int)(bits >> 23), 1 + 21);  // max |q| < 2^(e - 126); smallest: 2^-105
+    const float fold = __uint_as_float((uint32_t)(finite ? min(127 + 126 + 22 - e, 254) : 127) << 23);
+    unit = finite ? __uint_as_float((uint32_t)max(e - 22 + 1, 0) << 23) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t d[3] = {0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int i = 4 * w + b;
+          int v = (int)rintf(to_f32<DT>(raw[2 * c + (i >> 3)][i & 7]) * fold);
+#pragma unroll
+          for (int x = 0; x < 3; ++x) {
+            d[x] |= ((uint32_t)v & 255u) << (8 * b);
+            v = (v + 128) >> 8;  // what the signed digit leaves
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 3; ++x) digit[x][c][w] = (int)d[x];
+      }
+  }
+  struct Codes {
+    i32x4_t step[kSteps];
+    MOBA_DEV void read(int c, const uint8_t* p) { step[c] = *reinterpret_cast<const i32x4_t*>(p); }
+  };
+  template <int FMT> MOBA_DEV f32x4_t dot(const Codes& k) const {
+    i32x4_t s[3];
+#pragma unroll
+    for (int x = 2; x >= 0; --x) {
+      // the highest two digits in one integer: 127 256 (65 256 + 128) < 2^31
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[x][i] = x == 1 ? s[2][i] << 8 : 0;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+        s[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k.step[c], digit[x][c], s[x], 0, 0, 0);
+    }
+    f32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = fmaf((float)s[1][i], 256.0f, (float)s[0][i]) * unit;
+    return r;
+  }
+};
+
+template <int DT, int FMT, int NT>
+__global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a) {
+  constexpr int LD = 16 * NT + 4;  // floats of a joined row: neighbouring heads 4 banks apart
+  // a wave's tile (keys, then values of 32 tokens) and, when it has been used, its sums
+  constexpr int TILE = 2 * 32 * 16 * NT, SUMS = 16 * LD * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t tile_s[kWaves][TILE > SUMS ? TILE : SUMS];
   __shared__ float join_m[kWaves][16], join_l[kWaves][16];
-  __shared__ __attribute__((aligned(16))) uint32_t off_s[kWaves][32], mask_s[kWaves][32];
-  __shared__ __attribute__((aligned(16))) float ks_s[kWaves][32], vs_s[kWaves][32];
+  __shared__ uint32_t off_s[kWaves][64];
+  __shared__ __attribute__((aligned(16))) uint32_t mask_s[kWaves][64];
+  __shared__ __attribute__((aligned(16))) float ks_s[kWaves][64], vs_s[kWaves][64];
   __shared__ int2 items_s[kMaxItems];
   __shared__ uint32_t wave_sum[kWaves], found[2];
 
@@ -234,7 +318,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
   const uint32_t per = ((uint32_t)a.scan_n + 255) / 256, i0 = tid * per;
   const uint32_t i1 = min(i0 + per, (uint32_t)a.scan_n);
   uint32_t mine = 0;
-  for (uint32_t i = i0; i < i1; ++i) mine += units_of(scan_tokens(a, i)) * a.scan_mult;
+  for (uint32_t i = i0; i < i1; ++i) mine += shares_of(scan_tokens(a, i)) * a.scan_mult;
   uint32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -250,12 +334,12 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
     T += wave_sum[x];
   }
   uint32_t excl = base + incl - mine;
-  const uint32_t W = min((uint32_t)gridDim.x, T);
+  const uint32_t W = sharers(gridDim.x, T);
   if (blockIdx.x == 0) {  // for the second launch
     uint32_t s = excl;
     for (uint32_t i = i0; i < i1; ++i) {
       a.start[i] = s;
-      s += units_of(scan_tokens(a, i)) * a.scan_mult;
+      s += shares_of(scan_tokens(a, i)) * a.scan_mult;
     }
     if (tid == 0) a.start[a.scan_n] = T;
   }
@@ -267,7 +351,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
   if (x0 >= excl && x0 < excl + mine) {  // one thread has it
     uint32_t rem = x0 - excl, i = i0;
     for (;; ++i) {
-      const uint32_t n = units_of(scan_tokens(a, i)) * a.scan_mult;
+      const uint32_t n = shares_of(scan_tokens(a, i)) * a.scan_mult;
       if (rem < n) break;
       rem -= n;
     }
@@ -275,25 +359,66 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
     found[1] = rem;
   }
   __syncthreads();
-  uint32_t si = __builtin_amdgcn_readfirstlane(found[0]), rem = __builtin_amdgcn_readfirstlane(found[1]);
+  uint32_t si = __builtin_amdgcn_readfirstlane(found[0]), off = __builtin_amdgcn_readfirstlane(found[1]), in = 0;
   bool first_segment = true;
+  // what the scan entry after the present one is, asked for while that one is worked on
+  struct Peek {
+    int tokens, slot, length;
+  };
+  auto peek = [&](uint32_t i) __attribute__((always_inline)) {
+    Peek p;
+    i = min(i, (uint32_t)a.scan_n - 1);
+    const int r = moba ? (int)div_by(i, a.by_row) : (int)i;
+    p.slot = a.q_seq[r];
+    p.length = a.lengths[r];
+    p.tokens = moba ? a.tokens[i] : 0;
+    return p;
+  };
+  Peek coming = peek(si);
 
   while (left > 0) {
-    // ---- a segment: units [off, off + n) of entry e
-    const int scan_len = __builtin_amdgcn_readfirstlane(scan_tokens(a, si));
-    const uint32_t u = units_of(scan_len);
-    if (u == 0) { ++si; continue; }
-    const uint32_t in = rem / u, off = rem - in * u, n = min(left, u - off);
+    // ---- a segment: units [off, off + n) of entry e, the in-th of scan entry si
+    const int slot_id = __builtin_amdgcn_readfirstlane(coming.slot);
+    int len = __builtin_amdgcn_readfirstlane(coming.length);
+    len = slot_id < 0 || slot_id >= a.pool.B ? 0 : cut_length(a, len);
+    const int scan_len = moba ? __builtin_amdgcn_readfirstlane(coming.tokens) : len;
+    const uint32_t shares = shares_of(scan_len), u = units_of(scan_len);
+    if (shares == 0) {
+      coming = peek(++si);
+      continue;
+    }
+    if (off >= shares) {  // at the start only: the run begins in a later entry of the row
+      in = off / shares;
+      off -= in * shares;
+    }
+    const uint32_t taken = min(left, shares - off), n = min(off + taken, u) - min(off, u);
     const int e = (int)(si * a.scan_mult + in);
-    const int r = e / a.per_row, kh = (e % a.per_row) / a.NHB, blk = e % a.NHB;
+    if (first_segment && tid == 0) a.run_entry[wg] = e;
+    const uint32_t from = off;
+    left -= taken;
+    off += taken;
+    if (off == shares) {
+      off = 0;
+      if (++in == (uint32_t)a.scan_mult) {
+        in = 0;
+        coming = peek(++si);
+      }
+    }
+    if (n == 0) {  // the rest of an entry's share, without units
+      first_segment = false;
+      continue;
+    }
+    const int r = (int)div_by(e, a.by_row), of_row = e - r * a.per_row;
+    const int kh = (int)div_by(of_row, a.by_nhb), blk = of_row - kh * a.NHB;
     const int head0 = kh * a.G + blk * 16 * a.HB;             // of the entry
     const int heads = min(16 * a.HB, a.G - blk * 16 * a.HB);
-    const int len = moba ? __builtin_amdgcn_readfirstlane(row_length(a, r)) : scan_len;
-    const int v_lo = (int)off * kUnit, v_hi = min((int)(off + n) * kUnit, scan_len);
-    const int hb = w % a.HB, streams = kWaves / a.HB, stream = w / a.HB;
+    const int v_lo = (int)from * kUnit, v_hi = min((int)(from + n) * kUnit, scan_len);
+    const int hb = w & (a.HB - 1), streams = kWaves >> (a.HB - 1), stream = w >> (a.HB - 1);
     const int my_head = hb * 16 + c16;                         // in the entry
-    const int steps = (v_hi - v_lo + 31) / 32;
-    const int* trow = a.pool.table + (int64_t)a.q_seq[r] * a.pool.W;
+    // A wave's step is 64 tokens, found with one look; 32 where 64 would leave waves idle.
+    const int span_log = (n & (a.HB == 2 ? 0 : 1)) && n <= 8 ? 5 : (v_hi - v_lo) <= 32 * streams ? 5 : 6;
+    const int steps = (v_hi - v_lo + (1 << span_log) - 1) >> span_log;
+    const int* trow = a.pool.table + (int64_t)slot_id * a.pool.W;
     if (moba) {
       const int first_item = (int)div_by(v_lo, a.by_chunk), last_item = (int)div_by(v_hi - 1, a.by_chunk);
       const int2* it = a.items + (int64_t)e * a.max_items;
@@ -301,29 +426,37 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
       __syncthreads();
     }
 
-    u16x8_t qf[2 * NC];  // dims 64 c + 16 g + 8 x .. + 7 of the lane's head
+    typedef Query<DT, NT, digits<FMT, NT>()> Q;
+    u16x8_t raw[Q::kRaw];  // asked for first: its address waits for nothing
     {
       const uint16_t* qp = a.q + ((int64_t)r * a.Hq + head0 + min(my_head, heads - 1)) * a.pool.D;
 #pragma unroll
-      for (int c = 0; c < 2 * NC; ++c) {
-        const int d = 64 * (c >> 1) + 16 * g + 8 * (c & 1);
-        const u16x8_t x = ld8(qp + (d < a.pool.D ? d : 0));
-        qf[c] = d < a.pool.D && my_head < heads ? x : zero8();
+      for (int c = 0; c < Q::kRaw; ++c) {
+        const int d = Q::dim(c, g);
+        raw[c] = ld8(qp + (d < a.pool.D ? d : 0));
       }
     }
-    f32x4_t acc[4 * NC];
+    f32x4_t acc[NT];  // dims 16 t + 4 g + i of the lane's head
 #pragma unroll
-    for (int t = 0; t < 4 * NC; ++t) acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; ++t) acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
 
     const uint32_t heads_mask = heads == 32 ? ~0u : (1u << heads) - 1;
-    const uint32_t pieces = a.pool.Dp / 16;  // of a row of codes
+    const int pieces = a.pool.Dp / 16;  // of a row of codes
+    // Piece p of token t's row lies at place p ^ f(t) of its row in the tile, so that the
+    // same piece of 16 tokens lies in as many banks as it can (rows of 2^n pieces; the
+    // others' strides spread it by themselves).
+    const int f_shift = pieces == 8 ? 1 : pieces == 4 ? 2 : pieces == 2 ? 3 : 0;
+    const int f_mask = (pieces & (pieces - 1)) == 0 ? pieces - 1 : 0;
+    uint8_t* const tile = tile_s[w];
+    uint8_t* const tile_v = tile + 32 * 16 * NT;
+    const uint32_t tile_at = lds_addr(tile);
     auto look = [&](int step) __attribute__((always_inline)) {
       Look x;
-      const int v = v_lo + 32 * step + (lane & 31);
+      const int v = v_lo + (step << span_log) + lane;
       uint32_t t = v;
       x.mask = heads_mask;
-      bool ok = v < v_hi;
+      bool ok = lane < (1 << span_log) && v < v_hi;
       if (moba) {
         const uint32_t it = div_by(ok ? v : v_lo, a.by_chunk);
         const int2 item = items_s[it];
@@ -331,90 +464,113 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         x.mask = item.y;
         ok = ok && t < (uint32_t)len;
       }
-      const uint32_t lp = ok ? div_by(t, a.pool.by_page) : 0u;
+      t = ok ? t : 0u;
+      const uint32_t lp = div_by(t, a.pool.by_page);
       x.page = trow[lp];
       x.at = ok ? t - lp * a.pool.by_page.d : ~0u;
       return x;
     };
-    // Puts a step's places, from its page entries, where all lanes see them; loads its
-    // keys and the scales of the lane's token.  A step behind the last reads the pool's
-    // first row over and over: its loads are cheaper than a branch around them, behind
-    // which the compiler would wait for every load in flight.
-    auto fetch_keys = [&](const Look& x, Keys<NC>& k, Step& s, uint32_t (&voff)[8]) __attribute__((always_inline)) {
-      const bool ok = x.at != ~0u && x.page >= 0 && x.page < a.pool.num_pages;
+    // Puts a step's places, from its page entries, where all lanes see them, and asks for
+    // the scales of the lane's token.  A step behind the last, and a token that is not
+    // there, reads the pool's first row: such loads are cheaper than a branch around
+    // them, behind which the compiler would wait for every load in flight.
+    auto place = [&](const Look& x, Step& s) __attribute__((always_inline)) {
+      const bool ok = x.at != ~0u && (uint32_t)x.page < (uint32_t)a.pool.num_pages;
       const uint32_t row = ok ? ((uint32_t)x.page * a.pool.Hkv + kh) * a.pool.P + x.at : 0u;
-      off_s[w][lane & 31] = row * pieces;
-      s.live = (uint32_t)__ballot(ok);
+      off_s[w][lane] = row * (uint32_t)pieces;
+      s.live = __ballot(ok);
       s.mask = x.mask;
-      s.whole = s.live == ~0u && (!moba || __all(x.mask == heads_mask));
+      s.all = moba ? s.live & __ballot(x.mask == heads_mask) : s.live;
       s.ks = a.pool.ks[row];
       s.vs = a.pool.vs[row];
       wave_lds_sync();
+    };
+    // Keys and values of the 32 tokens from `half` (0 or 32) on are sent for in whole rows:
+    // lane l of load j has place x = 64 j + l of the tile, of token x / pieces.
+    uint32_t places[NT / 2];  // token, and piece above it
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const uint8_t* p = a.pool.k + ((uint64_t)off_s[w][16 * t + c16] << 4);
+    for (int j = 0; j < NT / 2; ++j) {
+      const int x = 64 * j + lane, t = (int)div_by(x, a.by_pieces), p = x - t * pieces;
+      places[j] = x < 32 * pieces ? t | (p ^ ((t >> f_shift) & f_mask)) << 16 : 31;  // else: behind the rows
+    }
+    uint32_t source[NT / 2];  // 16-byte piece of the pool for each place
+    auto aim = [&](int half) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int d = 64 * c + 16 * g;
-          k.reg[t][c] = load_once(reinterpret_cast<const u32x4_t*>(p + (d < a.pool.Dp ? d : 0)));
+      for (int j = 0; j < NT / 2; ++j) source[j] = off_s[w][half + (places[j] & 63)] + (places[j] >> 16);
+    };
+    auto send = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NT / 2; ++j) {
+        if (2 * j < pieces) {
+          load_tile(a.pool.k + ((uint64_t)source[j] << 4), tile_at + 1024 * j);
+          load_tile(a.pool.v + ((uint64_t)source[j] << 4), tile_at + 32 * 16 * NT + 1024 * j);
         }
-        const u32x4_t o = *reinterpret_cast<const u32x4_t*>(&off_s[w][16 * t + 4 * g]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) voff[4 * t + i] = o[i];
       }
-      wave_lds_sync();
     };
-    const int vd = 4 * NC * c16 < a.pool.Dp ? 4 * NC * c16 : 0;
-    auto fetch_values = [&](Values<NC>& v, const uint32_t (&voff)[8]) __attribute__((always_inline)) {
+    // The tile's keys and values, as the products take them.
+    typename Q::Codes keys[2];  // of token 16 t + l % 16
+    i32x2_t values[NT];         // dim 16 t + l % 16 of tokens 4 g + j and 16 + 4 g + j, j < 4
+    // (addresses are put together where they are used: held, they cost a wave of a SIMD)
+    const uint32_t key_at = c16 * a.pool.Dp + (Q::kBytes == 16 ? 0 : 8 * (g & 1));
+    const uint32_t key_f = 16 * ((c16 >> f_shift) & f_mask);  // the same for token 16 + c16
+    const int token_v = (c16 & 8 ? 16 : 0) + 4 * g + ((c16 >> 1) & 3);
+    const uint32_t value_at = token_v * a.pool.Dp + 8 * (c16 & 1);
+    const uint32_t value_f = 16 * ((token_v >> f_shift) & f_mask);
+    auto receive = [&]() __attribute__((always_inline)) {
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      const uint32_t at_key = opaque(key_at), at_value = opaque(value_at);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v.load(j, a.pool.v + ((uint64_t)voff[j] << 4) + vd);
-    };
-    // Scales of a step, from a lane per token to the scores' layout, and its scores in log2.
-    f32x4_t sc[2], vv[2];
-    u32x4_t mk[2];
-    auto scores = [&](const Keys<NC>& k, const Step& s) __attribute__((always_inline)) {
-      if (lane < 32) {
-        ks_s[w][lane] = s.ks * a.scale_log2;
-        vs_s[w][lane] = s.vs;
-        if (moba) mask_s[w][lane] = s.mask;
-      }
-      wave_lds_sync();
-      f32x4_t kk[2];
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        kk[t] = *reinterpret_cast<const f32x4_t*>(&ks_s[w][16 * t + 4 * g]);
-        vv[t] = *reinterpret_cast<const f32x4_t*>(&vs_s[w][16 * t + 4 * g]);
-        if (moba) mk[t] = *reinterpret_cast<const u32x4_t*>(&mask_s[w][16 * t + 4 * g]);
-      }
-      wave_lds_sync();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          u32x4_t lo, hi;
-          uint32_t x, y;
-          numbers4_16<FMT, DT>(k.reg[t][c][0], x, y); lo[0] = x; lo[1] = y;
-          numbers4_16<FMT, DT>(k.reg[t][c][1], x, y); lo[2] = x; lo[3] = y;
-          numbers4_16<FMT, DT>(k.reg[t][c][2], x, y); hi[0] = x; hi[1] = y;
-          numbers4_16<FMT, DT>(k.reg[t][c][3], x, y); hi[2] = x; hi[3] = y;
-          sc[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, lo), qf[2 * c], sc[t]);
-          sc[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, hi), qf[2 * c + 1], sc[t]);
+        for (int c = 0; c < Q::kSteps; ++c) {
+          // pieces behind the row: the query is 0 there, and the codes must be finite
+          const int piece = Q::kBytes == 16 ? 4 * c + g : 2 * c + (g >> 1);
+          keys[t].read(c, tile + at_key + t * 16 * a.pool.Dp + ((piece < pieces ? 16 * piece : 0) ^ key_f));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[t][i] *= kk[t][i];
+      for (int t = 0; t < NT; ++t) values[t] = read_tr8(tile_v + at_value + ((t < pieces ? 16 * t : 0) ^ value_f));
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the tile may be sent for again
+      asm volatile("" ::: "memory");
+    };
+    // Scales of a step, from a lane per token to where all lanes see them.
+    auto share = [&](const Step& s) __attribute__((always_inline)) {
+      ks_s[w][lane] = s.ks * a.scale_log2;
+      vs_s[w][lane] = s.vs;
+      if (moba) mask_s[w][lane] = s.mask;
+      wave_lds_sync();
+    };
+    // Scores of 32 tokens in log2.
+    Q query;
+    f32x4_t sc[2];
+    auto scores = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f32x4_t kk = lds4<f32x4_t>(&ks_s[w][half + 16 * t + 4 * g]);
+        sc[t] = query.template dot<FMT>(keys[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[t][i] *= kk[i];
       }
     };
     // The softmax of those scores and their product with the values.
-    auto weigh = [&](Values<NC>& v, const Step& s) __attribute__((always_inline)) {
+    auto weigh = [&](int half, const Step& s) __attribute__((always_inline)) {
+      const uint32_t live = (uint32_t)(s.live >> half);
+      const bool whole = (uint32_t)(s.all >> half) == ~0u;
+      f32x4_t vv[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vv[t] = lds4<f32x4_t>(&vs_s[w][half + 16 * t + 4 * g]);
       float p[8], wt[8], top = -INFINITY;
       uint32_t on = 0xff;  // bit j: the lane's head attends its token j
-      if (!s.whole) {
-        on = ((s.live >> (4 * g)) & 15) | (((s.live >> (16 + 4 * g)) & 15) << 4);
+      if (!whole) {
+        on = ((live >> (4 * g)) & 15) | (((live >> (16 + 4 * g)) & 15) << 4);
         if (moba) {
           uint32_t takes = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) takes |= ((mk[j >> 2][j & 3] >> my_head) & 1) << j;
+          for (int t = 0; t < 2; ++t) {
+            const u32x4_t mk = lds4<u32x4_t>(&mask_s[w][half + 16 * t + 4 * g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) takes |= ((mk[i] >> my_head) & 1) << (4 * t + i);
+          }
           on &= takes;
         }
 #pragma unroll
@@ -434,7 +590,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         m = to;
         l *= shrink;
 #pragma unroll
-        for (int t = 0; t < 4 * NC; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[t][i] *= shrink;
       }
@@ -445,7 +601,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         l += p[j];
         wt[j] = p[j] * vv[j >> 2][j & 3];
       }
-      if (!s.whole) {
+      if (!whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) wt[j] = (on >> j) & 1 ? wt[j] : 0.0f;  // a NaN scale that is not attended
       }
@@ -457,72 +613,77 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         unpack2<0>(hi[j], x, y);
         lo[j] = pack2<0>(wt[2 * j] - x, wt[2 * j + 1] - y);
       }
-      if (!s.whole) {
+      if (live != ~0u) {  // a token that is not there: its codes were never written, or may be a NaN's
+        uint32_t there[2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool there = (s.live >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1;
-#pragma unroll
-          for (int d = 0; d < NC; ++d) v.reg[j][d] = there ? v.reg[j][d] : 0;  // never written: may be a NaN's code
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t bits = (live >> (16 * x + 4 * g)) & 15;  // to a byte each
+          there[x] = ((bits & 1) | (bits & 2) << 7 | (bits & 4) << 14 | (bits & 8) << 21) * 255u;
         }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) values[t][x] &= (int)there[x];
       }
 #pragma unroll
-      for (int d = 0; d < NC; ++d) {
-        u32x4_t vt[4];
-        v.template operands<FMT>(d, vt);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt[b]), __builtin_bit_cast(u16x8_t, hi), acc[4 * d + b]);
-          acc[4 * d + b] = mfma16<0>(__builtin_bit_cast(u16x8_t, vt[b]), __builtin_bit_cast(u16x8_t, lo), acc[4 * d + b]);
-        }
+      for (int t = 0; t < NT; ++t) {
+        uint32_t v[4];
+        numbers4_16<FMT, 0>((uint32_t)values[t][0], v[0], v[1]);
+        numbers4_16<FMT, 0>((uint32_t)values[t][1], v[2], v[3]);
+        const u16x8_t vt = __builtin_bit_cast(u16x8_t, (u32x4_t){v[0], v[1], v[2], v[3]});
+        acc[t] = mfma16<0>(vt, __builtin_bit_cast(u16x8_t, hi), acc[t]);
+        acc[t] = mfma16<0>(vt, __builtin_bit_cast(u16x8_t, lo), acc[t]);
       }
     };
 
-    int k = stream;
-    if (k < steps) {
-      // Loads return in order: the page entries of a step are asked for before the keys
-      // and values of the one before it, so that waiting for them waits for nothing else.
-      uint32_t voff[8];
-      Look now = look(k), next = look(k + streams), after;
-      if constexpr (NC <= 2) {
-        // two steps in registers: one is on its way while the other is worked on
-        Keys<NC> ka, kb;
-        Values<NC> va, vb;
-        Step sa, sb;
-        fetch_keys(now, ka, sa, voff);
-        fetch_values(va, voff);
-        for (;;) {
-          after = look(k + 2 * streams);
-          fetch_keys(next, kb, sb, voff);
-          fetch_values(vb, voff);
-          scores(ka, sa);
-          weigh(va, sa);
+    if (stream < steps) {
+      // The halves of the wave's steps, in order: one is worked on, the next one's codes are
+      // on their way, and where the one after lies is known, so that it can be sent for as
+      // soon as the tile has been read.  Page entries are asked for one step ahead of that.
+      // Everything a wave waits for in memory it waits for at the tile.
+      struct Half {
+        Step s;
+        int half;
+        bool any;
+      } at, sent, aimed;
+      int k = stream;
+      Look page = look(k);
+      Step step;
+      bool second = false;
+      auto prepare = [&]() __attribute__((always_inline)) {
+        aimed.any = second || k < steps;
+        aimed.half = second ? 32 : 0;
+        if (second) {
+          second = false;
+        } else if (aimed.any) {
+          place(page, step);
           k += streams;
-          if (k >= steps) break;
-          next = look(k + 2 * streams);
-          fetch_keys(after, ka, sa, voff);
-          fetch_values(va, voff);
-          scores(kb, sb);
-          weigh(vb, sb);
-          k += streams;
-          if (k >= steps) break;
+          page = look(k);
+          second = (step.live >> 32) != 0;
         }
-      } else {
-        // registers for one: its keys make room after the scores, its values after theirs
-        Keys<NC> ka;
-        Values<NC> va;
-        Step sa, sb;
-        fetch_keys(now, ka, sa, voff);
-        fetch_values(va, voff);
-        for (; k < steps; k += streams) {
-          scores(ka, sa);
-          after = look(k + 2 * streams);
-          fetch_keys(next, ka, sb, voff);
-          next = after;
-          weigh(va, sa);
-          fetch_values(va, voff);
-          sa = sb;
-        }
-      }
+        aimed.s = step;
+        if (aimed.any) aim(aimed.half);
+      };
+      prepare();
+      send();
+      sent = aimed;
+      prepare();
+#pragma unroll
+      for (int c = 0; c < Q::kRaw; ++c)
+        if (Q::dim(c, g) >= a.pool.D || my_head >= heads) raw[c] = zero8();
+      query.set(raw);
+      do {
+        at = sent;
+        wave_prio<1>();  // the reads of the next half go out ahead of other waves' arithmetic
+        receive();
+        if (aimed.any) send();
+        wave_prio<0>();
+        sent = aimed;
+        prepare();
+        if (at.half == 0) share(at.s);
+        scores(at.half);
+        weigh(at.half, at.s);
+      } while (sent.any);
     }
 
     // ---- the four waves join; head h of block hb is in waves hb, hb + HB, ...
@@ -532,13 +693,10 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
       join_m[w][c16] = m;
       join_l[w][c16] = l;
     }
+    wave_lds_sync();
+    float* const sums = reinterpret_cast<float*>(tile);  // no load into the tile is on its way
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < NC; ++d) {
-        const f32x4_t x = {acc[4 * d][i], acc[4 * d + 1][i], acc[4 * d + 2][i], acc[4 * d + 3][i]};
-        *reinterpret_cast<f32x4_t*>(&join_o[w][c16][4 * NC * (4 * g + i) + 4 * d]) = x;
-      }
+    for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t*>(sums + c16 * LD + 16 * t + 4 * g) = acc[t];
     __syncthreads();
     const bool entire = n == u;
     const int D = a.pool.D;
@@ -552,7 +710,7 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
         const float my = join_m[y][h & 15];
         const float f = my == -INFINITY ? 0.0f : fast_exp2(my - top);
         z += join_l[y][h & 15] * f;
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&join_o[y][h & 15][d]);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(tile_s[y]) + (h & 15) * LD + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] += v[i] * f;
       }
@@ -569,52 +727,98 @@ __global__ __launch_bounds__(256, occupancy<NC>()) void attend_kernel(AttnArgs a
     }
     __syncthreads();  // the buffers are the next segment's
     first_segment = false;
-    left -= n;
-    rem += n;
-    if (rem == u * (uint32_t)a.scan_mult) { ++si; rem = 0; }
   }
 }
 
-// One workgroup per (entry, head) that spans several workgroups of the first launch:
-// their partials, weighted by 2^(m_j - m); cols (a power of two) threads of 4 dims each,
-// B / cols parts at once, whose sums are added in a fixed order.  An entry without
-// tokens gets zeros and -inf.
+// Joins the partials of the entries that span several workgroups of the first launch:
+// o = sum 2^(m_j - m) o_j, z = sum 2^(m_j - m) z_j, in an order that is fixed.  The
+// first workgroups have an entry each: a thread has 4 dims of a head and walks through
+// its parts.  Entries of many parts (fewer than one for every kManyParts runs) are left
+// to the others, one for each head and every kManyParts-th run: that run's
+// entry is theirs if the run is the first such one behind the entry's start; B / cols parts
+// at once, cols threads of 4 dims each (a power of two).
+struct Parts {
+  uint32_t w0, n;     // first workgroup, and how many (0: no units)
+  int64_t slot0;      // row of that one's partial of head 0
+  int hpe;
+  // workgroup w0 + j's: its first segment's (j > 0: its run begins within the entry)
+  MOBA_DEV int64_t slot(uint32_t j) const { return j == 0 ? slot0 : (int64_t)2 * (w0 + j) * hpe; }
+};
+MOBA_DEV Parts parts_of(const AttnArgs& a, int e, int wgs) {
+  Parts p;
+  p.hpe = 16 * a.HB;
+  const int si = a.scan_mult == 1 ? e : (int)div_by(e, a.by_row), in = e - si * a.scan_mult;
+  const uint32_t T = a.start[a.scan_n], s0 = a.start[si], all = a.start[si + 1] - s0;
+  const uint32_t shares = a.scan_mult == 1 ? all : div_by(all, a.by_row);
+  p.n = 0;
+  if (shares == 0) return p;
+  const Deal deal(T, sharers(wgs, T));
+  const uint32_t from = s0 + in * shares;
+  p.w0 = deal.owner(from);
+  p.n = deal.owner(from + shares - kBegin - 1) - p.w0 + 1;
+  p.slot0 = ((int64_t)2 * p.w0 + (deal.first(p.w0) < from ? 1 : 0)) * p.hpe;
+  return p;
+}
+template <int DT>
+MOBA_DEV void store_joined(const AttnArgs& a, int64_t row, int d, const f32x4_t& o, float top, float z) {
+  const float f = z == 0.0f ? 0.0f : 1.0f / z;
+  *reinterpret_cast<uint2*>(a.out + row * a.pool.D + d) =
+      make_uint2(pack2<DT>(o[0] * f, o[1] * f), pack2<DT>(o[2] * f, o[3] * f));
+  if (d == 0) a.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) * kLn2;
+}
+
 template <int DT, int B>
-__global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int cols, int per_entry) {
+__global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entries, int cols, int per_entry) {
   __shared__ float weight[kMaxWgs];
   __shared__ float red[2][B / 64];
   __shared__ __attribute__((aligned(16))) f32x4_t sums[B / 64][64];
-  const int hpe = 16 * a.HB, e = blockIdx.x / per_entry, h = blockIdx.x % per_entry;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int r = e / a.per_row, kh = (e % a.per_row) / a.NHB, blk = e % a.NHB;
-  if (h >= a.G - blk * hpe) return;
-  const int D = a.pool.D;
-  const int si = e / a.scan_mult;
-  const uint32_t T = a.start[a.scan_n], s0 = a.start[si], u = (a.start[si + 1] - s0) / a.scan_mult;
-  const int64_t row = (int64_t)r * a.Hq + kh * a.G + blk * hpe + h;
-  if (u == 0) {
-    for (int d = tid; d < D; d += B) a.out[row * D + d] = 0;
-    if (tid == 0) a.lse[row] = -INFINITY;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, D = a.pool.D;
+  int e = blockIdx.x, h = 0, run = 0;
+  const bool many = e >= entries;
+  if (many) {
+    h = (e - entries) % per_entry;
+    run = ((e - entries) / per_entry + 1) * kManyParts;
+    if (run >= (int)sharers(wgs, a.start[a.scan_n])) return;
+    e = a.run_entry[run];
+  }
+  const Parts p = parts_of(a, e, wgs);
+  const int r = (int)div_by(e, a.by_row), of_row = e - r * a.per_row;
+  const int kh = (int)div_by(of_row, a.by_nhb), blk = of_row - kh * a.NHB;
+  const int heads = min(p.hpe, a.G - blk * p.hpe);
+  const int64_t row0 = (int64_t)r * a.Hq + kh * a.G + blk * p.hpe;
+  if (!many) {
+    if (p.n == 1 || p.n > kManyParts) return;  // written by that workgroup; or left to the others
+    const int all = heads * (D / 4);
+    for (int x = tid; x < all; x += B) {
+      const int hx = (int)div_by(x, a.by_d4), d = 4 * (x - hx * (D / 4));
+      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, z = 0.0f;
+#pragma unroll 4
+      for (uint32_t j = 0; j < p.n; ++j) top = fmaxf(top, a.part_ml[2 * (p.slot(j) + hx)]);
+#pragma unroll 4
+      for (uint32_t j = 0; j < p.n; ++j) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p.slot(j) + hx));
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.part_o + (p.slot(j) + hx) * D + d);
+        const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
+        z += f * ml.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += v[i] * f;
+      }
+      store_joined<DT>(a, row0 + hx, d, o, top, z);  // no units: zeros and -inf
+    }
     return;
   }
-  const uint32_t W = min((uint32_t)wgs, T), from = s0 + (e % a.scan_mult) * u;
-  const Deal deal(T, W);
-  const uint32_t w0 = deal.owner(from), w1 = deal.owner(from + u - 1), parts = w1 - w0 + 1;
-  if (parts == 1) return;  // written by that workgroup
-  // workgroup x's partial of this entry: its first segment's, if its run begins within
-  // the entry (all but w0's do), else its last one's
-  const int64_t slot0 = ((int64_t)2 * w0 + (deal.first(w0) < from ? 1 : 0)) * hpe + h;
-  auto slot = [&](uint32_t j) { return j == 0 ? slot0 : (int64_t)2 * (w0 + j) * hpe + h; };
+  if (p.n <= kManyParts || h >= heads || (p.w0 / kManyParts + 1) * kManyParts != (uint32_t)run) return;
   float top = -INFINITY;
-  for (uint32_t j = tid; j < parts; j += B) top = fmaxf(top, a.part_ml[2 * slot(j)]);
+  for (uint32_t j = tid; j < p.n; j += B) top = fmaxf(top, a.part_ml[2 * (p.slot(j) + h)]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   if (lane == 0) red[0][w] = top;
   __syncthreads();
   for (int x = 0; x < B / 64; ++x) top = fmaxf(top, red[0][x]);
   float z = 0.0f;
-  for (uint32_t j = tid; j < parts; j += B) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot(j));
+  for (uint32_t j = tid; j < p.n; j += B) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p.slot(j) + h));
     const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
     weight[j] = f;
     z += f * ml.y;
@@ -629,8 +833,8 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int cols, 
   const int at = d < D ? d : 0;  // columns behind D repeat the first
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (uint32_t j = tid / cols; j < parts; j += groups) {
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + slot(j) * D + at);
+  for (uint32_t j = tid / cols; j < p.n; j += groups) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + (p.slot(j) + h) * D + at);
     const float f = weight[j];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += x[i] * f;
@@ -645,16 +849,13 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int cols, 
   for (int x = 0; x < B / 64; ++x)
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += sums[x][c][i];
-  const float f = z == 0.0f ? 0.0f : 1.0f / z;
-  *reinterpret_cast<uint2*>(a.out + row * D + d) =
-      make_uint2(pack2<DT>(o[0] * f, o[1] * f), pack2<DT>(o[2] * f, o[3] * f));
-  if (d == 0) a.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) * kLn2;
+  store_joined<DT>(a, row0 + h, d, o, top, z);
 }
 
 // Shape of a call: blocks of heads, entries, workgroups, and what its workspace holds.
 struct Shape {
   int G, HB, NHB, max_items, wgs;
-  int64_t entries, items_at, tokens_at, start_at, part_o_at, part_ml_at, bytes;
+  int64_t entries, items_at, tokens_at, start_at, run_at, part_o_at, part_ml_at, bytes;
 };
 Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_length) {
   Shape s;
@@ -664,7 +865,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.entries = (int64_t)Nq * Hkv * s.NHB;
   s.max_items = std::min(s.G, 16 * s.HB) * slots;
   // as many workgroups as the card holds at once, but no more than there can be units
-  const int per_cu = D > 64 ? 2 : 3;
+  const int per_cu = D > 128 ? 2 : D > 96 ? 3 : D > 64 ? 4 : 5;
   const int64_t longest = slots > 0 ? std::min<int64_t>((int64_t)s.max_items * chunk, max_length) : max_length;
   const int64_t units = s.entries * ((longest + kUnit - 1) / kUnit);
   s.wgs = (int)std::min<int64_t>(256 * per_cu, (units + 7) / 8 * 8);
@@ -674,6 +875,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.items_at = take(slots > 0 ? s.entries * s.max_items * 8 : 0);
   s.tokens_at = take(slots > 0 ? s.entries * 4 : 0);
   s.start_at = take((std::max<int64_t>(slots > 0 ? s.entries : Nq, 1) + 1) * 4);
+  s.run_at = take(s.wgs * 4);
   const int64_t rows = 2ll * s.wgs * 16 * s.HB;
   s.part_o_at = take(rows * D * 4);
   s.part_ml_at = take(rows * 8);
@@ -682,15 +884,22 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
 
 template <int DT, int FMT> void launch_attend(const AttnArgs& a, int wgs, hipStream_t st) {
   const dim3 grid(wgs), block(256);
-  if (a.pool.Dp <= 64) hipLaunchKernelGGL((attend_kernel<DT, FMT, 1>), grid, block, 0, st, a);
-  else if (a.pool.Dp <= 128) hipLaunchKernelGGL((attend_kernel<DT, FMT, 2>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((attend_kernel<DT, FMT, 4>), grid, block, 0, st, a);
+  const int tiles = a.pool.Dp / 16;
+  if (tiles <= 4) hipLaunchKernelGGL((attend_kernel<DT, FMT, 4>), grid, block, 0, st, a);
+  else if (tiles <= 6) hipLaunchKernelGGL((attend_kernel<DT, FMT, 6>), grid, block, 0, st, a);
+  else if (tiles <= 8) hipLaunchKernelGGL((attend_kernel<DT, FMT, 8>), grid, block, 0, st, a);
+  else if (tiles <= 12) hipLaunchKernelGGL((attend_kernel<DT, FMT, 12>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((attend_kernel<DT, FMT, 16>), grid, block, 0, st, a);
 }
 
-// Few joins have many parts each: wide workgroups then.
-template <int DT> void launch_join(const AttnArgs& a, unsigned joins, int wgs, int cols, int per_entry, hipStream_t st) {
-  if (joins <= 256) hipLaunchKernelGGL((join_kernel<DT, 1024>), dim3(joins), dim3(1024), 0, st, a, wgs, cols, per_entry);
-  else hipLaunchKernelGGL((join_kernel<DT, 256>), dim3(joins), dim3(256), 0, st, a, wgs, cols, per_entry);
+// Few entries have many parts each: wide workgroups then.
+template <int DT> void launch_join(const AttnArgs& a, int entries, int wgs, hipStream_t st) {
+  int cols = 16;
+  while (cols * 4 < a.pool.D) cols *= 2;
+  const int per_entry = std::min(a.G, 16 * a.HB);
+  const dim3 grid((unsigned)(entries + (wgs - 1) / kManyParts * per_entry));
+  if (entries <= 64) hipLaunchKernelGGL((join_kernel<DT, 1024>), grid, dim3(1024), 0, st, a, wgs, entries, cols, per_entry);
+  else hipLaunchKernelGGL((join_kernel<DT, 256>), grid, dim3(256), 0, st, a, wgs, entries, cols, per_entry);
 }
 
 }  // namespace
@@ -725,7 +934,7 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   chunk = std::min(chunk, max_length);  // a longer one ends where the row does
   const Shape s = shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length);
   // units, tokens and workgroups of the second launch are counted in 31 bits
-  if (max_length > 0x7fffff00 || s.entries * ((max_length + kUnit - 1ll) / kUnit) >= 1ll << 31 ||
+  if (max_length > 0x7fffff00 || s.entries * ((max_length + kUnit - 1ll) / kUnit + kBegin) >= 1ll << 31 ||
       s.entries * 16 * s.HB >= 1ll << 31) {
     moba_set_error("quantized_attention: more than 2^31 tokens of a row, units of 128 tokens or heads");
     return MOBA_ERR_ARG;
@@ -733,13 +942,14 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   char* p = (char*)work;
   a.q = (const uint16_t*)q;
   a.Hq = Hq; a.G = s.G; a.HB = s.HB; a.NHB = s.NHB; a.per_row = Hkv * s.NHB;
+  a.by_row = fast_div(a.per_row); a.by_nhb = fast_div(s.NHB);
   a.q_seq = q_seq; a.lengths = lengths; a.length_add = length_add; a.max_length = max_length;
   a.selected = selected; a.slots = slots; a.chunk = chunk; a.max_items = s.max_items;
-  a.by_chunk = fast_div(std::max(1, chunk)); a.by_d4 = fast_div(D / 4);
+  a.by_chunk = fast_div(std::max(1, chunk)); a.by_d4 = fast_div(D / 4); a.by_pieces = fast_div(a.pool.Dp / 16);
   a.items = (int2*)(p + s.items_at); a.tokens = (int*)(p + s.tokens_at);
   a.scan_n = selected != nullptr ? (int)s.entries : Nq;
   a.scan_mult = selected != nullptr ? 1 : a.per_row;
-  a.start = (uint32_t*)(p + s.start_at);
+  a.start = (uint32_t*)(p + s.start_at); a.run_entry = (int*)(p + s.run_at);
   a.scale_log2 = scale * kLog2e;
   a.part_o = (float*)(p + s.part_o_at); a.part_ml = (float*)(p + s.part_ml_at);
   a.out = (uint16_t*)out; a.lse = lse;
@@ -747,11 +957,7 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   if (selected != nullptr) hipLaunchKernelGGL(union_kernel, dim3((unsigned)s.entries), dim3(64), 0, st, a);
   if (dtype == 0) { if (format == 0) launch_attend<0, 0>(a, s.wgs, st); else launch_attend<0, 1>(a, s.wgs, st); }
   else { if (format == 0) launch_attend<1, 0>(a, s.wgs, st); else launch_attend<1, 1>(a, s.wgs, st); }
-  int cols = 16;
-  while (cols * 4 < D) cols *= 2;
-  const int per_entry = std::min(s.G, 16 * s.HB);
-  const unsigned joins = (unsigned)(s.entries * per_entry);
-  if (dtype == 0) launch_join<0>(a, joins, s.wgs, cols, per_entry, st);
-  else launch_join<1>(a, joins, s.wgs, cols, per_entry, st);
+  if (dtype == 0) launch_join<0>(a, (int)s.entries, s.wgs, st);
+  else launch_join<1>(a, (int)s.entries, s.wgs, st);
   return moba_launch_status("quantized_attention");
 }
