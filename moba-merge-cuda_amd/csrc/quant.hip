@@ -259,30 +259,14 @@ bool whole_pieces(const void* p, int64_t ts, int64_t hs) {
 // -------------------------------------------------------------------- read
 struct ReadArgs {
   QuantPool pool;
-  uint32_t total;  // N * Hkv * 2 * (D / 8) pieces of 8 codes
+  uint32_t total;  // N * Hkv * (D / 8) pieces of 8 codes
   FastDiv by_row, by_token;
   const int *seq, *pos;
   uint16_t *k_out, *v_out;
   int* status;
 };
 
-template <int DT, int FMT>
-__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
-  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  if (idx >= a.total) return;
-  const uint32_t row = div_by(idx, a.by_row), u = idx - row * a.by_row.d;
-  const uint32_t t = div_by(row, a.by_token), h = row - t * a.by_token.d;  // keys, then values
-  const bool is_v = h >= (uint32_t)a.pool.Hkv;
-  const int kh = (int)(is_v ? h - a.pool.Hkv : h), s = a.seq[t];
-  const int64_t cell = pool_row(a.pool, s, a.pos[t], kh);
-  uint16_t* dst = (is_v ? a.v_out : a.k_out) + ((int64_t)t * a.pool.Hkv + kh) * a.pool.D + 8 * u;
-  if (cell < 0) {  // padding, or no such cell: zeros
-    if (s != -1 && h == 0 && u == 0) report(a.status, s < 0 || s >= a.pool.B ? kBadSlot : kBadCell);
-    st8(dst, zero8());
-    return;
-  }
-  const uint2 w = *reinterpret_cast<const uint2*>((is_v ? a.pool.v : a.pool.k) + cell * a.pool.Dp + 8 * u);
-  const float scale = (is_v ? a.pool.vs : a.pool.ks)[cell];
+template <int DT, int FMT> MOBA_DEV void store_values(uint16_t* dst, uint2 w, float scale) {
   float x[4], y[4], v[8];
   numbers4<FMT>(w.x, x);
   numbers4<FMT>(w.y, y);
@@ -292,6 +276,30 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
     v[4 + i] = y[i] * scale;
   }
   st8(dst, pack8<DT>(v));
+}
+
+// A thread has 8 dims of a token's key and of its value: one search for both.
+template <int DT, int FMT>
+__global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
+  if (idx >= a.total) return;
+  const uint32_t row = div_by(idx, a.by_row), u = idx - row * a.by_row.d;
+  const uint32_t t = div_by(row, a.by_token);
+  const int kh = (int)(row - t * a.by_token.d), s = a.seq[t];
+  const int64_t cell = pool_row(a.pool, s, a.pos[t], kh);
+  const int64_t to = (int64_t)row * a.pool.D + 8 * u;
+  if (cell < 0) {  // padding, or no such cell: zeros
+    if (s != -1 && kh == 0 && u == 0) report(a.status, s < 0 || s >= a.pool.B ? kBadSlot : kBadCell);
+    st8(a.k_out + to, zero8());
+    st8(a.v_out + to, zero8());
+    return;
+  }
+  const int64_t from = cell * a.pool.Dp + 8 * u;
+  const uint2 k = *reinterpret_cast<const uint2*>(a.pool.k + from);
+  const uint2 v = *reinterpret_cast<const uint2*>(a.pool.v + from);
+  const float ks = a.pool.ks[cell], vs = a.pool.vs[cell];
+  store_values<DT, FMT>(a.k_out + to, k, ks);
+  store_values<DT, FMT>(a.v_out + to, v, vs);
 }
 
 // ------------------------------------------------------------------- means
@@ -403,8 +411,8 @@ extern "C" int moba_hip_quantized_read(int format, const void* k_codes, const vo
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) { moba_set_error("quantized_read: outputs must be 16-byte aligned"); return MOBA_ERR_ARG; }
   if ((int64_t)N * 2 * Hkv * D >= 1ll << 31) { moba_set_error("quantized_read: more than 2^31 elements in one call"); return MOBA_ERR_ARG; }
   a.by_row = fast_div(D / 8);
-  a.by_token = fast_div(2 * Hkv);
-  a.total = (uint32_t)N * 2 * Hkv * (D / 8);
+  a.by_token = fast_div(Hkv);
+  a.total = (uint32_t)N * Hkv * (D / 8);
   a.seq = token_seq; a.pos = token_pos;
   a.k_out = (uint16_t*)k_out; a.v_out = (uint16_t*)v_out; a.status = status;
   const dim3 grid((a.total + 255) / 256), block(256);

@@ -41,7 +41,7 @@ namespace {
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
-constexpr int kMaxWgs = 1280;   // of a launch, at most
+constexpr int kMaxWgs = 768;   // of a launch, at most
 constexpr int kRun = 4;         // units of a workgroup, at least
 constexpr int kBegin = 2;       // units' worth of time that beginning an entry takes
 constexpr int kManyParts = 16;  // of an entry, above which a workgroup joins one head
@@ -165,8 +165,10 @@ __global__ __launch_bounds__(64) void union_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ attention
 constexpr int kWaves = 4;  // of a workgroup
 // NT: 16-dim tiles of a head that the registers hold.  Workgroups of a CU: what registers
-// and LDS allow.
-template <int NT> constexpr int occupancy() { return NT <= 4 ? 5 : NT <= 6 ? 4 : NT <= 8 ? 3 : 2; }
+// allow without spills.  Measured with one more or one less (kernel, us): 64 rows of up
+// to 32K, 128 dims: 3 162, 2 141, 1 173; 32 rows of 256 dims: 2 107, 1 76; of 192: 2 54,
+// 1 62; 8 rows of 32 heads of 64 dims: 3 30, 2 31.5.
+template <int NT> constexpr int occupancy() { return NT <= 6 ? 3 : NT <= 12 ? 2 : 1; }
 
 // Where a step's tokens are, before the pool's rows are known.
 struct Look {
@@ -865,7 +867,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.entries = (int64_t)Nq * Hkv * s.NHB;
   s.max_items = std::min(s.G, 16 * s.HB) * slots;
   // as many workgroups as the card holds at once, but no more than there can be units
-  const int per_cu = D > 128 ? 2 : D > 96 ? 3 : D > 64 ? 4 : 5;
+  const int per_cu = D > 192 ? 1 : D > 96 ? 2 : 3;  // occupancy()
   const int64_t longest = slots > 0 ? std::min<int64_t>((int64_t)s.max_items * chunk, max_length) : max_length;
   const int64_t units = s.entries * ((longest + kUnit - 1) / kUnit);
   s.wgs = (int)std::min<int64_t>(256 * per_cu, (units + 7) / 8 * 8);
