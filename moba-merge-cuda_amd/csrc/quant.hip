@@ -46,7 +46,7 @@ struct AppendArgs {
   QuantPool pool;
   const uint16_t *q, *k, *v;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;  // token and head strides, elements
-  int Hq, R, lanes, inter;                     // lanes of a row, a power of two
+  int Hq, R, lanes, lanes_log, inter;          // lanes of a row, a power of two
   uint32_t rows;                               // N * (Hq + 2 Hkv)
   FastDiv by_token;                            // Hq + 2 Hkv
   const float2* cos_sin;
@@ -139,7 +139,7 @@ MOBA_DEV void store_scale(const AppendArgs& a, const Row& r, float scale) {
 template <int DT, int FMT>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t row = idx / a.lanes;
+  const uint32_t row = idx >> a.lanes_log;
   if (row >= a.rows) return;
   const int u = (int)(idx & (a.lanes - 1)), D = a.pool.D;
   Row r;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
 template <int DT, int FMT, bool WIDE>
 __global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
-  const uint32_t row = idx / a.lanes;
+  const uint32_t row = idx >> a.lanes_log;
   if (row >= a.rows) return;
   const int u = (int)(idx & (a.lanes - 1)), D = a.pool.D, half = a.R / 2;
   Row r;
@@ -243,8 +243,9 @@ template <int DT, int FMT> void launch_append(AppendArgs& a, bool wide, hipStrea
   const int D = a.pool.D;
   const bool pairs = wide && D % 16 == 0 && a.R % 16 == 0;
   const int units = pairs ? D / 16 : a.pool.Dp / 8;
-  a.lanes = 1;
-  while (a.lanes < units) a.lanes *= 2;
+  a.lanes_log = 0;
+  while ((1 << a.lanes_log) < units) ++a.lanes_log;
+  a.lanes = 1 << a.lanes_log;
   const dim3 grid((unsigned)(((uint64_t)a.rows * a.lanes + 255) / 256)), block(256);
   if (pairs) hipLaunchKernelGGL((append_pairs_kernel<DT, FMT>), grid, block, 0, st, a);
   else if (wide) hipLaunchKernelGGL((append_any_kernel<DT, FMT, true>), grid, block, 0, st, a);

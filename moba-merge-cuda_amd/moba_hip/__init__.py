@@ -13,5 +13,6 @@ from .kv_cache import ContiguousKVCache, DecodeResult, PagedKVCache  # noqa: F40
 from .prepared_decode import PreparedDecode  # noqa: F401
 from .prepared_shared import PreparedSharedDecode  # noqa: F401
 from .quantized import QuantizedPages, quantized_append, quantized_attention, quantized_read  # noqa: F401
+from .quantized_cache import PreparedQuantizedDecode, QuantizedKVCache  # noqa: F401
 from .rotary import RotaryTable, append_rotary  # noqa: F401
 from .shared_prefix import SharedPrefixPlan, shared_prefix_attention  # noqa: F401

@@ -88,13 +88,38 @@ class PagedKVCache:
             self.device = torch.device("cuda", torch.cuda.current_device())
             self._stream = torch.cuda.current_stream(self.device).cuda_stream
             dev = dict(device=self.device)
-            self.k_cache = torch.empty((pages, P, self.num_kv_heads, self.head_dim), dtype=dtype,
-                                       **dev)
-            self.v_cache = torch.empty_like(self.k_cache)
+            self._allocate(pages, P)
             self._table = torch.full((B, self._layout.table_width), -1, dtype=torch.int32, **dev)
             self._lengths = torch.zeros(B, dtype=torch.int32, **dev)
             self._means = torch.empty((B, -(-L // self.chunk_size), self.num_kv_heads,
                                        self.head_dim), dtype=dtype, **dev)
+
+    # ---------------------------------------------------------------- the pool
+    # (QuantizedKVCache has its own)
+    def _allocate(self, pages, page):
+        self.k_cache = torch.empty((pages, page, self.num_kv_heads, self.head_dim), dtype=self.dtype,
+                                   device=self.device)
+        self.v_cache = torch.empty_like(self.k_cache)
+
+    def _pool_tensors(self):
+        return self.k_cache, self.v_cache
+
+    def _write(self, k, v, seq, pos):
+        kernels.append_tokens(k.contiguous(), v.contiguous(), self.k_cache, self.v_cache, self._table,
+                              seq, pos)
+
+    def _write_rotary(self, k, v, seq, pos, rotary, q, offsets):
+        return append_rotary(k, v, self.k_cache, self.v_cache, self._table, seq, pos, rotary, q=q,
+                             offsets=offsets)
+
+    def _close_chunks(self, seq, chunks):
+        kernels.block_means(self.k_cache, self._table, self._means, seq, chunks, self.chunk_size)
+
+    def _read(self, slot, n):
+        tok = torch.arange(n, device=self.device)
+        P = self._layout.page_size
+        page = self._table[slot].long()[tok // P]
+        return self.k_cache[page, tok % P], self.v_cache[page, tok % P]
 
     # -------------------------------------------------------------- snapshots
     @property
@@ -125,8 +150,7 @@ class PagedKVCache:
         contract.tensors(specs, device=self.device, dtype=self.dtype, head_dim=self.head_dim)
 
     def _no_pool_alias(self, *tensors):
-        pools = (self.k_cache.untyped_storage().data_ptr(),
-                 self.v_cache.untyped_storage().data_ptr())
+        pools = {t.untyped_storage().data_ptr() for t in self._pool_tensors()}
         _require([(lambda: all(t.untyped_storage().data_ptr() not in pools for t in tensors),
                    "append inputs must not alias KV cache storage; clone first")])
 
@@ -184,12 +208,10 @@ class PagedKVCache:
             seq, pos, cseq, cchunk, *more = self._publish_layout(
                 plan.seq_arr, plan.pos_arr, plan.closed_arr[:, 0], plan.closed_arr[:, 1], *extra)
             if put is None:
-                kernels.append_tokens(k.contiguous(), v.contiguous(), self.k_cache, self.v_cache,
-                                      self._table, seq, pos)
+                self._write(k, v, seq, pos)
             else:
                 put(seq, pos, *more)
-            kernels.block_means(self.k_cache, self._table, self._means, cseq, cchunk,
-                                self.chunk_size)
+            self._close_chunks(cseq, cchunk)
         except Exception:  # a failed launch leaves the pool as it was
             self._layout._pool.assign(before)
             self._publish_layout()
@@ -231,8 +253,7 @@ class PagedKVCache:
             turned = []
 
             def put(seq, pos, offs):
-                turned.append(append_rotary(k, v, self.k_cache, self.v_cache, self._table, seq, pos,
-                                            rotary, q=q, offsets=offs))
+                turned.append(self._write_rotary(k, v, seq, pos, rotary, q, offs))
             done = self._store(k, v, ids, counts, put, (by_slot,))[0]
             return RotaryAppendResult(done.sequence_ids, done.positions, turned[0])
 
@@ -372,11 +393,7 @@ class PagedKVCache:
         with self._lock, torch.cuda.device(self.device):
             self._guard(under_lease=True)
             sid = self._layout.validate_ids([sequence_id])[0]
-            n = self.lengths[sid]
-            tok = torch.arange(n, device=self.device)
-            P = self._layout.page_size
-            page = self._table[sid].long()[tok // P]
-            return self.k_cache[page, tok % P], self.v_cache[page, tok % P]
+            return self._read(sid, self.lengths[sid])
 
 
 class ContiguousKVCache(PagedKVCache):

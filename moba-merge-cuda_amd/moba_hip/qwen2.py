@@ -28,6 +28,8 @@ import torch
 from .cache_layout import positive_int
 from .grouped_attention import moba_hip_attention
 from .kv_cache import PagedKVCache
+from .quantized import _check_format
+from .quantized_cache import QuantizedKVCache
 from .rotary import RotaryTable
 
 
@@ -83,7 +85,12 @@ def decode_layer(layer, norm, hidden, cos, sin, cache_or_plan, *, graph=False, t
 
 class Qwen2Session:
     def __init__(self, model, capacity, *, mode="moba", chunk=128, topk=4, page=16,
-                 backend="eager"):
+                 backend="eager", kv_format=None):
+        """``kv_format``: ``"int8"`` or ``"fp8"`` keeps the caches in 8 bits
+        (:class:`~moba_hip.QuantizedKVCache`); the prompt's own attention reads the keys
+        and values as they were projected."""
+        if kv_format is not None:
+            _check_format(kv_format)
         if mode not in ("dense", "moba"):
             raise ValueError("mode")
         if backend not in ("eager", "model_graph"):
@@ -101,8 +108,11 @@ class Qwen2Session:
         self.hq, self.hk = cfg.num_attention_heads, cfg.num_key_value_heads
         self.dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.hq
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
-        self.caches = [PagedKVCache(1, self.capacity, self.hk, self.dim, page_size=page,
-                                    chunk_size=self.chunk, dtype=self.dtype, device=self.device)
+        self.kv_format = kv_format
+        kind, more = ((PagedKVCache, {}) if kv_format is None else
+                      (QuantizedKVCache, {"format": kv_format}))
+        self.caches = [kind(1, self.capacity, self.hk, self.dim, page_size=page,
+                            chunk_size=self.chunk, dtype=self.dtype, device=self.device, **more)
                        for _ in model.model.layers]
         self.plans, self.graph, self.closed, self.failed = [], None, False, False
         self.token = torch.zeros((1, 1), device=self.device, dtype=torch.long)
