@@ -441,6 +441,117 @@ def test_a_long_context():
     _attend([131071], 14, 2, 64, 16, "fp8", torch.bfloat16)
 
 
+# ------------------------------------------------------------------- refusals
+def _refusal_state():
+    from moba_hip import QuantizedPages, RotaryTable
+    dev = dict(dtype=torch.int32, device="cuda")
+    pages = QuantizedPages.empty(4, 8, 2, 64, format="int8")
+    return dict(pages=pages, table=torch.zeros(2, 2, **dev), seq=torch.zeros(3, **dev), pos=torch.arange(3, **dev),
+                k=torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda"),
+                v=torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda"),
+                q=torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda"), rotary=RotaryTable(64, 9),
+                lengths=torch.ones(3, **dev))
+
+
+BAD_PAGES = {
+    "no pool": lambda p: tuple(p),
+    "codes of 16 bits": lambda p: p._replace(k=p.k.to(torch.int16)),
+    "fp8 beside int8": lambda p: p._replace(v=p.v.view(torch.float8_e4m3fn)),
+    "narrow rows": lambda p: p._replace(k=p.k[..., :48], v=p.v[..., :48]),
+    "another head_dim": lambda p: p._replace(head_dim=80),
+    "odd head_dim": lambda p: p._replace(head_dim=60),
+    "bool head_dim": lambda p: p._replace(head_dim=True),
+    "fewer values": lambda p: p._replace(v=p.v[:3]),
+    "scales of 16 bits": lambda p: p._replace(k_scale=p.k_scale.half()),
+    "scales of fewer pages": lambda p: p._replace(v_scale=p.v_scale[:2]),
+    "strided": lambda p: p._replace(k=p.k.transpose(1, 2).contiguous().transpose(1, 2)),
+    "one pool twice": lambda p: p._replace(v=p.k),
+    "on the CPU": lambda p: p._replace(k_scale=p.k_scale.cpu()),
+    "misaligned": lambda p: p._replace(k=torch.empty(p.k.numel() + 8, dtype=torch.int8, device="cuda")[8:].view(p.k.shape)),
+    "no tensor": lambda p: p._replace(v_scale=None),
+}
+
+
+@pytest.mark.parametrize("how", BAD_PAGES)
+def test_pools_that_are_refused(how):
+    from moba_hip import quantized_append, quantized_attention, quantized_read
+    st = _refusal_state()
+    bad = BAD_PAGES[how](st["pages"])
+    for call in (lambda: quantized_append(st["k"], st["v"], bad, st["table"], st["seq"], st["pos"]),
+                 lambda: quantized_read(bad, st["table"], st["seq"], st["pos"]),
+                 lambda: quantized_attention(st["q"], bad, st["table"], st["seq"], st["lengths"])):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(k=lambda st: st["k"][:2]), "invalid shape"), (dict(k=lambda st: st["k"].float()), "BF16 or FP16"),
+    (dict(k=lambda st: st["k"].half()), "match"), (dict(v=lambda st: st["v"][..., :32]), "invalid shape"),
+    (dict(k=lambda st: st["k"].requires_grad_(True)), "inference-only"),
+    (dict(k=lambda st: st["k"][:0], v=lambda st: st["v"][:0], seq=lambda st: st["seq"][:0],
+          pos=lambda st: st["pos"][:0], q=lambda st: None), "invalid shape"),
+    (dict(k=lambda st: st["k"].transpose(1, 2).contiguous().transpose(1, 2)), "contiguous"),
+    (dict(seq=lambda st: st["seq"].long()), "token_seq"), (dict(pos=lambda st: st["pos"][:2]), "token_pos"),
+    (dict(table=lambda st: st["table"].t()), "page_table"), (dict(table=lambda st: st["table"][:0]), "page_table"),
+    (dict(rotary=lambda st: None), "without rotary"), (dict(rotary=lambda st: 3), "RotaryTable"),
+    (dict(offsets=lambda st: st["seq"]), "offsets"), (dict(q=lambda st: st["q"][:, :0]), "invalid shape"),
+    (dict(q=lambda st: None, q_out=lambda st: st["q"]), "q_out without q"),
+    (dict(q_out=lambda st: st["q"]), "overlap"), (dict(q_out=lambda st: st["q"][:2]), "invalid shape"),
+    (dict(k=lambda st: st["pages"].k.view(torch.bfloat16).reshape(-1)[:384].view(3, 2, 64)), "alias"),
+])
+def test_appends_that_are_refused(change, message):
+    from moba_hip import quantized_append
+    st = _refusal_state()
+    args = {"q_out": None, "offsets": None, **st, **{n: f(st) for n, f in change.items()}}
+    with pytest.raises(ValueError, match=message):
+        quantized_append(args["k"], args["v"], args["pages"], args["table"], args["seq"], args["pos"],
+                         rotary=args["rotary"], q=args["q"], q_out=args["q_out"], offsets=args["offsets"])
+
+
+def test_a_replaced_table_of_angles_is_checked():
+    from moba_hip import quantized_append
+    st = _refusal_state()
+    st["rotary"].cos_sin = st["rotary"].cos_sin[:, :16].contiguous()
+    with pytest.raises(ValueError, match="cos_sin"):
+        quantized_append(st["k"], st["v"], st["pages"], st["table"], st["seq"], st["pos"], rotary=st["rotary"])
+
+
+@pytest.mark.parametrize("kw", [dict(dtype=torch.float32), dict(seq=lambda t: t[:0]), dict(seq=lambda t: t.long()),
+                                dict(pos=lambda t: t[:1]), dict(seq=lambda t: t[None])])
+def test_reads_that_are_refused(kw):
+    from moba_hip import quantized_read
+    st = _refusal_state()
+    seq, pos = (kw.get(n, lambda t: t)(st[n]) for n in ("seq", "pos"))
+    with pytest.raises(ValueError):
+        quantized_read(st["pages"], st["table"], seq, pos, dtype=kw.get("dtype", torch.bfloat16))
+
+
+@pytest.mark.parametrize("kw,message", [
+    (dict(scale=0.0), "scale"), (dict(scale=1e31), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(max_length=0), "max_length"), (dict(max_length=2.5), "max_length"), (dict(chunk_size=8), "without selected"),
+    (dict(selected=lambda st: torch.zeros(3, 4, 2, dtype=torch.int32, device="cuda")), "chunk_size"),
+    (dict(selected=lambda st: torch.zeros(3, 4, 17, dtype=torch.int32, device="cuda"), chunk_size=8), "1 to 16"),
+    (dict(selected=lambda st: torch.zeros(3, 2, 2, dtype=torch.int32, device="cuda"), chunk_size=8), "selected"),
+    (dict(selected=lambda st: torch.zeros(3, 4, 2, device="cuda"), chunk_size=8), "selected"),
+    (dict(selected=lambda st: torch.zeros(3, 4, 2, dtype=torch.int32, device="cuda"), chunk_size=0), "chunk_size"),
+    (dict(q=lambda st: st["q"][:, :3]), "multiple of Hkv"), (dict(q=lambda st: st["q"][:2]), "q_seq"),
+    (dict(q=lambda st: st["q"].float()), "BF16 or FP16"),
+    (dict(q=lambda st: torch.zeros(3 * 256 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(3, 4, 64)), "16-byte"),
+    (dict(q=lambda st: st["q"].transpose(0, 1).contiguous().transpose(0, 1)), "contiguous"),
+    (dict(lengths=lambda st: st["lengths"].long()), "lengths"), (dict(lengths=lambda st: st["lengths"][:1]), "lengths"),
+    (dict(out=lambda st: st["q"]), "overlap"), (dict(out=lambda st: st["q"].half()), "out must be"),
+    (dict(lse=lambda st: torch.zeros(3, 4, dtype=torch.float64, device="cuda")), "lse"),
+    (dict(lse=lambda st: st["pages"].k_scale.view(-1)[:12].view(3, 4)), "overlap"),
+])
+def test_attentions_that_are_refused(kw, message):
+    from moba_hip import quantized_attention
+    st = _refusal_state()
+    kw = {n: f(st) if callable(f) else f for n, f in kw.items()}
+    q, lengths = kw.pop("q", st["q"]), kw.pop("lengths", st["lengths"])
+    with pytest.raises(ValueError, match=message):
+        quantized_attention(q, st["pages"], st["table"], st["seq"], lengths, **kw)
+
+
 # --------------------------------------------------------- streams and graphs
 def _step(pages, table, rt, n, hq, hkv, d, seed):
     """State of a decode step of n slots, one token each."""
