@@ -117,74 +117,89 @@ template <int N> MOBA_DEV uint32_t row_max(const float (&v)[N], bool on, int lan
   return m;
 }
 
-// Eight codes of v from dim d on.
-template <int FMT> MOBA_DEV void store_codes(uint8_t* dst, const float* v, const RowScale& r) {
-  float y[8];
+// N codes (8 or 4) of v, from dst on.
+template <int FMT, int N> MOBA_DEV void store_codes(uint8_t* dst, const float* v, const RowScale& r) {
+  uint32_t w[N / 4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = r.finite ? to_code<FMT>(v[i], r) : 0.0f;
-  uint2 w;
-  w.x = codes4<FMT>(y[0], y[1], y[2], y[3]);
-  w.y = codes4<FMT>(y[4], y[5], y[6], y[7]);
-  *reinterpret_cast<uint2*>(dst) = w;
+  for (int j = 0; j < N / 4; ++j) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = r.finite ? to_code<FMT>(v[4 * j + i], r) : 0.0f;
+    w[j] = codes4<FMT>(y[0], y[1], y[2], y[3]);
+  }
+  if constexpr (N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = w[0];
 }
 
 MOBA_DEV void store_scale(const AppendArgs& a, const Row& r, float scale) {
   (r.is_v ? a.pool.vs : a.pool.ks)[r.cell] = scale;
 }
 
-// Rows of whole 16-byte pieces, R a multiple of 16 (0: nothing turns): a lane has
-// two pieces of 8 dims, those at 8u and 8u + R/2 of what turns, or the pieces c and
-// c + n of the 2n behind R, so that a pair's two values are in one lane and
-// neighbouring lanes have neighbouring pieces.
-template <int DT, int FMT>
+// Rows of whole pieces of VEC dims (8 or 4), R a multiple of two of them (0: nothing
+// turns): a lane has two pieces, those at VEC u and VEC u + R/2 of what turns, or the
+// pieces c and c + n of the 2n behind R, so that a pair's two values are in one lane and
+// neighbouring lanes have neighbouring pieces.  25K tokens of 12 + 2 + 2 heads of 40 dims, all
+// turned: 24 us in pieces of 4, 42 where each dim finds its partner.
+template <int DT, int FMT, int VEC>
 __global__ __launch_bounds__(256) void append_pairs_kernel(AppendArgs a) {
+  typedef uint32_t words __attribute__((ext_vector_type(VEC / 2)));
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;
   const uint32_t row = idx >> a.lanes_log;
   if (row >= a.rows) return;
   const int u = (int)(idx & (a.lanes - 1)), D = a.pool.D;
   Row r;
   if (!locate(a, row, u == 0, r)) return;
-  const int turning = r.turn != nullptr ? a.R / 16 : 0, from = turning * 16;
-  const int n = (D - from) / 16, c = u - turning;
-  const bool on = u < D / 16, turns = u < turning;
-  const int d0 = turns ? 8 * u : on ? from + 8 * c : 0, d1 = turns ? d0 + a.R / 2 : on ? d0 + 8 * n : 0;
-  const u32x4_t x = *reinterpret_cast<const u32x4_t*>(r.src + d0);
-  const u32x4_t y = *reinterpret_cast<const u32x4_t*>(r.src + d1);
-  float v[16];
+  const int turning = r.turn != nullptr ? a.R / (2 * VEC) : 0, from = turning * 2 * VEC;
+  const int n = (D - from) / (2 * VEC), c = u - turning;
+  const bool on = u < D / (2 * VEC), turns = u < turning;
+  const int d0 = turns ? VEC * u : on ? from + VEC * c : 0;
+  const int d1 = turns ? d0 + a.R / 2 : on ? d0 + VEC * n : 0;
+  const words x = *reinterpret_cast<const words*>(r.src + d0);
+  const words y = *reinterpret_cast<const words*>(r.src + d1);
+  float v[2 * VEC];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < VEC / 2; ++i) {
     unpack2<DT>(x[i], v[2 * i], v[2 * i + 1]);
-    unpack2<DT>(y[i], v[8 + 2 * i], v[9 + 2 * i]);
+    unpack2<DT>(y[i], v[VEC + 2 * i], v[VEC + 1 + 2 * i]);
   }
   if (turns) {
     if (a.inter) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {  // two pairs an access, as the table has them
-        const float4 w = *reinterpret_cast<const float4*>(r.turn + (i < 4 ? d0 / 2 + i : d1 / 2 + i - 4));
+      for (int i = 0; i < VEC; i += 2) {  // two pairs an access, as the table has them
+        const float4 w = *reinterpret_cast<const float4*>(r.turn + (i < VEC / 2 ? d0 / 2 + i : d1 / 2 + i - VEC / 2));
         rotate(v[2 * i], v[2 * i + 1], make_float2(w.x, w.y));
         rotate(v[2 * i + 2], v[2 * i + 3], make_float2(w.z, w.w));
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
+      for (int i = 0; i < VEC; i += 2) {
         const float4 w = *reinterpret_cast<const float4*>(r.turn + d0 + i);
-        rotate(v[i], v[8 + i], make_float2(w.x, w.y));
-        rotate(v[i + 1], v[9 + i], make_float2(w.z, w.w));
+        rotate(v[i], v[VEC + i], make_float2(w.x, w.y));
+        rotate(v[i + 1], v[VEC + 1 + i], make_float2(w.z, w.w));
       }
     }
   }
   if (r.cell < 0) {
     if (!on) return;
-    st8(r.q_dst + d0, pack8<DT>(v));
-    st8(r.q_dst + d1, pack8<DT>(v + 8));
+    words p, q;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      p[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+      q[i] = pack2<DT>(v[VEC + 2 * i], v[VEC + 1 + 2 * i]);
+    }
+    *reinterpret_cast<words*>(r.q_dst + d0) = p;
+    *reinterpret_cast<words*>(r.q_dst + d1) = q;
     return;
   }
   const RowScale s = row_scale<FMT>(row_max(v, on, a.lanes));
-  if (u == 0) store_scale(a, r, s.scale);
-  if (!on) return;
   uint8_t* dst = (r.is_v ? a.pool.v : a.pool.k) + r.cell * a.pool.Dp;
-  store_codes<FMT>(dst + d0, v, s);
-  store_codes<FMT>(dst + d1, v + 8, s);
+  if (u == 0) {
+    store_scale(a, r, s.scale);
+    if (D < a.pool.Dp) *reinterpret_cast<uint2*>(dst + D) = make_uint2(0, 0);  // behind D
+  }
+  if (!on) return;
+  store_codes<FMT, VEC>(dst + d0, v, s);
+  store_codes<FMT, VEC>(dst + d1, v + VEC, s);
 }
 
 // Any other row: a lane has 8 neighbouring dims and reads the partner of each one
@@ -235,19 +250,21 @@ __global__ __launch_bounds__(256) void append_any_kernel(AppendArgs a) {
   const RowScale s = row_scale<FMT>(row_max(v, on, a.lanes));
   if (u == 0) store_scale(a, r, s.scale);
   uint8_t* dst = (r.is_v ? a.pool.v : a.pool.k) + r.cell * a.pool.Dp;
-  if (on) store_codes<FMT>(dst + d, v, s);
+  if (on) store_codes<FMT, 8>(dst + d, v, s);
   else if (8 * u < a.pool.Dp) *reinterpret_cast<uint2*>(dst + 8 * u) = make_uint2(0, 0);  // behind D
 }
 
+// Pieces as wide as rows and R allow; else each dim finds its partner.
 template <int DT, int FMT> void launch_append(AppendArgs& a, bool wide, hipStream_t st) {
   const int D = a.pool.D;
-  const bool pairs = wide && D % 16 == 0 && a.R % 16 == 0;
-  const int units = pairs ? D / 16 : a.pool.Dp / 8;
+  const int vec = !wide ? 0 : D % 16 == 0 && a.R % 16 == 0 ? 8 : a.R % 8 == 0 ? 4 : 0;
+  const int units = vec ? D / (2 * vec) : a.pool.Dp / 8;
   a.lanes_log = 0;
   while ((1 << a.lanes_log) < units) ++a.lanes_log;
   a.lanes = 1 << a.lanes_log;
   const dim3 grid((unsigned)(((uint64_t)a.rows * a.lanes + 255) / 256)), block(256);
-  if (pairs) hipLaunchKernelGGL((append_pairs_kernel<DT, FMT>), grid, block, 0, st, a);
+  if (vec == 8) hipLaunchKernelGGL((append_pairs_kernel<DT, FMT, 8>), grid, block, 0, st, a);
+  else if (vec == 4) hipLaunchKernelGGL((append_pairs_kernel<DT, FMT, 4>), grid, block, 0, st, a);
   else if (wide) hipLaunchKernelGGL((append_any_kernel<DT, FMT, true>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((append_any_kernel<DT, FMT, false>), grid, block, 0, st, a);
 }
