@@ -44,7 +44,7 @@ constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 w
 constexpr int kMaxWgs = 768;   // of a launch, at most
 constexpr int kRun = 4;         // units of a workgroup, at least
 constexpr int kBegin = 2;       // units' worth of time that beginning an entry takes
-constexpr int kManyParts = 16;  // of an entry, above which a workgroup joins one head
+constexpr int kManyParts = 8;   // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects
 constexpr int kMaxItems = 32 * kMaxSlots;
 constexpr float kSlack = 6.0f;  // log2 by which scores may pass the running maximum
@@ -862,7 +862,12 @@ struct Shape {
 Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_length) {
   Shape s;
   s.G = Hq / Hkv;
-  s.HB = s.G > 16 ? 2 : 1;
+  // Two blocks of heads in an entry read its codes once for both; one block an entry joins
+  // half as wide sums and has twice as many entries.  32 heads of one kv head, 128 dims, us:
+  // 32 rows of 100K tokens and more (962 MB) two 294, one 324; 64 rows of 6.7K on average
+  // (105 MB, which stays in the last-level cache) 57 and 49; 48 heads, 105 MB: 73 and 65.
+  const int blocks = (s.G + 15) / 16;
+  s.HB = blocks % 2 == 0 && 2ll * Nq * Hkv * max_length * code_width(D) > 256ll << 20 ? 2 : 1;
   s.NHB = (s.G + 16 * s.HB - 1) / (16 * s.HB);
   s.entries = (int64_t)Nq * Hkv * s.NHB;
   s.max_items = std::min(s.G, 16 * s.HB) * slots;

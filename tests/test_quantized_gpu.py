@@ -294,6 +294,28 @@ def test_attention_of_selected_chunks(chunk, slots, hq, hkv, d, fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("chunk", [None, 64])
+@pytest.mark.parametrize("hq,hkv,d", [(17, 1, 64), (32, 1, 128), (64, 2, 40), (64, 1, 96), (30, 1, 256)])
+def test_two_blocks_of_heads_in_an_entry(fmt, chunk, hq, hkv, d):
+    """Tables that could map more than the last-level cache holds: more than 16 heads of a kv
+    head read its tokens together.  (Most of the table has no page.)"""
+    from moba_hip import quantized_attention
+    lengths, page = [700, 33, 1, 129], 16
+    pages, table = _filled(lengths, page, hkv, d, fmt, torch.bfloat16, width=2 ** 18 // page)
+    rows = list(enumerate(lengths)) * 4
+    assert 2 * len(rows) * hkv * 2 ** 18 * d > 256 << 20
+    dev = dict(dtype=torch.int32, device="cuda")
+    q_seq, lens = torch.tensor([s for s, _ in rows], **dev), torch.tensor([n for _, n in rows], **dev)
+    q = _randn(len(rows), hq, d, dtype=torch.bfloat16, seed=3, scale=2.0)
+    selected = None
+    if chunk:
+        g = torch.Generator().manual_seed(1)
+        selected = torch.randint(-1, 12, (len(rows), hq, 4), generator=g).to("cuda", torch.int32)
+    got = quantized_attention(q, pages, table, q_seq, lens, selected=selected, chunk_size=chunk)
+    check_attention(got, attention(q, pages, table, q_seq, lens, selected, chunk))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_rows_of_unlike_lengths_share_the_card(fmt):
     """One long row among short and empty ones, and several rows of one slot: entries that
     span many workgroups, workgroups that hold many entries."""
