@@ -462,7 +462,8 @@ int moba_hip_quantized_means(int format, const void* k_codes, const float* k_sca
                              int max_chunks, void* stream);
 
 /* Attention of q [Nq,Hq,D] over the pool: row r attends the first lengths[r] + length_add
- * (device; cut to [0, max_length]) tokens of slot q_seq[r], or with selected
+ * (device; cut to [0, max_length], max_length at most table_width * page_size and
+ * 0x7fff0000) tokens of slot q_seq[r], or with selected
  * [Nq,Hq,slots] (nullable, slots in [1,16]) those of them in the chunks of `chunk` tokens
  * that each head selected (-1 none, any order; chunks behind the length hold nothing).
  * out [Nq,Hq,D] (dtype), lse [Nq,Hq] fp32 natural log; a row or head that attends nothing
@@ -478,8 +479,7 @@ int moba_hip_quantized_attention(const void* q, int dtype, int Nq, int Hq, int H
                                  int length_add, int max_length, const int* selected, int slots,
                                  int chunk, void* work, void* out, float* lse, void* stream);
 
-/* Bytes of that workspace for the same arguments (-1 for bad ones), max_length before or
- * after it is cut to the table's table_width * page_size tokens. */
+/* Bytes of that workspace for the same arguments (-1 for bad ones). */
 int64_t moba_hip_quantized_attention_work(int Nq, int Hq, int Hkv, int D, int slots, int chunk,
                                           int max_length);
 

@@ -371,7 +371,7 @@ PyObject* quantized_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   QPool p;
   if (PyErr_Occurred() || !qpool_of(a[0], a[1], p) || !seq || seq->dim() != 1) return not_here();
   const int64_t n = seq->size(0);
-  if (n < 1 || !index_of(seq, p.idx, n) || !index_of(pos, p.idx, n) || n * 2 * p.hkv * p.d >= (1ll << 31))
+  if (n < 1 || !index_of(seq, p.idx, n) || !index_of(pos, p.idx, n) || n * p.hkv * (p.d / 8) >= (1ll << 31))
     return not_here();
   void* stream;
   if (!stream_of(p.idx, stream)) return not_here();
@@ -431,9 +431,9 @@ PyObject* quantized_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)p.d)
                        : PyFloat_Check(a[8]) ? PyFloat_AS_DOUBLE(a[8]) : 0.0;
   if (!(scale >= 0x1p-126 && scale < 1e30)) return not_here();
-  const int64_t blocks = (hq / p.hkv + 31) / 32;
-  if (n * hq >= (1ll << 31) || limit > 0x7fffff00 ||
-      n * p.hkv * blocks * std::max<int64_t>(32, (limit + 127) / 128) >= (1ll << 31))
+  const int64_t blocks = (hq / p.hkv + 15) / 16;
+  if (n * hq >= (1ll << 31) || limit > 0x7fff0000 ||
+      n * p.hkv * blocks * std::max<int64_t>(32, (limit + 127) / 128 + 2) >= (1ll << 31))
     return not_here();
   void* stream;
   if (!stream_of(p.idx, stream)) return not_here();

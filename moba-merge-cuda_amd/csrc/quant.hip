@@ -427,7 +427,7 @@ extern "C" int moba_hip_quantized_read(int format, const void* k_codes, const vo
   if (dtype != 0 && dtype != 1) { moba_set_error("quantized_read: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
   if (N < 1) { moba_set_error("quantized_read: nonempty N required"); return MOBA_ERR_ARG; }
   if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) { moba_set_error("quantized_read: outputs must be 16-byte aligned"); return MOBA_ERR_ARG; }
-  if ((int64_t)N * 2 * Hkv * D >= 1ll << 31) { moba_set_error("quantized_read: more than 2^31 elements in one call"); return MOBA_ERR_ARG; }
+  if ((int64_t)N * Hkv * (D / 8) >= 1ll << 31) { moba_set_error("quantized_read: more than 2^31 pieces of 8 elements in one call"); return MOBA_ERR_ARG; }
   a.by_row = fast_div(D / 8);
   a.by_token = fast_div(Hkv);
   a.total = (uint32_t)N * Hkv * (D / 8);

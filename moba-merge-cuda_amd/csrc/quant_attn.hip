@@ -26,9 +26,11 @@
 //         the scores of 4 + 4 tokens for one head;
 //   O^T = V^T P^T: those 8 weights are a lane's share of P^T as they are, if V^T is
 //         supplied with the same 8 tokens, which the transposed LDS read does.
-// Three waves a SIMD up to 128 dims then have 96 KB of a CU's reads on their way; with
-// tiles in registers it were two and 64 KB (64 rows of up to 32K tokens, 32/8 heads of
-// 128 dims, int8: 172 us against XX).
+// Kernel times at 64 rows of 256 to 32K tokens, 32 / 8 heads of 128 dims, int8 (831 MB):
+// 142 us, 5.9 TB/s, where a plain read of such blocks and their scales takes 139 and the
+// arithmetic alone 113; with codes loaded to registers two steps ahead 172; with runs
+// dealt by units alone (kBegin 0) 175.  One row of 128K tokens of 2 kv heads of 64 dims,
+// fp8 (36 MB): 13.5 and 6 to join.
 #include <algorithm>
 
 #include "quant.h"
@@ -41,9 +43,12 @@ namespace {
 typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
-constexpr int kMaxWgs = 768;   // of a launch, at most
+constexpr int kMaxWgs = 768;    // of a launch, at most
 constexpr int kRun = 4;         // units of a workgroup, at least
-constexpr int kBegin = 2;       // units' worth of time that beginning an entry takes
+// Units' worth of time that beginning and ending an entry takes (its length, slot, pages,
+// query and sums wait for each other, about 4 us).  256 rows of 64 to 4K tokens, one kv
+// head, us: 0 29, 1 21.9, 2 21.5, 3 20.9, 4 23; 64 rows of up to 32K: 179, 165, 163, 164, 163.
+constexpr int kBegin = 2;
 constexpr int kManyParts = 8;   // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects
 constexpr int kMaxItems = 32 * kMaxSlots;
@@ -418,7 +423,8 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
     const int hb = w & (a.HB - 1), streams = kWaves >> (a.HB - 1), stream = w >> (a.HB - 1);
     const int my_head = hb * 16 + c16;                         // in the entry
     // A wave's step is 64 tokens, found with one look; 32 where 64 would leave waves idle.
-    const int span_log = (n & (a.HB == 2 ? 0 : 1)) && n <= 8 ? 5 : (v_hi - v_lo) <= 32 * streams ? 5 : 6;
+    const bool uneven = a.HB == 1 && (n & 1) && n <= 8;
+    const int span_log = uneven || v_hi - v_lo <= 32 * streams ? 5 : 6;
     const int steps = (v_hi - v_lo + (1 << span_log) - 1) >> span_log;
     const int* trow = a.pool.table + (int64_t)slot_id * a.pool.W;
     if (moba) {
@@ -867,7 +873,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   // 32 rows of 100K tokens and more (962 MB) two 294, one 324; 64 rows of 6.7K on average
   // (105 MB, which stays in the last-level cache) 57 and 49; 48 heads, 105 MB: 73 and 65.
   const int blocks = (s.G + 15) / 16;
-  s.HB = blocks % 2 == 0 && 2ll * Nq * Hkv * max_length * code_width(D) > 256ll << 20 ? 2 : 1;
+  s.HB = blocks % 2 == 0 && 2.0 * Nq * Hkv * max_length * code_width(D) > 256 << 20 ? 2 : 1;
   s.NHB = (s.G + 16 * s.HB - 1) / (16 * s.HB);
   s.entries = (int64_t)Nq * Hkv * s.NHB;
   s.max_items = std::min(s.G, 16 * s.HB) * slots;
@@ -937,11 +943,11 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   if (max_length < 1) { moba_set_error("quantized_attention: max_length must be positive"); return MOBA_ERR_ARG; }
   if ((selected != nullptr) != (slots > 0) || slots > kMaxSlots || (selected != nullptr && chunk < 1)) { moba_set_error("quantized_attention: selected chunks need 1 to 16 slots and a chunk size"); return MOBA_ERR_ARG; }
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) || work == nullptr) { moba_set_error("quantized_attention: q, out and work must be 16-byte aligned"); return MOBA_ERR_ARG; }
-  max_length = (int)std::min<int64_t>(max_length, (int64_t)table_width * page_size);
+  if (max_length > (int64_t)table_width * page_size) { moba_set_error("quantized_attention: max_length exceeds what the table maps"); return MOBA_ERR_ARG; }
   chunk = std::min(chunk, max_length);  // a longer one ends where the row does
   const Shape s = shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length);
   // units, tokens and workgroups of the second launch are counted in 31 bits
-  if (max_length > 0x7fffff00 || s.entries * ((max_length + kUnit - 1ll) / kUnit + kBegin) >= 1ll << 31 ||
+  if (max_length > 0x7fff0000 || s.entries * ((max_length + kUnit - 1ll) / kUnit + kBegin) >= 1ll << 31 ||
       s.entries * 16 * s.HB >= 1ll << 31) {
     moba_set_error("quantized_attention: more than 2^31 tokens of a row, units of 128 tokens or heads");
     return MOBA_ERR_ARG;

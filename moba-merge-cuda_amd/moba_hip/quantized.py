@@ -230,8 +230,8 @@ def quantized_read(pages, page_table, token_seq, token_pos, *, dtype=torch.bfloa
     if n < 1:
         raise ValueError("token_seq must be nonempty")
     _check_index(token_pos, "token_pos", 1, dev, n)
-    if n * 2 * hkv * d >= 2 ** 31:
-        raise ValueError("read exceeds 2^31 elements")
+    if n * hkv * (d // 8) >= 2 ** 31:
+        raise ValueError("read exceeds 2^31 pieces of 8 elements")
     k, v = (torch.empty((n, hkv, d), dtype=dtype, device=dev) for _ in range(2))
     status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     pool, table = _pool_args(pages, page_table)
@@ -262,7 +262,10 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     outside the table (-1: padding) and a row or head with nothing to attend give
     zeros and an lse of -inf; a token in an unmapped page is not attended.  ``scale``
     (in [2^-126, 1e30]) defaults to D ** -0.5.  q and ``out`` are contiguous and 16-byte
-    aligned.  Nothing is read back, so a call can be captured into a graph."""
+    aligned.  Weights are summed before they are divided, up to 2^6 for a token, so that
+    values must stay below 2^122 / length in size.  Nothing is read back, so a call can
+    be captured into a graph; what becomes of its tensors on other streams and in a
+    graph: as in :func:`moba_hip.append_rotary`."""
     if out is None and lse is None:
         done = _lib.calls().quantized_attention(q, pages, page_table, q_seq, lengths, selected, chunk_size,
                                                 max_length, scale)
@@ -293,8 +296,8 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
         chunk = min(positive_int(chunk_size, "chunk_size"), limit)
     elif chunk_size is not None:
         raise ValueError("chunk_size without selected")
-    blocks = -(-(hq // hkv) // 32)
-    if limit > 0x7fffff00 or n * hkv * blocks * max(32, -(-limit // 128)) >= 2 ** 31:
+    blocks = -(-(hq // hkv) // 16)
+    if limit > 0x7fff0000 or n * hkv * blocks * max(32, -(-limit // 128) + 2) >= 2 ** 31:
         raise ValueError("attention exceeds 2^31 units of 128 tokens")
     pools = [_span(t) for t in pages[:4]]
     if out is None:

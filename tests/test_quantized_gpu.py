@@ -463,6 +463,54 @@ def test_a_long_context():
     _attend([131071], 14, 2, 64, 16, "fp8", torch.bfloat16)
 
 
+def test_more_rows_than_a_workgroup_has_threads():
+    """Each thread sums the shares of several rows; some rows are padding, some empty."""
+    _attend([40, 9], 2, 1, 64, 16, "fp8", torch.bfloat16,
+            rows=[(i % 3 if i % 3 < 2 else -1, (i * 11) % (41 if i % 3 == 0 else 10)) for i in range(3001)])
+
+
+def test_offsets_behind_32_bits():
+    """A pool of 2 x 36 GiB of codes whose last pages are used: bytes pass 2^35, pieces 2^31."""
+    from moba_hip import QuantizedPages, quantized_append, quantized_attention, quantized_read
+    n_pages, page, hkv, d = 36 << 16, 16, 8, 128
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("needs 90 GiB of device memory")
+    pages = QuantizedPages.empty(n_pages, page, hkv, d, format="int8")
+    first = n_pages - 6
+    table = torch.tensor([[first + 4, first, first + 5], [first + 2, first + 3, first + 1]],
+                         dtype=torch.int32, device="cuda")
+    lengths = [40, 33]
+    seq, pos = cells(lengths)
+    k, v = (_randn(len(seq), hkv, d, dtype=torch.bfloat16, seed=s) for s in (1, 2))
+    quantized_append(k, v, pages, table, seq, pos, check=True)
+    for x, y in zip((k, v), quantized_read(pages, table, seq, pos, check=True)):
+        c, s = stored(x, "int8")
+        want = c * s[..., None]
+        assert ((y.double() - want).abs() <= rounded(want, torch.bfloat16)).all()
+    q = _randn(2, 16, d, dtype=torch.bfloat16, seed=3)
+    rows = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    for selected, chunk in ((None, None), (torch.tensor([1, 4, -1], dtype=torch.int32, device="cuda")
+                                           .expand(2, 16, 3).contiguous(), 8)):
+        got = quantized_attention(q, pages, table, rows, lens, selected=selected, chunk_size=chunk)
+        check_attention(got, attention(q, pages, table, rows, lens, selected, chunk))
+
+
+def test_a_read_of_more_than_2_to_the_31_elements():
+    """A context of 2.1 million tokens of 8 heads of 128 dims, whose cells are a few."""
+    from moba_hip import quantized_read
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GiB of device memory")
+    pages, table = _filled([16], 16, 8, 128, "fp8", torch.bfloat16)
+    n = (2 ** 31 + 2 ** 20) // 1024
+    pos = torch.arange(n, dtype=torch.int32, device="cuda") % 16
+    k, v = quantized_read(pages, table, torch.zeros_like(pos), pos)
+    few = quantized_read(pages, table, torch.zeros_like(pos[:16]), pos[:16])
+    for x, y in zip((k, v), few):
+        assert torch.equal(x.view(-1, 16, 8, 128)[-5:], y.expand(5, 16, 8, 128))
+        assert torch.equal(x.view(-1, 16, 8, 128)[:5], y.expand(5, 16, 8, 128))
+
+
 # ------------------------------------------------------------------- refusals
 def _refusal_state():
     from moba_hip import QuantizedPages, RotaryTable
