@@ -325,7 +325,7 @@ PyObject* quantized_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     if (a[9] != Py_None && !((offsets = tensor_in(a[9])) && index_of(offsets, p.idx, p.slots))) return not_here();
   }
   const int64_t hq = q ? q->size(1) : 0;
-  if (n * (hq + 2 * p.hkv) * p.width >= (1ll << 31)) return not_here();
+  if (n * (hq + 2 * p.hkv) * p.width >= (1ll << 33)) return not_here();
   const at::Tensor* ins[3] = {k, v, q};
   Span spans[3];
   for (int i = 0; i < (q ? 3 : 2); ++i) {

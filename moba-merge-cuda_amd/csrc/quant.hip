@@ -395,7 +395,8 @@ extern "C" int moba_hip_quantized_append(const void* q, int64_t q_token_stride, 
   if (cos_sin != nullptr && (rotary_dim < 2 || rotary_dim > D || rotary_dim % 2 || max_pos < 1)) { moba_set_error("quantized_append: rotary_dim must be even, in [2, D], and the table nonempty"); return MOBA_ERR_ARG; }
   if ((uintptr_t)cos_sin & 15) { moba_set_error("quantized_append: the cos / sin table must be 16-byte aligned"); return MOBA_ERR_ARG; }
   if ((Hq > 0) != (q != nullptr) || (Hq > 0) != (q_out != nullptr) || (Hq > 0 && cos_sin == nullptr)) { moba_set_error("quantized_append: q, q_out and the cos / sin table go together with Hq > 0"); return MOBA_ERR_ARG; }
-  if ((int64_t)N * (Hq + 2ll * Hkv) * a.pool.Dp >= 1ll << 31) { moba_set_error("quantized_append: more than 2^31 elements in one call"); return MOBA_ERR_ARG; }
+  // 8 elements a lane, lanes of a row rounded up to a power of two: a launch of 2^31 threads
+  if ((int64_t)N * (Hq + 2ll * Hkv) * a.pool.Dp >= 1ll << 33) { moba_set_error("quantized_append: more than 2^33 elements in one call"); return MOBA_ERR_ARG; }
   a.q = (const uint16_t*)q; a.k = (const uint16_t*)k; a.v = (const uint16_t*)v;
   a.q_ts = q_token_stride; a.q_hs = q_head_stride;
   a.k_ts = k_token_stride; a.k_hs = k_head_stride;

@@ -72,6 +72,7 @@ class PreparedDecode:
             cache._guard()
             self.num_q_heads = positive_int(num_q_heads, "num_q_heads")
             _require([
+                (lambda: hasattr(cache, "k_cache"), "an 8-bit cache has its own prepare_decode"),
                 (lambda: self.num_q_heads % cache.num_kv_heads == 0,
                  "Hq must be a multiple of Hkv"),
                 (lambda: isinstance(check_finite, bool), "check_finite must be bool"),

@@ -38,6 +38,7 @@ class PreparedSharedDecode(PreparedDecode):
             capacity = cache._layout.max_seq_len
             self.max_length = capacity if max_length is None else positive_int(max_length, "max_length")
             _require([
+                (lambda: hasattr(cache, "k_cache"), "shared prefixes need a 16-bit cache (PagedKVCache)"),
                 (lambda: self.num_q_heads % cache.num_kv_heads == 0, "Hq must be a multiple of Hkv"),
                 (lambda: self.max_length <= capacity, "max_length exceeds max_seq_len"),
                 (lambda: isinstance(check_finite, bool), "check_finite must be bool"),

@@ -181,8 +181,8 @@ def quantized_append(k, v, pages, page_table, token_seq, token_pos, *, rotary=No
         hq = q.shape[1]
     elif q_out is not None:
         raise ValueError("q_out without q")
-    if n * (hq + 2 * hkv) * _code_width(d) >= 2 ** 31:
-        raise ValueError("append exceeds 2^31 elements")
+    if n * (hq + 2 * hkv) * _code_width(d) >= 2 ** 33:
+        raise ValueError("append exceeds 2^33 elements")
     pools = [_span(t) for t in pages[:4]]
     for t in (k, v, q):
         if t is not None and any(_meet(_span(t), at) for at in pools):

@@ -124,6 +124,7 @@ class PreparedQuantizedDecode(PreparedSharedDecode):
             cache._guard()
             self.num_q_heads = positive_int(num_q_heads, "num_q_heads")
             _require([
+                (lambda: isinstance(cache, QuantizedKVCache), "QuantizedKVCache required"),
                 (lambda: self.num_q_heads % cache.num_kv_heads == 0, "Hq must be a multiple of Hkv"),
                 (lambda: isinstance(check_finite, bool), "check_finite must be bool"),
                 (lambda: isinstance(stable_routes, bool), "stable_routes must be bool"),

@@ -74,7 +74,7 @@ def _refused(name, base, change, word=""):
     dict(kc=72), dict(vs=66), dict(dtype=2), dict(N=0), dict(Hq=-1), dict(Hq=2), dict(q=64), dict(q_out=64),
     dict(Hq=2, q=64, q_out=64), dict(cs=64, rotary=0, max_pos=4), dict(cs=64, rotary=66, max_pos=4),
     dict(cs=64, rotary=7, max_pos=4), dict(cs=64, rotary=8, max_pos=0), dict(cs=72, rotary=8, max_pos=4),
-    dict(N=2 ** 24)])
+    dict(N=2 ** 28)])
 def test_append_entry_refusals(change):
     _refused("moba_hip_quantized_append", APPEND, change, "quantized_append")
 

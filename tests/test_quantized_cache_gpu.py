@@ -250,3 +250,17 @@ def test_qwen2_session_in_8_bits(fmt, mode, topk):
         for a, b in zip(logits[None, "eager"][1:], logits[fmt, "eager"][1:]):
             cos = torch.nn.functional.cosine_similarity(a.float().flatten(), b.float().flatten(), dim=0)
             assert cos > 0.99
+
+
+def test_a_prepared_decode_of_another_cache_is_refused():
+    from moba_hip import PagedKVCache, PreparedDecode, PreparedQuantizedDecode, PreparedSharedDecode
+    args = (1, 8, 1, 64)
+    wide, narrow = PagedKVCache(*args, page_size=4, chunk_size=4), _cache(*args, page_size=4, chunk_size=4)
+    with pytest.raises(ValueError, match="8-bit"):
+        PreparedDecode(narrow, [0], 1)
+    with pytest.raises(ValueError, match="16-bit"):
+        PreparedSharedDecode(narrow, [0], [-1], 1)
+    with pytest.raises(ValueError, match="QuantizedKVCache"):
+        PreparedQuantizedDecode(wide, [0], 1)
+    for c in (wide, narrow):
+        c.prepare_decode([0], 1).close()    # nothing was leased

@@ -496,6 +496,31 @@ def test_offsets_behind_32_bits():
         check_attention(got, attention(q, pages, table, rows, lens, selected, chunk))
 
 
+@pytest.mark.parametrize("turn", [False, True])
+def test_an_append_of_more_than_2_to_the_31_elements(turn):
+    """A prompt of a million tokens of 8 heads of 128 dims, all alike before they turn."""
+    from moba_hip import RotaryTable, quantized_append, quantized_read
+    n, page, hkv, d = 2 ** 20 + 40, 64, 8, 128
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GiB of device memory")
+    pages = _pool(-(-n // page), page, hkv, d, "int8")
+    table = torch.arange(pages.k.shape[0], dtype=torch.int32, device="cuda")[None]
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    k, v = (_randn(1, hkv, d, dtype=torch.bfloat16, seed=s) for s in (1, 2))
+    rotary = RotaryTable(64, n) if turn else None
+    quantized_append(k.expand(n, hkv, d), v.expand(n, hkv, d), pages, table, torch.zeros_like(pos), pos,
+                     rotary=rotary)
+    small = _pool(1, 64, hkv, d, "int8")
+    for at in (0, n - 64, n // 2):
+        few = pos[at:at + 64]
+        got = quantized_read(pages, table, torch.zeros_like(few), few)
+        quantized_append(k.expand(64, hkv, d), v.expand(64, hkv, d), small, table[:, :1], torch.zeros_like(few),
+                         pos[:64], rotary=rotary,
+                         offsets=torch.tensor([at], dtype=torch.int32, device="cuda") if turn else None)
+        want = quantized_read(small, table[:, :1], torch.zeros_like(few), pos[:64])
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_a_read_of_more_than_2_to_the_31_elements():
     """A context of 2.1 million tokens of 8 heads of 128 dims, whose cells are a few."""
     from moba_hip import quantized_read
