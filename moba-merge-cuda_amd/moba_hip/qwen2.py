@@ -14,7 +14,8 @@ caller passes a transformers Qwen2 model).
   fused decode launches, the MLPs and the LM head, and the host work of a
   step is the page planning of each layer (native code) plus one replay.
   The decode position comes from the device length of layer 0's cache, so
-  replays need no new arguments.
+  replays need no new arguments.  With ``kv_format`` the caches are
+  :class:`~moba_hip.QuantizedKVCache`.
 * :class:`Qwen2Branches`: several continuations of one prompt decoded together
   (sampling, search).  The prompt is prefilled and stored once; a step runs all
   branches through every layer with one prepared shared step each, which turns,
