@@ -30,7 +30,7 @@
 // 142 us, 5.9 TB/s, where a plain read of such blocks and their scales takes 139 and the
 // arithmetic alone 113; with codes loaded to registers two steps ahead 172; with runs
 // dealt by units alone (kBegin 0) 175.  One row of 128K tokens of 2 kv heads of 64 dims,
-// fp8 (36 MB): 13.5 and 6 to join.
+// fp8 (36 MB): 13.5 and 5 to join.
 #include <algorithm>
 
 #include "quant.h"
@@ -68,8 +68,8 @@ struct AttnArgs {
   int2* items;                  // [entries][max_items]: chunk, mask of heads
   int* tokens;                  // [entries] tokens of the items, end to end
   int scan_n, scan_mult;        // dense: rows, entries per row; else entries, 1
-  uint32_t* start;              // [scan_n + 1] first unit of each
-  int* run_entry;               // [workgroups] entry of each run's first unit
+  uint32_t* start;              // [scan_n + 1] first share of each
+  int4* many;                   // [workgroups / kManyParts] the entry in which that run begins (join_kernel)
   float scale_log2;
   float *part_o, *part_ml;      // [2 workgroups][16 HB heads][D], [..][2]
   uint16_t* out;
@@ -89,9 +89,9 @@ MOBA_DEV int row_length(const AttnArgs& a, int r) {
 MOBA_DEV int scan_tokens(const AttnArgs& a, int i) {
   return a.selected != nullptr ? a.tokens[i] : row_length(a, i);
 }
-// Workgroups that share T units: all of the launch's, where each then has kRun units or
+// Workgroups for T shares: all of the launch's, where each then has kRun of them or
 // more (a run that ends inside an entry writes its sums of 16 heads, as much as a quarter
-// of a unit's codes), else fewer of them; up to one a CU for fewer units than that.
+// of a unit's codes), else fewer of them; up to one a CU for fewer shares than that.
 MOBA_DEV uint32_t sharers(uint32_t launched, uint32_t T) {
   return min(launched, max((T + kRun - 1) / kRun, min(T, 256u)));
 }
@@ -99,7 +99,7 @@ MOBA_DEV uint32_t units_of(int tokens) { return ((uint32_t)tokens + kUnit - 1) /
 // What an entry counts for in the deal: its units, and what beginning and ending it costs.
 MOBA_DEV uint32_t shares_of(int tokens) { return tokens > 0 ? units_of(tokens) + kBegin : 0; }
 
-// Workgroup w of W has units [first(w), first(w + 1)) of T >= W.
+// Workgroup w of W has shares [first(w), first(w + 1)) of T >= W.
 struct Deal {
   uint32_t q, r;
   MOBA_DEV Deal(uint32_t T, uint32_t W) : q(T / W), r(T % W) {}
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool moba = a.selected != nullptr;
 
-  // ---- the run of units that is this workgroup's
+  // ---- the run of shares that is this workgroup's
   const uint32_t per = ((uint32_t)a.scan_n + 255) / 256, i0 = tid * per;
   const uint32_t i1 = min(i0 + per, (uint32_t)a.scan_n);
   uint32_t mine = 0;
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
   uint32_t left = deal.first(wg + 1) - x0;
   if (x0 >= excl && x0 < excl + mine) {  // one thread has it
     uint32_t rem = x0 - excl, i = i0;
-    for (;; ++i) {
+    for (; i + 1 < i1; ++i) {
       const uint32_t n = shares_of(scan_tokens(a, i)) * a.scan_mult;
       if (rem < n) break;
       rem -= n;
@@ -368,6 +368,14 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
   __syncthreads();
   uint32_t si = __builtin_amdgcn_readfirstlane(found[0]), off = __builtin_amdgcn_readfirstlane(found[1]), in = 0;
   bool first_segment = true;
+  // Of every kManyParts-th run, for the second launch: the entry in which the run begins, its
+  // first workgroup, parts (0: this run has none of it) and the row of the first one's partial.
+  auto tell = [&](int e, uint32_t from, uint32_t shares, bool part) __attribute__((always_inline)) {
+    if (!first_segment || tid != 0 || wg % kManyParts != 0) return;
+    const uint32_t begin = x0 - from, w0 = deal.owner(begin);
+    const uint32_t n = part ? deal.owner(begin + shares - kBegin - 1) - w0 + 1 : 0;
+    a.many[wg / kManyParts] = make_int4(e, (int)w0, (int)n, (int)(2 * w0 + (deal.first(w0) < begin ? 1 : 0)));
+  };
   // what the scan entry after the present one is, asked for while that one is worked on
   struct Peek {
     int tokens, slot, length;
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
   Peek coming = peek(si);
 
   while (left > 0) {
-    // ---- a segment: units [off, off + n) of entry e, the in-th of scan entry si
+    // ---- a segment: n of entry e's units from `off` on; e is the in-th of scan entry si
     const int slot_id = __builtin_amdgcn_readfirstlane(coming.slot);
     int len = __builtin_amdgcn_readfirstlane(coming.length);
     len = slot_id < 0 || slot_id >= a.pool.B ? 0 : cut_length(a, len);
@@ -400,7 +408,6 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
     }
     const uint32_t taken = min(left, shares - off), n = min(off + taken, u) - min(off, u);
     const int e = (int)(si * a.scan_mult + in);
-    if (first_segment && tid == 0) a.run_entry[wg] = e;
     const uint32_t from = off;
     left -= taken;
     off += taken;
@@ -411,7 +418,8 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
         coming = peek(++si);
       }
     }
-    if (n == 0) {  // the rest of an entry's share, without units
+    if (n == 0) {  // the rest of an entry's shares, without units
+      tell(e, from, shares, false);
       first_segment = false;
       continue;
     }
@@ -694,6 +702,7 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
       } while (sent.any);
     }
 
+    tell(e, from, shares, true);
     // ---- the four waves join; head h of block hb is in waves hb, hb + HB, ...
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -740,11 +749,12 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
 
 // Joins the partials of the entries that span several workgroups of the first launch:
 // o = sum 2^(m_j - m) o_j, z = sum 2^(m_j - m) z_j, in an order that is fixed.  The
-// first workgroups have an entry each: a thread has 4 dims of a head and walks through
-// its parts.  Entries of many parts (fewer than one for every kManyParts runs) are left
-// to the others, one for each head and every kManyParts-th run: that run's
-// entry is theirs if the run is the first such one behind the entry's start; B / cols parts
-// at once, cols threads of 4 dims each (a power of two).
+// first workgroups have an entry each: a thread has 4 dims of a head and all its parts.
+// Entries of more than kManyParts parts are left to the others, one for each head and
+// every kManyParts-th run: the entry in which that run begins is theirs if it is the
+// first such run behind the entry's own begin; B / cols parts at once, cols threads of 4
+// dims each (a power of two).  A launch of 4 to 7 us that waits: for where the parts are,
+// then for maxima, sums and the first of the partials together.
 struct Parts {
   uint32_t w0, n;     // first workgroup, and how many (0: no units)
   int64_t slot0;      // row of that one's partial of head 0
@@ -758,7 +768,8 @@ MOBA_DEV Parts parts_of(const AttnArgs& a, int e, int wgs) {
   const int si = a.scan_mult == 1 ? e : (int)div_by(e, a.by_row), in = e - si * a.scan_mult;
   const uint32_t T = a.start[a.scan_n], s0 = a.start[si], all = a.start[si + 1] - s0;
   const uint32_t shares = a.scan_mult == 1 ? all : div_by(all, a.by_row);
-  p.n = 0;
+  p.w0 = p.n = 0;
+  p.slot0 = 0;
   if (shares == 0) return p;
   const Deal deal(T, sharers(wgs, T));
   const uint32_t from = s0 + in * shares;
@@ -775,50 +786,78 @@ MOBA_DEV void store_joined(const AttnArgs& a, int64_t row, int d, const f32x4_t&
   if (d == 0) a.lse[row] = z == 0.0f ? -INFINITY : (top + __log2f(z)) * kLn2;
 }
 
+// 4 dims of a head, of N parts at most; the loads behind the last part repeat it.
+template <int DT, int N> MOBA_DEV void join_few(const AttnArgs& a, const Parts& p, int64_t row, int h, int d) {
+  float2 ml[N];
+  f32x4_t v[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int64_t at = p.slot(min((uint32_t)j, p.n - 1)) + h;
+    ml[j] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+    v[j] = *reinterpret_cast<const f32x4_t*>(a.part_o + at * a.pool.D + d);
+  }
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, z = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = fmaxf(top, ml[j].x);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if ((uint32_t)j >= p.n) break;
+    const float f = ml[j].x == -INFINITY ? 0.0f : fast_exp2(ml[j].x - top);
+    z += f * ml[j].y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += v[j][i] * f;
+  }
+  store_joined<DT>(a, row, d, o, top, z);
+}
+
 template <int DT, int B>
 __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entries, int cols, int per_entry) {
   __shared__ float weight[kMaxWgs];
   __shared__ float red[2][B / 64];
   __shared__ __attribute__((aligned(16))) f32x4_t sums[B / 64][64];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, D = a.pool.D;
-  int e = blockIdx.x, h = 0, run = 0;
+  int e = blockIdx.x, h = 0;
   const bool many = e >= entries;
+  Parts p;
   if (many) {
+    const int run = ((e - entries) / per_entry + 1) * kManyParts;
     h = (e - entries) % per_entry;
-    run = ((e - entries) / per_entry + 1) * kManyParts;
+    const int4 t = a.many[run / kManyParts];  // not written for a run that there is not
     if (run >= (int)sharers(wgs, a.start[a.scan_n])) return;
-    e = a.run_entry[run];
+    e = t.x;
+    p.w0 = (uint32_t)t.y;
+    p.n = (uint32_t)t.z;
+    p.hpe = 16 * a.HB;
+    p.slot0 = (int64_t)t.w * p.hpe;
+    if (p.n <= kManyParts || (p.w0 / kManyParts + 1) * kManyParts != (uint32_t)run) return;
+  } else {
+    p = parts_of(a, e, wgs);
+    if (p.n == 1 || p.n > kManyParts) return;  // written by that workgroup; or left to the others
   }
-  const Parts p = parts_of(a, e, wgs);
   const int r = (int)div_by(e, a.by_row), of_row = e - r * a.per_row;
   const int kh = (int)div_by(of_row, a.by_nhb), blk = of_row - kh * a.NHB;
   const int heads = min(p.hpe, a.G - blk * p.hpe);
   const int64_t row0 = (int64_t)r * a.Hq + kh * a.G + blk * p.hpe;
   if (!many) {
-    if (p.n == 1 || p.n > kManyParts) return;  // written by that workgroup; or left to the others
-    const int all = heads * (D / 4);
-    for (int x = tid; x < all; x += B) {
+    for (int x = tid; x < heads * (D / 4); x += B) {
       const int hx = (int)div_by(x, a.by_d4), d = 4 * (x - hx * (D / 4));
-      f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-      float top = -INFINITY, z = 0.0f;
-#pragma unroll 4
-      for (uint32_t j = 0; j < p.n; ++j) top = fmaxf(top, a.part_ml[2 * (p.slot(j) + hx)]);
-#pragma unroll 4
-      for (uint32_t j = 0; j < p.n; ++j) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p.slot(j) + hx));
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.part_o + (p.slot(j) + hx) * D + d);
-        const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
-        z += f * ml.y;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += v[i] * f;
-      }
-      store_joined<DT>(a, row0 + hx, d, o, top, z);  // no units: zeros and -inf
+      if (p.n == 0) store_joined<DT>(a, row0 + hx, d, (f32x4_t){0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.0f);
+      else if (p.n <= 4) join_few<DT, 4>(a, p, row0 + hx, hx, d);
+      else join_few<DT, kManyParts>(a, p, row0 + hx, hx, d);
     }
     return;
   }
-  if (p.n <= kManyParts || h >= heads || (p.w0 / kManyParts + 1) * kManyParts != (uint32_t)run) return;
-  float top = -INFINITY;
-  for (uint32_t j = tid; j < p.n; j += B) top = fmaxf(top, a.part_ml[2 * (p.slot(j) + h)]);
+  if (h >= heads) return;
+  auto sums_of = [&](uint32_t j) { return *reinterpret_cast<const float2*>(a.part_ml + 2 * (p.slot(j) + h)); };
+  const int c = tid & (cols - 1), d = 4 * c, groups = B / cols;
+  const int at = d < D ? d : 0;  // columns behind D repeat the first
+  auto part = [&](uint32_t j) { return *reinterpret_cast<const f32x4_t*>(a.part_o + (p.slot(j) + h) * D + at); };
+  const uint32_t first = tid / cols;
+  const float2 mine = sums_of(min((uint32_t)tid, p.n - 1));
+  f32x4_t o = part(min(first, p.n - 1));
+  float top = mine.x;
+  for (uint32_t j = tid + B; j < p.n; j += B) top = fmaxf(top, sums_of(j).x);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   if (lane == 0) red[0][w] = top;
@@ -826,7 +865,7 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entrie
   for (int x = 0; x < B / 64; ++x) top = fmaxf(top, red[0][x]);
   float z = 0.0f;
   for (uint32_t j = tid; j < p.n; j += B) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (p.slot(j) + h));
+    const float2 ml = j == (uint32_t)tid ? mine : sums_of(j);
     const float f = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - top);
     weight[j] = f;
     z += f * ml.y;
@@ -837,12 +876,12 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entrie
   __syncthreads();
   z = 0.0f;
   for (int x = 0; x < B / 64; ++x) z += red[1][x];
-  const int c = tid & (cols - 1), d = 4 * c, groups = B / cols;
-  const int at = d < D ? d : 0;  // columns behind D repeat the first
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  const float f0 = weight[min(first, p.n - 1)];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = first < p.n ? o[i] * f0 : 0.0f;
 #pragma unroll 4
-  for (uint32_t j = tid / cols; j < p.n; j += groups) {
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + (p.slot(j) + h) * D + at);
+  for (uint32_t j = first + groups; j < p.n; j += groups) {
+    const f32x4_t x = part(j);
     const float f = weight[j];
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[i] += x[i] * f;
@@ -863,7 +902,7 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entrie
 // Shape of a call: blocks of heads, entries, workgroups, and what its workspace holds.
 struct Shape {
   int G, HB, NHB, max_items, wgs;
-  int64_t entries, items_at, tokens_at, start_at, run_at, part_o_at, part_ml_at, bytes;
+  int64_t entries, items_at, tokens_at, start_at, many_at, part_o_at, part_ml_at, bytes;
 };
 Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_length) {
   Shape s;
@@ -888,7 +927,7 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.items_at = take(slots > 0 ? s.entries * s.max_items * 8 : 0);
   s.tokens_at = take(slots > 0 ? s.entries * 4 : 0);
   s.start_at = take((std::max<int64_t>(slots > 0 ? s.entries : Nq, 1) + 1) * 4);
-  s.run_at = take(s.wgs * 4);
+  s.many_at = take(((s.wgs - 1) / kManyParts + 1) * 16);
   const int64_t rows = 2ll * s.wgs * 16 * s.HB;
   s.part_o_at = take(rows * D * 4);
   s.part_ml_at = take(rows * 8);
@@ -962,7 +1001,7 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   a.items = (int2*)(p + s.items_at); a.tokens = (int*)(p + s.tokens_at);
   a.scan_n = selected != nullptr ? (int)s.entries : Nq;
   a.scan_mult = selected != nullptr ? 1 : a.per_row;
-  a.start = (uint32_t*)(p + s.start_at); a.run_entry = (int*)(p + s.run_at);
+  a.start = (uint32_t*)(p + s.start_at); a.many = (int4*)(p + s.many_at);
   a.scale_log2 = scale * kLog2e;
   a.part_o = (float*)(p + s.part_o_at); a.part_ml = (float*)(p + s.part_ml_at);
   a.out = (uint16_t*)out; a.lse = lse;
