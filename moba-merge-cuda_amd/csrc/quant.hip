@@ -6,6 +6,11 @@
 // (2i, 2i + 1), y_a = x_a cos - x_b sin, y_b = x_a sin + x_b cos, fp32, here with
 // each product rounded), and are quantised from fp32, so that a stored key is
 // rounded once.  Several lanes hold a row; the maximum of |x| goes through them.
+//
+// Bound by memory where tokens are many: 32K tokens of 32 + 8 + 8 heads of 128 dims, all
+// turned (739 MB): 154 us, 4.8 TB/s, where a copy of 1 GiB runs at 5.1.  8 tokens of 12 +
+// 2 + 2 heads: 4.2 us, a launch and what waits for each other (slot and position, page,
+// store).  One pass: a row's scale is known before its values leave the registers.
 #include <algorithm>
 
 #include "quant.h"
@@ -296,7 +301,10 @@ template <int DT, int FMT> MOBA_DEV void store_values(uint16_t* dst, uint2 w, fl
   st8(dst, pack8<DT>(v));
 }
 
-// A thread has 8 dims of a token's key and of its value: one search for both.
+// A thread has 8 dims of a token's key and of its value: one search for both.  32K tokens
+// of 8 heads of 128 dims (204 MB): 39 us, 5.2 TB/s (a call 45; with key and value in threads
+// of their own 66).  Stores that pass the caches by took 33, but the reader
+// of the output, which comes next, would then find nothing of it there.
 template <int DT, int FMT>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x;

@@ -944,14 +944,16 @@ template <int DT, int FMT> void launch_attend(const AttnArgs& a, int wgs, hipStr
   else hipLaunchKernelGGL((attend_kernel<DT, FMT, 16>), grid, block, 0, st, a);
 }
 
-// Few entries have many parts each: wide workgroups then.
+// Wide workgroups for entries of 128 parts and more, if the work is even (us, 512 and 1024
+// threads): 2 entries of 384 parts 6.2, 5.4; 64 entries of 8 parts of 32 heads 7.2, 12.2; 256
+// entries of 3 parts 4.9, 7.6.  (256 threads: 9.5, 10.0, 5.9.)
 template <int DT> void launch_join(const AttnArgs& a, int entries, int wgs, hipStream_t st) {
   int cols = 16;
   while (cols * 4 < a.pool.D) cols *= 2;
   const int per_entry = std::min(a.G, 16 * a.HB);
   const dim3 grid((unsigned)(entries + (wgs - 1) / kManyParts * per_entry));
-  if (entries <= 64) hipLaunchKernelGGL((join_kernel<DT, 1024>), grid, dim3(1024), 0, st, a, wgs, entries, cols, per_entry);
-  else hipLaunchKernelGGL((join_kernel<DT, 256>), grid, dim3(256), 0, st, a, wgs, entries, cols, per_entry);
+  if (wgs >= 128ll * entries) hipLaunchKernelGGL((join_kernel<DT, 1024>), grid, dim3(1024), 0, st, a, wgs, entries, cols, per_entry);
+  else hipLaunchKernelGGL((join_kernel<DT, 512>), grid, dim3(512), 0, st, a, wgs, entries, cols, per_entry);
 }
 
 }  // namespace
