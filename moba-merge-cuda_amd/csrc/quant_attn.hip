@@ -44,7 +44,9 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
 constexpr int kMaxWgs = 768;    // of a launch, at most
-constexpr int kRun = 4;         // units of a workgroup, at least
+// Shares of a workgroup, at least (both launches, us): 256 rows of 64 to 4K tokens, one kv
+// head: 2 25.1, 4 24.1, 6 23.6, 8 26.1; one row of 128K: 21.0, 19.6, 19.2, 20.7.
+constexpr int kRun = 6;
 // Units' worth of time that beginning and ending an entry takes (its length, slot, pages,
 // query and sums wait for each other, about 4 us).  256 rows of 64 to 4K tokens, one kv
 // head, us: 0 29, 1 21.9, 2 21.5, 3 20.9, 4 23; 64 rows of up to 32K: 179, 165, 163, 164, 163.
