@@ -467,8 +467,8 @@ int moba_hip_quantized_means(int format, const void* k_codes, const float* k_sca
  * [Nq,Hq,slots] (nullable, slots in [1,16]) those of them in the chunks of `chunk` tokens
  * that each head selected (-1 none, any order; chunks behind the length hold nothing).
  * out [Nq,Hq,D] (dtype), lse [Nq,Hq] fp32 natural log; a row or head that attends nothing
- * (a slot outside [0, B) too) gets zeros and -inf.  A token in an unmapped page is not
- * attended.  scale in [2^-126, 1e30].  work: moba_hip_quantized_attention_work bytes, of
+ * (a slot outside [0, B) too) gets zeros and -inf, a head whose query is not finite NaN.
+ * A token in an unmapped page is not attended.  scale in [2^-126, 1e30].  work: moba_hip_quantized_attention_work bytes, of
  * this call alone until it is done.  q, out and work 16-byte aligned.  Two launches,
  * three with selected; results do not depend on timing. */
 int moba_hip_quantized_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,

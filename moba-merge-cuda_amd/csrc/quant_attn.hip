@@ -225,8 +225,24 @@ template <int DT, int NT> struct Query<DT, NT, false> {
   static MOBA_DEV int dim(int c, int g) { return 32 * c + 8 * g; }
   u16x8_t part[kSteps];
   MOBA_DEV void set(const u16x8_t (&raw)[kRaw]) {
+    u16x8_t top = zero8();
 #pragma unroll
-    for (int c = 0; c < kSteps; ++c) part[c] = raw[c];
+    for (int c = 0; c < kSteps; ++c) {
+      part[c] = raw[c];
+      top = __builtin_elementwise_max(top, raw[c] & (uint16_t)0x7fff);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bits = max(bits, (uint32_t)top[e]);
+    // A query that is not finite: its scores are NaN.  As it is, keys of one sign would make
+    // all of them -inf, which is what a row has that attends nothing.
+    const uint64_t bad = __ballot(bits >= (DT == 0 ? 0x7f80u : 0x7c00u));
+    if (bad != 0) {  // the same for all four lanes of a head
+      const uint32_t nan = (bad >> (threadIdx.x & 15)) & 0x0001000100010001ull ? 0x7fff7fffu : 0u;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+        part[c] = __builtin_bit_cast(u16x8_t, __builtin_bit_cast(u32x4_t, part[c]) | nan);
+    }
   }
   struct Codes {
     uint2 step[kSteps];
@@ -685,11 +701,11 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
       prepare();
       send();
       sent = aimed;
-      prepare();
 #pragma unroll
       for (int c = 0; c < Q::kRaw; ++c)
         if (Q::dim(c, g) >= a.pool.D || my_head >= heads) raw[c] = zero8();
-      query.set(raw);
+      query.set(raw);  // while the tile is on its way: the next `prepare` waits for it
+      prepare();
       do {
         at = sent;
         wave_prio<1>();  // the reads of the next half go out ahead of other waves' arithmetic

@@ -260,10 +260,12 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     chunks of ``chunk_size`` that it names (-1: none, any order, a chunk named twice
     counts once): MoBA's decode with :attr:`DecodeResult.selected_blocks`.  A slot
     outside the table (-1: padding) and a row or head with nothing to attend give
-    zeros and an lse of -inf; a token in an unmapped page is not attended.  ``scale``
-    (in [2^-126, 1e30]) defaults to D ** -0.5.  q and ``out`` are contiguous and 16-byte
-    aligned.  Weights are summed before they are divided, up to 2^6 for a token, so that
-    values must stay below 2^122 / length in size.  Nothing is read back, so a call can
+    zeros and an lse of -inf; a token in an unmapped page is not attended.  A head whose
+    query holds an infinity or a NaN gets NaN.  ``scale`` (in [2^-126, 1e30]) defaults to
+    D ** -0.5.  q and ``out`` are contiguous and 16-byte aligned.  Scores, and before their
+    scales the products of q with the codes (up to 127 or 448), must be finite in fp32.
+    Weights are summed before they are divided, up to 2^6 for a token, so that values must
+    stay below 2^122 / length in size.  Nothing is read back, so a call can
     be captured into a graph; what becomes of its tensors on other streams and in a
     graph: as in :func:`moba_hip.append_rotary`."""
     if out is None and lse is None:

@@ -1,0 +1,45 @@
+"""Queries of an 8-bit cache that are not finite."""
+import pytest
+import torch
+
+from quant_check import attention, cells, make_table
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to("cuda", dtype)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,d", [(4, 64), (4, 128), (20, 40), (4, 256)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_query_that_is_not_finite_gives_nan(fmt, dtype, hq, d, bad):
+    """Keys of one sign in the dim of an infinity: its scores are all +inf or all -inf, and
+    the softmax of either is no number.  The other heads and rows are as they were, and a row
+    that attends nothing is zeros whatever its query holds."""
+    from moba_hip import QuantizedPages, quantized_append, quantized_attention
+    n, dim = 70, 3
+    table, n_pages = make_table([n], 16, 0)
+    pages = QuantizedPages.empty(n_pages, 16, 1, d, format=fmt)
+    seq, pos = cells([n])
+    k = _rand((n, 1, d), dtype, 1)
+    k[..., dim] = -k[..., dim].abs() - 0.5
+    quantized_append(k, _rand((n, 1, d), dtype, 2), pages, table, seq, pos)
+    q = _rand((3, hq, d), dtype, 3)
+    dev = dict(dtype=torch.int32, device="cuda")
+    rows, lens = torch.zeros(3, **dev), torch.tensor([n, 33, 0], **dev)
+    for selected in (None, torch.tensor([0, 2], **dev).expand(3, hq, 2).contiguous()):
+        chunk = None if selected is None else 20
+        want = attention(q, pages, table, rows, lens, selected, chunk)
+        other = q.clone()
+        other[0, 1, dim] = other[2, 0, d - 1] = bad
+        out, lse = quantized_attention(other, pages, table, rows, lens, selected=selected, chunk_size=chunk)
+        assert torch.isnan(out[0, 1]).all() and torch.isnan(lse[0, 1])
+        kept = torch.ones(3, hq, dtype=torch.bool, device="cuda")
+        kept[0, 1] = kept[2] = False
+        assert ((out.double() - want[0]).abs() <= want[2])[kept].all()
+        assert ((lse.double() - want[1]).abs() <= want[3])[kept].all()
+        assert (out[2] == 0).all() and (lse[2] == -float("inf")).all()
