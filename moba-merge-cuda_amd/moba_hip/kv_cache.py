@@ -362,6 +362,10 @@ class PagedKVCache:
         return PreparedSharedDecode(self, sequence_ids, prefix_ids, num_q_heads, rotary=rotary,
                                     max_length=max_length, check_finite=check_finite)
 
+    def _check_decode(self, q, ids, counts, topk, dense):
+        """Raises what keeps the queries of tokens that are to be appended from being
+        attended, before any of them is stored.  (QuantizedKVCache has such limits.)"""
+
     @torch.no_grad()
     def append_and_attend(self, q, k, v, *, sequence_ids, cu_seqlens=None, topk=4, mode="moba"):
         with self._lock, torch.cuda.device(self.device):
@@ -374,6 +378,7 @@ class PagedKVCache:
             contract.query_grid(q, self.num_kv_heads)
             ids = self._layout.validate_ids(_ints(sequence_ids, "sequence_ids"), unique=True)
             counts = contract.append_counts(k.shape[0], ids, cu_seqlens)
+            self._check_decode(q, ids, counts, topk, dense)
             done, seq, pos = self._store(k, v, ids, counts)
             return self._decode(q, done.sequence_ids, done.positions, seq, pos, topk, dense)
 

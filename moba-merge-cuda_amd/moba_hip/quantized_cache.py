@@ -78,6 +78,22 @@ class QuantizedKVCache(PagedKVCache):
         pos = torch.arange(n, device=self.device, dtype=torch.int32)
         return quantized_read(self.pages, self._table, torch.full_like(pos, slot), pos, dtype=self.dtype)
 
+    def _route_size(self, nq, hq, last, lengths, topk):
+        """(remote chunks of a head, chunks to score) of nq routed queries, the farthest at
+        position ``last`` of a cache of ``lengths``; raises what the route does not take."""
+        remote = min(int(topk) - 1, self._candidates(lengths))
+        width = max(remote, last // self.chunk_size) if remote else 0
+        _require([(lambda: width * hq * nq < 2 ** 31, "route score grid exceeds int32 capacity"),
+                  *_route_rules(hq, self.num_kv_heads, width)])
+        return remote, width
+
+    def _check_decode(self, q, ids, counts, topk, dense):
+        if dense:
+            return
+        lengths = np.array(self.lengths)
+        lengths[list(ids)] += counts
+        self._route_size(q.shape[0], q.shape[1], int(lengths[list(ids)].max()) - 1, lengths, topk)
+
     def _decode(self, q, ids, pos, dev_ids, dev_pos, topk, dense):
         q = q.contiguous()
         if q.data_ptr() & 15:
@@ -85,10 +101,7 @@ class QuantizedKVCache(PagedKVCache):
         nq, hq, d = q.shape
         selected = None
         if not dense:
-            remote = min(int(topk) - 1, self._candidates())
-            width = max(remote, max(pos) // self.chunk_size) if remote else 0
-            _require([(lambda: width * hq * nq < 2 ** 31, "route score grid exceeds int32 capacity"),
-                      *_route_rules(hq, self.num_kv_heads, width)])
+            remote, width = self._route_size(nq, hq, max(pos), None, topk)
             selected = torch.empty((nq, hq, remote + 1), dtype=torch.int32, device=self.device)
             scores = (torch.empty((nq, hq, width), dtype=torch.float32, device=self.device)
                       if remote else None)
