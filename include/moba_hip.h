@@ -479,7 +479,9 @@ int moba_hip_quantized_attention(const void* q, int dtype, int Nq, int Hq, int H
                                  int length_add, int max_length, const int* selected, int slots,
                                  int chunk, void* work, void* out, float* lse, void* stream);
 
-/* Bytes of that workspace for the same arguments (-1 for bad ones). */
+/* Bytes of that workspace for the same arguments; -1 for bad ones, and for a call that
+ * passes its counters: 2^31 heads or units of 128 tokens, or 2^32 threads of a launch (512
+ * for each row, kv head and block of up to 16 or 32 query heads, and a few more). */
 int64_t moba_hip_quantized_attention_work(int Nq, int Hq, int Hkv, int D, int slots, int chunk,
                                           int max_length);
 

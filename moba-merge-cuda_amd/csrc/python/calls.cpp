@@ -431,18 +431,16 @@ PyObject* quantized_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)p.d)
                        : PyFloat_Check(a[8]) ? PyFloat_AS_DOUBLE(a[8]) : 0.0;
   if (!(scale >= 0x1p-126 && scale < 1e30)) return not_here();
-  const int64_t blocks = (hq / p.hkv + 15) / 16;
-  if (n * hq >= (1ll << 31) || limit > 0x7fff0000 ||
-      n * p.hkv * blocks * std::max<int64_t>(32, (limit + 127) / 128 + 2) >= (1ll << 31))
-    return not_here();
+  if (n * hq >= (1ll << 31)) return not_here();
+  const int64_t size = moba_hip_quantized_attention_work((int)n, (int)hq, (int)p.hkv, (int)p.d, (int)slots, (int)chunk,
+                                                         (int)limit);
+  if (size < 0) return not_here();
   void* stream;
   if (!stream_of(p.idx, stream)) return not_here();
   const auto options = q->options().requires_grad(false);
   at::Tensor out = at::empty({n, hq, p.d}, options);
   at::Tensor lse = at::empty({n, hq}, options.dtype(at::kFloat));
-  at::Tensor work = at::empty({moba_hip_quantized_attention_work((int)n, (int)hq, (int)p.hkv, (int)p.d, (int)slots,
-                                                                 (int)chunk, (int)limit)},
-                              options.dtype(at::kByte));
+  at::Tensor work = at::empty({size}, options.dtype(at::kByte));
   const int rc = moba_hip_quantized_attention(
       q->data_ptr(), type, (int)n, (int)hq, (int)p.hkv, (int)p.d, (float)scale, p.code, p.k->data_ptr(),
       p.v->data_ptr(), (const float*)p.ks->data_ptr(), (const float*)p.vs->data_ptr(), (int)p.pages, (int)p.page,

@@ -919,8 +919,8 @@ __global__ __launch_bounds__(B) void join_kernel(AttnArgs a, int wgs, int entrie
 
 // Shape of a call: blocks of heads, entries, workgroups, and what its workspace holds.
 struct Shape {
-  int G, HB, NHB, max_items, wgs;
-  int64_t entries, items_at, tokens_at, start_at, many_at, part_o_at, part_ml_at, bytes;
+  int G, HB, NHB, max_items, wgs, join_threads;
+  int64_t joins, entries, items_at, tokens_at, start_at, many_at, part_o_at, part_ml_at, bytes;
 };
 Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_length) {
   Shape s;
@@ -940,6 +940,11 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   const int64_t units = s.entries * ((longest + kUnit - 1) / kUnit);
   s.wgs = (int)std::min<int64_t>(256 * per_cu, (units + 7) / 8 * 8);
   if (s.wgs < 8) s.wgs = 8;
+  // Wide workgroups join entries of 128 parts and more, if the work is even (us, 512 and 1024
+  // threads): 2 entries of 384 parts 6.2, 5.4; 64 entries of 8 parts of 32 heads 7.2, 12.2; 256
+  // entries of 3 parts 4.9, 7.6.  (256 threads: 9.5, 10.0, 5.9.)
+  s.join_threads = s.wgs >= 128 * s.entries ? 1024 : 512;
+  s.joins = s.entries + (s.wgs - 1) / kManyParts * std::min(s.G, 16 * s.HB);  // workgroups
   auto take = [&](int64_t n) { const int64_t at = s.bytes; s.bytes += (n + 255) / 256 * 256; return at; };
   s.bytes = 0;
   s.items_at = take(slots > 0 ? s.entries * s.max_items * 8 : 0);
@@ -962,26 +967,31 @@ template <int DT, int FMT> void launch_attend(const AttnArgs& a, int wgs, hipStr
   else hipLaunchKernelGGL((attend_kernel<DT, FMT, 16>), grid, block, 0, st, a);
 }
 
-// Wide workgroups for entries of 128 parts and more, if the work is even (us, 512 and 1024
-// threads): 2 entries of 384 parts 6.2, 5.4; 64 entries of 8 parts of 32 heads 7.2, 12.2; 256
-// entries of 3 parts 4.9, 7.6.  (256 threads: 9.5, 10.0, 5.9.)
-template <int DT> void launch_join(const AttnArgs& a, int entries, int wgs, hipStream_t st) {
+template <int DT> void launch_join(const AttnArgs& a, const Shape& s, hipStream_t st) {
   int cols = 16;
   while (cols * 4 < a.pool.D) cols *= 2;
-  const int per_entry = std::min(a.G, 16 * a.HB);
-  const dim3 grid((unsigned)(entries + (wgs - 1) / kManyParts * per_entry));
-  if (wgs >= 128ll * entries) hipLaunchKernelGGL((join_kernel<DT, 1024>), grid, dim3(1024), 0, st, a, wgs, entries, cols, per_entry);
-  else hipLaunchKernelGGL((join_kernel<DT, 512>), grid, dim3(512), 0, st, a, wgs, entries, cols, per_entry);
+  const int entries = (int)s.entries, per_entry = std::min(a.G, 16 * a.HB);
+  const dim3 grid((unsigned)s.joins), block(s.join_threads);
+  if (s.join_threads == 1024) hipLaunchKernelGGL((join_kernel<DT, 1024>), grid, block, 0, st, a, s.wgs, entries, cols, per_entry);
+  else hipLaunchKernelGGL((join_kernel<DT, 512>), grid, block, 0, st, a, s.wgs, entries, cols, per_entry);
+}
+
+// Tokens of a row, units and heads are counted in 31 bits, the threads of a launch in 32 (the
+// runtime refuses a launch of more, by when the first one would have been made).
+bool countable(const Shape& s, int max_length) {
+  return max_length <= 0x7fff0000 && s.entries * ((max_length + kUnit - 1ll) / kUnit + kBegin) < 1ll << 31 &&
+         s.entries * 16 * s.HB < 1ll << 31 && s.joins * s.join_threads < 1ll << 32;
 }
 
 }  // namespace
 
 extern "C" int64_t moba_hip_quantized_attention_work(int Nq, int Hq, int Hkv, int D, int slots, int chunk,
                                                      int max_length) {
-  if (Nq < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || D < 8 || D > 256 || slots < 0 || slots > kMaxSlots ||
-      (slots > 0 && chunk < 1) || max_length < 1)
+  if (Nq < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || (int64_t)Nq * Hq >= 1ll << 31 || D < 8 || D > 256 || slots < 0 ||
+      slots > kMaxSlots || (slots > 0 && chunk < 1) || max_length < 1)
     return -1;
-  return shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length).bytes;
+  const Shape s = shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length);
+  return countable(s, max_length) ? s.bytes : -1;
 }
 
 extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, int Hq, int Hkv, int D,
@@ -1004,11 +1014,10 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) || work == nullptr) { moba_set_error("quantized_attention: q, out and work must be 16-byte aligned"); return MOBA_ERR_ARG; }
   if (max_length > (int64_t)table_width * page_size) { moba_set_error("quantized_attention: max_length exceeds what the table maps"); return MOBA_ERR_ARG; }
   chunk = std::min(chunk, max_length);  // a longer one ends where the row does
-  const Shape s = shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length);
-  // units, tokens and workgroups of the second launch are counted in 31 bits
-  if (max_length > 0x7fff0000 || s.entries * ((max_length + kUnit - 1ll) / kUnit + kBegin) >= 1ll << 31 ||
-      s.entries * 16 * s.HB >= 1ll << 31) {
-    moba_set_error("quantized_attention: more than 2^31 tokens of a row, units of 128 tokens or heads");
+  const bool heads = (int64_t)Nq * Hq < 1ll << 31;
+  const Shape s = heads ? shape_of(Nq, Hq, Hkv, D, slots, chunk, max_length) : Shape();
+  if (!heads || !countable(s, max_length)) {
+    moba_set_error("quantized_attention: more than 2^31 tokens of a row, units of 128 tokens or heads, or 2^32 threads of a launch");
     return MOBA_ERR_ARG;
   }
   char* p = (char*)work;
@@ -1029,7 +1038,7 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   if (selected != nullptr) hipLaunchKernelGGL(union_kernel, dim3((unsigned)s.entries), dim3(64), 0, st, a);
   if (dtype == 0) { if (format == 0) launch_attend<0, 0>(a, s.wgs, st); else launch_attend<0, 1>(a, s.wgs, st); }
   else { if (format == 0) launch_attend<1, 0>(a, s.wgs, st); else launch_attend<1, 1>(a, s.wgs, st); }
-  if (dtype == 0) launch_join<0>(a, (int)s.entries, s.wgs, st);
-  else launch_join<1>(a, (int)s.entries, s.wgs, st);
+  if (dtype == 0) launch_join<0>(a, s, st);
+  else launch_join<1>(a, s, st);
   return moba_launch_status("quantized_attention");
 }

@@ -247,6 +247,15 @@ def quantized_read(pages, page_table, token_seq, token_pos, *, dtype=torch.bfloa
     return k, v
 
 
+def _attention_work(n, hq, hkv, d, slots, chunk, limit):
+    """Bytes of the workspace of an attention; raises for one that passes its counters."""
+    size = -1 if n * hq >= 2 ** 31 else _lib.load().moba_hip_quantized_attention_work(
+        n, hq, hkv, d, slots, chunk, limit)
+    if size < 0:
+        raise ValueError("attention exceeds 2^31 units of 128 tokens or 2^23 blocks of 16 heads")
+    return size
+
+
 def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, chunk_size=None,
                         max_length=None, scale=None, out=None, lse=None):
     """Softmax attention of q [Nq,Hq,D] (bf16 or fp16) over an 8-bit pool: row r attends
@@ -265,9 +274,10 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     D ** -0.5.  q and ``out`` are contiguous and 16-byte aligned.  Scores, and before their
     scales the products of q with the codes (up to 127 or 448), must be finite in fp32.
     Weights are summed before they are divided, up to 2^6 for a token, so that values must
-    stay below 2^122 / length in size.  Nothing is read back, so a call can
-    be captured into a graph; what becomes of its tensors on other streams and in a
-    graph: as in :func:`moba_hip.append_rotary`."""
+    stay below 2^122 / length in size.  A call takes less than 2^31 units
+    of 128 tokens and 2^23 blocks of up to 16 query heads of a row and kv head.  Nothing is
+    read back, so a call can be captured into a graph; what becomes of its tensors on other
+    streams and in a graph: as in :func:`moba_hip.append_rotary`."""
     if out is None and lse is None:
         done = _lib.calls().quantized_attention(q, pages, page_table, q_seq, lengths, selected, chunk_size,
                                                 max_length, scale)
@@ -298,9 +308,7 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
         chunk = min(positive_int(chunk_size, "chunk_size"), limit)
     elif chunk_size is not None:
         raise ValueError("chunk_size without selected")
-    blocks = -(-(hq // hkv) // 16)
-    if limit > 0x7fff0000 or n * hkv * blocks * max(32, -(-limit // 128) + 2) >= 2 ** 31:
-        raise ValueError("attention exceeds 2^31 units of 128 tokens")
+    size = _attention_work(n, hq, hkv, d, slots, chunk, limit)
     pools = [_span(t) for t in pages[:4]]
     if out is None:
         out = torch.empty_like(q)
@@ -315,7 +323,6 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     read = pools + [_span(t) for t in (q, page_table, q_seq, lengths, selected) if t is not None]
     if any(_meet(_span(out), at) for at in read) or any(_meet(_span(lse), at) for at in [*read, _span(out)]):
         raise ValueError("out and lse must not overlap each other, the inputs or the pool")
-    size = _lib.load().moba_hip_quantized_attention_work(n, hq, hkv, d, slots, chunk, limit)
     work = torch.empty(size, dtype=torch.uint8, device=dev)
     pool, table = _pool_args(pages, page_table)
     _on_device(pages.k.get_device(), "moba_hip_quantized_attention", q.data_ptr(), _DTYPES[q.dtype], n, hq,

@@ -24,16 +24,18 @@ from .kv_cache import DecodeResult, PagedKVCache
 from .ops import _lib
 from .ops import decode as kernels
 from .prepared_shared import PreparedSharedDecode
-from .quantized import (_FORMATS, QuantizedPages, _check_format, _check_head_dim, _pool_args,
-                        quantized_append, quantized_attention, quantized_read)
+from .quantized import (_FORMATS, QuantizedPages, _attention_work, _check_format, _check_head_dim,
+                        _pool_args, quantized_append, quantized_attention, quantized_read)
 
 _ROUTE_WIDTH = 8192   # chunks that moba_hip_decode_route scores
 _ROUTE_GROUP = 64     # query heads of a kv head
 
 
-def _route_rules(hq, hkv, width):
+def _route_rules(nq, hq, hkv, width):
     return [(lambda: hq // hkv <= _ROUTE_GROUP, "at most 64 query heads per kv head are routed"),
-            (lambda: width <= _ROUTE_WIDTH, "at most 8192 chunks are routed")]
+            (lambda: width <= _ROUTE_WIDTH, "at most 8192 chunks are routed"),
+            (lambda: nq * hkv * -(-(hq // hkv) // 16) < 2 ** 23,   # 2^32 threads
+             "at most 2^23 blocks of 16 query heads are routed")]
 
 
 class QuantizedKVCache(PagedKVCache):
@@ -84,15 +86,16 @@ class QuantizedKVCache(PagedKVCache):
         remote = min(int(topk) - 1, self._candidates(lengths))
         width = max(remote, last // self.chunk_size) if remote else 0
         _require([(lambda: width * hq * nq < 2 ** 31, "route score grid exceeds int32 capacity"),
-                  *_route_rules(hq, self.num_kv_heads, width)])
+                  *_route_rules(nq, hq, self.num_kv_heads, width)])
         return remote, width
 
     def _check_decode(self, q, ids, counts, topk, dense):
-        if dense:
-            return
+        nq, hq, d = q.shape
         lengths = np.array(self.lengths)
         lengths[list(ids)] += counts
-        self._route_size(q.shape[0], q.shape[1], int(lengths[list(ids)].max()) - 1, lengths, topk)
+        limit = int(lengths[list(ids)].max())
+        slots = 0 if dense else self._route_size(nq, hq, limit - 1, lengths, topk)[0] + 1
+        _attention_work(nq, hq, self.num_kv_heads, d, slots, min(self.chunk_size, limit), limit)
 
     def _decode(self, q, ids, pos, dev_ids, dev_pos, topk, dense):
         q = q.contiguous()
@@ -154,7 +157,7 @@ class PreparedQuantizedDecode(PreparedSharedDecode):
             self.remote = 0 if self.dense else min(topk - 1, width)
             if not self.dense:
                 _require([(lambda: rows * hq * width < 2 ** 31, "route score grid exceeds int32 capacity"),
-                          *_route_rules(hq, cache.num_kv_heads, width)])
+                          *_route_rules(rows, hq, cache.num_kv_heads, width)])
             self.prefix_lengths = (0,) * rows
             self.rotary = rotary
             if rotary is not None:
@@ -185,9 +188,9 @@ class PreparedQuantizedDecode(PreparedSharedDecode):
             self.selected = torch.full((rows, hq, self.remote + 1), -1, device=dev, dtype=torch.int32)
             self.scores = torch.empty((rows, hq, width), device=dev, dtype=torch.float32)
         slots, chunk = (0, 0) if self.dense else (self.remote + 1, min(c.chunk_size, self.max_length))
-        size = _lib.load().moba_hip_quantized_attention_work(rows, hq, c.num_kv_heads, d, slots, chunk,
-                                                             self.max_length)
-        self._work = torch.empty(size, device=dev, dtype=torch.uint8)
+        self._work = torch.empty(
+            _attention_work(rows, hq, c.num_kv_heads, d, slots, chunk, self.max_length), device=dev,
+            dtype=torch.uint8)
 
     def _launches(self, rows, width):
         """(entry, arguments without the stream) of a step, in order: the first, those that

@@ -1,0 +1,41 @@
+"""CPU tests of the largest calls that the 8-bit operators take."""
+import pytest
+
+from moba_hip.ops import _lib
+from moba_hip.quantized import _attention_work
+
+MILLION = 2 ** 20
+# the largest number of rows of 2 kv heads: 512 threads join each row and kv head, and 95
+# times `group` workgroups wait for entries of many parts
+LAST = {1: (2 ** 23 - 96) // 2, 2: (2 ** 23 - 191) // 2, 16: (2 ** 23 - 1521) // 2}
+
+
+@pytest.mark.parametrize("group", LAST)
+def test_the_threads_of_a_launch_bound_an_attention(group):
+    """2^32 threads are more than a launch holds."""
+    work = _lib.load().moba_hip_quantized_attention_work
+    rows = LAST[group]
+    assert work(rows, 2 * group, 2, 64, 0, 0, 32) > 0
+    assert work(rows + 1, 2 * group, 2, 64, 0, 0, 32) == -1
+    assert _attention_work(rows, 2 * group, 2, 64, 0, 0, 32) == work(rows, 2 * group, 2, 64, 0, 0, 32)
+    with pytest.raises(ValueError, match="blocks of 16 heads"):
+        _attention_work(rows + 1, 2 * group, 2, 64, 0, 0, 32)
+
+
+@pytest.mark.parametrize("args", [
+    (MILLION, 8, 8, 64, 0, 0, 32), (MILLION, 8, 8, 64, 4, 16, 32),     # 2^23 entries
+    (2 ** 16, 2 ** 15, 1, 64, 0, 0, 32),                               # 2^31 heads
+    (2 ** 13, 8, 8, 64, 0, 0, 2 ** 22),                                # 2^31 units and two an entry
+    (1, 8, 8, 64, 0, 0, 0x7fff0001), (2 ** 33, 8, 8, 64, 0, 0, 32)])
+def test_attentions_that_pass_a_counter(args):
+    with pytest.raises(ValueError, match="2\\^31"):
+        _attention_work(*args)
+
+
+def test_the_entry_refuses_what_the_workspace_refuses():
+    """Before anything is launched."""
+    lib = _lib.load()
+    for rows, hq in ((LAST[2] + 1, 4), (2 ** 29, 4), (2 ** 30, 4)):
+        rc = lib.moba_hip_quantized_attention(64, 0, rows, hq, 2, 64, 1.0, 0, 64, 64, 64, 64, 4, 16, 64, 2, 2, 64, 64,
+                                              0, 32, None, 0, 0, 64, 64, 64, None)
+        assert rc == _lib.MOBA_ERR_ARG and "threads of a launch" in lib.moba_hip_last_error().decode()
