@@ -454,7 +454,8 @@ int moba_hip_quantized_read(int format, const void* k_codes, const void* v_codes
                             int dtype, void* k_out, void* v_out, int* status, void* stream);
 
 /* moba_hip_block_means of an 8-bit pool: the means of the stored values of closed chunks,
- * in the same canonical order, rounded to dtype. */
+ * in the same canonical order, rounded to dtype.  One launch, more where the items have 2^26
+ * pieces of 8 dims or more together. */
 int moba_hip_quantized_means(int format, const void* k_codes, const float* k_scale, int num_pages,
                              int page_size, int Hkv, int D, const int* table, int B,
                              int table_width, const int* item_seq, const int* item_chunk_or_pos,

@@ -463,14 +463,18 @@ extern "C" int moba_hip_quantized_means(int format, const void* k_codes, const f
   if (rc) return rc;
   if (dtype != 0 && dtype != 1) { moba_set_error("quantized_means: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
   if (chunk < 1 || chunk > 64 * kMeansPer || max_chunks < 1) { moba_set_error("quantized_means: chunk must be in [1,1024], the means nonempty"); return MOBA_ERR_ARG; }
-  if ((int64_t)n_items * Hkv * (D / 8) >= 1ll << 31 || (int64_t)max_chunks * chunk >= 1ll << 31) { moba_set_error("quantized_means: more than 2^31 pieces or positions"); return MOBA_ERR_ARG; }
-  const dim3 grid((unsigned)((int64_t)n_items * Hkv * (D / 8))), block(64);
+  const int64_t per_item = (int64_t)Hkv * (D / 8);
+  const int most = (int)(((1ll << 26) - 1) / per_item);  // items of a launch: 2^32 threads are too many
+  if (n_items * per_item >= 1ll << 31 || most < 1 || (int64_t)max_chunks * chunk >= 1ll << 31) { moba_set_error("quantized_means: more than 2^31 pieces or positions, or 2^26 pieces of an item"); return MOBA_ERR_ARG; }
   hipStream_t st = (hipStream_t)stream;
-#define MOBA_MEANS(DT_, FMT_)                                                                       \
-  hipLaunchKernelGGL((means_kernel<DT_, FMT_>), grid, block, 0, st, p, item_seq, item_chunk_or_pos, \
-                     mode, chunk, (uint16_t*)means, max_chunks)
-  if (dtype == 0) { if (format == 0) MOBA_MEANS(0, 0); else MOBA_MEANS(0, 1); }
-  else { if (format == 0) MOBA_MEANS(1, 0); else MOBA_MEANS(1, 1); }
+#define MOBA_MEANS(DT_, FMT_)                                                                      \
+  hipLaunchKernelGGL((means_kernel<DT_, FMT_>), grid, block, 0, st, p, item_seq + at,               \
+                     item_chunk_or_pos + at, mode, chunk, (uint16_t*)means, max_chunks)
+  for (int at = 0; at < n_items; at += std::min(most, n_items - at)) {
+    const dim3 grid((unsigned)(std::min(most, n_items - at) * per_item)), block(64);
+    if (dtype == 0) { if (format == 0) MOBA_MEANS(0, 0); else MOBA_MEANS(0, 1); }
+    else { if (format == 0) MOBA_MEANS(1, 0); else MOBA_MEANS(1, 1); }
+  }
 #undef MOBA_MEANS
   return moba_launch_status("quantized_means");
 }

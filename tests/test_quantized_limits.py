@@ -39,3 +39,11 @@ def test_the_entry_refuses_what_the_workspace_refuses():
         rc = lib.moba_hip_quantized_attention(64, 0, rows, hq, 2, 64, 1.0, 0, 64, 64, 64, 64, 4, 16, 64, 2, 2, 64, 64,
                                               0, 32, None, 0, 0, 64, 64, 64, None)
         assert rc == _lib.MOBA_ERR_ARG and "threads of a launch" in lib.moba_hip_last_error().decode()
+
+
+@pytest.mark.parametrize("hkv,d", [(2 ** 23, 64), (2 ** 21, 256)])
+def test_an_item_of_the_means_that_no_launch_holds(hkv, d):
+    """64 threads for 8 dims of a kv head: 2^26 of these are 2^32."""
+    lib = _lib.load()
+    rc = lib.moba_hip_quantized_means(0, 64, 64, 1, 16, hkv, d, 64, 2, 1, 64, 64, 1, 0, 8, 0, 64, 2, None)
+    assert rc == _lib.MOBA_ERR_ARG and "quantized_means" in lib.moba_hip_last_error().decode()

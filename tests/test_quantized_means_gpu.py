@@ -90,3 +90,31 @@ def test_steps_that_close_long_chunks(graph, fmt, chunk):
     assert cache.lengths == (2 * chunk + 3, chunk + 4)
     for slot in (0, 1):
         _check_means(cache, slot)
+
+
+def test_more_items_than_a_launch_holds():
+    """32 767 items of 64 kv heads of 256 dims fill a launch; of the items around its end, some
+    close a chunk, and the others, as a step's rows do, none."""
+    from quant_check import cells, make_table
+    from moba_hip import QuantizedPages, quantized_append
+    from moba_hip.ops import _lib
+    hk, dim, page, most = 64, 256, 4, 32767
+    table, n_pages = make_table([2] * 5, page, 0)
+    pages = QuantizedPages.empty(n_pages, page, hk, dim)
+    seq, pos = cells([2] * 5)
+    k = _rand((10, hk, dim), torch.bfloat16, 1)
+    quantized_append(k, k, pages, table, seq, pos)
+    dev = dict(dtype=torch.int32, device="cuda")
+    n = most + 100
+    item_seq, item_pos = torch.zeros(n, **dev), torch.zeros(n, **dev)
+    for slot, at in ((1, most - 1), (2, most), (3, n - 1)):
+        item_seq[at], item_pos[at] = slot, 1
+    means = torch.full((5, 1, hk, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    _lib.call("moba_hip_quantized_means", 0, pages.k.data_ptr(), pages.k_scale.data_ptr(), n_pages, page, hk, dim,
+              table.data_ptr(), 5, 1, item_seq.data_ptr(), item_pos.data_ptr(), n, 1, 2, 0, means.data_ptr(), 1,
+              torch.cuda.current_stream().cuda_stream)
+    assert (means[[0, 4]] == 7).all()
+    for slot in (1, 2, 3):
+        x, _, _ = numbers(pages, table, slot, torch.arange(2, device="cuda"))
+        want, size = x.mean(0), x.abs().mean(0)
+        assert ((means[slot, 0].double() - want).abs() <= rounded(want, means.dtype) + size * 9 * 2.0 ** -24).all()
