@@ -430,7 +430,7 @@ PyObject* quantized_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   }
   const double scale = a[8] == Py_None ? 1.0 / std::sqrt((double)p.d)
                        : PyFloat_Check(a[8]) ? PyFloat_AS_DOUBLE(a[8]) : 0.0;
-  if (!(scale >= 0x1p-126 && scale < 1e30)) return not_here();
+  if (!(scale >= 0x1p-126 && scale <= 1e30)) return not_here();
   if (n * hq >= (1ll << 31)) return not_here();
   const int64_t size = moba_hip_quantized_attention_work((int)n, (int)hq, (int)p.hkv, (int)p.d, (int)slots, (int)chunk,
                                                          (int)limit);

@@ -1008,7 +1008,7 @@ extern "C" int moba_hip_quantized_attention(const void* q, int dtype, int Nq, in
   if (rc) return rc;
   if (dtype != 0 && dtype != 1) { moba_set_error("quantized_attention: dtype must be 0 (bf16) or 1 (fp16)"); return MOBA_ERR_ARG; }
   if (Nq < 1 || Hq < 1 || Hq % Hkv) { moba_set_error("quantized_attention: nonempty q, Hq a multiple of Hkv required"); return MOBA_ERR_ARG; }
-  if (!(scale >= 0x1p-126f && scale < 1e30f)) { moba_set_error("quantized_attention: scale must be in [2^-126, 1e30]"); return MOBA_ERR_ARG; }
+  if (!(scale >= 0x1p-126f && scale <= 1e30f)) { moba_set_error("quantized_attention: scale must be in [2^-126, 1e30]"); return MOBA_ERR_ARG; }
   if (max_length < 1) { moba_set_error("quantized_attention: max_length must be positive"); return MOBA_ERR_ARG; }
   if ((selected != nullptr) != (slots > 0) || slots > kMaxSlots || (selected != nullptr && chunk < 1)) { moba_set_error("quantized_attention: selected chunks need 1 to 16 slots and a chunk size"); return MOBA_ERR_ARG; }
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)work) & 15) || work == nullptr) { moba_set_error("quantized_attention: q, out and work must be 16-byte aligned"); return MOBA_ERR_ARG; }

@@ -47,3 +47,13 @@ def test_an_item_of_the_means_that_no_launch_holds(hkv, d):
     lib = _lib.load()
     rc = lib.moba_hip_quantized_means(0, 64, 64, 1, 16, hkv, d, 64, 2, 1, 64, 64, 1, 0, 8, 0, 64, 2, None)
     assert rc == _lib.MOBA_ERR_ARG and "quantized_means" in lib.moba_hip_last_error().decode()
+
+
+def test_the_ends_of_scale():
+    """The entry takes both ends: what it refuses here is the length."""
+    lib = _lib.load()
+    for scale, word in ((2.0 ** -126, "max_length"), (1e30, "max_length"), (1e30 * (1 - 2.0 ** -50), "max_length"),
+                        (2.0 ** -127, "scale"), (1.1e30, "scale"), (float("inf"), "scale")):
+        rc = lib.moba_hip_quantized_attention(64, 0, 1, 4, 2, 64, scale, 0, 64, 64, 64, 64, 4, 16, 64, 2, 2, 64, 64,
+                                              0, 0, None, 0, 0, 64, 64, 64, None)
+        assert rc == _lib.MOBA_ERR_ARG and f"{word} must be" in lib.moba_hip_last_error().decode()

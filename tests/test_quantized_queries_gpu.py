@@ -43,3 +43,23 @@ def test_a_query_that_is_not_finite_gives_nan(fmt, dtype, hq, d, bad):
         assert ((out.double() - want[0]).abs() <= want[2])[kept].all()
         assert ((lse.double() - want[1]).abs() <= want[3])[kept].all()
         assert (out[2] == 0).all() and (lse[2] == -float("inf")).all()
+
+
+@pytest.mark.parametrize("fmt,d", [("int8", 64), ("int8", 128), ("fp8", 64)])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1e30 * (1 - 2.0 ** -50), 1e30])
+def test_the_ends_of_scale(fmt, d, scale):
+    """Queries so small that scores are ordinary ones; with outputs of the caller too, which
+    the other host path serves."""
+    from quant_check import check_attention
+    from moba_hip import QuantizedPages, quantized_append, quantized_attention
+    table, n_pages = make_table([50], 16, 0)
+    pages = QuantizedPages.empty(n_pages, 16, 1, d, format=fmt)
+    seq, pos = cells([50])
+    k = _rand((50, 1, d), torch.bfloat16, 1)
+    quantized_append(k, k, pages, table, seq, pos)
+    q = (_rand((1, 4, d), torch.float32, 3) / max(scale, 1.0)).bfloat16()
+    dev = dict(dtype=torch.int32, device="cuda")
+    args = q, pages, table, torch.tensor([0], **dev), torch.tensor([50], **dev)
+    want = attention(*args, scale=scale)
+    check_attention(quantized_attention(*args, scale=scale), want)
+    check_attention(quantized_attention(*args, scale=scale, out=torch.empty_like(q)), want)
