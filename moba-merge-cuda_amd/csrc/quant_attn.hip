@@ -53,13 +53,13 @@ constexpr int kRun = 6;
 constexpr int kBegin = 2;
 constexpr int kManyParts = 8;   // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects
-constexpr int kMaxItems = 32 * kMaxSlots;
+constexpr int kMaxItems = 16 * kMaxSlots;  // of an entry
 constexpr float kSlack = 6.0f;  // log2 by which scores may pass the running maximum
 
 struct AttnArgs {
   QuantPool pool;
   const uint16_t* q;
-  int Hq, G, HB, NHB;           // query heads per kv head; blocks of 16 in an entry (1, 2); entries per kv head
+  int Hq, G, HB, NHB;           // query heads per kv head; blocks of 16 in an entry (1, or 2 if dense); entries per kv head
   int per_row;                  // entries per row: Hkv * NHB
   FastDiv by_row, by_nhb;       // per_row, NHB
   const int *q_seq, *lengths;
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(64) void union_kernel(AttnArgs a) {
   __shared__ uint32_t mask_s[kMaxItems];
   const int e = blockIdx.x, lane = threadIdx.x;
   const int r = e / a.per_row, kh = (e % a.per_row) / a.NHB, blk = e % a.NHB;
-  const int g0 = blk * 16 * a.HB, heads = min(16 * a.HB, a.G - g0), E = heads * a.slots;
+  const int g0 = blk * 16, heads = min(16, a.G - g0), E = heads * a.slots;
   const int len = row_length(a, r);
   const int* sel = a.selected + ((int64_t)r * a.Hq + kh * a.G + g0) * a.slots;
   for (int x = lane; x < E; x += 64) {
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
     for (int t = 0; t < NT; ++t) acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
 
-    const uint32_t heads_mask = heads == 32 ? ~0u : (1u << heads) - 1;
+    const uint32_t heads_mask = moba ? (1u << heads) - 1 : 0;  // selected chunks: heads <= 16
     const int pieces = a.pool.Dp / 16;  // of a row of codes
     // Piece p of token t's row lies at place p ^ f(t) of its row in the tile, so that the
     // same piece of 16 tokens lies in as many banks as it can (rows of 2^n pieces; the
@@ -927,13 +927,18 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.G = Hq / Hkv;
   // Two blocks of heads in an entry read its codes once for both; one block an entry joins
   // half as wide sums and has twice as many entries.  32 heads of one kv head, 128 dims, us:
-  // 32 rows of 100K tokens and more (962 MB) two 294, one 324; 64 rows of 6.7K on average
-  // (105 MB, which stays in the last-level cache) 57 and 49; 48 heads, 105 MB: 73 and 65.
+  // 32 rows of 100K tokens and more (950 MB) two 240, one 300; 64 rows of 20K (328 MB) 100 and
+  // 118; of 6.7K (110 MB, which stays in the last-level cache) 46 and 46; of 1K 21.9 and 21.6.
+  // The lengths are on the device: the rule goes by what max_length lets be read, so that
+  // short rows in a long table pay a little (8 rows of 2K, 64 heads of 2, 15.5 instead of 14.3).
+  // With selected chunks one block, always: each reads what its own 16 heads chose, where two
+  // read the other's too.  64 rows of 100K, one and two: 4 chunks of 64 a head 35, 56; 4 of 512
+  // 92, 128; 9 of 1024 of which heads share nine in ten 141, 189; that all heads agree on 64, 62.
   const int blocks = (s.G + 15) / 16;
-  s.HB = blocks % 2 == 0 && 2.0 * Nq * Hkv * max_length * code_width(D) > 256 << 20 ? 2 : 1;
+  s.HB = slots == 0 && blocks % 2 == 0 && 2.0 * Nq * Hkv * max_length * code_width(D) > 256 << 20 ? 2 : 1;
   s.NHB = (s.G + 16 * s.HB - 1) / (16 * s.HB);
   s.entries = (int64_t)Nq * Hkv * s.NHB;
-  s.max_items = std::min(s.G, 16 * s.HB) * slots;
+  s.max_items = std::min(s.G, 16) * slots;
   // as many workgroups as the card holds at once, but no more than there can be units
   const int per_cu = D > 192 ? 1 : D > 96 ? 2 : 3;  // occupancy()
   const int64_t longest = slots > 0 ? std::min<int64_t>((int64_t)s.max_items * chunk, max_length) : max_length;

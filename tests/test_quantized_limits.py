@@ -57,3 +57,11 @@ def test_the_ends_of_scale():
         rc = lib.moba_hip_quantized_attention(64, 0, 1, 4, 2, 64, scale, 0, 64, 64, 64, 64, 4, 16, 64, 2, 2, 64, 64,
                                               0, 0, None, 0, 0, 64, 64, 64, None)
         assert rc == _lib.MOBA_ERR_ARG and f"{word} must be" in lib.moba_hip_last_error().decode()
+
+
+def test_selected_chunks_have_one_block_of_heads_an_entry():
+    """However long the table: a workspace for chunks that each head selects is made for what
+    they hold, and two blocks of heads would have twice the partials."""
+    work = _lib.load().moba_hip_quantized_attention_work
+    assert work(64, 32, 1, 128, 4, 64, 131072) == work(64, 32, 1, 128, 4, 64, 8192)
+    assert work(64, 32, 1, 128, 0, 0, 131072) > 1.9 * work(64, 32, 1, 128, 0, 0, 8192)
