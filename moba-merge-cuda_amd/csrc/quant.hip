@@ -8,7 +8,7 @@
 // rounded once.  Several lanes hold a row; the maximum of |x| goes through them.
 //
 // Bound by memory where tokens are many: 32K tokens of 32 + 8 + 8 heads of 128 dims, all
-// turned (739 MB): 154 us, 4.8 TB/s, where a copy of 1 GiB runs at 5.1.  8 tokens of 12 +
+// turned (739 MB): 154 to 158 us, 4.7 TB/s, where a copy of 1 GiB runs at 5.1.  8 tokens of 12 +
 // 2 + 2 heads: 4.2 us, a launch and what waits for each other (slot and position, page,
 // store).  One pass: a row's scale is known before its values leave the registers.
 #include <algorithm>

@@ -8,8 +8,9 @@
 // Codes are exact in the 16-bit types, so q . c runs on the matrix units in q's type
 // with fp32 sums.  The weight w_t = exp(s_t - m) s^v_t has the range of s^v and is
 // split in two bf16 parts (w = hi + lo, off by 2^-17 of w), each multiplied by the
-// codes: bf16 for its range, two parts for fp16's precision.  The second product costs
-// 8 of 24 matrix instructions, in a kernel that waits for memory.
+// codes: bf16 for its range, two parts for fp16's precision.  At 128 dims the second
+// product costs 8 of 24 matrix instructions (fp8) or of 28 (int8), in a kernel that waits
+// for memory.
 //
 // Bound by the reads of codes and scales.  Work is cut into units of 128 tokens of a
 // (row, kv head, block of query heads); all units of the call, laid end to end, are
@@ -26,11 +27,11 @@
 //         the scores of 4 + 4 tokens for one head;
 //   O^T = V^T P^T: those 8 weights are a lane's share of P^T as they are, if V^T is
 //         supplied with the same 8 tokens, which the transposed LDS read does.
-// Kernel times at 64 rows of 256 to 32K tokens, 32 / 8 heads of 128 dims, int8 (831 MB):
-// 142 us, 5.9 TB/s, where a plain read of such blocks and their scales takes 139 and the
-// arithmetic alone 113; with codes loaded to registers two steps ahead 172; with runs
-// dealt by units alone (kBegin 0) 175.  One row of 128K tokens of 2 kv heads of 64 dims,
-// fp8 (36 MB): 13.5 and 5 to join.
+// Calls at 64 rows of 256 to 32K tokens, 32 / 8 heads of 128 dims, int8 (831 MB): 139 to
+// 141 us, 5.9 TB/s, where a plain read of such blocks and their scales takes 139; the first
+// form with codes loaded to registers two steps ahead took 172 in this kernel alone.  One
+// row of 128K tokens of 2 kv heads of 64 dims, fp8 (36 MB): 18.4 us; under the profiler
+// this kernel takes 14.5 of it and the join 4.8.
 #include <algorithm>
 
 #include "quant.h"
@@ -44,12 +45,17 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
 constexpr int kMaxWgs = 768;    // of a launch, at most
-// Shares of a workgroup, at least (both launches, us): 256 rows of 64 to 4K tokens, one kv
-// head: 2 25.1, 4 24.1, 6 23.6, 8 26.1; one row of 128K: 21.0, 19.6, 19.2, 20.7.
+// Shares of a workgroup, at least.  Calls, us, at 2, 4, 6, 8: 256 rows of 64 to 4K tokens, one
+// kv head 24.1, 23.2, 22.6, 25.2, two 35.5, 36.7, 36.8, 36.6; one row of 128K tokens of 64 dims
+// 20.3, 18.7, 18.4, 20.0, of 96 dims 23.2, 20.8, 19.8, 19.9; 128 rows of up to 300 tokens 12.6,
+// 14.0, 13.9, 13.9; 64 rows of up to 32K within 1%.
 constexpr int kRun = 6;
 // Units' worth of time that beginning and ending an entry takes (its length, slot, pages,
-// query and sums wait for each other, about 4 us).  256 rows of 64 to 4K tokens, one kv
-// head, us: 0 29, 1 21.9, 2 21.5, 3 20.9, 4 23; 64 rows of up to 32K: 179, 165, 163, 164, 163.
+// query and sums wait for each other, about 4 us).  Calls, us, at 0, 1, 2, 3, 4: 256 rows of 64
+// to 4K tokens, one kv head 31.3, 25.2, 22.6, 21.7, 23.4, two 50.0, 39.4, 36.8, 34.7, 36.9; 64
+// rows of up to 32K 157, 147, 142, 141, 141; 32 such rows of 256 dims 94, 83, 78, 77, 76, of 192
+// 61.3, 58.5, 58.5, 59.9, 60.4; 32 rows of 512 tokens 14.2, 17.1, 15.4, 16.3, 14.6; 56 short rows
+// of 256 dims 68.4, 61.4, 61.7, 62.5, 63.9; one row of 64K 17.3, 18.5, 18.4, 18.7, 18.5.
 constexpr int kBegin = 2;
 constexpr int kManyParts = 8;   // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects

@@ -12,8 +12,8 @@ A row of D values (one head of one token) stands as codes c and a scale s, x ~ c
                                              ties to the even one
 
 with top 127 (``"int8"``) or 448 (``"fp8"``, the 8-bit float e4m3).  int8 is off by at
-most a / 254; fp8 by 2^-4 of each value (a / 2^19 where that is more), so it keeps small
-values next to large ones.  A row that holds an infinity or a NaN has codes 0
+most a / 254; fp8 by 2^-4 of each value (a / 458752, half the smallest step, where that is
+more), so it keeps small values next to large ones.  A row that holds an infinity or a NaN has codes 0
 and scale NaN: it reads back as NaN.
 """
 from __future__ import annotations
@@ -42,7 +42,8 @@ class QuantizedPages(NamedTuple):
     """A pool of 8-bit pages: codes ``k``, ``v`` [pages,Hkv,page_size,Dp] (int8 or
     float8_e4m3fn; Dp: head_dim rounded up to 16) and scales ``k_scale``, ``v_scale``
     [pages,Hkv,page_size] fp32; contiguous, the codes 16-byte aligned.  head_dim is a
-    multiple of 8, at most 256."""
+    multiple of 8, at most 256.  A cell that is attended holds what an append wrote there:
+    finite codes, those behind head_dim 0."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -272,7 +273,8 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     zeros and an lse of -inf; a token in an unmapped page is not attended.  A head whose
     query holds an infinity or a NaN gets NaN.  ``scale`` (in [2^-126, 1e30]) defaults to
     D ** -0.5.  q and ``out`` are contiguous and 16-byte aligned.  Scores, and before their
-    scales the products of q with the codes (up to 127 or 448), must be finite in fp32.
+    scales the products of q with the codes (up to 127 or 448), must be finite in fp32;
+    against int8 keys of more than 64 dims a head's queries are held to 2^-22 of the largest.
     Weights are summed before they are divided, up to 2^6 for a token, so that values must
     stay below 2^122 / length in size.  A call takes less than 2^31 units
     of 128 tokens and 2^23 blocks of up to 16 query heads of a row and kv head.  Nothing is

@@ -4,8 +4,9 @@ scales (:mod:`moba_hip.quantized`), at half the bytes of a 16-bit cache.
 Constructor, operations, errors and lifecycle are the 16-bit cache's, with
 ``format="int8"`` or ``"fp8"``; ``dtype`` is the type of its inputs and outputs.  Keys
 and values are quantised as they are appended; chunk means, routing and attention are
-those of the stored values.  Sequences behind shared prefixes are the 16-bit cache's
-alone.
+those of the stored values.  At most 64 query heads of a kv head and 8192 chunks are
+routed; what is refused for that is refused before anything is stored.  Sequences behind
+shared prefixes are the 16-bit cache's alone.
 
 :class:`PreparedQuantizedDecode` is its prepared decode: the page delta and positions, the
 quantising append (with a ``rotary`` table the keys and queries turn inside it), the mean
