@@ -223,6 +223,13 @@ struct Step {
 // at most 2^-22 of the largest |q|, and exact for what lies less than 2^11 (fp16) or
 // 2^14 (bf16) below it.  Turning 128 dims of 32 int8 keys takes a wave 96
 // instructions; joining three integer sums of 8 scores takes 40.
+// Where a few values are so much larger than the rest that the digits lose what the rest
+// add to a score, the wave multiplies its queries as they are, with the keys turned: as
+// soon as for one head the digits' errors come to more than 2^-20 of sum min(|q|, 2^14
+// units), in which a large value counts as one of 2^14 units (2^-8 to 2^-7 of the largest).
+// Values of a normal distribution are far from that: one in 10^3 (fp16) or 10^4 (bf16) has
+// an error.  64 rows of up to 32K with such queries: 173 us instead of 140; a loop of their
+// own for them took 192 dims from 59 to 70 (registers).
 template <int FMT, int NT> constexpr bool digits() { return FMT == 0 && NT > 4; }
 template <int DT, int NT, bool DIGITS> struct Query;
 template <int DT, int NT> struct Query<DT, NT, false> {
@@ -271,6 +278,7 @@ template <int DT, int NT> struct Query<DT, NT, true> {
   static constexpr int kSteps = (NT + 3) / 4, kBytes = 16;  // of 64 dims: 16 of a lane's token
   i32x4_t digit[3][kSteps];  // lowest first
   float unit;                // 2^-k
+  bool whole;                // the digits do for all heads of the wave
   static constexpr int kRaw = 2 * kSteps;
   static MOBA_DEV int dim(int c, int g) { return 64 * (c >> 1) + 16 * g + 8 * (c & 1); }
   MOBA_DEV void set(const u16x8_t (&raw)[kRaw]) {
@@ -287,6 +295,7 @@ template <int DT, int NT> struct Query<DT, NT, true> {
     const int e = max((int)(bits >> 23), 1 + 21);  // max |q| < 2^(e - 126); smallest: 2^-105
     const float fold = __uint_as_float((uint32_t)(finite ? min(127 + 126 + 22 - e, 254) : 127) << 23);
     unit = finite ? __uint_as_float((uint32_t)max(e - 22 + 1, 0) << 23) : __uint_as_float(0x7fc00000u);
+    float lost = 0.0f;  // in units; NaN for a query that is not finite, as its scores
 #pragma unroll
     for (int c = 0; c < kSteps; ++c)
 #pragma unroll
@@ -295,16 +304,32 @@ template <int DT, int NT> struct Query<DT, NT, true> {
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           const int i = 4 * w + b;
-          int v = (int)rintf(to_f32<DT>(raw[2 * c + (i >> 3)][i & 7]) * fold);
+          const float x = to_f32<DT>(raw[2 * c + (i >> 3)][i & 7]) * fold, near = rintf(x);
+          lost += fabsf(x - near);
+          int v = (int)near;
 #pragma unroll
-          for (int x = 0; x < 3; ++x) {
-            d[x] |= ((uint32_t)v & 255u) << (8 * b);
+          for (int y = 0; y < 3; ++y) {
+            d[y] |= ((uint32_t)v & 255u) << (8 * b);
             v = (v + 128) >> 8;  // what the signed digit leaves
           }
         }
 #pragma unroll
-        for (int x = 0; x < 3; ++x) digit[x][c][w] = (int)d[x];
+        for (int y = 0; y < 3; ++y) digit[y][c][w] = (int)d[y];
       }
+    whole = true;
+    if (__any(lost > 0.0f)) {
+      float held = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kRaw; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) held += fminf(fabsf(to_f32<DT>(raw[c][i]) * fold), 0x1p14f);
+#pragma unroll
+      for (int off = 16; off < 64; off <<= 1) {
+        lost += __shfl_xor(lost, off, 64);
+        held += __shfl_xor(held, off, 64);
+      }
+      whole = !__any(lost > 0x1p-20f * held);
+    }
   }
   struct Codes {
     i32x4_t step[kSteps];
@@ -325,6 +350,29 @@ template <int DT, int NT> struct Query<DT, NT, true> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = fmaf((float)s[1][i], 256.0f, (float)s[0][i]) * unit;
     return r;
+  }
+  // q . c of two tiles without digits; row: the query in memory, null for no head.
+  MOBA_DEV void dot_as_it_is(const Codes (&k)[2], const uint16_t* row, int D, int g, f32x4_t (&s)[2]) const {
+    s[0] = s[1] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < kRaw; ++c) {
+      const int d = dim(c, g);
+      u16x8_t x = zero8();
+      if (row != nullptr && d < D) x = ld8(row + d);
+      asm volatile("" ::: "memory");  // one load's registers at a time
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint32_t w[4];
+        numbers4_16<0, DT>((uint32_t)k[t].step[c >> 1][2 * (c & 1)], w[0], w[1]);
+        numbers4_16<0, DT>((uint32_t)k[t].step[c >> 1][2 * (c & 1) + 1], w[2], w[3]);
+        s[t] = mfma16<DT>(__builtin_bit_cast(u16x8_t, (u32x4_t){w[0], w[1], w[2], w[3]}), x, s[t]);
+      }
+    }
+    const float nan = unit - unit;  // of a query that is not finite
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] += nan;
   }
 };
 
@@ -584,10 +632,22 @@ __global__ __launch_bounds__(256, occupancy<NT>()) void attend_kernel(AttnArgs a
     Q query;
     f32x4_t sc[2];
     auto scores = [&](int half) __attribute__((always_inline)) {
+      bool done = false;
+      if constexpr (digits<FMT, NT>()) {
+        if (__builtin_expect(!query.whole, 0)) {
+          const int h = (int)opaque((uint32_t)my_head);  // (no address is held between halves)
+          const uint16_t* row = a.q + ((int64_t)r * a.Hq + head0 + h) * a.pool.D;
+          query.dot_as_it_is(keys, h < heads ? row : nullptr, a.pool.D, (int)opaque((uint32_t)g), sc);
+          done = true;
+        }
+      }
+      if (!done) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) sc[t] = query.template dot<FMT>(keys[t]);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const f32x4_t kk = lds4<f32x4_t>(&ks_s[w][half + 16 * t + 4 * g]);
-        sc[t] = query.template dot<FMT>(keys[t]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[t][i] *= kk[i];
       }

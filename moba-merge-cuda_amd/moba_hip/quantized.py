@@ -273,8 +273,7 @@ def quantized_attention(q, pages, page_table, q_seq, lengths, *, selected=None, 
     zeros and an lse of -inf; a token in an unmapped page is not attended.  A head whose
     query holds an infinity or a NaN gets NaN.  ``scale`` (in [2^-126, 1e30]) defaults to
     D ** -0.5.  q and ``out`` are contiguous and 16-byte aligned.  Scores, and before their
-    scales the products of q with the codes (up to 127 or 448), must be finite in fp32;
-    against int8 keys of more than 64 dims a head's queries are held to 2^-22 of the largest.
+    scales the products of q with the codes (up to 127 or 448), must be finite in fp32.
     Weights are summed before they are divided, up to 2^6 for a token, so that values must
     stay below 2^122 / length in size.  A call takes less than 2^31 units
     of 128 tokens and 2^23 blocks of up to 16 query heads of a row and kv head.  Nothing is

@@ -63,3 +63,30 @@ def test_the_ends_of_scale(fmt, d, scale):
     want = attention(*args, scale=scale)
     check_attention(quantized_attention(*args, scale=scale), want)
     check_attention(quantized_attention(*args, scale=scale, out=torch.empty_like(q)), want)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,large", [(torch.bfloat16, 2.0 ** 13), (torch.bfloat16, 2.0 ** 18),
+                                         (torch.bfloat16, 1e9), (torch.float16, 60000.0)])
+@pytest.mark.parametrize("hq,d", [(4, 64), (6, 96), (20, 128), (3, 192), (4, 256)])
+def test_a_large_value_in_a_query_leaves_the_others_their_digits(fmt, dtype, large, hq, d):
+    """One dim of some heads' queries is much larger than the others, and the keys are zero
+    there: scores are those of the other dims, which the bound goes by."""
+    from quant_check import check_attention
+    from moba_hip import QuantizedPages, quantized_append, quantized_attention
+    n, dim = 300, 5
+    table, n_pages = make_table([n], 16, 0)
+    pages = QuantizedPages.empty(n_pages, 16, 1, d, format=fmt)
+    seq, pos = cells([n])
+    k = _rand((n, 1, d), dtype, 1)
+    k[..., dim] = 0.0
+    quantized_append(k, _rand((n, 1, d), dtype, 2), pages, table, seq, pos)
+    q = _rand((3, hq, d), dtype, 3)
+    q[0, :, dim], q[1, ::2, dim] = large, -large / 3
+    dev = dict(dtype=torch.int32, device="cuda")
+    args = q, pages, table, torch.zeros(3, **dev), torch.tensor([n, 257, n], **dev)
+    check_attention(quantized_attention(*args), attention(*args))
+    # the large value itself, against a key that has it
+    k[7, 0, dim] = 1.0 / large
+    quantized_append(k, _rand((n, 1, d), dtype, 2), pages, table, seq, pos)
+    check_attention(quantized_attention(*args), attention(*args))
