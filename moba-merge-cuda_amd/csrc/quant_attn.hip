@@ -31,7 +31,7 @@
 // 141 us, 5.9 TB/s, where a plain read of such blocks and their scales takes 139; the first
 // form with codes loaded to registers two steps ahead took 172 in this kernel alone.  One
 // row of 128K tokens of 2 kv heads of 64 dims, fp8 (36 MB): 18.4 us; under the profiler
-// this kernel takes 14.5 of it and the join 4.8.
+// this kernel takes 14.4 of it and the join 4.7.
 #include <algorithm>
 
 #include "quant.h"
@@ -46,16 +46,16 @@ typedef int32_t i32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kUnit = 128;      // tokens of a unit: one step of each of the 4 waves
 constexpr int kMaxWgs = 768;    // of a launch, at most
 // Shares of a workgroup, at least.  Calls, us, at 2, 4, 6, 8: 256 rows of 64 to 4K tokens, one
-// kv head 24.1, 23.2, 22.6, 25.2, two 35.5, 36.7, 36.8, 36.6; one row of 128K tokens of 64 dims
-// 20.3, 18.7, 18.4, 20.0, of 96 dims 23.2, 20.8, 19.8, 19.9; 128 rows of up to 300 tokens 12.6,
-// 14.0, 13.9, 13.9; 64 rows of up to 32K within 1%.
+// kv head 24.4, 23.3, 22.8, 25.0, two 37.0, 36.5, 36.2, 36.8; one row of 128K tokens of 64 dims
+// 20.3, 18.7, 18.5, 20.0, of 96 dims 23.4, 20.9, 19.9, 19.8; 128 rows of up to 300 tokens 12.1,
+// 13.9, 13.8, 13.7; 64 rows of up to 32K within 1%.
 constexpr int kRun = 6;
 // Units' worth of time that beginning and ending an entry takes (its length, slot, pages,
 // query and sums wait for each other, about 4 us).  Calls, us, at 0, 1, 2, 3, 4: 256 rows of 64
-// to 4K tokens, one kv head 31.3, 25.2, 22.6, 21.7, 23.4, two 50.0, 39.4, 36.8, 34.7, 36.9; 64
-// rows of up to 32K 157, 147, 142, 141, 141; 32 such rows of 256 dims 94, 83, 78, 77, 76, of 192
-// 61.3, 58.5, 58.5, 59.9, 60.4; 32 rows of 512 tokens 14.2, 17.1, 15.4, 16.3, 14.6; 56 short rows
-// of 256 dims 68.4, 61.4, 61.7, 62.5, 63.9; one row of 64K 17.3, 18.5, 18.4, 18.7, 18.5.
+// to 4K tokens, one kv head 31.1, 25.4, 22.8, 21.7, 23.5, two 50.3, 39.2, 36.2, 35.0, 37.3; 64
+// rows of up to 32K 157, 145, 139, 139, 142; 32 such rows of 256 dims 94, 83, 77, 77, 77, of 192
+// 61.5, 58.7, 59.3, 60.9, 60.3; 32 rows of 512 tokens 13.6, 16.9, 15.4, 16.1, 14.6; 56 short rows
+// of 256 dims 70.2, 64.1, 63.9, 63.6, 64.8; one row of 64K 17.0, 18.2, 18.3, 18.3, 18.3.
 constexpr int kBegin = 2;
 constexpr int kManyParts = 8;   // of an entry, above which a workgroup joins one head
 constexpr int kMaxSlots = 16;   // chunks that a head selects
@@ -993,10 +993,10 @@ Shape shape_of(int Nq, int Hq, int Hkv, int D, int slots, int chunk, int max_len
   s.G = Hq / Hkv;
   // Two blocks of heads in an entry read its codes once for both; one block an entry joins
   // half as wide sums and has twice as many entries.  32 heads of one kv head, 128 dims, us:
-  // 32 rows of 100K tokens and more (950 MB) two 240, one 300; 64 rows of 20K (328 MB) 100 and
-  // 118; of 6.7K (110 MB, which stays in the last-level cache) 46 and 46; of 1K 21.9 and 21.6.
+  // 32 rows of 100K tokens and more (950 MB) two 253, one 307; 64 rows of 20K (328 MB) 102 and
+  // 115; of 6.7K (110 MB, which stays in the last-level cache) 47 and 46; of 1K 22.5 and 22.0.
   // The lengths are on the device: the rule goes by what max_length lets be read, so that
-  // short rows in a long table pay a little (8 rows of 2K, 64 heads of 2, 15.5 instead of 14.3).
+  // short rows in a long table pay a little (8 rows of 2K, 64 heads of 2, 15.5 instead of 14.2).
   // With selected chunks one block, always: each reads what its own 16 heads chose, where two
   // read the other's too.  64 rows of 100K, one and two: 4 chunks of 64 a head 35, 56; 4 of 512
   // 92, 128; 9 of 1024 of which heads share nine in ten 141, 189; that all heads agree on 64, 62.
